@@ -329,6 +329,122 @@ int ming_ln_modulate(ming_ctx* ctx, const uint16_t* x, int64_t ldx,
                      const uint16_t* scale, uint16_t* y, int64_t ldy, int rows,
                      int D, float eps);
 
+/* ---- rows that choose their own weights ------------------------------------------
+ * A mixture of experts (the language encoder's feed-forward: a router, grouped
+ * products, a weighted sum; the reference's LlmOps, ming-ops.cc:250-428) and
+ * projections over a batch of requests that each bring their own adapter. The
+ * choices are device data: nothing here waits for the GPU or allocates, so
+ * every call below but the creations and ming_adapters_set / _clear can be
+ * captured, and a replay takes the choices that are in memory then. Scratch is
+ * the caller's (ws, 16-byte aligned, at least the bytes the size function
+ * names; it holds nothing between calls, and calls or graphs that may run at
+ * the same time need one each). Strides in elements.
+ *
+ * The router: per row of logits [rows][ld] (f32 when logits_f32, else bf16)
+ * the scores s = softmax(l) or sigmoid(l) over n_experts, the keys s + bias
+ * (bias f32 [n_experts], NULL: none) and the top_k largest keys, ties to the
+ * lowest index. With n_groups > 1 the experts are that many equal consecutive
+ * groups, and only the top_groups groups with the largest sums of their two
+ * best keys take part. ids [rows][top_k] holds the chosen experts, best first,
+ * weights [rows][top_k] their scores (without the bias), divided by the row's
+ * sum of them when `normalize`, times scale. An expert whose logit is -inf or
+ * NaN, or whose key is, is never chosen; a row with fewer than top_k experts
+ * left ends in ids of -1 with weights of 0. A logit of +inf counts as the
+ * largest finite one. Scores, keys and sums are in f64. n_experts <= 1024, a
+ * multiple of n_groups <= 64; top_k <= 64 and <= the experts of top_groups
+ * groups. */
+#define MING_SCORE_SOFTMAX 0
+#define MING_SCORE_SIGMOID 1
+int ming_topk_route(ming_ctx* ctx, const void* logits, int64_t ld, int logits_f32,
+                    const float* bias, int rows, int n_experts, int top_k, int n_groups,
+                    int top_groups, int score, int normalize, float scale, int32_t* ids,
+                    float* weights);
+
+/* The plan of a grouped product: the n entries of ids (a router's [rows][top_k],
+ * flat) in the order of their group, entries of one group in their own order.
+ * offsets [n_groups + 1]: group g is places offsets[g] .. offsets[g + 1] - 1;
+ * order [n]: the entry at each place; place [n]: each entry's place. Entries
+ * whose id is outside [0, n_groups) are in no group: their place is -1, and so
+ * is order from offsets[n_groups] on. n_groups <= 1024, n <= 2^30. */
+size_t ming_group_rows_workspace_bytes(int n, int n_groups);
+int ming_group_rows(ming_ctx* ctx, const int32_t* ids, int n, int n_groups, int32_t* offsets,
+                    int32_t* order, int32_t* place, void* ws, size_t ws_bytes);
+
+/* A stack of n_experts projections of one shape, resident: codes [n_experts][N]
+ * [K*bits/32], scales and biases [n_experts][N][K/64] as ming_qweight_create
+ * takes them, or dense bf16 [n_experts][N][K]. K % 64 == 0, N % 8 == 0, one
+ * expert's weights below 2 GiB, n_experts <= 1024. Quantized scales and biases
+ * must be exact in fp16 (MING_ERR_RANGE otherwise). */
+typedef struct ming_experts ming_experts;
+int ming_experts_create(ming_ctx* ctx, int n_experts, int N, int K, int bits, int group,
+                        const uint32_t* codes, const uint16_t* scales, const uint16_t* biases,
+                        int src_on_device, ming_experts** out);
+int ming_experts_create_dense(ming_ctx* ctx, int n_experts, int N, int K, const uint16_t* w,
+                              int src_on_device, ming_experts** out);
+int ming_experts_destroy(ming_experts* ex);
+int ming_experts_shape(const ming_experts* ex, int* n_experts, int* N, int* K, int* bits);
+
+/* Each place's row times its own expert: for places p of expert e's group
+ * (offsets, n and order from ming_group_rows over n_experts groups),
+ *   ming_experts_lin:     y[p] = x[r] . W_e^T
+ *   ming_experts_swiglu:  y[p] = bf16(silu(x[r] . G_e^T) * (x[r] . U_e^T)), G_e
+ *                         the first N/2 rows of W_e, U_e the others: y is N/2
+ *                         wide, the products stay in f32 up to the one rounding
+ * with r = order[p] / fan (a token's row for each of its fan choices), or p
+ * itself where order is NULL (x already in place order). Rows of y from
+ * offsets[n_experts] on are left as they were. x [x_rows][ldx], 16-byte
+ * aligned, ldx % 8 == 0, x_rows * ldx below 2^30; y [n][ldy], 16-byte aligned,
+ * ldy % 8 == 0; they share no memory. Quantized stacks multiply fp16
+ * activations from some rows an expert on, with ming_lin's range rule (see
+ * MING_ERR_RANGE); on the general and the wide route they take bf16 ones at
+ * any size, and more time. */
+size_t ming_experts_workspace_bytes(const ming_experts* ex, int x_rows);
+int ming_experts_lin(ming_ctx* ctx, const ming_experts* ex, const uint16_t* x, int64_t ldx,
+                     int x_rows, const int32_t* order, int fan, const int32_t* offsets, int n,
+                     uint16_t* y, int64_t ldy, void* ws, size_t ws_bytes);
+int ming_experts_swiglu(ming_ctx* ctx, const ming_experts* ex, const uint16_t* x, int64_t ldx,
+                        int x_rows, const int32_t* order, int fan, const int32_t* offsets,
+                        int n, uint16_t* y, int64_t ldy, void* ws, size_t ws_bytes);
+
+/* The expert rows back to their tokens: out[t] = bf16(add[t] + sum over j <
+ * top_k of weights[t][j] * y[place[t * top_k + j]]), f32, j in order, one
+ * rounding. A place outside [0, n) adds nothing. add [tokens][ldadd] may be NULL
+ * or out itself. N, strides multiples of 8, 16-byte aligned. */
+int ming_experts_combine(ming_ctx* ctx, const uint16_t* y, int64_t ldy, int n,
+                         const int32_t* place, const float* weights, int tokens, int top_k,
+                         const uint16_t* add, int64_t ldadd, uint16_t* out, int64_t ldo, int N);
+
+/* Adapters for the rows of many requests beside one projection shape [N][K]: up
+ * to `capacity` of them (<= 4096), each of a rank of its own up to max_rank
+ * (<= MING_MAX_LORA_RANK). Factors as ming_qweight_bind_lora's; every value and
+ * fold must be finite (MING_ERR_RANGE: an infinite factor would reach the rows
+ * of other requests that share a tile). _set replaces what `id` held, _clear
+ * empties it; both wait for the context's stream, and no call or replay that
+ * reads the bank may be running elsewhere. */
+typedef struct ming_adapters ming_adapters;
+int ming_adapters_create(ming_ctx* ctx, int N, int K, int capacity, int max_rank,
+                         ming_adapters** out);
+int ming_adapters_destroy(ming_adapters* bank);
+int ming_adapters_set(ming_adapters* bank, int id, int rank, const uint16_t* A,
+                      const uint16_t* B, float fold, int src_on_device);
+int ming_adapters_clear(ming_adapters* bank, int id);
+/* Rank bound at id, 0 when none. */
+int ming_adapters_rank(const ming_adapters* bank, int id);
+
+/* ming_lin with an adapter a row: y[m] = x[m] . W^T + row_scale[m] * fold_a *
+ * B_a (A_a x[m]), a = row_adapter[m] (device int32 [M]; row_scale device f32
+ * [M], NULL: all 1). A row whose id names no bound adapter, or whose strength
+ * is 0, is ming_lin's row without adapters. The adapters' sum joins the f32
+ * result before the one rounding; a row's bits do not depend on the other rows'
+ * adapters (but for the sign of a zero). Slots bound on the weight take no part.
+ * x and y as ming_lin's; they share no memory. */
+size_t ming_lin_adapters_workspace_bytes(ming_ctx* ctx, const ming_qweight* qw,
+                                         const ming_adapters* bank, int M);
+int ming_lin_adapters(ming_ctx* ctx, const ming_qweight* qw, const ming_adapters* bank,
+                      const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, int M,
+                      const int32_t* row_adapter, const float* row_scale, void* ws,
+                      size_t ws_bytes);
+
 /* ---- the pack quantizer (ming-quant-family.cc:31-59's recipe target) -----------
  * Device f32 w [N, K] -> the pack layout ming_qweight_create reads: bits 8
  * symmetric (s = bf16(max|w|/127), code = clamp(rint(w/s), -127, 127) +

@@ -1,0 +1,268 @@
+"""The experts' ragged products (plain and SwiGLU-gated; w4, w8 and dense
+stacks) against 64-bit products: uneven groups, rows at every tile edge, places
+that were dropped, strides, routes, captured calls, and the whole feed-forward
+from logits to tokens."""
+import numpy as np
+import pytest
+import torch
+
+import ming_dit_amd as m
+import rows_ref as ref
+from helpers import bf16, f32, from_dev, randn, sync, to_dev
+
+pytestmark = pytest.mark.gpu
+SENTINEL = 0x4242
+
+
+def run(ctx, ex, gated, x, offsets, order, n, fan=1, padx=0, pady=0):
+    """y of one call, with sentinels behind the last group and in the padding."""
+    width = ex.N // 2 if gated else ex.N
+    rows = x.shape[0]
+    xs = np.full((max(rows, 1), ex.K + padx), 0x7fc0, np.uint16)   # NaN beside the columns
+    xs[:rows, :ex.K] = x
+    xd, y = to_dev(xs), to_dev(np.full((n + 3, width + pady), SENTINEL, np.uint16))
+    ws = torch.empty(max(1, ex.workspace_bytes(rows)), dtype=torch.uint8, device="cuda")
+    call = ctx.experts_swiglu if gated else ctx.experts_lin
+    od = None if order is None else to_dev(order)
+    offd = to_dev(offsets)
+    sync()
+    call(ex, xd, rows, od, offd, n, y, fan=fan, ws=ws, ldx=ex.K + padx, ldy=width + pady)
+    ctx.synchronize()
+    y = from_dev(y)
+    held = int(offsets[-1])
+    assert np.all(y[held:] == SENTINEL) and np.all(y[:, width:] == SENTINEL)
+    return y[:held, :width]
+
+
+def check(got, w, x, offsets, src, gated, bits):
+    want, bound = ref.products(f32(x), w, offsets, src, gated, bits)
+    got = f32(got).astype(np.float64)
+    assert got.shape == want.shape
+    worst = np.max(np.abs(got - want) / bound) if got.size else 0.0
+    assert worst <= 1.0, worst
+    if got.size > 1000:
+        assert ref.rel(got, want) <= ref.REL
+
+
+COUNTS = {
+    "one row": [0, 1, 0],
+    "a row each": [1] * 7,
+    "edges": [15, 0, 16, 17, 1, 0, 63],
+    "tiles": [64, 65, 0, 127, 128, 129],
+    "uneven": [0, 300, 2, 0, 0, 31],
+    "large": [255, 256, 257, 513],
+}
+
+
+@pytest.mark.parametrize("bits", [4, 8, 16])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("what", COUNTS)
+def test_products(ctx, bits, gated, what):
+    counts = COUNTS[what]
+    E, K, N = len(counts), 192, 144
+    ex, w = ref.make_experts(ctx, 11000, E, N, K, bits)
+    offsets, order, src = ref.plan_of(counts, n=sum(counts) + 11, fan=2, seed=E, x_rows=50)
+    x = bf16(randn(11100, (50, K)))
+    got = run(ctx, ex, gated, x, offsets, order, order.size, fan=2, padx=8, pady=8)
+    check(got, w, x, offsets, src, gated, bits)
+    ex.close()
+
+
+@pytest.mark.parametrize("bits", [4, 8, 16])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("N,K", [(16, 64), (272, 128), (528, 1088), (1040, 576)])
+def test_product_shapes(ctx, bits, gated, N, K):
+    """Narrow and odd widths, one K group to many; places in the rows' order."""
+    counts = [3, 0, 70, 40]
+    ex, w = ref.make_experts(ctx, 11200, 4, N, K, bits)
+    offsets, _, _ = ref.plan_of(counts)
+    n = sum(counts)
+    x = bf16(randn(11300, (n, K)))
+    got = run(ctx, ex, gated, x, offsets, None, n)
+    check(got, w, x, offsets, np.arange(n), gated, bits)
+    ex.close()
+
+
+@pytest.mark.parametrize("E", [63, 64, 65, 200, 1000])
+def test_many_experts(ctx, E):
+    rng = np.random.default_rng(E)
+    counts = rng.integers(0, 4, E) * (rng.random(E) < 0.5)
+    counts[E - 1] = 2
+    ex, w = ref.make_experts(ctx, 11400, E, 16, 64, 16)
+    offsets, order, src = ref.plan_of(counts, fan=1, seed=E, x_rows=30)
+    x = bf16(randn(11500, (30, 64)))
+    got = run(ctx, ex, False, x, offsets, order, order.size)
+    check(got, w, x, offsets, src, False, 16)
+    ex.close()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_wide_and_general_routes_take_any_finite_row(ctx, bits):
+    """fp16 holds magnitudes below 2^16; the other routes multiply bf16."""
+    counts = [200, 0, 130]
+    ex, w = ref.make_experts(ctx, 11600, 3, 64, 128, bits)
+    offsets, order, src = ref.plan_of(counts, x_rows=64)
+    x = bf16(randn(11700, (64, 128)))
+    x[5, 7] = bf16(np.float32([3.0e6]))[0]
+    try:
+        for route in ("wide", "general"):
+            ctx.set_route(route)
+            got = run(ctx, ex, True, x, offsets, order, order.size)
+            check(got, w, x, offsets, src, True, bits)
+    finally:
+        ctx.set_route("auto")
+    ex.close()
+
+
+def test_a_bad_row_stays_its_own(ctx):
+    """NaN and infinity in one token reach that token's places alone."""
+    counts = [5, 100, 0, 64]
+    ex, w = ref.make_experts(ctx, 11800, 4, 64, 128, 16)
+    offsets, order, src = ref.plan_of(counts, x_rows=40)
+    x = bf16(randn(11900, (40, 128)))
+    clean = run(ctx, ex, True, x, offsets, order, order.size)
+    x[3, 0], x[3, 1] = 0x7fc0, 0x7f80
+    got = run(ctx, ex, True, x, offsets, order, order.size)
+    assert np.isnan(f32(got[src == 3])).all()
+    assert np.array_equal(got[src != 3], clean[src != 3])
+    ex.close()
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_captured_products_follow_the_plan(ctx, bits):
+    """A captured call replays with the plan that is in memory then, on a stream
+    and context of its own, with eager calls between."""
+    s = torch.cuda.Stream()
+    c = m.Ctx(0, s.cuda_stream)
+    E, N, K, T, k = 9, 96, 192, 70, 3
+    n = T * k
+    ex, w = ref.make_experts(c, 12000, E, N, K, bits)
+    rng = np.random.default_rng(1)
+    ids = torch.zeros(n, dtype=torch.int32, device="cuda")
+    x, y = to_dev(np.zeros((T, K), np.uint16)), to_dev(np.zeros((n, N // 2), np.uint16))
+    off = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+    order, place = torch.zeros_like(ids), torch.zeros_like(ids)
+    ws = torch.empty(max(1, ex.workspace_bytes(T)), dtype=torch.uint8, device="cuda")
+
+    def call():
+        c.group_rows(ids, n, E, off, order, place)
+        c.experts_swiglu(ex, x, T, order, off, n, y, fan=k, ws=ws)
+
+    sync()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s, capture_error_mode="thread_local"):
+        call()
+    for it in range(3):
+        hi = rng.integers(-1, E if it else 2, n).astype(np.int32)
+        hx = bf16(randn(12100 + it, (T, K)))
+        ids.copy_(to_dev(hi))
+        x.copy_(to_dev(hx))
+        y.fill_(0)
+        sync()
+        g.replay()
+        sync()
+        got = from_dev(y)
+        offsets, horder, _ = ref.group(hi, E)
+        held = int(offsets[-1])
+        check(got[:held], w, hx, offsets, horder[:held] // k, True, bits)
+        assert not got[held:].any()
+        y.fill_(0)
+        sync()
+        call()
+        c.synchronize()
+        assert np.array_equal(from_dev(y), got)
+    del g
+    ex.close()
+    c.close()
+
+
+@pytest.mark.parametrize("bits", [4, 8, 16])
+@pytest.mark.parametrize("T", [1, 6, 150])
+def test_feed_forward(ctx, orc, bits, T):
+    """Logits to tokens: route, group, gate and up, down, the weighted sum onto
+    the shared output, each step from what the one before left."""
+    E, k, H, F = 12, 4, 192, 160
+    n = T * k
+    gu, wgu = ref.make_experts(ctx, 12200, E, 2 * F, H, bits)
+    # down takes K = F rounded up to whole groups: 192 columns, the last 32 zero
+    FP = 192
+    dn, wdn = ref.make_experts(ctx, 12300, E, H, FP, bits)
+    x = bf16(randn(12400 + T, (T, H)))
+    logits = randn(12500 + T, (T, E), 2.0)
+    shared = bf16(randn(12600 + T, (T, H)))
+    i32 = lambda size: torch.empty(size, dtype=torch.int32, device="cuda")
+    ids, off, order, place = i32((T, k)), i32(E + 1), i32(n), i32(n)
+    wt = torch.empty((T, k), dtype=torch.float32, device="cuda")
+    h, y = to_dev(np.zeros((n, FP), np.uint16)), to_dev(np.zeros((n, H), np.uint16))
+    out = to_dev(shared)
+    xd, ld = to_dev(x), to_dev(logits)
+    ws = torch.empty(max(gu.workspace_bytes(T), dn.workspace_bytes(n), 1), dtype=torch.uint8,
+                     device="cuda")
+    sync()
+    ctx.topk_route(ld, T, E, k, ids, wt, score="sigmoid", scale=1.5)
+    ctx.group_rows(ids, n, E, off, order, place)
+    ctx.experts_swiglu(gu, xd, T, order, off, n, h, fan=k, ws=ws, ldy=FP)
+    ctx.experts_lin(dn, h, n, None, off, n, y, ws=ws)
+    ctx.experts_combine(y, n, place, wt, T, k, out, H, add=out)
+    ctx.synchronize()
+    wid, ww = ref.route(logits, k, score="sigmoid", scale=1.5)
+    assert np.array_equal(from_dev(ids), wid)
+    offsets, worder, wplace = ref.group(wid.reshape(-1), E)
+    assert np.array_equal(from_dev(order), worder) and np.array_equal(from_dev(off), offsets)
+    hh = from_dev(h)
+    check(hh[:, :F], wgu, x, offsets, worder // k, True, bits)
+    assert not hh[:, F:].any()
+    check(from_dev(y), wdn, hh, offsets, np.arange(n), False, bits)
+    want, bound = ref.combine(f32(from_dev(y)), wplace.reshape(T, k), from_dev(wt), f32(shared), n)
+    assert np.all(np.abs(f32(from_dev(out)) - want) <= bound)
+    # and the chain in 64 bits: four roundings to bf16 (h, y, out, and the
+    # weights' to f32 or fp16 beside them), each at most BF16 / sqrt(3)
+    h64, _ = ref.products(f32(x), wgu, offsets, worder // k, True, bits)
+    h64 = np.concatenate([h64, np.zeros((n, FP - F))], 1)
+    y64, _ = ref.products(h64, wdn, offsets, np.arange(n), False, bits)
+    o64, _ = ref.combine(y64, wplace.reshape(T, k), ww, f32(shared), n)
+    assert ref.rel(f32(from_dev(out)), o64) <= 2 * ref.REL
+    gu.close()
+    dn.close()
+
+
+def test_products_refusals(ctx):
+    ex, _ = ref.make_experts(ctx, 12700, 3, 40, 64, 16)
+    x, y = to_dev(np.zeros((8, 64), np.uint16)), to_dev(np.zeros((8, 40), np.uint16))
+    off = torch.zeros(4, dtype=torch.int32, device="cuda")
+    order = torch.zeros(8, dtype=torch.int32, device="cuda")
+    ok = dict(ex=ex, x=x, x_rows=8, order=order, offsets=off, n=8, y=y, fan=1)
+    for kw in ({"n": -1}, {"fan": 0}, {"x_rows": -1}, {"x_rows": 0}, {"ldx": 56}, {"ldx": 68},
+               {"ldy": 32}, {"ldy": 42}, {"x": None}, {"y": None}, {"offsets": None},
+               {"y": x}, {"x": x.data_ptr() + 2}, {"order": None, "x_rows": 7},
+               {"x_rows": 1 << 26}):
+        with pytest.raises(m.MingError):
+            ctx.experts_lin(**dict(ok, **kw))
+    with pytest.raises(m.MingError, match="16"):     # 40 rows are not two halves of eights
+        ctx.experts_swiglu(**ok)
+    ctx.experts_lin(**dict(ok, n=0))
+    other = m.Ctx(0)
+    with pytest.raises(m.MingError, match="another"):
+        other.experts_lin(**ok)
+    other.close()
+    with pytest.raises(m.MingError):                  # the context outlives its stacks
+        m._check(m.lib().ming_ctx_destroy(ctx.h))
+    ex.close()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_create_refusals(ctx, bits):
+    pack, _ = ref.stack(12800, 2, 16, 64, bits)
+    for kw in ({"bits": 5}, {"group": 32}):
+        with pytest.raises(m.MingError):
+            m.Experts.quantized(ctx, pack["codes"], pack["scales"], pack["biases"],
+                                kw.get("bits", bits), kw.get("group", 64))
+    bad = pack["scales"].copy()
+    bad[1, 3, 0] = 0x7f00                             # about 2^127
+    with pytest.raises(m.MingError, match="fp16") as e:
+        m.Experts.quantized(ctx, pack["codes"], bad, pack["biases"], bits)
+    assert e.value.code == m.ERR_RANGE
+    with pytest.raises(m.MingError):
+        m.Experts.dense(ctx, np.zeros((2, 12, 64), np.uint16))
+    with pytest.raises(m.MingError):
+        m.Experts.dense(ctx, np.zeros((2, 16, 72), np.uint16))

@@ -1,0 +1,231 @@
+// The experts' products over ragged groups of rows: y[p] = x[row(p)] . W_e^T
+// for the rows p of expert e's group, plain or SwiGLU-gated (kernels.h).
+#include "common.h"
+#include "kernels.h"
+#include "row_groups.h"
+
+namespace ming {
+namespace {
+
+__device__ __forceinline__ floatx4_t mfma16(const uint4& w, const uint4& x, floatx4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w),
+                                                 __builtin_bit_cast(bf16x8_t, x), c, 0, 0, 0);
+}
+__device__ __forceinline__ float byte_f(uint32_t w, int i) { return (float)((w >> (8 * i)) & 0xffu); }
+__device__ __forceinline__ float f16_lo(uint32_t u) {
+  return (float)__builtin_bit_cast(_Float16, (uint16_t)(u & 0xffffu));
+}
+__device__ __forceinline__ float f16_hi(uint32_t u) {
+  return (float)__builtin_bit_cast(_Float16, (uint16_t)(u >> 16));
+}
+
+// One 64-group of weight row n, the 16 values k 16g..16g+15, as the A operands
+// of two v_mfma_f32_16x16x32_bf16: dense weights as they are, codes as the
+// integers they hold (exact in bf16).
+template <int BITS>
+struct Raw {
+  uint4 v[BITS == 16 ? 2 : 1];
+};
+template <int BITS>
+__device__ __forceinline__ void load_group(const ExpertsArgs& a, const void* w, int n, int kt,
+                                           int g, Raw<BITS>& r) {
+  if constexpr (BITS == 16) {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(w) +
+                                                    (long long)n * a.K + 64 * kt + 16 * g);
+    r.v[0] = p[0];
+    r.v[1] = p[1];
+  } else {
+    // [kt][n][fk][kk] words: k 16 kk + 8 fk + 0..7
+    const uint32_t* p = static_cast<const uint32_t*>(w) + ((long long)kt * a.NW + n) * (2 * BITS);
+    if constexpr (BITS == 4) {
+      r.v[0] = make_uint4(p[g], p[4 + g], 0, 0);
+    } else {
+      const uint2 c = *reinterpret_cast<const uint2*>(p + 2 * g);
+      const uint2 d = *reinterpret_cast<const uint2*>(p + 8 + 2 * g);
+      r.v[0] = make_uint4(c.x, c.y, d.x, d.y);
+    }
+  }
+}
+template <int BITS>
+__device__ __forceinline__ void operands(const Raw<BITS>& r, uint4& w0, uint4& w1) {
+  if constexpr (BITS == 16) {
+    w0 = r.v[0];
+    w1 = r.v[1];
+  } else {
+    auto bytes = [](uint32_t c, uint32_t d) {
+      uint4 o;
+      o.x = pack_bf16x2_rne(byte_f(c, 0), byte_f(c, 1));
+      o.y = pack_bf16x2_rne(byte_f(c, 2), byte_f(c, 3));
+      o.z = pack_bf16x2_rne(byte_f(d, 0), byte_f(d, 1));
+      o.w = pack_bf16x2_rne(byte_f(d, 2), byte_f(d, 3));
+      return o;
+    };
+    if constexpr (BITS == 4) {
+      // nibbles {k0,k4,k1,k5,k2,k6,k3,k7}: the even ones are k0..k3 by byte
+      auto word = [&](uint32_t c) {
+        uint32_t lo = c & 0x0F0F0F0Fu, hi = (c >> 4) & 0x0F0F0F0Fu;
+        asm("" : "+v"(lo), "+v"(hi));   // kept as two masks, a conversion a byte
+        return bytes(lo, hi);
+      };
+      w0 = word(r.v[0].x);
+      w1 = word(r.v[0].y);
+    } else {
+      w0 = bytes(r.v[0].x, r.v[0].y);
+      w1 = bytes(r.v[0].z, r.v[0].w);
+    }
+  }
+}
+
+// ---- few rows an expert --------------------------------------------------------
+// A block takes 16 output columns of one expert with rows, 16 of its rows at a
+// time, its WK waves each a residue class of K's 64-groups; the sums meet in
+// LDS and are added in class order, so the bits depend on K alone. Quantized
+// weights multiply as integers: scale * sum(q x) + bias * sum(x) a group, in
+// f32, the activations as the bf16 they are (no range limit). Bound by HBM:
+// the weights of the experts that have rows, once.
+template <int BITS, bool GATED, int WK>
+__global__ __launch_bounds__(64 * WK) void experts_rows_kernel(const ExpertsArgs a) {
+  constexpr int CT = GATED ? 2 : 1;
+  constexpr int U = WK == 4 ? 1 : 4 / CT;  // groups of a wave in flight
+  const RowGroup rg =
+      find_group(a.offsets, a.E, a.n, (int)blockIdx.y, [](int) { return 1; });
+  if (rg.e < 0) return;
+  const int lane = (int)threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int n0 = (int)blockIdx.x * 16;
+  const int KT = a.K / 64;
+  const long long words = (long long)a.NW * a.K * BITS / 32;
+  const void* const w = BITS == 16
+                            ? (const void*)(a.w16 + (long long)rg.e * a.NW * a.K)
+                            : (const void*)(a.codes + (long long)rg.e * words);
+  const uint32_t* const sbp = a.sb + (long long)rg.e * a.NW * KT;
+  const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+  __shared__ floatx4_t red[WK][CT][64];
+  for (int r0 = 0; r0 < rg.rows; r0 += 16) {
+    const bool row = c < rg.rows - r0;     // lanes past the rows multiply row r0, never store
+    const int p = rg.p0 + r0 + (row ? c : 0);
+    int src = p;
+    if (a.order) {
+      src = a.order[p] / a.fan;
+      src = src < 0 ? 0 : src < a.x_rows ? src : a.x_rows - 1;
+    }
+    const uint16_t* const xr = a.x + (long long)src * a.ldx + 16 * g;
+    floatx4_t acc[CT];
+#pragma unroll
+    for (int t = 0; t < CT; ++t) acc[t] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k0 = wave; k0 < KT; k0 += WK * U) {
+      Raw<BITS> wr[U][CT];
+      uint4 x[U][2];
+      [[maybe_unused]] uint4 sb[U][CT];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int kt = k0 + WK * u;
+        if (kt < KT) {
+          const uint4* xp = reinterpret_cast<const uint4*>(xr + 64 * kt);
+          x[u][0] = xp[0];
+          x[u][1] = xp[1];
+#pragma unroll
+          for (int t = 0; t < CT; ++t) {
+            // columns past N (a multiple of 8) compute the last ones, never store
+            const int n = n0 + c;
+            load_group<BITS>(a, w, (n < a.N ? n : a.N - 1) + t * a.N, kt, g, wr[u][t]);
+            if constexpr (BITS != 16) {
+              const int ns = n0 + 4 * g;
+              sb[u][t] = *reinterpret_cast<const uint4*>(sbp + (long long)kt * a.NW + t * a.N +
+                                                         (ns < a.N ? ns : a.N - 4));
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (k0 + WK * u < KT) {
+          [[maybe_unused]] floatx4_t sx;
+          const floatx4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+          if constexpr (BITS != 16) sx = mfma16(ones, x[u][1], mfma16(ones, x[u][0], zero));
+#pragma unroll
+          for (int t = 0; t < CT; ++t) {
+            uint4 w0, w1;
+            operands<BITS>(wr[u][t], w0, w1);
+            if constexpr (BITS == 16) {
+              acc[t] = mfma16(w0, x[u][0], acc[t]);
+              acc[t] = mfma16(w1, x[u][1], acc[t]);
+            } else {
+              const floatx4_t d = mfma16(w1, x[u][1], mfma16(w0, x[u][0], zero));
+              const uint32_t* sp = &sb[u][t].x;
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                acc[t][r] += __builtin_fmaf(f16_lo(sp[r]), d[r], f16_hi(sp[r]) * sx[r]);
+            }
+          }
+        }
+      }
+    }
+    // lane (m = c, g): columns 4g + 0..3 of the 16, row m
+#pragma unroll
+    for (int t = 0; t < CT; ++t) red[wave][t][lane] = acc[t];
+    __syncthreads();
+    const int n = n0 + 4 * g;
+    if (wave == 0 && row && n < a.N) {
+      floatx4_t v[CT];
+#pragma unroll
+      for (int t = 0; t < CT; ++t) {
+        v[t] = red[0][t][lane];
+#pragma unroll
+        for (int j = 1; j < WK; ++j) v[t] += red[j][t][lane];
+      }
+      if constexpr (GATED) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[0][r] = silu_f(v[0][r]) * v[1][r];
+      }
+      *reinterpret_cast<uint2*>(a.y + (long long)(rg.p0 + r0 + c) * a.ldy + n) =
+          make_uint2(pack_bf16x2_rne(v[0][0], v[0][1]), pack_bf16x2_rne(v[0][2], v[0][3]));
+    }
+    __syncthreads();                       // the sums are read: the next rows' may come
+  }
+}
+
+template <int BITS, bool GATED>
+void rows_shape(const ExpertsArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)(a.n < a.E ? a.n : a.E));
+  if (a.K <= 512)
+    hipLaunchKernelGGL((experts_rows_kernel<BITS, GATED, 4>), grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((experts_rows_kernel<BITS, GATED, 8>), grid, dim3(512), 0, s, a);
+}
+
+}  // namespace
+
+hipError_t launch_experts_rows(int bits, bool gated, const ExpertsArgs& a, hipStream_t s) {
+  if (a.n <= 0 || a.N <= 0) return hipSuccess;
+  if (a.K % 64 || a.N % 8 || a.NW != a.N * (gated ? 2 : 1) || a.E < 1 || a.fan < 1 || a.x_rows < 1)
+    return hipErrorInvalidValue;
+  switch (bits) {
+    case 4: gated ? rows_shape<4, true>(a, s) : rows_shape<4, false>(a, s); break;
+    case 8: gated ? rows_shape<8, true>(a, s) : rows_shape<8, false>(a, s); break;
+    case 16: gated ? rows_shape<16, true>(a, s) : rows_shape<16, false>(a, s); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+hipError_t validate_experts_kernels() {
+  hipFuncAttributes fa;
+  const void* fns[] = {
+#define MING_EXPERTS_ROWS(BITS)                                               \
+  reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 4>),        \
+      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 8>),    \
+      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 4>),     \
+      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 8>)
+      MING_EXPERTS_ROWS(4), MING_EXPERTS_ROWS(8), MING_EXPERTS_ROWS(16)
+#undef MING_EXPERTS_ROWS
+  };
+  for (const void* f : fns) {
+    const hipError_t e = hipFuncGetAttributes(&fa, f);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+}  // namespace ming

@@ -1,0 +1,349 @@
+// Host side of the mixture's operators: the router, the grouping, the resident
+// expert stacks with their ragged products, and the weighted sum.
+#include <algorithm>
+#include <new>
+#include <string>
+
+#include "../../include/ming_dit_amd.h"
+#include "kernels.h"
+#include "rt.h"
+
+using ming::rt_fail;
+using ming::rt_ok;
+
+struct ming_experts {
+  ming_ctx* ctx = nullptr;
+  int E = 0, N = 0, K = 0, bits = 0;
+  uint32_t* codes = nullptr;   // bits 4 / 8: the fast resident layout, an expert after another
+  uint32_t* sb = nullptr;
+  uint16_t* w16 = nullptr;     // bits 16
+};
+
+namespace {
+
+struct DeviceGuard {
+  int prev = -1;
+  explicit DeviceGuard(int dev) {
+    if (hipGetDevice(&prev) != hipSuccess) prev = -1;
+    if (prev != dev) (void)hipSetDevice(dev);
+  }
+  ~DeviceGuard() {
+    int cur = -1;
+    if (prev >= 0 && hipGetDevice(&cur) == hipSuccess && cur != prev) (void)hipSetDevice(prev);
+  }
+};
+
+hipStream_t stream_of(const ming_ctx* c) { return (hipStream_t)ming_ctx_stream(c); }
+bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
+int hip_fail(hipError_t e, const char* what) {
+  return rt_fail(MING_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
+}
+// Two address ranges of rows x stride (the last row `width` wide), 2-byte elements.
+bool overlap(const void* a, int64_t ra, int64_t lda, int64_t wa, const void* b, int64_t rb,
+             int64_t ldb, int64_t wb) {
+  if (ra <= 0 || rb <= 0) return false;
+  const uint64_t a0 = (uint64_t)(uintptr_t)a, b0 = (uint64_t)(uintptr_t)b;
+  return a0 < b0 + 2 * (uint64_t)((rb - 1) * ldb + wb) &&
+         b0 < a0 + 2 * (uint64_t)((ra - 1) * lda + wa);
+}
+
+// One launch, timed when the context profiles.
+template <class F>
+int run(ming_ctx* c, ming::RtBucket b, double flops, double bytes, const char* what, F&& launch) {
+  void* ev = nullptr;
+  if (!ming::rt_profile_begin(c, &ev)) return hip_fail(hipErrorOutOfMemory, what);
+  const hipError_t e = launch();
+  const bool timed = ming::rt_profile_end(c, ev, b, flops, bytes);
+  if (e != hipSuccess) return hip_fail(e, what);
+  if (!timed) return hip_fail(hipErrorOutOfMemory, what);
+  return MING_OK;
+}
+
+int products(const char* who, bool gated, ming_ctx* c, const ming_experts* ex, const uint16_t* x,
+             int64_t ldx, int x_rows, const int32_t* order, int fan, const int32_t* offsets, int n,
+             uint16_t* y, int64_t ldy, void* ws, size_t ws_bytes) {
+  auto bad = [&](int code, const char* why) { return rt_fail(code, std::string(who) + ": " + why); };
+  if (!c || !ex || !x || !offsets || !y) return bad(MING_ERR_ARG, "null argument");
+  if (ex->ctx != c) return bad(MING_ERR_ARG, "experts of another context");
+  if (n < 0 || x_rows < 0 || fan < 1) return bad(MING_ERR_ARG, "a count out of range");
+  const int N = gated ? ex->N / 2 : ex->N;
+  if (gated && ex->N % 16 != 0)
+    return bad(MING_ERR_SHAPE, "gate and up rows need N % 16 == 0");
+  if (ldx < ex->K || ldx % 8 != 0 || ldy < N || ldy % 8 != 0)
+    return bad(MING_ERR_SHAPE, "need ldx >= K and ldy >= the output's width, multiples of 8");
+  if (!aligned(x, 16) || !aligned(y, 16) || !aligned(offsets, 4) || !aligned(order, 4))
+    return bad(MING_ERR_ARG, "x and y must be 16-byte, offsets and order 4-byte aligned");
+  if (n == 0) return rt_ok();
+  if (x_rows == 0) return bad(MING_ERR_ARG, "places without rows of x");
+  if (!order && x_rows < n) return bad(MING_ERR_SHAPE, "without an order x needs n rows");
+  if ((uint64_t)x_rows * (uint64_t)ldx >= (1ull << 30))
+    return bad(MING_ERR_SHAPE, "x_rows * ldx must be below 2^30");
+  if (overlap(x, x_rows, ldx, ex->K, y, n, ldy, N))
+    return bad(MING_ERR_ARG, "x and y share memory");
+  (void)ws;
+  (void)ws_bytes;
+  DeviceGuard g(ming::rt_device(c));
+  ming::ExpertsArgs a{};
+  a.x = x; a.ldx = ldx;
+  a.codes = ex->codes; a.sb = ex->sb; a.w16 = ex->w16;
+  a.offsets = offsets; a.order = order;
+  a.E = ex->E; a.fan = fan; a.x_rows = x_rows; a.n = n;
+  a.N = N; a.NW = ex->N; a.K = ex->K;
+  a.y = y; a.ldy = ldy;
+  const double flops = 2.0 * n * (double)ex->N * ex->K;
+  const double wb = ex->bits == 16 ? 2.0 * ex->N * ex->K
+                                   : (double)ex->N * ex->K * ex->bits / 8 + 4.0 * ex->N * (ex->K / 64);
+  const int rc = run(c, ming::kRtExperts, flops,
+                     wb * std::min(n, ex->E) + 2.0 * x_rows * ex->K + 2.0 * n * N, who, [&] {
+                       return ming::launch_experts_rows(ex->bits, gated, a, stream_of(c));
+                     });
+  if (rc != MING_OK) return rc;
+  ming::rt_note_rows(c, ex->bits, 2ull * (uint64_t)n * (uint64_t)ex->N * (uint64_t)ex->K);
+  return rt_ok();
+}
+
+// What both creations check.
+int check_stack(ming_ctx* c, int E, int N, int K) {
+  if (!c) return rt_fail(MING_ERR_ARG, "ming_experts_create: null argument");
+  if (E < 1 || E > ming::kGroupMax)
+    return rt_fail(MING_ERR_SHAPE, "ming_experts_create: 1 to 1024 experts");
+  if (N <= 0 || K <= 0 || K % 64 != 0 || N % 8 != 0)
+    return rt_fail(MING_ERR_SHAPE, "ming_experts_create: need K % 64 == 0 and N % 8 == 0");
+  if ((uint64_t)N * (uint64_t)K >= (1ull << 30))
+    return rt_fail(MING_ERR_SHAPE, "ming_experts_create: an expert's N * K must be below 2^30");
+  return MING_OK;
+}
+
+// Host or device memory copied to a new device buffer on the context's stream.
+hipError_t copy_in(ming_ctx* c, void** dst, const void* src, size_t bytes, int on_device) {
+  hipError_t e = hipMalloc(dst, bytes);
+  if (e == hipSuccess)
+    e = hipMemcpyAsync(*dst, src, bytes, on_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice,
+                       stream_of(c));
+  return e;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ming_topk_route(ming_ctx* c, const void* logits, int64_t ld, int logits_f32, const float* bias,
+                    int rows, int n_experts, int top_k, int n_groups, int top_groups, int score,
+                    int normalize, float scale, int32_t* ids, float* weights) {
+  auto bad = [](int code, const char* why) {
+    return rt_fail(code, std::string("ming_topk_route: ") + why);
+  };
+  if (!c || !logits || !ids || !weights) return bad(MING_ERR_ARG, "null argument");
+  if (rows < 0) return bad(MING_ERR_ARG, "rows < 0");
+  if (score != MING_SCORE_SOFTMAX && score != MING_SCORE_SIGMOID)
+    return bad(MING_ERR_ARG, "no such score");
+  if (n_experts < 1 || n_experts > ming::kRouteMaxExperts || n_groups < 1 || n_groups > 64 ||
+      n_experts % n_groups != 0)
+    return bad(MING_ERR_SHAPE, "1 to 1024 experts in at most 64 equal groups");
+  if (top_groups < 1 || top_groups > n_groups)
+    return bad(MING_ERR_SHAPE, "top_groups must be 1 to n_groups");
+  if (top_k < 1 || top_k > 64 || top_k > n_experts / n_groups * top_groups)
+    return bad(MING_ERR_SHAPE, "top_k must be 1 to 64 and fit in the chosen groups");
+  if (ld < n_experts) return bad(MING_ERR_SHAPE, "need ld >= n_experts");
+  if (!aligned(logits, logits_f32 ? 4 : 2) || !aligned(bias, 4) || !aligned(ids, 4) ||
+      !aligned(weights, 4))
+    return bad(MING_ERR_ARG, "a misaligned pointer");
+  if (rows == 0) return rt_ok();
+  DeviceGuard g(ming::rt_device(c));
+  ming::RouteArgs a{};
+  a.logits = logits; a.ld = ld; a.f32 = logits_f32 != 0; a.bias = bias;
+  a.rows = rows; a.E = n_experts; a.k = top_k; a.G = n_groups; a.top_groups = top_groups;
+  a.sigmoid = score == MING_SCORE_SIGMOID; a.normalize = normalize != 0; a.scale = scale;
+  a.ids = ids; a.weights = weights;
+  const int rc = run(c, ming::kRtRoute, 0.0, (double)rows * n_experts * (logits_f32 ? 4 : 2),
+                     "ming_topk_route", [&] { return ming::launch_topk_route(a, stream_of(c)); });
+  if (rc != MING_OK) return rc;
+  ming::rt_note_rows(c, 0, 0);
+  return rt_ok();
+}
+
+size_t ming_group_rows_workspace_bytes(int n, int n_groups) {
+  if (n <= 0 || n > (1 << 30) || n_groups < 1 || n_groups > ming::kGroupMax) return 0;
+  return ming::group_rows_bytes(n, n_groups);
+}
+
+int ming_group_rows(ming_ctx* c, const int32_t* ids, int n, int n_groups, int32_t* offsets,
+                    int32_t* order, int32_t* place, void* ws, size_t ws_bytes) {
+  auto bad = [](int code, const char* why) {
+    return rt_fail(code, std::string("ming_group_rows: ") + why);
+  };
+  if (n < 0 || n > (1 << 30)) return bad(MING_ERR_ARG, "n must be 0 to 2^30");
+  if (!c || !offsets || (n > 0 && (!ids || !order || !place)))
+    return bad(MING_ERR_ARG, "null argument");
+  if (n_groups < 1 || n_groups > ming::kGroupMax)
+    return bad(MING_ERR_SHAPE, "1 to 1024 groups");
+  if (!aligned(ids, 4) || !aligned(offsets, 4) || !aligned(order, 4) || !aligned(place, 4))
+    return bad(MING_ERR_ARG, "a misaligned pointer");
+  const size_t need = ming::group_rows_bytes(n, n_groups);
+  if (need > 0 && (!ws || !aligned(ws, 16)))
+    return bad(MING_ERR_ARG, "ws must be given, 16-byte aligned");
+  if (ws_bytes < need)
+    return rt_fail(MING_ERR_SHAPE, "ming_group_rows: the call needs " + std::to_string(need) +
+                                       " bytes of workspace, " + std::to_string(ws_bytes) +
+                                       " given");
+  DeviceGuard g(ming::rt_device(c));
+  ming::GroupRowsArgs a{};
+  a.ids = ids; a.n = n; a.G = n_groups;
+  a.offsets = offsets; a.order = order; a.place = place;
+  a.counts = static_cast<uint32_t*>(ws);
+  const int rc = run(c, ming::kRtGroup, 0.0, 12.0 * n + 4.0 * n_groups, "ming_group_rows",
+                     [&] { return ming::launch_group_rows(a, stream_of(c)); });
+  if (rc != MING_OK) return rc;
+  ming::rt_note_rows(c, 0, 0);
+  return rt_ok();
+}
+
+int ming_experts_destroy(ming_experts* ex) {
+  if (!ex) return rt_ok();
+  DeviceGuard g(ming::rt_device(ex->ctx));
+  (void)hipStreamSynchronize(stream_of(ex->ctx));
+  if (ex->codes) (void)hipFree(ex->codes);
+  if (ex->sb) (void)hipFree(ex->sb);
+  if (ex->w16) (void)hipFree(ex->w16);
+  ming::rt_release(ex->ctx);
+  delete ex;
+  return rt_ok();
+}
+
+int ming_experts_create_dense(ming_ctx* c, int n_experts, int N, int K, const uint16_t* w,
+                              int src_on_device, ming_experts** out) {
+  if (!out || !w) return rt_fail(MING_ERR_ARG, "ming_experts_create: null argument");
+  *out = nullptr;
+  if (const int rc = check_stack(c, n_experts, N, K)) return rc;
+  DeviceGuard g(ming::rt_device(c));
+  auto* ex = new (std::nothrow) ming_experts();
+  if (!ex) return rt_fail(MING_ERR_ALLOC, "ming_experts_create: out of memory");
+  ex->ctx = c; ex->E = n_experts; ex->N = N; ex->K = K; ex->bits = 16;
+  ming::rt_retain(c);
+  void* d = nullptr;
+  hipError_t e = copy_in(c, &d, w, (size_t)n_experts * N * K * 2, src_on_device);
+  ex->w16 = (uint16_t*)d;
+  if (e == hipSuccess) e = hipStreamSynchronize(stream_of(c));
+  if (e != hipSuccess) {
+    (void)hipGetLastError();
+    ming_experts_destroy(ex);
+    return e == hipErrorOutOfMemory
+               ? rt_fail(MING_ERR_ALLOC, "ming_experts_create: device allocation failed")
+               : hip_fail(e, "ming_experts_create");
+  }
+  *out = ex;
+  return rt_ok();
+}
+
+int ming_experts_create(ming_ctx* c, int n_experts, int N, int K, int bits, int group,
+                        const uint32_t* codes, const uint16_t* scales, const uint16_t* biases,
+                        int src_on_device, ming_experts** out) {
+  if (!out || !codes || !scales || !biases)
+    return rt_fail(MING_ERR_ARG, "ming_experts_create: null argument");
+  *out = nullptr;
+  if (const int rc = check_stack(c, n_experts, N, K)) return rc;
+  if (bits != 4 && bits != 8)
+    return rt_fail(MING_ERR_SHAPE, "ming_experts_create: bits must be 4 or 8");
+  if (group != 64) return rt_fail(MING_ERR_SHAPE, "ming_experts_create: group must be 64");
+  DeviceGuard g(ming::rt_device(c));
+  auto* ex = new (std::nothrow) ming_experts();
+  if (!ex) return rt_fail(MING_ERR_ALLOC, "ming_experts_create: out of memory");
+  ex->ctx = c; ex->E = n_experts; ex->N = N; ex->K = K; ex->bits = bits;
+  ming::rt_retain(c);
+  const size_t words = (size_t)N * K * bits / 32, pairs = (size_t)N * (K / 64);
+  const size_t E = (size_t)n_experts;
+  hipStream_t s = stream_of(c);
+  void *dc = nullptr, *ds = nullptr, *db = nullptr;
+  int *flag = nullptr, inexact = 0;
+  hipError_t e = copy_in(c, &dc, codes, E * words * 4, src_on_device);
+  if (e == hipSuccess) e = copy_in(c, &ds, scales, E * pairs * 2, src_on_device);
+  if (e == hipSuccess) e = copy_in(c, &db, biases, E * pairs * 2, src_on_device);
+  if (e == hipSuccess) e = hipMalloc(&ex->codes, E * words * 4);
+  if (e == hipSuccess) e = hipMalloc(&ex->sb, E * pairs * 4);
+  if (e == hipSuccess) e = hipMalloc(&flag, sizeof(int));
+  if (e == hipSuccess) e = hipMemsetAsync(flag, 0, sizeof(int), s);
+  for (size_t i = 0; i < E && e == hipSuccess; ++i)
+    e = ming::launch_repack_fast(bits, (const uint32_t*)dc + i * words,
+                                 (const uint16_t*)ds + i * pairs, (const uint16_t*)db + i * pairs,
+                                 N, K, ex->codes + i * words, ex->sb + i * pairs, flag, s);
+  if (e == hipSuccess) e = hipMemcpyAsync(&inexact, flag, sizeof(int), hipMemcpyDeviceToHost, s);
+  if (e == hipSuccess) e = hipStreamSynchronize(s);
+  for (void* p : {dc, ds, db, (void*)flag})
+    if (p) (void)hipFree(p);
+  if (e != hipSuccess || inexact) {
+    (void)hipGetLastError();
+    ming_experts_destroy(ex);
+    if (inexact)
+      return rt_fail(MING_ERR_RANGE,
+                     "ming_experts_create: a scale or bias is not exact in fp16 (create the "
+                     "stack from dense weights)");
+    return e == hipErrorOutOfMemory
+               ? rt_fail(MING_ERR_ALLOC, "ming_experts_create: device allocation failed")
+               : hip_fail(e, "ming_experts_create");
+  }
+  *out = ex;
+  return rt_ok();
+}
+
+int ming_experts_shape(const ming_experts* ex, int* n_experts, int* N, int* K, int* bits) {
+  if (!ex) return rt_fail(MING_ERR_ARG, "ming_experts_shape: null argument");
+  if (n_experts) *n_experts = ex->E;
+  if (N) *N = ex->N;
+  if (K) *K = ex->K;
+  if (bits) *bits = ex->bits;
+  return rt_ok();
+}
+
+size_t ming_experts_workspace_bytes(const ming_experts* ex, int x_rows) {
+  // the fp16 copy of x that the tiles of a quantized stack multiply
+  if (!ex || x_rows <= 0 || ex->bits == 16) return 0;
+  return (size_t)x_rows * ex->K * 2;
+}
+
+int ming_experts_lin(ming_ctx* c, const ming_experts* ex, const uint16_t* x, int64_t ldx,
+                     int x_rows, const int32_t* order, int fan, const int32_t* offsets, int n,
+                     uint16_t* y, int64_t ldy, void* ws, size_t ws_bytes) {
+  return products("ming_experts_lin", false, c, ex, x, ldx, x_rows, order, fan, offsets, n, y, ldy,
+                  ws, ws_bytes);
+}
+
+int ming_experts_swiglu(ming_ctx* c, const ming_experts* ex, const uint16_t* x, int64_t ldx,
+                        int x_rows, const int32_t* order, int fan, const int32_t* offsets, int n,
+                        uint16_t* y, int64_t ldy, void* ws, size_t ws_bytes) {
+  return products("ming_experts_swiglu", true, c, ex, x, ldx, x_rows, order, fan, offsets, n, y,
+                  ldy, ws, ws_bytes);
+}
+
+int ming_experts_combine(ming_ctx* c, const uint16_t* y, int64_t ldy, int n, const int32_t* place,
+                         const float* weights, int tokens, int top_k, const uint16_t* add,
+                         int64_t ldadd, uint16_t* out, int64_t ldo, int N) {
+  auto bad = [](int code, const char* why) {
+    return rt_fail(code, std::string("ming_experts_combine: ") + why);
+  };
+  if (!c || !out || !place || !weights || (n > 0 && !y)) return bad(MING_ERR_ARG, "null argument");
+  if (n < 0 || tokens < 0 || top_k < 1) return bad(MING_ERR_ARG, "a count out of range");
+  if (N <= 0 || N % 8 != 0 || (n > 0 && ldy < N) || ldo < N || (add && ldadd < N) ||
+      ldy % 8 != 0 || ldo % 8 != 0 || (add && ldadd % 8 != 0))
+    return bad(MING_ERR_SHAPE, "N and the strides must be multiples of 8, strides >= N");
+  if (!aligned(y, 16) || !aligned(out, 16) || !aligned(add, 16) || !aligned(place, 4) ||
+      !aligned(weights, 4))
+    return bad(MING_ERR_ARG, "y, add and out must be 16-byte, place and weights 4-byte aligned");
+  if (tokens == 0) return rt_ok();
+  if (n > 0 && overlap(y, n, ldy, N, out, tokens, ldo, N))
+    return bad(MING_ERR_ARG, "y and out share memory");
+  if (add && !(add == out && ldadd == ldo) && overlap(add, tokens, ldadd, N, out, tokens, ldo, N))
+    return bad(MING_ERR_ARG, "add and out share memory but are not the same rows");
+  DeviceGuard g(ming::rt_device(c));
+  ming::CombineArgs a{};
+  a.y = y; a.ldy = ldy; a.n = n; a.place = place; a.weights = weights;
+  a.add = add; a.ldadd = ldadd; a.out = out; a.ldo = ldo;
+  a.tokens = tokens; a.k = top_k; a.N = N;
+  const int rc = run(c, ming::kRtCombine, 0.0,
+                     2.0 * tokens * (double)N * (top_k + (add ? 2 : 1)), "ming_experts_combine",
+                     [&] { return ming::launch_combine(a, stream_of(c)); });
+  if (rc != MING_OK) return rc;
+  ming::rt_note_rows(c, 0, 0);
+  return rt_ok();
+}
+
+}  // extern "C"

@@ -187,6 +187,7 @@ __device__ __forceinline__ void gemv_body(const GemvArgs& a) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] += bf16_to_f32(a.bias[n + r]);
   }
+  if (a.delta) v += *reinterpret_cast<const floatx4_t*>(a.delta + (long long)c * a.N + n);
   *reinterpret_cast<uint2*>(a.y + (long long)c * a.ldy + n) =
       make_uint2(pack_bf16x2_rne(v[0], v[1]), pack_bf16x2_rne(v[2], v[3]));
 }

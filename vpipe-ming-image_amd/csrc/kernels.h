@@ -45,6 +45,21 @@ struct QprojMore {
   QprojSeg seg;
 };
 
+// Adapters that rows choose (adapters.hip): row m adds T[m] . B_a^T of adapter a
+// = rid[m] (-1: none), T[m] = strength * fold * (x[m] . A_a^T) in bf16.
+struct AdapterEntry {
+  const uint16_t* A;    // [r8][K], rows past the rank zero
+  const uint16_t* B;    // [N][r8], columns past the rank zero
+  int r8;               // rank padded to 8; 0: nothing bound
+  float fold;
+};
+struct RowAdapters {
+  const int32_t* rid;   // [M]
+  const uint16_t* t;    // [M][ldt]
+  int ldt;
+  const AdapterEntry* table;
+};
+
 struct QprojArgs {
   const uint16_t* x;
   long long ldx;
@@ -90,6 +105,8 @@ struct QprojArgs {
   // optional bias [N] bf16, added to the f32 result before the output's one
   // bf16 rounding (dense weights: ming_lin_bias)
   const uint16_t* bias;
+  // optional f32 [M][N], added like the bias: what rows' own adapters add
+  const float* delta;
 };
 
 // wide: bits 4/8 run with bf16 activations and the weight as a bf16 pair
@@ -158,6 +175,7 @@ struct LoraXaArgs {
   // optional (fast kernel only): bias [n_cols] bf16, T = bf16(coef * sum +
   // bias) -- the dense split-K GEMM's ming_lin_bias
   const uint16_t* bias;
+  const float* delta;   // or f32 [M][n_cols], added the same way (QprojArgs::delta)
   // fast kernel only: a dense weight's split-K GEMM. Column c is row c of
   // A[0], coefficient 1 (grp and coef unused), in tiles of `tile`
   bool ident;
@@ -269,6 +287,7 @@ struct GemvArgs {
   long long ldy;
   int M, N, K;
   const uint16_t* bias;   // optional bias [N] bf16, added before the rounding
+  const float* delta;     // optional f32 [M][N], added before the rounding
 };
 hipError_t launch_gemv(int bits, const GemvArgs& a, hipStream_t s);
 // Up to kGemvBatch GEMVs of one shape over one x in one launch (grid y =
@@ -358,6 +377,98 @@ hipError_t launch_dense_fast(const QprojArgs& a, int rf, hipStream_t s);
 int dense_fast_rf(int M, int N, int nw = 1);
 bool dense_merge_pays(int M, int N, int nw);
 hipError_t validate_dense_fast_kernels();
+
+// ---- many requests' adapters (adapters.hip) --------------------------------------
+// rid[m] = ids[m] where it names a bound adapter and the row's strength is not
+// zero, else -1; t[m][0, r32) = bf16(scale[m] * fold * x[m] . A^T), r32 the rank
+// rounded up to 32 (zeros past the rank). ldt a multiple of 32.
+struct RowXaArgs {
+  const uint16_t* x;
+  long long ldx;
+  int M, K;
+  const int32_t* ids;
+  const float* scale;   // optional
+  const AdapterEntry* table;
+  int cap;
+  int32_t* rid;
+  uint16_t* t;
+  int ldt;
+};
+hipError_t launch_row_xa(const RowXaArgs& a, hipStream_t s);
+// d[m][n] = T[m] . B_a[n] in f32, a = rid[m]; -0 for rows without an adapter,
+// which any sum takes without a change. N % 4 == 0.
+hipError_t launch_row_delta(const RowAdapters& r, int M, int N, float* d, hipStream_t s);
+// *flag = 1 where any of n bf16 values is not finite
+hipError_t launch_check_finite(const uint16_t* v, long long n, int* flag, hipStream_t s);
+hipError_t validate_adapter_kernels();
+
+// ---- a mixture's router, grouping and weighted sum (routing.hip) ---------------
+constexpr int kRouteMaxExperts = 1024;
+struct RouteArgs {
+  const void* logits;   // [rows][ld], f32 or bf16
+  long long ld;
+  int f32;
+  const float* bias;    // optional [E], added to the scores for the choice alone
+  long long rows;
+  int E, k, G, top_groups;
+  int sigmoid, normalize;
+  float scale;
+  int32_t* ids;         // [rows][k]
+  float* weights;
+};
+hipError_t launch_topk_route(const RouteArgs& a, hipStream_t s);
+constexpr int kGroupMax = 1024;
+struct GroupRowsArgs {
+  const int32_t* ids;   // [n]
+  long long n;
+  int G;
+  int32_t* offsets;     // [G + 1]
+  int32_t* order;       // [n]
+  int32_t* place;       // [n]
+  uint32_t* counts;     // group_rows_bytes(n, G)
+  int chunk, bits;      // set by the launch
+};
+size_t group_rows_bytes(long long n, int G);
+hipError_t launch_group_rows(GroupRowsArgs a, hipStream_t s);
+struct CombineArgs {
+  const uint16_t* y;
+  long long ldy;
+  int n;                // rows of y
+  const int32_t* place; // [tokens][k]
+  const float* weights;
+  const uint16_t* add;  // optional
+  long long ldadd;
+  uint16_t* out;
+  long long ldo;
+  long long tokens;
+  int k, N;
+  int tpr;              // set by the launch
+};
+hipError_t launch_combine(CombineArgs a, hipStream_t s);
+hipError_t validate_routing_kernels();
+
+// ---- the experts' ragged products (experts.hip) ---------------------------------
+// Rows [offsets[e], offsets[e + 1]) of y are expert e's: y[p] = x[row(p)] .
+// W_e^T with row(p) = order ? order[p] / fan : p, kept inside [0, x_rows). W is
+// a stack of E projections of NW rows: NW = N, or gated 2 N, the gate's N rows
+// before the up projection's, y = bf16(silu(gate) * up) of the f32 results.
+// Weights: bits 16 w16 [E][NW][K]; bits 4 / 8 the fast resident layout
+// (launch_repack_fast) an expert after another.
+struct ExpertsArgs {
+  const uint16_t* x;
+  long long ldx;
+  const uint32_t* codes;
+  const uint32_t* sb;
+  const uint16_t* w16;
+  const int32_t* offsets;
+  const int32_t* order;   // optional
+  int E, fan, x_rows, n;
+  int N, NW, K;
+  uint16_t* y;
+  long long ldy;
+};
+hipError_t launch_experts_rows(int bits, bool gated, const ExpertsArgs& a, hipStream_t s);
+hipError_t validate_experts_kernels();
 
 hipError_t validate_qproj_kernels();
 hipError_t validate_qproj_fast_kernels();

@@ -368,6 +368,13 @@ __global__ __launch_bounds__(NT, 1) void qproj_kernel(const QprojArgs a) {
             for (int e = 0; e < 4; ++e)
               if (n + e < a.N) r[e] += bf16_to_f32(a.bias[n + e]);
           }
+          if (a.delta) {
+            const float4 d = *reinterpret_cast<const float4*>(a.delta + (long long)m * a.N + n);
+            r[0] += d.x;
+            r[1] += d.y;
+            r[2] += d.z;
+            r[3] += d.w;
+          }
           uint2 v;
           v.x = pack_bf16x2_rne(r[0], r[1]);
           v.y = pack_bf16x2_rne(r[2], r[3]);

@@ -1005,11 +1005,15 @@ __global__ __launch_bounds__(512, 1) void lora_xa_fast_kernel(const LoraXaArgs a
         uint2 v;
         if (f == 0.0f) {
           v = make_uint2(0, 0);
-        } else if (a.bias) {
-          // the dense split-K GEMM with a bias (coef 1): one rounding
+        } else if (a.bias || a.delta) {
+          // the dense split-K GEMM with a bias or its rows' adapters (coef 1):
+          // one rounding
           float r[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) r[e] = f * acc[i][j][4 * q + e] + bf16_to_f32(a.bias[c + e]);
+          for (int e = 0; e < 4; ++e)
+            r[e] = f * acc[i][j][4 * q + e] +
+                   (a.bias ? bf16_to_f32(a.bias[c + e])
+                           : a.delta[(long long)m * a.n_cols + c + e]);
           v.x = pack_bf16x2_rne(r[0], r[1]);
           v.y = pack_bf16x2_rne(r[2], r[3]);
         } else {
@@ -1060,12 +1064,14 @@ __global__ void lora_xa_reduce_kernel(const float* part, int kslices, int M,
     }
     const float co = a.ident ? 1.0f : a.coef[c >> 3];
     uint4 o = make_uint4(0, 0, 0, 0);
-    if (co != 0.0f && a.bias) {
-      // the dense split-K GEMM with a bias (coef 1): one rounding
+    if (co != 0.0f && (a.bias || a.delta)) {
+      // the dense split-K GEMM with a bias or its rows' adapters (coef 1): one
+      // rounding
       float r[8] = {co * s0.x, co * s0.y, co * s0.z, co * s0.w,
                     co * s1.x, co * s1.y, co * s1.z, co * s1.w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) r[e] += bf16_to_f32(a.bias[c + e]);
+      for (int e = 0; e < 8; ++e)
+        r[e] += a.bias ? bf16_to_f32(a.bias[c + e]) : a.delta[(size_t)m * n_cols + c + e];
       o.x = pack_bf16x2_rne(r[0], r[1]);
       o.y = pack_bf16x2_rne(r[2], r[3]);
       o.z = pack_bf16x2_rne(r[4], r[5]);

@@ -38,6 +38,18 @@ int rt_take_range_fault(ming_ctx* c, const char* who);
 // whose projections are all dense); returns the previous mark.
 bool rt_set_copies_unread(ming_ctx* c, bool unread);
 
+int rt_route(const ming_ctx* c);
+// the device word fp16 copies raise (QprojArgs::range), NULL on routes without
+int* rt_range_word(const ming_ctx* c);
+// Event timing around one launch of a family (ming_ctx_set_profiling): begin
+// before it, end after; false where an event could not be had.
+enum RtBucket { kRtRoute, kRtGroup, kRtExperts, kRtCombine };
+bool rt_profile_begin(ming_ctx* c, void** ev);
+bool rt_profile_end(ming_ctx* c, void* ev, RtBucket b, double flops, double bytes);
+// counts what was dispatched: a grouped product of `bits` weights, or one of the
+// small kernels (bits 0)
+void rt_note_rows(ming_ctx* c, int bits, uint64_t flops);
+
 // Fused forms the block driver uses (same bits as the public calls they
 // replace):
 // y = rmsnorm(x) and the context's fp16 copy of y, which the next projections

@@ -106,14 +106,16 @@ namespace {
 // marks, ming-dit.cc:1689-1717, as HIP events around each launch).
 enum Bucket {
   kBQ4, kBQ8, kBDense, kBF4, kBF8, kBCvt, kBXa, kBRms, kBQkRope, kBRopeTab, kBSwiglu, kBResid,
-  kBModulate, kBBias, kBLn, kBQuant, kBAttn, kBNormRes, kBGemv, kBP4, kBP8, kBCount
+  kBModulate, kBBias, kBLn, kBQuant, kBAttn, kBNormRes, kBGemv, kBP4, kBP8, kBRowXa, kBRoute,
+  kBGroup, kBExperts, kBCombine, kBCount
 };
 const char* const kBucketName[kBCount] = {
     "qproj.w4", "qproj.w8", "qproj.dense", "qproj_fast.w4", "qproj_fast.w8",
     "cvt_f16", "lora_xa", "rmsnorm",
     "qk_norm_rope", "rope_table", "swiglu", "residual", "modulate",
     "bias_act", "ln_modulate", "quantize", "attention", "norm_residual", "gemv",
-    "qproj_pair.w4", "qproj_pair.w8"};
+    "qproj_pair.w4", "qproj_pair.w8", "row_adapters", "topk_route", "group_rows", "experts",
+    "experts_combine"};
 
 hipEvent_t take_event(ming_ctx* c) {
   if (!c->pool.empty()) {
@@ -187,6 +189,16 @@ struct ming_qweight {
   // context-refiner weights' generations, so a direct rebinding of one of
   // them is never served stale rows
   uint64_t bind_gen = 0;
+};
+
+// Adapters beside a projection's shape, chosen row by row (ming_lin_adapters).
+// The table is read on the device when a call runs; T's row stride is fixed by
+// max_rank, so a captured call stays in bounds whatever is bound later.
+struct ming_adapters {
+  ming_ctx* ctx = nullptr;
+  int N = 0, K = 0, cap = 0, max_rank = 0, ldt = 0;
+  std::vector<LoraBind> bound;
+  ming::AdapterEntry* table = nullptr;   // [cap], device
 };
 
 namespace {
@@ -435,6 +447,9 @@ hipError_t validate_kernels(int device) {
   if (e == hipSuccess) e = ming::validate_dense_fast_kernels();
   if (e == hipSuccess) e = ming::validate_gemv_kernels();
   if (e == hipSuccess) e = ming::validate_attention_kernels();
+  if (e == hipSuccess) e = ming::validate_adapter_kernels();
+  if (e == hipSuccess) e = ming::validate_routing_kernels();
+  if (e == hipSuccess) e = ming::validate_experts_kernels();
   if (known) done[device] = e == hipSuccess;
   return e;
 }
@@ -906,6 +921,11 @@ static bool overlap(const uint16_t* a, int64_t lda, int na, const uint16_t* b, i
 struct Carve {
   char* base = nullptr;
   size_t cap = 0, used = 0;
+  // measure: the call plans, sets `need` and launches nothing
+  bool measure = false;
+  size_t need = 0;
+  const char* who = "ming_lin_noalloc";
+  const char* what = "the no-alloc array";
   static size_t aligned256(size_t b) { return (b + 255) & ~(size_t)255; }
   // a 256-byte-aligned region of `bytes` (callers check the total first)
   void* take(size_t bytes) {
@@ -915,9 +935,18 @@ struct Carve {
   }
 };
 
+// Row adapters (ming_lin_adapters): one projection, scratch carved from the
+// caller's workspace, no slots.
+struct RowsCall {
+  const ming_adapters* bank;
+  const int32_t* ids;
+  const float* scale;
+};
+
 static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const LinOut* outs,
                      const uint16_t* x, int64_t ldx, int M, const float* scales,
-                     const uint16_t* xh_src, Carve* carve = nullptr) {
+                     const uint16_t* xh_src, Carve* carve = nullptr,
+                     const RowsCall* rows = nullptr) {
   for (int i = 0; i < n; ++i)
     if (outs[i].took_fast) *outs[i].took_fast = false;
   if (!c || !x || n < 1 || n > ming::kMaxXaSources)
@@ -945,6 +974,41 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
   if (M == 0) return ok();
   DeviceGuard g(c->device);
 
+  // What rows' own adapters take: their rows' adapter indices, T, and for the
+  // launches without tiles for it the f32 plane of what they add.
+  ming::RowAdapters ra{};
+  size_t rows_need = 0;
+  if (rows) {
+    ra.ldt = rows->bank->ldt;
+    ra.table = rows->bank->table;
+    rows_need = Carve::aligned256((size_t)M * 4) + Carve::aligned256((size_t)M * ra.ldt * 2);
+  }
+  auto rows_room = [&](size_t need) {
+    carve->need = need;
+    if (need <= carve->cap - carve->used) return (int)MING_OK;
+    return fail(MING_ERR_SHAPE, std::string(carve->who) + ": the call needs " +
+                                    std::to_string(need) + " bytes of scratch; " + carve->what +
+                                    " holds " + std::to_string(carve->cap));
+  };
+  // T of every row's adapter, then (plane) the f32 plane; the projections follow
+  auto rows_launch = [&](float* plane, int N) {
+    ming::RowXaArgs xr{};
+    xr.x = x; xr.ldx = ldx; xr.M = M; xr.K = K;
+    xr.ids = rows->ids; xr.scale = rows->scale;
+    xr.table = ra.table; xr.cap = rows->bank->cap;
+    xr.rid = const_cast<int32_t*>(ra.rid); xr.t = const_cast<uint16_t*>(ra.t); xr.ldt = ra.ldt;
+    MING_HIP(profiled(c, kBRowXa, 0.0, 2.0 * M * K,
+                      [&] { return ming::launch_row_xa(xr, c->stream); }),
+             "row adapters' x.A launch");
+    c->eng.lora_xa += 1;
+    c->eng.lora_proj += 1;
+    if (plane)
+      MING_HIP(profiled(c, kBRowXa, 0.0, 4.0 * M * N,
+                        [&] { return ming::launch_row_delta(ra, M, N, plane, c->stream); }),
+               "row adapters' up-projection launch");
+    return (int)MING_OK;
+  };
+
   // A handful of rows and no live adapter (the adaLN and timestep
   // projections run at M = 1): the GEMV streams each weight once instead of
   // running a 256-row tile. It reads bf16 x in f32, so any route but the
@@ -959,10 +1023,20 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
           if (sg.slot[sl].rank > 0 && scales && scales[sl] != 0.0f) gemv = false;
     }
     if (gemv) {
+      float* plane = nullptr;
+      if (rows) {
+        const size_t need = rows_need + Carve::aligned256((size_t)M * qs[0]->N * 4);
+        if (const int rc = rows_room(need)) return rc;
+        if (carve->measure) return ok();
+        ra.rid = (const int32_t*)carve->take((size_t)M * 4);
+        ra.t = (const uint16_t*)carve->take((size_t)M * ra.ldt * 2);
+        plane = (float*)carve->take((size_t)M * qs[0]->N * 4);
+        if (const int rc = rows_launch(plane, qs[0]->N)) return rc;
+      }
       for (int i = 0; i < n; ++i) {
         const ming_qweight* q = qs[i];
         const ming::GemvArgs ga{x, ldx, q->codes_t, q->sb, q->w16, outs[i].y, outs[i].ldy,
-                                M, q->N, K, outs[i].bias};
+                                M, q->N, K, outs[i].bias, plane};
         const double wbytes = q->bits == 16
                                   ? 2.0 * q->N * K
                                   : (double)q->N * K * q->bits / 8 + 4.0 * q->N * (K / 64);
@@ -1084,7 +1158,7 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
           (uint64_t)q->segs[si].N * (uint64_t)q->b_ld[si] * 2 > (1ull << 31))
         tail_fits[i] = false;
     fast[i] = q->bits != 16 && q->fast && c->route == MING_ROUTE_AUTO && tail_fits[i] &&
-              (uint64_t)M * (uint64_t)K * 2 <= (1ull << 31);
+              (uint64_t)M * (uint64_t)K * 2 <= (1ull << 31) && !rows;
     any_fast = any_fast || fast[i];
   }
   // Per projection: the fast route's K split on few tiles; a dense weight with
@@ -1124,7 +1198,7 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
     }
     // fused, a gated output lands while other tiles still read x: one that
     // shares memory with x goes by the plane
-    if (dense && dense_plan[i].slices == 0 && q->N % 8 == 0 && tail_fits[i] &&
+    if (dense && dense_plan[i].slices == 0 && q->N % 8 == 0 && tail_fits[i] && !rows &&
         !(o.gate && overlap(o.y, o.ldy, q->N, x, ldx, K, M)))
       dense_rf[i] = ming::dense_fast_rf(M, q->N);
     if (o.gate && !fast[i] && !dense_rf[i]) up_bytes = std::max(up_bytes, (size_t)M * q->N * 2);
@@ -1173,8 +1247,20 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
   uint16_t* T = nullptr;
   float* part = nullptr;
   uint16_t* up = nullptr;
+  float* plane = nullptr;
   const uint16_t* xh = xh_src;
-  if (carve) {
+  if (carve && rows) {
+    const size_t plane_bytes = (size_t)M * qs[0]->N * 4;
+    const size_t need = rows_need + Carve::aligned256(plane_bytes) + Carve::aligned256(xh_bytes) +
+                        Carve::aligned256(part_bytes);
+    if (const int rc = rows_room(need)) return rc;
+    if (carve->measure) return ok();
+    ra.rid = (const int32_t*)carve->take((size_t)M * 4);
+    ra.t = (const uint16_t*)carve->take((size_t)M * ra.ldt * 2);
+    if (plane_bytes) plane = (float*)carve->take(plane_bytes);
+    if (xh_bytes) xh = (const uint16_t*)carve->take(xh_bytes);
+    if (part_bytes) part = (float*)carve->take(part_bytes);
+  } else if (carve) {
     if (up_bytes > 0) return fail(MING_ERR_ARG, "ming_lin_noalloc: no gated projection");
     const size_t need = Carve::aligned256(t_bytes) + Carve::aligned256(xh_bytes) +
                         Carve::aligned256(part_bytes);
@@ -1206,6 +1292,8 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
   // The fast x.A stages every element of x through LDS: its DMA waves
   // write the fp16 copy as they go, in place of the conversion launch.
   const bool xh_in_xa = need_xh && t_cols > 0 && xa_fast;
+  if (rows)
+    if (const int rc = rows_launch(plane, qs[0]->N)) return rc;
   if (t_cols > 0) {
     xa.x = x; xa.ldx = ldx; xa.K = K; xa.M = M;
     xa.n_cols = t_cols; xa.t = T; xa.ldt = t_cols;
@@ -1326,6 +1414,7 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
     a.yh = nullptr; a.ldyh = 0;
     a.range = range_word(c);
     a.bias = o.bias;   // set for dense weights only
+    a.delta = plane;
     const bool fused_gate = fast[i] || dense_rf[i] > 0;
     if (o.gate && !fused_gate) {
       a.y = up; a.ldy = q->N;
@@ -1351,7 +1440,7 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
     if (dense_plan[i].slices > 0) {
       ming::LoraXaArgs da{};
       da.x = x; da.ldx = ldx; da.A[0] = q->w16; da.K = K; da.M = M;
-      da.n_cols = q->N; da.t = a.y; da.ldt = (int)a.ldy; da.bias = o.bias;
+      da.n_cols = q->N; da.t = a.y; da.ldt = (int)a.ldy; da.bias = o.bias; da.delta = plane;
       da.ident = true; da.tile = dense_plan[i].tile;
       const int dks = dense_plan[i].slices;
       MING_HIP(profiled(c, bk, base_flops, 2.0 * M * K + wbytes + 2.0 * M * q->N,
@@ -1442,6 +1531,183 @@ int ming_lin_noalloc(ming_ctx* c, const ming_qweight* qc, const uint16_t* x,
   o.y = y;
   o.ldy = ldy;
   return lin_multi(c, 1, &qc, &o, x, ldx, M, scales, nullptr, &cv);
+}
+
+// ---- adapters that rows choose -------------------------------------------------
+int ming_adapters_create(ming_ctx* c, int N, int K, int capacity, int max_rank,
+                         ming_adapters** out) {
+  if (!c || !out) return fail(MING_ERR_ARG, "ming_adapters_create: null argument");
+  *out = nullptr;
+  if (N <= 0 || K <= 0 || K % 64 != 0 || N % 8 != 0)
+    return fail(MING_ERR_SHAPE, "ming_adapters_create: need K % 64 == 0 and N % 8 == 0");
+  if (capacity <= 0 || capacity > 4096)
+    return fail(MING_ERR_SHAPE, "ming_adapters_create: capacity must be 1 to 4096");
+  if (max_rank <= 0 || max_rank > MING_MAX_LORA_RANK)
+    return fail(MING_ERR_SHAPE, "ming_adapters_create: max_rank out of range");
+  DeviceGuard g(c->device);
+  auto* b = new (std::nothrow) ming_adapters();
+  if (!b) return fail(MING_ERR_ALLOC, "ming_adapters_create: out of memory");
+  b->ctx = c; b->N = N; b->K = K; b->cap = capacity; b->max_rank = max_rank;
+  b->ldt = round_up(max_rank, 32);
+  b->bound.resize(capacity);
+  c->live_weights += 1;
+  const size_t bytes = (size_t)capacity * sizeof(ming::AdapterEntry);
+  if (hipMalloc(&b->table, bytes) != hipSuccess) {
+    b->table = nullptr;
+    ming_adapters_destroy(b);
+    return fail(MING_ERR_ALLOC, "ming_adapters_create: allocation failed");
+  }
+  hipError_t e = hipMemsetAsync(b->table, 0, bytes, c->stream);
+  if (e == hipSuccess) e = hipStreamSynchronize(c->stream);
+  if (e != hipSuccess) {
+    ming_adapters_destroy(b);
+    return hip_fail(e, "ming_adapters_create");
+  }
+  *out = b;
+  return ok();
+}
+
+int ming_adapters_destroy(ming_adapters* b) {
+  if (!b) return ok();
+  DeviceGuard g(b->ctx->device);
+  (void)hipStreamSynchronize(b->ctx->stream);
+  for (LoraBind& l : b->bound) {
+    if (l.A) (void)hipFree(l.A);
+    if (l.B) (void)hipFree(l.B);
+  }
+  if (b->table) (void)hipFree(b->table);
+  b->ctx->live_weights -= 1;
+  delete b;
+  return ok();
+}
+
+// The table's entry `id` becomes `nb` and what it held is freed, both behind
+// every queued reader (the stream drains first).
+static int adapters_replace(ming_adapters* b, int id, const LoraBind& nb) {
+  ming_ctx* c = b->ctx;
+  const ming::AdapterEntry e{nb.A, nb.B, nb.rank8, nb.fold};
+  hipError_t h = hipStreamSynchronize(c->stream);
+  if (h == hipSuccess)
+    h = hipMemcpyAsync(b->table + id, &e, sizeof(e), hipMemcpyHostToDevice, c->stream);
+  if (h == hipSuccess) h = hipStreamSynchronize(c->stream);
+  if (h != hipSuccess) return hip_fail(h, "ming_adapters: table update");
+  LoraBind& old = b->bound[id];
+  if (old.A) (void)hipFree(old.A);
+  if (old.B) (void)hipFree(old.B);
+  old = nb;
+  return MING_OK;
+}
+
+int ming_adapters_set(ming_adapters* b, int id, int rank, const uint16_t* A, const uint16_t* B,
+                      float fold, int src_on_device) {
+  if (!b || !A || !B) return fail(MING_ERR_ARG, "ming_adapters_set: null argument");
+  if (id < 0 || id >= b->cap) return fail(MING_ERR_ARG, "ming_adapters_set: id out of range");
+  if (rank <= 0 || rank > b->max_rank)
+    return fail(MING_ERR_SHAPE, "ming_adapters_set: rank must be 1 to the bank's max_rank");
+  if (!std::isfinite(fold)) return fail(MING_ERR_RANGE, "ming_adapters_set: fold is not finite");
+  ming_ctx* c = b->ctx;
+  DeviceGuard g(c->device);
+  const int r8 = round_up(rank, 8);
+  const size_t K = (size_t)b->K, N = (size_t)b->N;
+  LoraBind nb;
+  nb.rank = rank; nb.rank8 = r8; nb.fold = fold;
+  int* flag = nullptr;
+  int bad = 0;
+  auto drop = [&] {
+    if (nb.A) (void)hipFree(nb.A);
+    if (nb.B) (void)hipFree(nb.B);
+    if (flag) (void)hipFree(flag);
+  };
+  if (hipMalloc(&nb.A, (size_t)r8 * K * 2) != hipSuccess ||
+      hipMalloc(&nb.B, N * r8 * 2) != hipSuccess || hipMalloc(&flag, sizeof(int)) != hipSuccess) {
+    (void)hipGetLastError();
+    drop();
+    return fail(MING_ERR_ALLOC, "ming_adapters_set: allocation failed");
+  }
+  const hipMemcpyKind kind = src_on_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice;
+  hipError_t e = hipMemsetAsync(nb.A, 0, (size_t)r8 * K * 2, c->stream);
+  if (e == hipSuccess) e = hipMemsetAsync(nb.B, 0, N * r8 * 2, c->stream);
+  if (e == hipSuccess) e = hipMemsetAsync(flag, 0, sizeof(int), c->stream);
+  if (e == hipSuccess) e = hipMemcpyAsync(nb.A, A, (size_t)rank * K * 2, kind, c->stream);
+  if (e == hipSuccess)
+    e = hipMemcpy2DAsync(nb.B, (size_t)r8 * 2, B, (size_t)rank * 2, (size_t)rank * 2, N, kind,
+                         c->stream);
+  if (e == hipSuccess) e = ming::launch_check_finite(nb.A, (long long)(r8 * K), flag, c->stream);
+  if (e == hipSuccess) e = ming::launch_check_finite(nb.B, (long long)(N * r8), flag, c->stream);
+  if (e == hipSuccess) e = hipMemcpyAsync(&bad, flag, sizeof(int), hipMemcpyDeviceToHost, c->stream);
+  if (e == hipSuccess) e = hipStreamSynchronize(c->stream);
+  if (e != hipSuccess || bad) {
+    drop();
+    return e != hipSuccess ? hip_fail(e, "ming_adapters_set: upload")
+                           : fail(MING_ERR_RANGE, "ming_adapters_set: a factor is not finite");
+  }
+  (void)hipFree(flag);
+  flag = nullptr;
+  const int rc = adapters_replace(b, id, nb);
+  if (rc != MING_OK) {
+    drop();
+    return rc;
+  }
+  return ok();
+}
+
+int ming_adapters_clear(ming_adapters* b, int id) {
+  if (!b) return fail(MING_ERR_ARG, "ming_adapters_clear: null argument");
+  if (id < 0 || id >= b->cap) return fail(MING_ERR_ARG, "ming_adapters_clear: id out of range");
+  DeviceGuard g(b->ctx->device);
+  const int rc = adapters_replace(b, id, LoraBind{});
+  return rc == MING_OK ? ok() : rc;
+}
+
+int ming_adapters_rank(const ming_adapters* b, int id) {
+  return b && id >= 0 && id < b->cap ? b->bound[id].rank : 0;
+}
+
+// Shared by the call and its size: the projection planned with its rows'
+// adapters, its scratch from `cv`.
+static int lin_adapters(ming_ctx* c, const ming_qweight* qw, const ming_adapters* bank,
+                        const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, int M,
+                        const int32_t* ids, const float* scale, Carve* cv) {
+  if (!c || !qw || !bank) return fail(MING_ERR_ARG, "ming_lin_adapters: null argument");
+  if (bank->ctx != c) return fail(MING_ERR_ARG, "ming_lin_adapters: bank of another context");
+  if (bank->N != qw->N || bank->K != qw->K)
+    return fail(MING_ERR_SHAPE, "ming_lin_adapters: the bank's shape is not the weight's");
+  cv->who = "ming_lin_adapters";
+  cv->what = "the workspace";
+  LinOut o;
+  o.y = y;
+  o.ldy = ldy;
+  const RowsCall rows{bank, ids, scale};
+  return lin_multi(c, 1, &qw, &o, x, ldx, M, nullptr, nullptr, cv, &rows);
+}
+
+size_t ming_lin_adapters_workspace_bytes(ming_ctx* c, const ming_qweight* qw,
+                                         const ming_adapters* bank, int M) {
+  if (!c || !qw || !bank || M <= 0) return 0;
+  Carve cv;
+  cv.measure = true;
+  cv.cap = SIZE_MAX;
+  // nothing is launched or read: any aligned address stands for the operands
+  auto* any = reinterpret_cast<uint16_t*>((uintptr_t)256);
+  const int rc = lin_adapters(c, qw, bank, any, qw->K, any, qw->N, M, nullptr, nullptr, &cv);
+  return rc == MING_OK ? cv.need : 0;
+}
+
+int ming_lin_adapters(ming_ctx* c, const ming_qweight* qw, const ming_adapters* bank,
+                      const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, int M,
+                      const int32_t* row_adapter, const float* row_scale, void* ws,
+                      size_t ws_bytes) {
+  if (!row_adapter || !ws) return fail(MING_ERR_ARG, "ming_lin_adapters: null argument");
+  if (!aligned(ws, 16) || !aligned(row_adapter, 4) || !aligned(row_scale, 4))
+    return fail(MING_ERR_ARG,
+                "ming_lin_adapters: ws must be 16-byte, ids and strengths 4-byte aligned");
+  if (qw && x && y && M > 0 && ldx >= qw->K && ldy >= qw->N &&
+      overlap(x, ldx, qw->K, y, ldy, qw->N, M))
+    return fail(MING_ERR_ARG, "ming_lin_adapters: x and y share memory");
+  Carve cv;
+  cv.base = static_cast<char*>(ws);
+  cv.cap = ws_bytes;
+  return lin_adapters(c, qw, bank, x, ldx, y, ldy, M, row_adapter, row_scale, &cv);
 }
 
 int ming_lin_swiglu(ming_ctx* c, const ming_qweight* w, const uint16_t* x,
@@ -1875,6 +2141,35 @@ int ming_quantize_pack(ming_ctx* c, const float* w, int N, int K, int bits,
 }  // extern "C"
 
 namespace ming {
+int rt_route(const ming_ctx* c) { return c->route; }
+int* rt_range_word(const ming_ctx* c) { return range_word(c); }
+bool rt_profile_begin(ming_ctx* c, void** ev) {
+  *ev = nullptr;
+  if (!c->profiling || c->no_events) return true;
+  hipEvent_t a = take_event(c);
+  if (!a || hipEventRecord(a, c->stream) != hipSuccess) return false;
+  *ev = a;
+  return true;
+}
+bool rt_profile_end(ming_ctx* c, void* ev, RtBucket b, double flops, double bytes) {
+  if (!ev) return true;
+  hipEvent_t a = (hipEvent_t)ev, e = take_event(c);
+  if (!e || hipEventRecord(e, c->stream) != hipSuccess) {
+    c->pool.push_back(a);
+    if (e) c->pool.push_back(e);
+    return false;
+  }
+  c->recs.push_back({kBRoute + (int)b, a, e, flops, bytes});
+  return true;
+}
+void rt_note_rows(ming_ctx* c, int bits, uint64_t flops) {
+  if (bits == 4) c->eng.gemm_q4 += 1;
+  else if (bits == 8) c->eng.gemm_q8 += 1;
+  else if (bits == 16) c->eng.gemm_dense += 1;
+  else c->eng.elementwise += 1;
+  c->eng.gemm_flops += flops;
+}
+
 int rt_fail(int code, const std::string& why) { return fail(code, why); }
 int rt_ok() { return ok(); }
 int rt_device(const ming_ctx* c) { return c ? c->device : -1; }

@@ -42,7 +42,7 @@ def close_all():
     weights before their contexts. Registered with atexit when the first
     handle opens; safe to call at any time."""
     objs = list(_open)
-    for kind in (Model, QWeight, Pack, Ctx):
+    for kind in (Model, Experts, Adapters, QWeight, Pack, Ctx):
         for o in objs:
             if isinstance(o, kind):
                 try:
@@ -265,6 +265,28 @@ def lib():
         "ming_model_lora_modules": ([vp, i32], i32),
         "ming_model_lora_skipped": ([vp, i32], i32),
         "ming_model_lora_report": ([vp, i32], C.c_char_p),
+        "ming_topk_route": ([vp, vp, i64, i32, vp, i32, i32, i32, i32, i32, i32, i32, f32, vp,
+                             vp], i32),
+        "ming_group_rows_workspace_bytes": ([i32, i32], C.c_size_t),
+        "ming_group_rows": ([vp, vp, i32, i32, vp, vp, vp, vp, C.c_size_t], i32),
+        "ming_experts_create": ([vp, i32, i32, i32, i32, i32, vp, vp, vp, i32,
+                                 C.POINTER(vp)], i32),
+        "ming_experts_create_dense": ([vp, i32, i32, i32, vp, i32, C.POINTER(vp)], i32),
+        "ming_experts_destroy": ([vp], i32),
+        "ming_experts_shape": ([vp] + [C.POINTER(i32)] * 4, i32),
+        "ming_experts_workspace_bytes": ([vp, i32], C.c_size_t),
+        "ming_experts_lin": ([vp, vp, vp, i64, i32, vp, i32, vp, i32, vp, i64, vp,
+                              C.c_size_t], i32),
+        "ming_experts_swiglu": ([vp, vp, vp, i64, i32, vp, i32, vp, i32, vp, i64, vp,
+                                 C.c_size_t], i32),
+        "ming_experts_combine": ([vp, vp, i64, i32, vp, vp, i32, i32, vp, i64, vp, i64, i32], i32),
+        "ming_adapters_create": ([vp, i32, i32, i32, i32, C.POINTER(vp)], i32),
+        "ming_adapters_destroy": ([vp], i32),
+        "ming_adapters_set": ([vp, i32, i32, vp, vp, f32, i32], i32),
+        "ming_adapters_clear": ([vp, i32], i32),
+        "ming_adapters_rank": ([vp, i32], i32),
+        "ming_lin_adapters_workspace_bytes": ([vp, vp, vp, i32], C.c_size_t),
+        "ming_lin_adapters": ([vp, vp, vp, vp, i64, vp, i64, i32, vp, vp, vp, C.c_size_t], i32),
         "ming_schedule_sigmas": ([i32, f32, C.POINTER(f32)], i32),
         "ming_model_denoise": ([vp, C.POINTER(DenoiseArgs), C.POINTER(f32), STEP_FN,
                                 vp], i32),
@@ -499,6 +521,76 @@ class Ctx:
                                         _ptr(biases)))
 
 
+    # ---- rows that choose their own weights ----
+    def topk_route(self, logits, rows: int, n_experts: int, top_k: int, ids, weights, bias=None,
+                   n_groups: int = 1, top_groups: int = 1, score: str = "softmax",
+                   normalize: bool = True, scale: float = 1.0, ld=None):
+        """ming_topk_route: ids int32 and weights f32 [rows][top_k] of logits (a
+        4-byte element type is f32, a 2-byte one bf16)."""
+        _check(lib().ming_topk_route(self.h, _ptr(logits), n_experts if ld is None else ld,
+                                     int(_itemsize(logits) == 4), _ptr(bias), rows, n_experts,
+                                     top_k, n_groups, top_groups, SCORES[score], int(normalize),
+                                     scale, _ptr(ids), _ptr(weights)))
+
+    def group_rows(self, ids, n: int, n_groups: int, offsets, order, place, ws=None):
+        """ming_group_rows: int32 offsets [n_groups + 1], order [n], place [n]."""
+        _check(lib().ming_group_rows(self.h, _ptr(ids), n, n_groups, _ptr(offsets), _ptr(order),
+                                     _ptr(place), _ptr(ws), _nbytes(ws)))
+
+    def experts_lin(self, ex: "Experts", x, x_rows: int, order, offsets, n: int, y, fan: int = 1,
+                    ws=None, ldx=None, ldy=None):
+        """y[p] = x[order[p] // fan] . W_e^T over ming_group_rows' plan; order
+        None: x is in place order."""
+        _check(lib().ming_experts_lin(self.h, ex.h, _ptr(x), ex.K if ldx is None else ldx, x_rows,
+                                      _ptr(order), fan, _ptr(offsets), n, _ptr(y),
+                                      ex.N if ldy is None else ldy, _ptr(ws), _nbytes(ws)))
+
+    def experts_swiglu(self, ex: "Experts", x, x_rows: int, order, offsets, n: int, y,
+                       fan: int = 1, ws=None, ldx=None, ldy=None):
+        """y[p] = silu(gate) * up over a stack of gate rows, then up rows."""
+        _check(lib().ming_experts_swiglu(self.h, ex.h, _ptr(x), ex.K if ldx is None else ldx,
+                                         x_rows, _ptr(order), fan, _ptr(offsets), n, _ptr(y),
+                                         ex.N // 2 if ldy is None else ldy, _ptr(ws),
+                                         _nbytes(ws)))
+
+    def experts_combine(self, y, n: int, place, weights, tokens: int, top_k: int, out, N: int,
+                        add=None, ldy=None, ldadd=None, ldo=None):
+        """out[t] = add[t] + sum_j weights[t][j] * y[place[t][j]]."""
+        _check(lib().ming_experts_combine(self.h, _ptr(y), N if ldy is None else ldy, n,
+                                          _ptr(place), _ptr(weights), tokens, top_k, _ptr(add),
+                                          N if ldadd is None else ldadd, _ptr(out),
+                                          N if ldo is None else ldo, N))
+
+    def lin_adapters(self, qw: "QWeight", bank: "Adapters", x, y, M: int, row_adapter,
+                     row_scale, ws, ldx=None, ldy=None):
+        """ming_lin with the adapter row_adapter[m] of `bank` on row m, at the
+        strength row_scale[m] (None: all 1); ws of at least
+        lin_adapters_workspace_bytes, kept until the call has run."""
+        _check(lib().ming_lin_adapters(self.h, qw.h, bank.h, _ptr(x), qw.K if ldx is None else ldx,
+                                       _ptr(y), qw.N if ldy is None else ldy, M,
+                                       _ptr(row_adapter), _ptr(row_scale), _ptr(ws), _nbytes(ws)))
+
+    def lin_adapters_workspace_bytes(self, qw: "QWeight", bank: "Adapters", M: int) -> int:
+        return int(lib().ming_lin_adapters_workspace_bytes(self.h, qw.h, bank.h, M))
+
+
+SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def _itemsize(t) -> int:
+    return t.element_size() if hasattr(t, "element_size") else t.itemsize
+
+
+def _nbytes(t) -> int:
+    if t is None:
+        return 0
+    return t.numel() * t.element_size() if hasattr(t, "element_size") else t.nbytes
+
+
+def group_rows_workspace_bytes(n: int, n_groups: int) -> int:
+    return int(lib().ming_group_rows_workspace_bytes(n, n_groups))
+
+
 class QWeight:
     """A resident projection weight (ming_qweight)."""
 
@@ -557,6 +649,81 @@ class QWeight:
     def close(self):
         if self.h:
             lib().ming_qweight_destroy(self.h)
+            self.h = None
+
+    def __del__(self, _fin=_finalize):
+        _fin(self)
+
+
+class Experts:
+    """A resident stack of projections of one shape (ming_experts)."""
+
+    def __init__(self, ctx: Ctx, h):
+        self.ctx = ctx
+        self.h = h
+        ctx._weights.add(self)
+        _track(self)
+        v = [C.c_int() for _ in range(4)]
+        _check(lib().ming_experts_shape(h, *[C.byref(i) for i in v]))
+        self.n_experts, self.N, self.K, self.bits = (i.value for i in v)
+
+    @classmethod
+    def quantized(cls, ctx: Ctx, codes, scales, biases, bits: int, group: int = 64,
+                  on_device: bool = False):
+        """codes [E][N][K * bits / 32], scales and biases [E][N][K / 64]."""
+        E, N, words = (int(v) for v in codes.shape)
+        h = C.c_void_p()
+        _check(lib().ming_experts_create(ctx.h, E, N, words * 32 // bits, bits, group,
+                                         _ptr(codes), _ptr(scales), _ptr(biases),
+                                         int(on_device), C.byref(h)))
+        return cls(ctx, h)
+
+    @classmethod
+    def dense(cls, ctx: Ctx, w, on_device: bool = False):
+        """w bf16 [E][N][K]."""
+        E, N, K = (int(v) for v in w.shape)
+        h = C.c_void_p()
+        _check(lib().ming_experts_create_dense(ctx.h, E, N, K, _ptr(w), int(on_device),
+                                               C.byref(h)))
+        return cls(ctx, h)
+
+    def workspace_bytes(self, x_rows: int) -> int:
+        return int(lib().ming_experts_workspace_bytes(self.h, x_rows))
+
+    def close(self):
+        if self.h:
+            lib().ming_experts_destroy(self.h)
+            self.h = None
+
+    def __del__(self, _fin=_finalize):
+        _fin(self)
+
+
+class Adapters:
+    """Adapters that rows choose, beside one projection shape (ming_adapters)."""
+
+    def __init__(self, ctx: Ctx, N: int, K: int, capacity: int, max_rank: int):
+        h = C.c_void_p()
+        _check(lib().ming_adapters_create(ctx.h, N, K, capacity, max_rank, C.byref(h)))
+        self.ctx, self.h = ctx, h
+        self.N, self.K, self.capacity, self.max_rank = N, K, capacity, max_rank
+        ctx._weights.add(self)
+        _track(self)
+
+    def set(self, id: int, A, B, fold: float = 1.0, on_device: bool = False):
+        """A bf16 [rank][K], B bf16 [N][rank]."""
+        _check(lib().ming_adapters_set(self.h, id, int(A.shape[0]), _ptr(A), _ptr(B), fold,
+                                       int(on_device)))
+
+    def clear(self, id: int):
+        _check(lib().ming_adapters_clear(self.h, id))
+
+    def rank(self, id: int) -> int:
+        return lib().ming_adapters_rank(self.h, id)
+
+    def close(self):
+        if self.h:
+            lib().ming_adapters_destroy(self.h)
             self.h = None
 
     def __del__(self, _fin=_finalize):
