@@ -104,7 +104,7 @@ __device__ __forceinline__ void operands(const GroupRaw<BITS>& r, uint4& w0, uin
 }
 
 template <int BITS, int WK, int CT, int CL>
-__device__ __forceinline__ void gemv_body(const GemvArgs& a) {
+__device__ __forceinline__ void gemv_body(const GemvArgs& a, const float* delta = nullptr) {
   constexpr int NC = WK * CL;                // residue classes of the groups
   constexpr int U = NC == 4 ? 1 : 4 / (CL * CT);   // groups of a class in flight
   const int lane = (int)threadIdx.x & 63;
@@ -187,7 +187,7 @@ __device__ __forceinline__ void gemv_body(const GemvArgs& a) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] += bf16_to_f32(a.bias[n + r]);
   }
-  if (a.delta) v += *reinterpret_cast<const floatx4_t*>(a.delta + (long long)c * a.N + n);
+  if (delta) v += *reinterpret_cast<const floatx4_t*>(delta + (long long)c * a.N + n);
   *reinterpret_cast<uint2*>(a.y + (long long)c * a.ldy + n) =
       make_uint2(pack_bf16x2_rne(v[0], v[1]), pack_bf16x2_rne(v[2], v[3]));
 }
@@ -195,6 +195,11 @@ __device__ __forceinline__ void gemv_body(const GemvArgs& a) {
 template <int BITS, int WK, int CT>
 __global__ __launch_bounds__(64 * WK) void gemv_kernel(const GemvArgs a) {
   gemv_body<BITS, WK, CT, 1>(a);
+}
+
+template <int BITS, int WK, int CT>
+__global__ __launch_bounds__(64 * WK) void gemv_delta_kernel(const GemvArgs a, const float* delta) {
+  gemv_body<BITS, WK, CT, 1>(a, delta);
 }
 
 template <int BITS, int CL>
@@ -209,9 +214,12 @@ __global__ __launch_bounds__(256) void gemv_batch_kernel(const GemvBatch b) {
 }
 
 template <int BITS, int WK, int CT>
-void launch_shape(const GemvArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((gemv_kernel<BITS, WK, CT>), dim3((unsigned)((a.N + 16 * CT - 1) / (16 * CT))),
-                     dim3(64 * WK), 0, s, a);
+void launch_shape(const GemvArgs& a, const float* delta, hipStream_t s) {
+  const dim3 grid((unsigned)((a.N + 16 * CT - 1) / (16 * CT)));
+  if (delta)
+    hipLaunchKernelGGL((gemv_delta_kernel<BITS, WK, CT>), grid, dim3(64 * WK), 0, s, a, delta);
+  else
+    hipLaunchKernelGGL((gemv_kernel<BITS, WK, CT>), grid, dim3(64 * WK), 0, s, a);
 }
 template <int BITS, int CL>
 void launch_batch_shape(const GemvBatch& b, hipStream_t s) {
@@ -233,14 +241,14 @@ void launch_batch_shape(const GemvBatch& b, hipStream_t s) {
 constexpr int kShortK = 512;
 
 template <int BITS>
-void launch_one(const GemvArgs& a, hipStream_t s) {
+void launch_one(const GemvArgs& a, const float* d, hipStream_t s) {
   if constexpr (BITS != 16) {
     if (a.N > 3 * 256 * 16) {
-      a.K <= kShortK ? launch_shape<BITS, 4, 2>(a, s) : launch_shape<BITS, 8, 2>(a, s);
+      a.K <= kShortK ? launch_shape<BITS, 4, 2>(a, d, s) : launch_shape<BITS, 8, 2>(a, d, s);
       return;
     }
   }
-  a.K <= kShortK ? launch_shape<BITS, 4, 1>(a, s) : launch_shape<BITS, 8, 1>(a, s);
+  a.K <= kShortK ? launch_shape<BITS, 4, 1>(a, d, s) : launch_shape<BITS, 8, 1>(a, d, s);
 }
 
 template <int BITS>
@@ -267,12 +275,16 @@ hipError_t launch_gemv_batch(int bits, const GemvBatch& b, hipStream_t s) {
 }
 
 hipError_t launch_gemv(int bits, const GemvArgs& a, hipStream_t s) {
+  return launch_gemv_delta(bits, a, nullptr, s);
+}
+
+hipError_t launch_gemv_delta(int bits, const GemvArgs& a, const float* delta, hipStream_t s) {
   if (a.M <= 0 || a.N <= 0) return hipSuccess;
   if (a.M > kGemvMaxM || a.K % 64 != 0) return hipErrorInvalidValue;
   switch (bits) {
-    case 4: launch_one<4>(a, s); break;
-    case 8: launch_one<8>(a, s); break;
-    case 16: launch_one<16>(a, s); break;
+    case 4: launch_one<4>(a, delta, s); break;
+    case 8: launch_one<8>(a, delta, s); break;
+    case 16: launch_one<16>(a, delta, s); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
@@ -284,6 +296,8 @@ hipError_t validate_gemv_kernels() {
 #define MING_GEMV_ALL(BITS)                                             \
   reinterpret_cast<const void*>(&gemv_kernel<BITS, 4, 1>),              \
       reinterpret_cast<const void*>(&gemv_kernel<BITS, 8, 1>),          \
+      reinterpret_cast<const void*>(&gemv_delta_kernel<BITS, 4, 1>),    \
+      reinterpret_cast<const void*>(&gemv_delta_kernel<BITS, 8, 1>),    \
       reinterpret_cast<const void*>(&gemv_batch_kernel<BITS, 1>),       \
       reinterpret_cast<const void*>(&gemv_batch_kernel<BITS, 2>)
       MING_GEMV_ALL(4), MING_GEMV_ALL(8), MING_GEMV_ALL(16),
@@ -291,7 +305,11 @@ hipError_t validate_gemv_kernels() {
       reinterpret_cast<const void*>(&gemv_kernel<4, 4, 2>),
       reinterpret_cast<const void*>(&gemv_kernel<4, 8, 2>),
       reinterpret_cast<const void*>(&gemv_kernel<8, 4, 2>),
-      reinterpret_cast<const void*>(&gemv_kernel<8, 8, 2>)};
+      reinterpret_cast<const void*>(&gemv_kernel<8, 8, 2>),
+      reinterpret_cast<const void*>(&gemv_delta_kernel<4, 4, 2>),
+      reinterpret_cast<const void*>(&gemv_delta_kernel<4, 8, 2>),
+      reinterpret_cast<const void*>(&gemv_delta_kernel<8, 4, 2>),
+      reinterpret_cast<const void*>(&gemv_delta_kernel<8, 8, 2>)};
   for (const void* f : fns) {
     const hipError_t e = hipFuncGetAttributes(&fa, f);
     if (e != hipSuccess) return e;

@@ -287,9 +287,10 @@ struct GemvArgs {
   long long ldy;
   int M, N, K;
   const uint16_t* bias;   // optional bias [N] bf16, added before the rounding
-  const float* delta;     // optional f32 [M][N], added before the rounding
 };
 hipError_t launch_gemv(int bits, const GemvArgs& a, hipStream_t s);
+// The same with f32 [M][N] added before the rounding (what rows' adapters add).
+hipError_t launch_gemv_delta(int bits, const GemvArgs& a, const float* delta, hipStream_t s);
 // Up to kGemvBatch GEMVs of one shape over one x in one launch (grid y =
 // entry): the per-block adaLN projections of a forward, each entry's bits
 // those of launch_gemv on it.

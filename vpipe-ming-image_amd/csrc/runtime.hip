@@ -1036,13 +1036,13 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
       for (int i = 0; i < n; ++i) {
         const ming_qweight* q = qs[i];
         const ming::GemvArgs ga{x, ldx, q->codes_t, q->sb, q->w16, outs[i].y, outs[i].ldy,
-                                M, q->N, K, outs[i].bias, plane};
+                                M, q->N, K, outs[i].bias};
         const double wbytes = q->bits == 16
                                   ? 2.0 * q->N * K
                                   : (double)q->N * K * q->bits / 8 + 4.0 * q->N * (K / 64);
         MING_HIP(profiled(c, kBGemv, 2.0 * M * (double)q->N * K,
                           wbytes + 2.0 * M * K + 2.0 * M * q->N,
-                          [&] { return ming::launch_gemv(q->bits, ga, c->stream); }),
+                          [&] { return ming::launch_gemv_delta(q->bits, ga, plane, c->stream); }),
                  "gemv launch");
         if (q->bits == 4) c->eng.gemm_q4 += 1;
         else if (q->bits == 8) c->eng.gemm_q8 += 1;
