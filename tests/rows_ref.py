@@ -164,4 +164,23 @@ def plan_of(counts, n=None, fan=1, seed=0, x_rows=None):
     return offsets, order, order[:held] // fan
 
 
+def experts_cut(E, N, K, bits, n):
+    """Which kernel the plan gives n places: 0 the few-row one, else the tiles' cut."""
+    import ming_dit_amd as m
+    return m.lib()._ZN4ming11experts_cutEiiiii(E, N, K, bits, n)
+
+
+def set_experts_cut(ctx, cut):
+    """Experts' products on ctx take this cut whatever their size; -1 the plan's."""
+    import ctypes as C
+
+    import ming_dit_amd as m
+    f = m.lib()._ZN4ming18rt_set_experts_cutEP8ming_ctxi
+    f.argtypes, f.restype = [C.c_void_p, C.c_int], None
+    f(ctx.h, cut)
+
+
+CUTS = {16: (0, 2, 4), 8: (0, 2, 8), 4: (0, 2, 4)}
+
+
 __all__ = ["route", "group", "products", "combine", "adapters", "rel", "REL", "orc"]

@@ -144,6 +144,39 @@ def test_routes(ctx, bits, route, M):
     qw.close()
 
 
+@pytest.mark.parametrize("bits", [4, 8, 16])
+@pytest.mark.parametrize("M,N,K", [(3, 264, 320), (37, 1024, 2048), (300, 264, 320),
+                                   (1300, 1280, 256)])
+def test_rows_without_an_adapter_are_plain_rows(ctx, bits, M, N, K):
+    """Strength 0, an id of none, of nothing bound and out of range: ming_lin's
+    bits, all of them; and a row's own bits do not depend on its neighbours'
+    adapters (the sign of a zero aside)."""
+    qw, _ = weight(ctx, 14200, N, K, bits)
+    bank, _ = make_bank(ctx, 14300, N, K, (16, 0, 40))
+    x = bf16(randn(14400 + M, (M, K)))
+    xd, y = to_dev(x), to_dev(np.zeros((M, N), np.uint16))
+    sync()
+    ctx.lin(qw, xd, y, M)
+    ctx.synchronize()
+    plain = from_dev(y)
+    none = np.resize(np.array([-1, 1, 3, 2 ** 31 - 1, -2 ** 31]), M)
+    assert np.array_equal(call(ctx, qw, bank, x, none, None), plain)
+    off = np.zeros(M, np.float32)
+    off[::2] = -0.0
+    assert np.array_equal(call(ctx, qw, bank, x, np.full(M, 2), off), plain)
+    mixed = np.where(np.arange(M) % 3 == 0, 0, none)
+    a = call(ctx, qw, bank, x, mixed, None)
+    b = call(ctx, qw, bank, x, np.where(mixed == 0, 0, 2), None)
+    mine = mixed == 0
+    same = (a == b) | ((a | b) & 0x7fff == 0)
+    assert same[mine].all()
+    same = (a == plain) | ((a | plain) & 0x7fff == 0)
+    assert same[~mine].all()
+    assert not np.array_equal(a[mine], plain[mine])
+    bank.close()
+    qw.close()
+
+
 @pytest.mark.parametrize("bits", [16])
 def test_a_bad_row_stays_its_own(ctx, bits):
     N, K = 264, 320

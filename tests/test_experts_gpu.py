@@ -83,6 +83,65 @@ def test_product_shapes(ctx, bits, gated, N, K):
     ex.close()
 
 
+@pytest.fixture()
+def cut(ctx):
+    yield lambda c: ref.set_experts_cut(ctx, c)
+    ref.set_experts_cut(ctx, -1)
+
+
+@pytest.mark.parametrize("bits", [4, 8, 16])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("N,K,counts", [
+    (528, 1088, [1, 64, 65, 0, 127, 128, 129, 63, 2, 200, 130, 100]),
+    (560, 576, [255, 256, 257, 1, 513, 0, 192, 193, 321, 449]),
+    (2064, 64, [300, 700, 15, 0, 1, 900]),
+    (272, 1216, [40, 1000]), (16, 128, [70, 0, 9])])
+def test_every_kernel(ctx, cut, bits, gated, N, K, counts):
+    """Each kernel on groups that end at and beside every tile height, one K stage
+    to odd counts of them, columns that end inside a tile; rows gathered and rows
+    in place order to the same bits, twice."""
+    E, n = len(counts), sum(counts)
+    ex, w = ref.make_experts(ctx, 12900, E, N, K, bits)
+    offsets, order, src = ref.plan_of(counts, n=n + 70, fan=3, seed=N, x_rows=300)
+    x = bf16(randn(12950, (300, K)))
+    for c in ref.CUTS[bits]:
+        cut(c)
+        got = run(ctx, ex, gated, x, offsets, order, order.size, fan=3, padx=8, pady=16)
+        check(got, w, x, offsets, src, gated, bits)
+        assert np.array_equal(run(ctx, ex, gated, x[src], offsets, None, n), got)
+    ex.close()
+
+
+def test_the_plan_takes_each_kernel():
+    """Few rows: no tiles; a batch's: the low cut; long batches: the tall one."""
+    for bits, cuts in ref.CUTS.items():
+        assert [ref.experts_cut(64, 2048, 2048, bits, n) for n in (8, 2048, 34816)] == list(cuts)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_tiles_report_what_fp16_cannot_hold(ctx, cut, bits):
+    E, N, K, counts = 3, 560, 576, [300, 10, 400]
+    ex, w = ref.make_experts(ctx, 13000, E, N, K, bits)
+    offsets, order, src = ref.plan_of(counts, x_rows=64)
+    x = bf16(randn(13100, (64, K)))
+    x[5, 7] = bf16(np.float32([7.0e4]))[0]
+    cut(2)
+    with pytest.raises(m.MingError) as e:
+        run(ctx, ex, True, x, offsets, order, order.size)
+    assert e.value.code == m.ERR_RANGE
+    ctx.set_route("wide")
+    try:
+        check(run(ctx, ex, True, x, offsets, order, order.size), w, x, offsets, src, True, bits)
+    finally:
+        ctx.set_route("auto")
+    xd, y = to_dev(x), to_dev(np.zeros((order.size, N), np.uint16))
+    ws = torch.empty(ex.workspace_bytes(64) - 16, dtype=torch.uint8, device="cuda")
+    for bad in (None, ws):
+        with pytest.raises(m.MingError, match="ws|workspace"):
+            ctx.experts_lin(ex, xd, 64, to_dev(order), to_dev(offsets), order.size, y, ws=bad)
+    ex.close()
+
+
 @pytest.mark.parametrize("E", [63, 64, 65, 200, 1000])
 def test_many_experts(ctx, E):
     rng = np.random.default_rng(E)
@@ -114,8 +173,10 @@ def test_wide_and_general_routes_take_any_finite_row(ctx, bits):
     ex.close()
 
 
-def test_a_bad_row_stays_its_own(ctx):
+@pytest.mark.parametrize("kernel", [0, 2, 4])
+def test_a_bad_row_stays_its_own(ctx, cut, kernel):
     """NaN and infinity in one token reach that token's places alone."""
+    cut(kernel)
     counts = [5, 100, 0, 64]
     ex, w = ref.make_experts(ctx, 11800, 4, 64, 128, 16)
     offsets, order, src = ref.plan_of(counts, x_rows=40)
@@ -128,12 +189,13 @@ def test_a_bad_row_stays_its_own(ctx):
     ex.close()
 
 
-@pytest.mark.parametrize("bits", [4, 16])
-def test_captured_products_follow_the_plan(ctx, bits):
+@pytest.mark.parametrize("bits,kernel", [(4, 0), (16, 0), (4, 2), (8, 8), (16, 4)])
+def test_captured_products_follow_the_plan(bits, kernel):
     """A captured call replays with the plan that is in memory then, on a stream
     and context of its own, with eager calls between."""
     s = torch.cuda.Stream()
     c = m.Ctx(0, s.cuda_stream)
+    ref.set_experts_cut(c, kernel)
     E, N, K, T, k = 9, 96, 192, 70, 3
     n = T * k
     ex, w = ref.make_experts(c, 12000, E, N, K, bits)

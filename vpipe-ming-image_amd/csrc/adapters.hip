@@ -17,24 +17,105 @@ namespace {
 // Bound by the reads of x and, for few rows, of A.
 constexpr int XW = 8;
 
+// The adapter of row m and the factor of its T, -1 for none.
+__device__ __forceinline__ int resolve(const RowXaArgs& a, int m, float* coef) {
+  if (m >= a.M) return -1;
+  const int id = a.ids[m];
+  const float s = a.scale ? a.scale[m] : 1.0f;
+  if (id < 0 || id >= a.cap || s == 0.0f || a.table[id].r8 == 0) return -1;
+  *coef = s * a.table[id].fold;
+  return id;
+}
+
+// The chunk list of row tile `tile` (at most 256 rows, a thread each): the chunks
+// of each adapter where the tile's first row of it stands.
+__device__ __forceinline__ void row_chunks(const RowXaArgs& a, int tile, int* ids, int* sums) {
+  const int tid = (int)threadIdx.x, lane = tid & 63;
+  const int mains = a.rows_main / 256;
+  const int m0 = tile < mains ? 256 * tile : a.rows_main + (tile - mains) * a.rest;
+  const int end = tile < mains ? m0 + 256 : m0 + a.rest;
+  float unused;
+  const int m = m0 + tid;
+  const int id = tid < 256 && m < end ? resolve(a, m, &unused) : -1;
+  if (tid < 256) ids[tid] = id;
+  __syncthreads();
+  bool first = id >= 0;
+  const int4* const q = reinterpret_cast<const int4*>(ids);
+  for (int r = 0; r < tid && r < 256; r += 4) {
+    const int4 v = q[r >> 2];
+    if (v.x == id || (r + 1 < tid && v.y == id) || (r + 2 < tid && v.z == id) ||
+        (r + 3 < tid && v.w == id))
+      first = false;
+  }
+  AdapterEntry e = {};
+  if (first) e = a.table[id];
+  const int chunks = first ? (e.r8 + 31) / 32 : 0;
+  RowChunk* const out = reinterpret_cast<RowChunk*>(a.chunks) + (long long)tile * a.stride;
+  int base = 0;
+  for (int s = 0; s < a.slices; ++s) {     // chunk c of adapter id is slice (id + c) % slices'
+    const int c0 = (s + a.slices - (id < 0 ? 0 : id) % a.slices) % a.slices;
+    const int n = chunks > c0 ? (chunks - c0 + a.slices - 1) / a.slices : 0;
+    int run = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(run, o, 64);
+      if (lane >= o) run += v;
+    }
+    __syncthreads();                       // the last slice's sums are read
+    if (lane == 63) sums[tid >> 6] = run;
+    __syncthreads();
+    int at = base + run - n;
+    for (int w = 0; w < 4; ++w) {
+      if (w < (tid >> 6)) at += sums[w];
+      base += sums[w];
+    }
+    for (int i = 0; i < n; ++i) {
+      const int c = c0 + i * a.slices;
+      const int groups = e.r8 - 32 * c >= 32 ? 4 : (e.r8 - 32 * c) / 8;
+      out[at + i] = RowChunk{e.B + 32 * c, id,
+                             (uint32_t)e.r8 | (uint32_t)c << 12 | (uint32_t)(groups - 1) << 20};
+    }
+    if (tid == 0) a.counts[tile * a.slices + s] = base;
+  }
+  // T's row of zeros
+  if (tile == 0)
+    for (int i = tid; i < a.ldt; i += 64 * XW) a.t[(long long)a.M * a.ldt + i] = 0;
+}
+
 __global__ __launch_bounds__(64 * XW) void row_xa_kernel(const RowXaArgs a) {
-  __shared__ float red[XW][16][64];
+  __shared__ __align__(16) float red[XW][16][64];
+  const int xtiles = (a.M + 31) / 32;
+  if ((int)blockIdx.x >= xtiles) {           // the lists' blocks
+    if (blockIdx.y == 0)
+      row_chunks(a, (int)blockIdx.x - xtiles, reinterpret_cast<int*>(&red[0][0][0]),
+                 reinterpret_cast<int*>(&red[1][0][0]));
+    return;
+  }
   const int lane = (int)threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int fr = lane & 31, fk = lane >> 5;
   const int m0 = (int)blockIdx.x * 32;
   const int m = m0 + fr;
   // the row's adapter; both halves of the wave hold the same 32 rows
-  int id = -1;
   float coef = 0.0f;
-  if (m < a.M) {
-    id = a.ids[m];
-    coef = a.scale ? a.scale[m] : 1.0f;
-    if (id < 0 || id >= a.cap || coef == 0.0f) id = -1;
-    if (id >= 0) {
-      if (a.table[id].r8 == 0) id = -1;
-      else coef *= a.table[id].fold;
-    }
+  const int id = resolve(a, m, &coef);
+  if (a.xh) {
+    // the fp16 copy of the block's rows, grid y sharing out the columns
+    const int k8 = a.K / 8, c0 = k8 * (int)blockIdx.y / (int)gridDim.y;
+    const int c1 = k8 * ((int)blockIdx.y + 1) / (int)gridDim.y;
+    uint32_t seen = 0;
+    for (int r = wave; r < 32 && m0 + r < a.M; r += XW)
+      for (int c = c0 + lane; c < c1; c += 64) {
+        const uint4 v = *reinterpret_cast<const uint4*>(a.x + (long long)(m0 + r) * a.ldx + 8 * c);
+        seen = range_track4(seen, v);
+        uint4 f;
+        f.x = bf16x2_to_f16x2(v.x);
+        f.y = bf16x2_to_f16x2(v.y);
+        f.z = bf16x2_to_f16x2(v.z);
+        f.w = bf16x2_to_f16x2(v.w);
+        *reinterpret_cast<uint4*>(a.xh + (long long)(m0 + r) * a.K + 8 * c) = f;
+      }
+    range_report(a.range, seen);
   }
   if (blockIdx.y == 0 && wave == 0 && fk == 0 && m < a.M) a.rid[m] = id;
   const int KT = a.K / 64;
@@ -129,11 +210,14 @@ __global__ void check_finite_kernel(const uint16_t* v, long long n, int* flag) {
 
 hipError_t launch_row_xa(const RowXaArgs& a, hipStream_t s) {
   if (a.M <= 0) return hipSuccess;
-  if (a.K % 64 || a.ldt % 32) return hipErrorInvalidValue;
+  if (a.K % 64 || a.ldt % 32 || (a.counts && (a.rows_main % 256 || a.rest < 1 || a.rest > 256 || a.slices < 1)))
+    return hipErrorInvalidValue;
   const int tiles = (a.M + 31) / 32;
+  const int lists = a.counts ? row_tiles(a.M, a.rows_main, a.rest) : 0;
   int y = 1;
   while (y < 32 && tiles * y < 512) y *= 2;
-  hipLaunchKernelGGL(row_xa_kernel, dim3((unsigned)tiles, (unsigned)y), dim3(64 * XW), 0, s, a);
+  hipLaunchKernelGGL(row_xa_kernel, dim3((unsigned)(tiles + lists), (unsigned)y), dim3(64 * XW), 0,
+                     s, a);
   return hipGetLastError();
 }
 

@@ -30,7 +30,8 @@ namespace {
 constexpr int DBN = 256, DBK = 64, NW = 8;
 
 // EPI: 0 plain; 1 a.bias added before the output's one rounding; 2 gated by
-// a.g (the fused SwiGLU); 3 plain, a.nw projections over one x. One instance
+// a.g (the fused SwiGLU); 3 plain, a.nw projections over one x; 4 plain with
+// rows' own adapters as the tail (a.rows). One instance
 // each: with the first three in one the 256-row tile's epilogue spilled
 // registers.
 template <int RF, int EPI>
@@ -202,12 +203,100 @@ __global__ __launch_bounds__(64 * NW, 1) void dense_fast_kernel(const QprojArgs 
           dma16_sb(base, xoff[i], lds_addr(S + 64 * (XD * wave + i)));
       });
 
+  if constexpr (EPI == 4) {
+    // ---- the chunks of the adapters that the tile's rows name, two of 32 ranks a
+    // stage, each over all the tile's rows: those with another adapter read T's
+    // row of zeros (an odd last chunk's second half: all of them) ----
+    const RowAdapters& ra = a.rows;
+    const int n = ra.counts[tm], stages = (n + 1) / 2;
+    if (n > 0) {
+      // uniform reads through the scalar cache: a vector load would count with
+      // the DMAs
+      typedef const __attribute__((address_space(4))) uint64_t* Const64;
+      const Const64 list = (Const64)(uintptr_t)(ra.chunks + (long long)tm * ra.stride);
+      uint32_t trow[XD], bn[WD];
+      int rid[XD];
+#pragma unroll
+      for (int i = 0; i < XD; ++i) {
+        const int p = 64 * (XD * wave + i) + lane;
+        int mr = m0 + row_of(p);
+        mr = mr < mlast ? mr : mlast;
+        rid[i] = ra.rid[mr];
+        trow[i] = (uint32_t)(((long long)mr * ra.ldt + 8 * (chunk_of(p) & 3)) * 2);
+      }
+#pragma unroll
+      for (int i = 0; i < WD; ++i) {
+        const int r = n0 + row_of(64 * (WD * wave + i) + lane);
+        bn[i] = (uint32_t)(r < nlast ? r : nlast);
+      }
+      auto issue_r = [&](int st, const uint4* S) {
+        const int e0 = 2 * st, e1 = 2 * st + 1 < n ? 2 * st + 1 : e0;
+        const uint64_t p0 = list[2 * e0], p1 = list[2 * e1];
+        const uint32_t s0 = (uint32_t)(list[2 * e0 + 1] >> 32);
+        const uint32_t s1 = (uint32_t)(list[2 * e1 + 1] >> 32);
+#pragma unroll
+        for (int i = 0; i < WD; ++i) {
+          const int c = chunk_of(64 * (WD * wave + i) + lane);
+          const uint32_t sh = (c & 4) ? s1 : s0;
+          const uint32_t live = sh >> 20, cc = (uint32_t)(c & 3);
+          // past the chunk's live groups T is zero: any of its columns will do
+          dma16_v(reinterpret_cast<const void*>(((c & 4) ? p1 : p0) +
+                                                (uint64_t)(bn[i] * ((sh & 0xfffu) * 2u) +
+                                                           (cc < live ? cc : live) * 16u)),
+                  lds_addr(S + 64 * (WD * wave + i)));
+        }
+      };
+      auto issue_s = [&](int st, const uint4* S) {
+        const int e0 = 2 * st, e1 = 2 * st + 1;
+        const uint64_t v0 = list[2 * e0 + 1], v1 = list[2 * (e1 < n ? e1 : e0) + 1];
+        const int id0 = (int)(uint32_t)v0, id1 = e1 < n ? (int)(uint32_t)v1 : -2;
+        const uint32_t c0 = ((uint32_t)(v0 >> 32) >> 12 & 0xffu) * 64u;
+        const uint32_t c1 = ((uint32_t)(v1 >> 32) >> 12 & 0xffu) * 64u;
+#pragma unroll
+        for (int i = 0; i < XD; ++i) {
+          const bool hi = chunk_of(64 * (XD * wave + i) + lane) & 4;
+          dma16_sb(ra.t, rid[i] == (hi ? id1 : id0) ? trow[i] + (hi ? c1 : c0) : ra.zero,
+                   lds_addr(S + 64 * (XD * wave + i)));
+        }
+      };
+      // Two buffers, the next stage in flight under a stage's MFMAs: most tiles
+      // have one stage or two, and the pipelined walk would leave the 256-row
+      // tile short of registers.
+      auto stage = [&](int st, const uint4* X, const uint4* W, const uint4* Xn, const uint4* Wn) {
+        ring_wait<0>();                    // landed, and the other buffer is read
+        if (st + 1 < stages) {
+          issue_r(st + 1, Wn);
+          issue_s(st + 1, Xn);
+        }
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          read_frags(X, W, kk, wa, xb);
+#pragma unroll
+          for (int i = 0; i < RF; ++i)
+#pragma unroll
+            for (int j = 0; j < JF; ++j)
+              acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                  __builtin_bit_cast(bf16x8_t, wa[j]), __builtin_bit_cast(bf16x8_t, xb[i]),
+                  acc[j][i], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      issue_r(0, wslot(0));
+      issue_s(0, xslot(0));
+      for (int st = 0; st < stages; st += 2) {
+        stage(st, xslot(0), wslot(0), xslot(1), wslot(1));
+        if (st + 1 < stages) stage(st + 1, xslot(1), wslot(1), xslot(0), wslot(0));
+      }
+      ring_wait<0>();                      // every wave's reads done: LDS free
+    }
+  }
+
   // ---- LoRA tail: T and gathered B, two chunks of 32 ranks a stage ----
   int sg = 0;
   for (int i = 1; i < a.nseg; ++i)
     if (n0 >= a.seg[i].n_begin) sg = i;
   const QprojSeg& s = EPI == 3 && wsel > 0 ? a.more[wsel - 1].seg : a.seg[sg];
-  const int chunks = s.chunks;
+  const int chunks = EPI == 4 ? 0 : s.chunks;
   if (chunks > 0) {
     const int grp0 = s.grp0;
     // a padding group's T columns are exactly 0: any finite B will do, the
@@ -392,7 +481,9 @@ template <int RF>
 static void launch_rf(const QprojArgs& a, hipStream_t s) {
   const int nw = a.nw > 1 ? a.nw : 1;
   const dim3 grid((unsigned)(((a.M + 64 * RF - 1) / (64 * RF)) * ((a.N + DBN - 1) / DBN) * nw));
-  if (nw > 1)
+  if (a.rows.counts)
+    hipLaunchKernelGGL((dense_fast_kernel<RF, 4>), grid, dim3(64 * NW), 0, s, a);
+  else if (nw > 1)
     hipLaunchKernelGGL((dense_fast_kernel<RF, 3>), grid, dim3(64 * NW), 0, s, a);
   else if (a.bias)
     hipLaunchKernelGGL((dense_fast_kernel<RF, 1>), grid, dim3(64 * NW), 0, s, a);
@@ -405,7 +496,7 @@ static void launch_rf(const QprojArgs& a, hipStream_t s) {
 hipError_t launch_dense_fast(const QprojArgs& a, int rf, hipStream_t s) {
   if (a.M <= 0 || a.N <= 0) return hipSuccess;
   if (a.N % 8 != 0 || a.K % 64 != 0 || a.kslices > 1 || a.yh || (a.bias && a.g) ||
-      (a.nw > 1 && (a.nw > 3 || a.nseg != 1 || a.bias || a.g)))
+      (a.rows.counts && (a.nw > 1 || a.bias || a.g)) || (a.nw > 1 && (a.nw > 3 || a.nseg != 1 || a.bias || a.g)))
     return hipErrorInvalidValue;
   switch (rf) {
     case 1: launch_rf<1>(a, s); break;
@@ -423,7 +514,8 @@ static hipError_t validate_rf() {
   const void* fns[] = {reinterpret_cast<const void*>(&dense_fast_kernel<RF, 0>),
                        reinterpret_cast<const void*>(&dense_fast_kernel<RF, 1>),
                        reinterpret_cast<const void*>(&dense_fast_kernel<RF, 2>),
-                       reinterpret_cast<const void*>(&dense_fast_kernel<RF, 3>)};
+                       reinterpret_cast<const void*>(&dense_fast_kernel<RF, 3>),
+                       reinterpret_cast<const void*>(&dense_fast_kernel<RF, 4>)};
   for (const void* f : fns) {
     const hipError_t e = hipFuncGetAttributes(&fa, f);
     if (e != hipSuccess) return e;

@@ -31,7 +31,7 @@ __device__ __forceinline__ void load_group(const ExpertsArgs& a, const void* w, 
                                            int g, Raw<BITS>& r) {
   if constexpr (BITS == 16) {
     const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(w) +
-                                                    (long long)n * a.K + 64 * kt + 16 * g);
+                                                    ((long long)kt * a.NW + n) * 64 + 16 * g);
     r.v[0] = p[0];
     r.v[1] = p[1];
   } else {
@@ -83,17 +83,17 @@ __device__ __forceinline__ void operands(const Raw<BITS>& r, uint4& w0, uint4& w
 // weights multiply as integers: scale * sum(q x) + bias * sum(x) a group, in
 // f32, the activations as the bf16 they are (no range limit). Bound by HBM:
 // the weights of the experts that have rows, once.
-template <int BITS, bool GATED, int WK>
+template <int BITS, bool GATED, int WK, int CO>
 __global__ __launch_bounds__(64 * WK) void experts_rows_kernel(const ExpertsArgs a) {
-  constexpr int CT = GATED ? 2 : 1;
-  constexpr int U = WK == 4 ? 1 : 4 / CT;  // groups of a wave in flight
+  constexpr int CT = GATED ? 2 * CO : CO;  // column tiles: the outputs', then the up rows'
+  constexpr int U = WK == 4 || CT > 4 ? 1 : 4 / CT;   // groups of a wave in flight
   const RowGroup rg =
-      find_group(a.offsets, a.E, a.n, (int)blockIdx.y, [](int) { return 1; });
+      find_group(a.offsets, a.E, a.n, [](int) { return 1; }, [](int) { return (int)blockIdx.y; });
   if (rg.e < 0) return;
   const int lane = (int)threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
-  const int n0 = (int)blockIdx.x * 16;
+  const int n0 = (int)blockIdx.x * 16 * CO;
   const int KT = a.K / 64;
   const long long words = (long long)a.NW * a.K * BITS / 32;
   const void* const w = BITS == 16
@@ -128,11 +128,11 @@ __global__ __launch_bounds__(64 * WK) void experts_rows_kernel(const ExpertsArgs
 #pragma unroll
           for (int t = 0; t < CT; ++t) {
             // columns past N (a multiple of 8) compute the last ones, never store
-            const int n = n0 + c;
-            load_group<BITS>(a, w, (n < a.N ? n : a.N - 1) + t * a.N, kt, g, wr[u][t]);
+            const int n = n0 + 16 * (t % CO) + c;
+            load_group<BITS>(a, w, (n < a.N ? n : a.N - 1) + t / CO * a.N, kt, g, wr[u][t]);
             if constexpr (BITS != 16) {
-              const int ns = n0 + 4 * g;
-              sb[u][t] = *reinterpret_cast<const uint4*>(sbp + (long long)kt * a.NW + t * a.N +
+              const int ns = n0 + 16 * (t % CO) + 4 * g;
+              sb[u][t] = *reinterpret_cast<const uint4*>(sbp + (long long)kt * a.NW + t / CO * a.N +
                                                          (ns < a.N ? ns : a.N - 4));
             }
           }
@@ -162,49 +162,74 @@ __global__ __launch_bounds__(64 * WK) void experts_rows_kernel(const ExpertsArgs
         }
       }
     }
-    // lane (m = c, g): columns 4g + 0..3 of the 16, row m
+    // lane (m = c, g): columns 4g + 0..3 of each 16, row m; wave t finishes tile t
 #pragma unroll
     for (int t = 0; t < CT; ++t) red[wave][t][lane] = acc[t];
     __syncthreads();
-    const int n = n0 + 4 * g;
-    if (wave == 0 && row && n < a.N) {
-      floatx4_t v[CT];
+    const int n = n0 + 16 * wave + 4 * g;
+    if (wave < CO && row && n < a.N) {
+      floatx4_t v = red[0][wave][lane];
 #pragma unroll
-      for (int t = 0; t < CT; ++t) {
-        v[t] = red[0][t][lane];
-#pragma unroll
-        for (int j = 1; j < WK; ++j) v[t] += red[j][t][lane];
-      }
+      for (int j = 1; j < WK; ++j) v += red[j][wave][lane];
       if constexpr (GATED) {
+        floatx4_t u = red[0][CO + wave][lane];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[0][r] = silu_f(v[0][r]) * v[1][r];
+        for (int j = 1; j < WK; ++j) u += red[j][CO + wave][lane];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = silu_f(v[r]) * u[r];
       }
       *reinterpret_cast<uint2*>(a.y + (long long)(rg.p0 + r0 + c) * a.ldy + n) =
-          make_uint2(pack_bf16x2_rne(v[0][0], v[0][1]), pack_bf16x2_rne(v[0][2], v[0][3]));
+          make_uint2(pack_bf16x2_rne(v[0], v[1]), pack_bf16x2_rne(v[2], v[3]));
     }
     __syncthreads();                       // the sums are read: the next rows' may come
   }
 }
 
-template <int BITS, bool GATED>
-void rows_shape(const ExpertsArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)(a.n < a.E ? a.n : a.E));
+template <int BITS, bool GATED, int CO>
+void rows_wide(const ExpertsArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)((a.N + 16 * CO - 1) / (16 * CO)), (unsigned)(a.n < a.E ? a.n : a.E));
   if (a.K <= 512)
-    hipLaunchKernelGGL((experts_rows_kernel<BITS, GATED, 4>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((experts_rows_kernel<BITS, GATED, 4, CO>), grid, dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((experts_rows_kernel<BITS, GATED, 8>), grid, dim3(512), 0, s, a);
+    hipLaunchKernelGGL((experts_rows_kernel<BITS, GATED, 8, CO>), grid, dim3(512), 0, s, a);
+}
+
+template <int BITS, bool GATED>
+void rows_shape(const ExpertsArgs& a, int co, hipStream_t s) {
+  co == 2 ? rows_wide<BITS, GATED, 2>(a, s) : rows_wide<BITS, GATED, 1>(a, s);
+}
+
+// w [NW][K] -> [K / 64][NW][64], 16 bytes a thread and step.
+__global__ void repack_dense_kernel(const uint16_t* w, int NW, int K, uint16_t* out) {
+  const long long total = (long long)NW * K / 8;
+  for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total;
+       i += (long long)gridDim.x * blockDim.x) {
+    const int c = (int)(i & 7);
+    const long long r = i >> 3;
+    const int n = (int)(r % NW), kt = (int)(r / NW);
+    reinterpret_cast<uint4*>(out)[i] =
+        *reinterpret_cast<const uint4*>(w + (long long)n * K + 64 * kt + 8 * c);
+  }
 }
 
 }  // namespace
 
-hipError_t launch_experts_rows(int bits, bool gated, const ExpertsArgs& a, hipStream_t s) {
+hipError_t launch_repack_dense(const uint16_t* w, int NW, int K, uint16_t* out, hipStream_t s) {
+  if (NW <= 0 || K <= 0 || K % 64) return hipErrorInvalidValue;
+  const long long blocks = ((long long)NW * K / 8 + 255) / 256;
+  hipLaunchKernelGGL(repack_dense_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256),
+                     0, s, w, NW, K, out);
+  return hipGetLastError();
+}
+
+hipError_t launch_experts_rows(int bits, bool gated, const ExpertsArgs& a, int co, hipStream_t s) {
   if (a.n <= 0 || a.N <= 0) return hipSuccess;
   if (a.K % 64 || a.N % 8 || a.NW != a.N * (gated ? 2 : 1) || a.E < 1 || a.fan < 1 || a.x_rows < 1)
     return hipErrorInvalidValue;
   switch (bits) {
-    case 4: gated ? rows_shape<4, true>(a, s) : rows_shape<4, false>(a, s); break;
-    case 8: gated ? rows_shape<8, true>(a, s) : rows_shape<8, false>(a, s); break;
-    case 16: gated ? rows_shape<16, true>(a, s) : rows_shape<16, false>(a, s); break;
+    case 4: gated ? rows_shape<4, true>(a, co, s) : rows_shape<4, false>(a, co, s); break;
+    case 8: gated ? rows_shape<8, true>(a, co, s) : rows_shape<8, false>(a, co, s); break;
+    case 16: gated ? rows_shape<16, true>(a, co, s) : rows_shape<16, false>(a, co, s); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
@@ -213,12 +238,14 @@ hipError_t launch_experts_rows(int bits, bool gated, const ExpertsArgs& a, hipSt
 hipError_t validate_experts_kernels() {
   hipFuncAttributes fa;
   const void* fns[] = {
-#define MING_EXPERTS_ROWS(BITS)                                               \
-  reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 4>),        \
-      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 8>),    \
-      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 4>),     \
-      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 8>)
-      MING_EXPERTS_ROWS(4), MING_EXPERTS_ROWS(8), MING_EXPERTS_ROWS(16)
+#define MING_EXPERTS_ROWS(BITS, CO)                                               \
+  reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 4, CO>),        \
+      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 8, CO>),    \
+      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 4, CO>),     \
+      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 8, CO>)
+      reinterpret_cast<const void*>(&repack_dense_kernel),
+      MING_EXPERTS_ROWS(4, 1), MING_EXPERTS_ROWS(8, 1), MING_EXPERTS_ROWS(16, 1),
+      MING_EXPERTS_ROWS(4, 2), MING_EXPERTS_ROWS(8, 2), MING_EXPERTS_ROWS(16, 2)
 #undef MING_EXPERTS_ROWS
   };
   for (const void* f : fns) {

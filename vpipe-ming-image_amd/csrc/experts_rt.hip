@@ -1,6 +1,7 @@
 // Host side of the mixture's operators: the router, the grouping, the resident
 // expert stacks with their ragged products, and the weighted sum.
 #include <algorithm>
+#include <cmath>
 #include <new>
 #include <string>
 
@@ -16,8 +17,49 @@ struct ming_experts {
   int E = 0, N = 0, K = 0, bits = 0;
   uint32_t* codes = nullptr;   // bits 4 / 8: the fast resident layout, an expert after another
   uint32_t* sb = nullptr;
-  uint16_t* w16 = nullptr;     // bits 16
+  uint16_t* w16 = nullptr;     // bits 16: [E][K / 64][N][64]
 };
+
+namespace ming {
+
+// Which kernel takes n places: 0 the few-row one, else the tiles, cut every
+// 64 (dense) or 32 (quantized) * max places. The groups' sizes are on the device,
+// so it goes by what an even router gives: live experts, rows of each. Of both the
+// times below are fits (us) to [8 to 256][256 to 4096, 512 to 4096] at 2 to 34816
+// places; where they are close, so are the kernels.
+//   few rows, dense: 2.5 + bytes / 5.9 TB/s, longer by the rows' own reads (swiglu
+//     of [64][2048, 2048], 8 places: 13.7, the tiles 17.0); w4 and w8: the codes'
+//     conversion, 2.8 and 3.9 weights a ps ([128][1024, 2048] w8 gated, 32 places:
+//     19.2, the tiles 25); 16 rows a pass over the weights.
+//   tiles: a start and the K stages of one, then the weights at 6.1 TB/s, a round
+//     of the chip (one dense block a CU) at least that again (the same, 64 places:
+//     62.0, few rows 56.2; 128: 80.2 and 83.2). Out of cold caches the tiles lose a
+//     little more: they have to win by 8%.
+// Cuts: dense, 128 rows up to 192 an expert, then 256 ([64][2048, 2048] gated at
+// 128 rows 121 us, 147 cut at 256; at 544 rows 317 and 359). w4, 64 rows, three
+// blocks a CU, then 128, two ([128][1024, 2048] gated at 128 rows 102 both, at 272
+// 186 and 166); w8, 64 rows, then 256 (at 64 rows 75, at 272 214 and 202).
+int experts_cut(int E, int N, int K, int bits, int n) {
+  const double live = E * (1.0 - std::exp(-(double)n / E)), rows = n / live;
+  const double weights = live * N * (double)K, stages = K / 64.0;
+  const double passes = rows > 16.0 ? rows / 16.0 : 1.0;
+  double few, tile;
+  if (bits == 16) {
+    const double one = 256.0 * K * 2 / 6.1e6;            // a tile's weights, us
+    const double all = live * ((N + 255) / 256), round = std::floor(all / 256.0) * 256.0;
+    few = 2.5 + weights * 2 / 5.9e6 * (1.0 + rows / 40.0) * passes;
+    tile = round * one + std::max(4.0 + 0.4 * stages, 2.5 + (all - round) * one);
+  } else {
+    few = 3.0 + weights / (bits == 4 ? 2.8e6 : 3.9e6) * passes;
+    tile = 2.5 + std::max(4.6 + 0.5 * stages, 2.5 + weights * bits / 8 / 4.5e6);
+  }
+  if (few < 1.08 * tile) return 0;
+  if (bits == 16) return rows < 192.0 ? 2 : 4;
+  if (bits == 4) return rows < 160.0 ? 2 : 4;
+  return rows < 200.0 ? 2 : 8;
+}
+
+}  // namespace ming
 
 namespace {
 
@@ -80,8 +122,18 @@ int products(const char* who, bool gated, ming_ctx* c, const ming_experts* ex, c
     return bad(MING_ERR_SHAPE, "x_rows * ldx must be below 2^30");
   if (overlap(x, x_rows, ldx, ex->K, y, n, ldy, N))
     return bad(MING_ERR_ARG, "x and y share memory");
-  (void)ws;
-  (void)ws_bytes;
+  // the quantized tiles multiply fp16, which the other routes are chosen against
+  const int cut = ex->bits != 16 && ming::rt_route(c) != MING_ROUTE_AUTO ? 0
+                  : ming::rt_experts_cut(c) >= 0
+                      ? ming::rt_experts_cut(c)
+                      : ming::experts_cut(ex->E, ex->N, ex->K, ex->bits, n);
+  const size_t xh_bytes = cut && ex->bits != 16 ? (size_t)x_rows * ex->K * 2 : 0;
+  if (xh_bytes > 0 && (!ws || !aligned(ws, 16)))
+    return bad(MING_ERR_ARG, "ws must be given, 16-byte aligned");
+  if (ws_bytes < xh_bytes)
+    return rt_fail(MING_ERR_SHAPE, std::string(who) + ": the call needs " +
+                                       std::to_string(xh_bytes) + " bytes of workspace, " +
+                                       std::to_string(ws_bytes) + " given");
   DeviceGuard g(ming::rt_device(c));
   ming::ExpertsArgs a{};
   a.x = x; a.ldx = ldx;
@@ -93,10 +145,21 @@ int products(const char* who, bool gated, ming_ctx* c, const ming_experts* ex, c
   const double flops = 2.0 * n * (double)ex->N * ex->K;
   const double wb = ex->bits == 16 ? 2.0 * ex->N * ex->K
                                    : (double)ex->N * ex->K * ex->bits / 8 + 4.0 * ex->N * (ex->K / 64);
-  const int rc = run(c, ming::kRtExperts, flops,
-                     wb * std::min(n, ex->E) + 2.0 * x_rows * ex->K + 2.0 * n * N, who, [&] {
-                       return ming::launch_experts_rows(ex->bits, gated, a, stream_of(c));
-                     });
+  const int rc = run(
+      c, ming::kRtExperts, flops, wb * std::min(n, ex->E) + 2.0 * x_rows * ex->K + 2.0 * n * N, who,
+      [&] {
+        if (cut == 0)
+          return ming::launch_experts_rows(ex->bits, gated, a, gated ? 1 : 2, stream_of(c));
+        if (ex->bits == 16) return ming::launch_experts_tile(gated, a, cut, stream_of(c));
+        // one conversion of x to fp16 for all experts' rows
+        auto* xh = static_cast<uint16_t*>(ws);
+        const hipError_t e = ming::launch_bf16_to_f16(x, ldx, xh, ex->K, x_rows, ex->K,
+                                                      stream_of(c), ming::rt_range_word(c));
+        if (e != hipSuccess) return e;
+        a.x = xh;
+        a.ldx = ex->K;
+        return ming::launch_experts_qtile(ex->bits, gated, a, cut, stream_of(c));
+      });
   if (rc != MING_OK) return rc;
   ming::rt_note_rows(c, ex->bits, 2ull * (uint64_t)n * (uint64_t)ex->N * (uint64_t)ex->K);
   return rt_ok();
@@ -215,15 +278,28 @@ int ming_experts_create_dense(ming_ctx* c, int n_experts, int N, int K, const ui
   if (!out || !w) return rt_fail(MING_ERR_ARG, "ming_experts_create: null argument");
   *out = nullptr;
   if (const int rc = check_stack(c, n_experts, N, K)) return rc;
+  if (src_on_device && !aligned(w, 16))
+    return rt_fail(MING_ERR_ARG, "ming_experts_create: device weights must be 16-byte aligned");
   DeviceGuard g(ming::rt_device(c));
   auto* ex = new (std::nothrow) ming_experts();
   if (!ex) return rt_fail(MING_ERR_ALLOC, "ming_experts_create: out of memory");
   ex->ctx = c; ex->E = n_experts; ex->N = N; ex->K = K; ex->bits = 16;
   ming::rt_retain(c);
-  void* d = nullptr;
-  hipError_t e = copy_in(c, &d, w, (size_t)n_experts * N * K * 2, src_on_device);
-  ex->w16 = (uint16_t*)d;
-  if (e == hipSuccess) e = hipStreamSynchronize(stream_of(c));
+  const size_t one = (size_t)N * K;
+  hipStream_t s = stream_of(c);
+  void* stage = nullptr;                 // an expert's source, where it is on the host
+  hipError_t e = hipMalloc(&ex->w16, (size_t)n_experts * one * 2);
+  if (e == hipSuccess && !src_on_device) e = hipMalloc(&stage, one * 2);
+  for (int i = 0; i < n_experts && e == hipSuccess; ++i) {
+    const uint16_t* src = w + i * one;
+    if (stage) {
+      e = hipMemcpyAsync(stage, src, one * 2, hipMemcpyHostToDevice, s);
+      src = static_cast<const uint16_t*>(stage);
+    }
+    if (e == hipSuccess) e = ming::launch_repack_dense(src, N, K, ex->w16 + i * one, s);
+  }
+  if (e == hipSuccess) e = hipStreamSynchronize(s);
+  if (stage) (void)hipFree(stage);
   if (e != hipSuccess) {
     (void)hipGetLastError();
     ming_experts_destroy(ex);

@@ -58,6 +58,19 @@ struct RowAdapters {
   const uint16_t* t;    // [M][ldt]
   int ldt;
   const AdapterEntry* table;
+  // For the tile kernels' tails: per row tile the 32-rank chunks of the adapters
+  // its rows name (RowChunk, `stride` a tile), how many (split: where each slice's
+  // end), and T's row of zeros as a byte offset from t.
+  const uint4* chunks;
+  const int32_t* counts;
+  int stride;
+  uint32_t zero;
+};
+// A chunk of a tile's tail as the kernels read it (one 16-byte scalar load).
+struct RowChunk {
+  const uint16_t* B;    // the adapter's factor at the chunk's first rank
+  int32_t id;
+  uint32_t shape;       // r8 | chunk << 12 | (live 8-rank groups - 1) << 20
 };
 
 struct QprojArgs {
@@ -107,6 +120,9 @@ struct QprojArgs {
   const uint16_t* bias;
   // optional f32 [M][N], added like the bias: what rows' own adapters add
   const float* delta;
+  // rows' own adapters as a tail of the tiles (launch_qproj_fast and
+  // launch_dense_fast; no segments' adapters then), counts NULL: none
+  RowAdapters rows;
 };
 
 // wide: bits 4/8 run with bf16 activations and the weight as a bf16 pair
@@ -394,7 +410,20 @@ struct RowXaArgs {
   int32_t* rid;
   uint16_t* t;
   int ldt;
+  // optional: the chunk lists of row tiles (RowAdapters) of 256 rows up to
+  // rows_main, then of `rest` rows, and T's row of zeros, row M
+  uint4* chunks;
+  int32_t* counts;
+  int stride, rows_main, rest;
+  int slices;           // of a split launch, else 1: counts [tiles][slices], where each ends
+  // optional: the fp16 copy of x, [M][K], and the word it raises (QprojArgs::range)
+  uint16_t* xh;
+  int* range;
 };
+// Row tiles of the lists, and chunks a tile may need.
+inline int row_tiles(int M, int rows_main, int rest) {
+  return rows_main / 256 + (M > rows_main ? (M - rows_main + rest - 1) / rest : 0);
+}
 hipError_t launch_row_xa(const RowXaArgs& a, hipStream_t s);
 // d[m][n] = T[m] . B_a[n] in f32, a = rid[m]; -0 for rows without an adapter,
 // which any sum takes without a change. N % 4 == 0.
@@ -453,7 +482,7 @@ hipError_t validate_routing_kernels();
 // W_e^T with row(p) = order ? order[p] / fan : p, kept inside [0, x_rows). W is
 // a stack of E projections of NW rows: NW = N, or gated 2 N, the gate's N rows
 // before the up projection's, y = bf16(silu(gate) * up) of the f32 results.
-// Weights: bits 16 w16 [E][NW][K]; bits 4 / 8 the fast resident layout
+// Weights: bits 16 w16 [E][K / 64][NW][64] (launch_repack_dense); bits 4 / 8 the fast resident layout
 // (launch_repack_fast) an expert after another.
 struct ExpertsArgs {
   const uint16_t* x;
@@ -468,8 +497,27 @@ struct ExpertsArgs {
   uint16_t* y;
   long long ldy;
 };
-hipError_t launch_experts_rows(int bits, bool gated, const ExpertsArgs& a, hipStream_t s);
+// One projection [NW][K] into [K / 64][NW][64]: a stage of a tile is then one run
+// of memory. In rows of a power of two the same 128 bytes of every row lie on a
+// few of the memory's channels ([64][2048, 2048], 512 rows: 128.7 us by rows, 96.5
+// with K = 2112).
+hipError_t launch_repack_dense(const uint16_t* w, int NW, int K, uint16_t* out, hipStream_t s);
+// few rows an expert, any weights: 16 rows and 16 * co columns (co 1, 2) a block
+// (experts.hip)
+hipError_t launch_experts_rows(int bits, bool gated, const ExpertsArgs& a, int co, hipStream_t s);
 hipError_t validate_experts_kernels();
+// dense weights, tiles (experts_tile.hip): groups cut every 64 * max places, max 2
+// or 4; x_rows * ldx and NW * K below 2^30, y 16-byte aligned with ldy % 8 == 0
+hipError_t launch_experts_tile(bool gated, const ExpertsArgs& a, int max, hipStream_t s);
+hipError_t validate_experts_tile_kernels();
+// w4 and w8, the same with x as its fp16 copy (experts_qtile.hip): groups cut
+// every 32 * max places, max 2 or, of w4, 4, of w8, 8
+hipError_t launch_experts_qtile(int bits, bool gated, const ExpertsArgs& a, int max,
+                                hipStream_t s);
+hipError_t validate_experts_qtile_kernels();
+// Which of them takes n places of a stack of N weight rows: 0 the few-row kernel,
+// else the tiles' cut (`max`).
+int experts_cut(int E, int N, int K, int bits, int n);
 
 hipError_t validate_qproj_kernels();
 hipError_t validate_qproj_fast_kernels();

@@ -34,6 +34,11 @@ __device__ __forceinline__ void dma4_sb(const void* base, uint32_t off, uint32_t
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
                :: "v"(off), "s"(base), "s"(lds) : "m0");
 }
+// The same with a 64-bit address a lane, for sources with no base in common.
+__device__ __forceinline__ void dma16_v(const void* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+               :: "v"(src), "s"(lds) : "m0");
+}
 #pragma clang diagnostic pop
 
 // LDS byte address of a __shared__ object: the low half of its generic

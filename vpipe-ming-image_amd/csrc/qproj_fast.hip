@@ -31,69 +31,14 @@
 #include <atomic>
 
 #include "common.h"
+#include "deq_frag.h"
 #include "kernels.h"
 #include "lds_ring.h"
 
 namespace ming {
 namespace {
 
-typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-
 constexpr int BM = 256, BN = 256, BK = 64;
-
-// 8 codes (one w4 word) -> 8 fp16 dequantized values. The word's nibbles
-// are ordered {k0,k4,k1,k5,k2,k6,k3,k7}, so lo = w & 0x0F0F0F0F holds
-// k0..k3 one per byte and hi = (w >> 4) & 0x0F0F0F0F holds k4..k7; one
-// v_perm per pair then lays a code under the 0x64 magic byte.
-__device__ __forceinline__ uint4 deq_w4(uint32_t w, half2v s2, half2v b2) {
-  const half2v k1024 = {(_Float16)1024.0f, (_Float16)1024.0f};
-  const uint32_t lo = w & 0x0F0F0F0Fu;
-  const uint32_t hi = (w >> 4) & 0x0F0F0F0Fu;
-  uint32_t v[4];
-  v[0] = __builtin_amdgcn_perm(0x64646464u, lo, 0x05010400u);
-  v[1] = __builtin_amdgcn_perm(0x64646464u, lo, 0x05030402u);
-  v[2] = __builtin_amdgcn_perm(0x64646464u, hi, 0x05010400u);
-  v[3] = __builtin_amdgcn_perm(0x64646464u, hi, 0x05030402u);
-  uint4 o;
-  uint32_t* op = &o.x;
-#pragma unroll
-  for (int p = 0; p < 4; ++p) {
-    const half2v c = __builtin_bit_cast(half2v, v[p]) - k1024;
-    op[p] = __builtin_bit_cast(uint32_t, c * s2 + b2);
-  }
-  return o;
-}
-
-// 8 codes (two w8 words, bytes in k order) -> 8 fp16.
-__device__ __forceinline__ uint4 deq_w8(uint32_t w0, uint32_t w1, half2v s2,
-                                        half2v b2) {
-  const half2v k1024 = {(_Float16)1024.0f, (_Float16)1024.0f};
-  uint32_t v[4];
-  v[0] = __builtin_amdgcn_perm(0x64646464u, w0, 0x05010400u);
-  v[1] = __builtin_amdgcn_perm(0x64646464u, w0, 0x05030402u);
-  v[2] = __builtin_amdgcn_perm(0x64646464u, w1, 0x05010400u);
-  v[3] = __builtin_amdgcn_perm(0x64646464u, w1, 0x05030402u);
-  uint4 o;
-  uint32_t* op = &o.x;
-#pragma unroll
-  for (int p = 0; p < 4; ++p) {
-    const half2v c = __builtin_bit_cast(half2v, v[p]) - k1024;
-    op[p] = __builtin_bit_cast(uint32_t, c * s2 + b2);
-  }
-  return o;
-}
-
-// Code-chunk swizzle inside a row group: chunk h of row n sits at
-// n*CPR + (h ^ sw(n)), so the 16 rows a fragment read serves per LDS cycle
-// land on distinct banks (rows are 32 B (w4) / 64 B (w8) apart).
-template <int CPR>
-__device__ __forceinline__ int wswz(int n) {
-  return CPR == 2 ? ((n >> 3) & 1) : ((n >> 2) & 3);
-}
-template <int CPR>
-__device__ __forceinline__ int wchunk(int n, int h) {
-  return n * CPR + (h ^ wswz<CPR>(n));
-}
 
 // SPLIT (a.kslices > 1, a projection of few tiles): block b is slice
 // b / tiles of tile b % tiles. The slice runs its share of K (the last one
@@ -106,7 +51,13 @@ __device__ __forceinline__ int wchunk(int n, int h) {
 // side; the epilogue meets the two in LDS and writes only the SwiGLU. MULTI
 // (qproj_merged_kernel): a.nw projections over one x, their column tiles side
 // by side in the tile grid.
-template <int BITS, bool SPLIT, bool PAIR, int RF, int NW, bool MULTI = false>
+//
+// ROWS (qproj_rows_kernel): instead of the segments' adapters the tail runs the
+// chunks of the adapters that the tile's rows name (a.rows), each over all its
+// rows: those with another adapter read T's row of zeros. Split, the slices share
+// them out by adapter and chunk alone, so that a row's sum does not depend on
+// which others are in its tile.
+template <int BITS, bool SPLIT, bool PAIR, int RF, int NW, bool MULTI = false, bool ROWS = false>
 __device__ __forceinline__ void qproj_fast_body(const QprojArgs& a) {
   constexpr int WCH = BITS == 4 ? 512 : 1024;    // 16-B code chunks per stage
   constexpr int CPR = BITS == 4 ? 2 : 4;         // code chunks per row
@@ -411,8 +362,106 @@ __device__ __forceinline__ void qproj_fast_body(const QprojArgs& a) {
   if (KT - kt == 2) body(kt + 1, st1, st2, st0);
   ring_wait<0>();                               // drained; LDS free
 
+  if constexpr (ROWS) {
+    const RowAdapters& ra = a.rows;
+    const int32_t* const ends = ra.counts + (SPLIT ? tm * a.kslices + ks : tm);
+    const int ch0 = SPLIT && ks > 0 ? ends[-1] : 0;
+    const int n = ends[0] - ch0;
+    if (n > 0) {
+      // uniform reads through the scalar cache: a vector load would count with
+      // the DMAs
+      typedef const __attribute__((address_space(4))) uint64_t* Const64;
+      const Const64 list = (Const64)(uintptr_t)(ra.chunks + (long long)tm * ra.stride + ch0);
+      uint32_t trow[TD], bn[BD];
+      int rid[TD], tc[TD], bc[BD];
+#pragma unroll
+      for (int i = 0; i < TD; ++i) {
+        const int p = 64 * (TD * wave + i) + lane;
+        const int row = p >> 2;
+        tc[i] = (p & 3) ^ ((row >> 2) & 3);
+        int m = m0 + row;
+        m = m < mlast ? m : mlast;
+        rid[i] = ra.rid[m];
+        trow[i] = (uint32_t)(((long long)m * ra.ldt + 8 * tc[i]) * 2);
+      }
+#pragma unroll
+      for (int i = 0; i < BD; ++i) {
+        const int p = 64 * (BD * wave + i) + lane;
+        const int row = p >> 2;
+        bc[i] = (p & 3) ^ ((row >> 2) & 3);
+        bn[i] = (uint32_t)(n0 + row < nlast ? n0 + row : nlast);
+      }
+      auto issue_c = [&](int ch, const uint4* X) {
+        const uint64_t ptr = list[2 * ch], meta = list[2 * ch + 1];
+        const int id = (int)(uint32_t)meta;
+        const uint32_t shape = (uint32_t)(meta >> 32);
+        const uint32_t r16 = (shape & 0xfffu) * 2u, c64 = (shape >> 12 & 0xffu) * 64u;
+        const int live = (int)(shape >> 20);
+#pragma unroll
+        for (int i = 0; i < TD; ++i)
+          dma16_sb(ra.t, rid[i] == id ? trow[i] + c64 : ra.zero,
+                   lds_addr(X + 64 * (TD * wave + i)));
+        // past the chunk's live groups T is zero: any of its columns of B will do
+#pragma unroll
+        for (int i = 0; i < BD; ++i)
+          dma16_sb(reinterpret_cast<const void*>(ptr),
+                   bn[i] * r16 + (uint32_t)(bc[i] < live ? bc[i] : live) * 16u,
+                   lds_addr(X + TRG + 64 * (BD * wave + i)));
+      };
+      uint4 ta[JT], tb[RF];
+      auto read_c = [&](const uint4* X, int kk, uint4 (&av)[JT], uint4 (&bv)[RF]) {
+        const int c = 2 * kk + fk;
+#pragma unroll
+        for (int j = 0; j < JT; ++j) av[j] = X[TRG + swz4(32 * JT * wave + 32 * j + fr, c)];
+#pragma unroll
+        for (int i = 0; i < RF; ++i) bv[i] = X[swz4(32 * i + fr, c)];
+      };
+      auto body_c = [&](int ch, const uint4* C, const uint4* Nx, const uint4* Pv) {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          uint4 an[JT], bn_[RF];
+          if (kk == 0) {
+            issue_c(ch + 2 < n ? ch + 2 : n - 1, Pv);
+            read_c(C, 1, an, bn_);
+          } else {
+            read_c(Nx, 0, an, bn_);
+          }
+#pragma unroll
+          for (int i = 0; i < RF; ++i)
+#pragma unroll
+            for (int j = 0; j < JT; ++j)
+              acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                  __builtin_bit_cast(bf16x8_t, ta[j]), __builtin_bit_cast(bf16x8_t, tb[i]),
+                  acc[j][i], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+          if (kk == 0) {
+            ring_wait<TPER>();                     // chunk ch + 1 landed, ch done
+            __builtin_amdgcn_sched_barrier(0);
+          }
+#pragma unroll
+          for (int j = 0; j < JT; ++j) ta[j] = an[j];
+#pragma unroll
+          for (int i = 0; i < RF; ++i) tb[i] = bn_[i];
+        }
+      };
+      issue_c(0, st0);
+      issue_c(n > 1 ? 1 : 0, st1);
+      ring_wait<TPER>();
+      read_c(st0, 0, ta, tb);
+      int ch = 0;
+      for (; ch + 3 <= n; ch += 3) {
+        body_c(ch, st0, st1, st2);
+        body_c(ch + 1, st1, st2, st0);
+        body_c(ch + 2, st2, st0, st1);
+      }
+      if (n - ch >= 1) body_c(ch, st0, st1, st2);
+      if (n - ch == 2) body_c(ch + 1, st1, st2, st0);
+      ring_wait<0>();
+    }
+  }
+
   // ---- LoRA tail: T and gathered B chunks of 32 ranks, same ring ----
-  const int chunks32 = (!SPLIT || ks == a.kslices - 1) ? seg.chunks : 0;
+  const int chunks32 = ROWS ? 0 : (!SPLIT || ks == a.kslices - 1) ? seg.chunks : 0;
   if (chunks32 > 0) {
     // PAIR: the second half of the waves gathers the up projection's B (its segment, its
     // groups); both T chunks are staged for every wave
@@ -724,6 +773,11 @@ __global__ __launch_bounds__(64 * NW, 1) void qproj_pair_kernel(const QprojArgs 
 template <int BITS, bool SPLIT, int RF, int NW>
 __global__ __launch_bounds__(64 * NW, 1) void qproj_merged_kernel(const QprojArgs a) {
   qproj_fast_body<BITS, SPLIT, false, RF, NW, true>(a);
+}
+
+template <int BITS, bool SPLIT, int RF, int NW>
+__global__ __launch_bounds__(64 * NW, 1) void qproj_rows_kernel(const QprojArgs a) {
+  qproj_fast_body<BITS, SPLIT, false, RF, NW, false, true>(a);
 }
 
 // The split projection's end (grid y: the projection of a merged launch): y =
@@ -1343,8 +1397,11 @@ bool qproj_merge_pays(int M, int N, int K, int nw) {
 template <int BITS, bool SPLIT, int RF, int NW>
 static void launch_tiles(const QprojArgs& a, hipStream_t s) {
   const int tiles = ((a.M + 32 * RF - 1) / (32 * RF)) * ((a.N + BN - 1) / BN);
-  hipLaunchKernelGGL((qproj_fast_kernel<BITS, SPLIT, RF, NW>),
-                     dim3((unsigned)(SPLIT ? tiles * a.kslices : tiles)), dim3(64 * NW), 0, s, a);
+  const dim3 grid((unsigned)(SPLIT ? tiles * a.kslices : tiles));
+  if (a.rows.counts)
+    hipLaunchKernelGGL((qproj_rows_kernel<BITS, SPLIT, RF, NW>), grid, dim3(64 * NW), 0, s, a);
+  else
+    hipLaunchKernelGGL((qproj_fast_kernel<BITS, SPLIT, RF, NW>), grid, dim3(64 * NW), 0, s, a);
 }
 template <int BITS>
 static void launch_rows(const QprojArgs& a, int rf, hipStream_t s) {
@@ -1420,6 +1477,13 @@ static hipError_t launch_plan(const QprojArgs& a, const RowPlan& p, F&& rows) {
   if (a.g) h.g = a.g + r * a.ldg;
   if (a.yh) h.yh = a.yh + r * a.ldyh;
   if (a.t) h.t = a.t + r * a.ldt;
+  if (a.rows.counts) {
+    h.rows.rid = a.rows.rid + r;
+    h.rows.t = a.rows.t + r * a.rows.ldt;
+    h.rows.zero = a.rows.zero - (uint32_t)(r * a.rows.ldt * 2);
+    h.rows.chunks = a.rows.chunks + r / 256 * a.rows.stride;
+    h.rows.counts = a.rows.counts + r / 256;
+  }
   for (int i = 0; i + 1 < a.nw; ++i) h.more[i].y = a.more[i].y + r * a.ldy;
   rows(h, p.rf_rest);
   return hipGetLastError();
@@ -1699,6 +1763,16 @@ hipError_t validate_qproj_fast_kernels() {
                        reinterpret_cast<const void*>(&qproj_fast_kernel<8, true, 8, 4>),
                        reinterpret_cast<const void*>(&qproj_pair_kernel<8, 4, 8>),
                        reinterpret_cast<const void*>(&qproj_pair_kernel<8, 6, 8>),
+#define MING_QPROJ_ROWS(BITS)                                              \
+  reinterpret_cast<const void*>(&qproj_rows_kernel<BITS, false, 2, 8>),    \
+      reinterpret_cast<const void*>(&qproj_rows_kernel<BITS, false, 4, 8>), \
+      reinterpret_cast<const void*>(&qproj_rows_kernel<BITS, false, 6, 8>), \
+      reinterpret_cast<const void*>(&qproj_rows_kernel<BITS, false, 8, 4>), \
+      reinterpret_cast<const void*>(&qproj_rows_kernel<BITS, true, 2, 8>), \
+      reinterpret_cast<const void*>(&qproj_rows_kernel<BITS, true, 4, 8>), \
+      reinterpret_cast<const void*>(&qproj_rows_kernel<BITS, true, 8, 4>)
+                       MING_QPROJ_ROWS(4), MING_QPROJ_ROWS(8),
+#undef MING_QPROJ_ROWS
                        reinterpret_cast<const void*>(&qproj_split_reduce_kernel),
                        reinterpret_cast<const void*>(&repack_fast_kernel),
                        reinterpret_cast<const void*>(&repack_sbf_kernel),

@@ -15,12 +15,13 @@ struct RowGroup {
   int index;   // the block's index inside the group
 };
 
-// Block `b` of a grid in which group e has units(rows of e) consecutive blocks.
-// Offsets are kept inside [0, n] and ascending, so a plan that is not one can
-// name wrong rows but none outside.
-template <class Units>
+// The group of unit pick(total) where group e has units(rows of e) consecutive
+// ones; none where pick says -1. Offsets are kept inside [0, n] and a group that
+// ends before it begins is empty, so a plan that is not one can name wrong rows
+// but none outside.
+template <class Units, class Pick>
 __device__ __forceinline__ RowGroup find_group(const int32_t* __restrict__ offsets, int E, int n,
-                                               int b, Units&& units) {
+                                               Units&& units, Pick&& pick) {
   const int lane = (int)threadIdx.x & 63;
   const int per = (E + 63) / 64;
   const int e0 = lane * per;
@@ -41,9 +42,10 @@ __device__ __forceinline__ RowGroup find_group(const int32_t* __restrict__ offse
     const int v = __shfl_up(run, o, 64);
     if (lane >= o) run += v;
   }
-  const uint64_t past = __ballot(run > b);
   RowGroup g = {-1, 0, 0, 0};
-  if (!past) return g;
+  const int b = pick(__builtin_amdgcn_readlane(run, 63));
+  const uint64_t past = __ballot(run > b);
+  if (b < 0 || !past) return g;
   const int w = __builtin_ctzll(past);     // the lane whose groups hold the block
   int left = b - (__builtin_amdgcn_readlane(run, w) - __builtin_amdgcn_readlane(sum, w));
   int e = w * per;

@@ -39,6 +39,9 @@ int rt_take_range_fault(ming_ctx* c, const char* who);
 bool rt_set_copies_unread(ming_ctx* c, bool unread);
 
 int rt_route(const ming_ctx* c);
+// Experts' products on the context take this cut (experts_cut), -1: the plan's (tests).
+void rt_set_experts_cut(ming_ctx* c, int cut);
+int rt_experts_cut(const ming_ctx* c);
 // the device word fp16 copies raise (QprojArgs::range), NULL on routes without
 int* rt_range_word(const ming_ctx* c);
 // Event timing around one launch of a family (ming_ctx_set_profiling): begin

@@ -83,6 +83,7 @@ struct ming_ctx {
   // growing it keeps the old buffer (until the context goes) instead of freeing it
   bool part_captured = false;
   size_t part_cap = SIZE_MAX;  // rt_set_part_cap
+  int experts_cut = -1;        // rt_set_experts_cut
   std::vector<void*> part_kept;
   int route = MING_ROUTE_AUTO;
   // device word raised by any fp16 copy that could not hold its value
@@ -450,6 +451,8 @@ hipError_t validate_kernels(int device) {
   if (e == hipSuccess) e = ming::validate_adapter_kernels();
   if (e == hipSuccess) e = ming::validate_routing_kernels();
   if (e == hipSuccess) e = ming::validate_experts_kernels();
+  if (e == hipSuccess) e = ming::validate_experts_tile_kernels();
+  if (e == hipSuccess) e = ming::validate_experts_qtile_kernels();
   if (known) done[device] = e == hipSuccess;
   return e;
 }
@@ -981,7 +984,7 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
   if (rows) {
     ra.ldt = rows->bank->ldt;
     ra.table = rows->bank->table;
-    rows_need = Carve::aligned256((size_t)M * 4) + Carve::aligned256((size_t)M * ra.ldt * 2);
+    rows_need = Carve::aligned256((size_t)M * 4) + Carve::aligned256((size_t)(M + 1) * ra.ldt * 2);
   }
   auto rows_room = [&](size_t need) {
     carve->need = need;
@@ -991,8 +994,8 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
                                     " holds " + std::to_string(carve->cap));
   };
   // T of every row's adapter, then (plane) the f32 plane; the projections follow
+  ming::RowXaArgs xr{};
   auto rows_launch = [&](float* plane, int N) {
-    ming::RowXaArgs xr{};
     xr.x = x; xr.ldx = ldx; xr.M = M; xr.K = K;
     xr.ids = rows->ids; xr.scale = rows->scale;
     xr.table = ra.table; xr.cap = rows->bank->cap;
@@ -1029,7 +1032,7 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
         if (const int rc = rows_room(need)) return rc;
         if (carve->measure) return ok();
         ra.rid = (const int32_t*)carve->take((size_t)M * 4);
-        ra.t = (const uint16_t*)carve->take((size_t)M * ra.ldt * 2);
+        ra.t = (const uint16_t*)carve->take((size_t)(M + 1) * ra.ldt * 2);
         plane = (float*)carve->take((size_t)M * qs[0]->N * 4);
         if (const int rc = rows_launch(plane, qs[0]->N)) return rc;
       }
@@ -1152,13 +1155,15 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
   bool any_fast = false;
   for (int i = 0; i < n; ++i) {
     const ming_qweight* q = qs[i];
-    tail_fits[i] = (uint64_t)M * (uint64_t)t_cols * 2 <= (1ull << 31);
+    tail_fits[i] = (uint64_t)M * (uint64_t)t_cols * 2 <= (1ull << 31) &&
+                   (!rows || ((uint64_t)(M + 1) * (uint64_t)ra.ldt * 2 <= (1ull << 31) &&
+                              (uint64_t)q->N * (uint64_t)ra.ldt * 2 <= (1ull << 31)));
     for (int si = 0; si < (int)q->segs.size() && t_cols > 0; ++si)
       if (qa[i].seg[si].chunks > 0 &&
           (uint64_t)q->segs[si].N * (uint64_t)q->b_ld[si] * 2 > (1ull << 31))
         tail_fits[i] = false;
     fast[i] = q->bits != 16 && q->fast && c->route == MING_ROUTE_AUTO && tail_fits[i] &&
-              (uint64_t)M * (uint64_t)K * 2 <= (1ull << 31) && !rows;
+              (uint64_t)M * (uint64_t)K * 2 <= (1ull << 31);
     any_fast = any_fast || fast[i];
   }
   // Per projection: the fast route's K split on few tiles; a dense weight with
@@ -1198,7 +1203,7 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
     }
     // fused, a gated output lands while other tiles still read x: one that
     // shares memory with x goes by the plane
-    if (dense && dense_plan[i].slices == 0 && q->N % 8 == 0 && tail_fits[i] && !rows &&
+    if (dense && dense_plan[i].slices == 0 && q->N % 8 == 0 && tail_fits[i] &&
         !(o.gate && overlap(o.y, o.ldy, q->N, x, ldx, K, M)))
       dense_rf[i] = ming::dense_fast_rf(M, q->N);
     if (o.gate && !fast[i] && !dense_rf[i]) up_bytes = std::max(up_bytes, (size_t)M * q->N * 2);
@@ -1250,14 +1255,45 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
   float* plane = nullptr;
   const uint16_t* xh = xh_src;
   if (carve && rows) {
-    const size_t plane_bytes = (size_t)M * qs[0]->N * 4;
-    const size_t need = rows_need + Carve::aligned256(plane_bytes) + Carve::aligned256(xh_bytes) +
-                        Carve::aligned256(part_bytes);
+    // The tile kernels take the rows' adapters as a tail over lists of their
+    // chunks, one a row tile; the other launches an f32 plane.
+    const bool tail = fast[0] || dense_rf[0] > 0;
+    size_t plane_bytes = 0, list_bytes = 0, count_bytes = 0;
+    if (tail) {
+      ming::RowPlan rp{0, 2 * dense_rf[0], 0.0};
+      if (fast[0])
+        rp = split_ks[0] >= 2
+                 ? ming::RowPlan{0, qa[0].split_rf, 0.0}
+                 : ming::plan_rows(M, (qs[0]->N + 255) / 256, K / 64, false);
+      xr.rows_main = rp.rows_main / 256 * 256;
+      xr.rest = 32 * rp.rf_rest;
+      const int tiles = ming::row_tiles(M, xr.rows_main, xr.rest);
+      // at most an adapter a row of the tile
+      const int most = std::max(xr.rows_main > 0 ? 256 : 0, xr.rest);
+      xr.stride = std::min({most, M, rows->bank->cap}) * (ra.ldt / 32);
+      list_bytes = (size_t)tiles * xr.stride * sizeof(ming::RowChunk);
+      xr.slices = fast[0] && split_ks[0] >= 2 ? split_ks[0] : 1;
+      count_bytes = (size_t)tiles * xr.slices * 4;
+    } else {
+      plane_bytes = (size_t)M * qs[0]->N * 4;
+    }
+    const size_t need = rows_need + Carve::aligned256(plane_bytes) +
+                        Carve::aligned256(list_bytes) + Carve::aligned256(count_bytes) +
+                        Carve::aligned256(xh_bytes) + Carve::aligned256(part_bytes);
     if (const int rc = rows_room(need)) return rc;
     if (carve->measure) return ok();
     ra.rid = (const int32_t*)carve->take((size_t)M * 4);
-    ra.t = (const uint16_t*)carve->take((size_t)M * ra.ldt * 2);
+    ra.t = (const uint16_t*)carve->take((size_t)(M + 1) * ra.ldt * 2);
     if (plane_bytes) plane = (float*)carve->take(plane_bytes);
+    if (tail) {
+      xr.chunks = (uint4*)carve->take(list_bytes);
+      xr.counts = (int32_t*)carve->take(count_bytes);
+      ra.chunks = xr.chunks;
+      ra.counts = xr.counts;
+      ra.stride = xr.stride;
+      ra.zero = (uint32_t)((size_t)M * ra.ldt * 2);
+      qa[0].rows = ra;
+    }
     if (xh_bytes) xh = (const uint16_t*)carve->take(xh_bytes);
     if (part_bytes) part = (float*)carve->take(part_bytes);
   } else if (carve) {
@@ -1292,8 +1328,14 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
   // The fast x.A stages every element of x through LDS: its DMA waves
   // write the fp16 copy as they go, in place of the conversion launch.
   const bool xh_in_xa = need_xh && t_cols > 0 && xa_fast;
-  if (rows)
+  if (rows) {
+    if (need_xh) {
+      // the rows' x.A reads every element of x: it writes the fp16 copy too
+      xr.xh = const_cast<uint16_t*>(xh);
+      xr.range = range_word(c);
+    }
     if (const int rc = rows_launch(plane, qs[0]->N)) return rc;
+  }
   if (t_cols > 0) {
     xa.x = x; xa.ldx = ldx; xa.K = K; xa.M = M;
     xa.n_cols = t_cols; xa.t = T; xa.ldt = t_cols;
@@ -1314,7 +1356,7 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
              "lora_xa launch");
     c->eng.lora_xa += 1;
   }
-  if (need_xh && !xh_in_xa) {
+  if (need_xh && !xh_in_xa && !rows) {
     uint16_t* dst = const_cast<uint16_t*>(xh);
     MING_HIP(profiled(c, kBCvt, 0.0, 4.0 * M * K,
                       [&] { return ming::launch_bf16_to_f16(x, ldx, dst, K, M, K,
@@ -2142,6 +2184,8 @@ int ming_quantize_pack(ming_ctx* c, const float* w, int N, int K, int bits,
 
 namespace ming {
 int rt_route(const ming_ctx* c) { return c->route; }
+void rt_set_experts_cut(ming_ctx* c, int cut) { c->experts_cut = cut; }
+int rt_experts_cut(const ming_ctx* c) { return c->experts_cut; }
 int* rt_range_word(const ming_ctx* c) { return range_word(c); }
 bool rt_profile_begin(ming_ctx* c, void** ev) {
   *ev = nullptr;
