@@ -33,6 +33,7 @@
 // order, sb [kt][n] = bf16 scale | bf16 bias << 16; dense w [n][k].
 #include "common.h"
 #include "kernels.h"
+#include "row_adapters.h"
 
 namespace ming {
 namespace {
@@ -104,7 +105,7 @@ __device__ __forceinline__ void operands(const GroupRaw<BITS>& r, uint4& w0, uin
 }
 
 template <int BITS, int WK, int CT, int CL>
-__device__ __forceinline__ void gemv_body(const GemvArgs& a, const float* delta = nullptr) {
+__device__ __forceinline__ void gemv_body(const GemvArgs& a, const RowAdapters* ra = nullptr) {
   constexpr int NC = WK * CL;                // residue classes of the groups
   constexpr int U = NC == 4 ? 1 : 4 / (CL * CT);   // groups of a class in flight
   const int lane = (int)threadIdx.x & 63;
@@ -187,7 +188,11 @@ __device__ __forceinline__ void gemv_body(const GemvArgs& a, const float* delta 
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] += bf16_to_f32(a.bias[n + r]);
   }
-  if (delta) v += *reinterpret_cast<const floatx4_t*>(delta + (long long)c * a.N + n);
+  if (ra) {
+    float r[4] = {v[0], v[1], v[2], v[3]};
+    add_row_adapter(*ra, c, n, r);
+    v = floatx4_t{r[0], r[1], r[2], r[3]};
+  }
   *reinterpret_cast<uint2*>(a.y + (long long)c * a.ldy + n) =
       make_uint2(pack_bf16x2_rne(v[0], v[1]), pack_bf16x2_rne(v[2], v[3]));
 }
@@ -198,8 +203,8 @@ __global__ __launch_bounds__(64 * WK) void gemv_kernel(const GemvArgs a) {
 }
 
 template <int BITS, int WK, int CT>
-__global__ __launch_bounds__(64 * WK) void gemv_delta_kernel(const GemvArgs a, const float* delta) {
-  gemv_body<BITS, WK, CT, 1>(a, delta);
+__global__ __launch_bounds__(64 * WK) void gemv_rows_kernel(const GemvArgs a, const RowAdapters ra) {
+  gemv_body<BITS, WK, CT, 1>(a, &ra);
 }
 
 template <int BITS, int CL>
@@ -214,10 +219,10 @@ __global__ __launch_bounds__(256) void gemv_batch_kernel(const GemvBatch b) {
 }
 
 template <int BITS, int WK, int CT>
-void launch_shape(const GemvArgs& a, const float* delta, hipStream_t s) {
+void launch_shape(const GemvArgs& a, const RowAdapters* ra, hipStream_t s) {
   const dim3 grid((unsigned)((a.N + 16 * CT - 1) / (16 * CT)));
-  if (delta)
-    hipLaunchKernelGGL((gemv_delta_kernel<BITS, WK, CT>), grid, dim3(64 * WK), 0, s, a, delta);
+  if (ra)
+    hipLaunchKernelGGL((gemv_rows_kernel<BITS, WK, CT>), grid, dim3(64 * WK), 0, s, a, *ra);
   else
     hipLaunchKernelGGL((gemv_kernel<BITS, WK, CT>), grid, dim3(64 * WK), 0, s, a);
 }
@@ -241,7 +246,7 @@ void launch_batch_shape(const GemvBatch& b, hipStream_t s) {
 constexpr int kShortK = 512;
 
 template <int BITS>
-void launch_one(const GemvArgs& a, const float* d, hipStream_t s) {
+void launch_one(const GemvArgs& a, const RowAdapters* d, hipStream_t s) {
   if constexpr (BITS != 16) {
     if (a.N > 3 * 256 * 16) {
       a.K <= kShortK ? launch_shape<BITS, 4, 2>(a, d, s) : launch_shape<BITS, 8, 2>(a, d, s);
@@ -275,16 +280,16 @@ hipError_t launch_gemv_batch(int bits, const GemvBatch& b, hipStream_t s) {
 }
 
 hipError_t launch_gemv(int bits, const GemvArgs& a, hipStream_t s) {
-  return launch_gemv_delta(bits, a, nullptr, s);
+  return launch_gemv_rows(bits, a, nullptr, s);
 }
 
-hipError_t launch_gemv_delta(int bits, const GemvArgs& a, const float* delta, hipStream_t s) {
+hipError_t launch_gemv_rows(int bits, const GemvArgs& a, const RowAdapters* ra, hipStream_t s) {
   if (a.M <= 0 || a.N <= 0) return hipSuccess;
   if (a.M > kGemvMaxM || a.K % 64 != 0) return hipErrorInvalidValue;
   switch (bits) {
-    case 4: launch_one<4>(a, delta, s); break;
-    case 8: launch_one<8>(a, delta, s); break;
-    case 16: launch_one<16>(a, delta, s); break;
+    case 4: launch_one<4>(a, ra, s); break;
+    case 8: launch_one<8>(a, ra, s); break;
+    case 16: launch_one<16>(a, ra, s); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
@@ -296,8 +301,8 @@ hipError_t validate_gemv_kernels() {
 #define MING_GEMV_ALL(BITS)                                             \
   reinterpret_cast<const void*>(&gemv_kernel<BITS, 4, 1>),              \
       reinterpret_cast<const void*>(&gemv_kernel<BITS, 8, 1>),          \
-      reinterpret_cast<const void*>(&gemv_delta_kernel<BITS, 4, 1>),    \
-      reinterpret_cast<const void*>(&gemv_delta_kernel<BITS, 8, 1>),    \
+      reinterpret_cast<const void*>(&gemv_rows_kernel<BITS, 4, 1>),    \
+      reinterpret_cast<const void*>(&gemv_rows_kernel<BITS, 8, 1>),    \
       reinterpret_cast<const void*>(&gemv_batch_kernel<BITS, 1>),       \
       reinterpret_cast<const void*>(&gemv_batch_kernel<BITS, 2>)
       MING_GEMV_ALL(4), MING_GEMV_ALL(8), MING_GEMV_ALL(16),
@@ -306,10 +311,10 @@ hipError_t validate_gemv_kernels() {
       reinterpret_cast<const void*>(&gemv_kernel<4, 8, 2>),
       reinterpret_cast<const void*>(&gemv_kernel<8, 4, 2>),
       reinterpret_cast<const void*>(&gemv_kernel<8, 8, 2>),
-      reinterpret_cast<const void*>(&gemv_delta_kernel<4, 4, 2>),
-      reinterpret_cast<const void*>(&gemv_delta_kernel<4, 8, 2>),
-      reinterpret_cast<const void*>(&gemv_delta_kernel<8, 4, 2>),
-      reinterpret_cast<const void*>(&gemv_delta_kernel<8, 8, 2>)};
+      reinterpret_cast<const void*>(&gemv_rows_kernel<4, 4, 2>),
+      reinterpret_cast<const void*>(&gemv_rows_kernel<4, 8, 2>),
+      reinterpret_cast<const void*>(&gemv_rows_kernel<8, 4, 2>),
+      reinterpret_cast<const void*>(&gemv_rows_kernel<8, 8, 2>)};
   for (const void* f : fns) {
     const hipError_t e = hipFuncGetAttributes(&fa, f);
     if (e != hipSuccess) return e;

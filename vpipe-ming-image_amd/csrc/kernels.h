@@ -48,7 +48,7 @@ struct QprojMore {
 // Adapters that rows choose (adapters.hip): row m adds T[m] . B_a^T of adapter a
 // = rid[m] (-1: none), T[m] = strength * fold * (x[m] . A_a^T) in bf16.
 struct AdapterEntry {
-  const uint16_t* A;    // [r8][K], rows past the rank zero
+  const uint16_t* A;    // in operand order (launch_repack_adapter), rows past the rank zero
   const uint16_t* B;    // [N][r8], columns past the rank zero
   int r8;               // rank padded to 8; 0: nothing bound
   float fold;
@@ -191,7 +191,10 @@ struct LoraXaArgs {
   // optional (fast kernel only): bias [n_cols] bf16, T = bf16(coef * sum +
   // bias) -- the dense split-K GEMM's ming_lin_bias
   const uint16_t* bias;
-  const float* delta;   // or f32 [M][n_cols], added the same way (QprojArgs::delta)
+  // or what rows' own adapters add (rid NULL: nothing); with one slice as the f32
+  // plane [M][n_cols] of it
+  RowAdapters rows;
+  const float* delta;
   // fast kernel only: a dense weight's split-K GEMM. Column c is row c of
   // A[0], coefficient 1 (grp and coef unused), in tiles of `tile`
   bool ident;
@@ -305,8 +308,8 @@ struct GemvArgs {
   const uint16_t* bias;   // optional bias [N] bf16, added before the rounding
 };
 hipError_t launch_gemv(int bits, const GemvArgs& a, hipStream_t s);
-// The same with f32 [M][N] added before the rounding (what rows' adapters add).
-hipError_t launch_gemv_delta(int bits, const GemvArgs& a, const float* delta, hipStream_t s);
+// The same with what the rows' own adapters add (optional), before the rounding.
+hipError_t launch_gemv_rows(int bits, const GemvArgs& a, const RowAdapters* ra, hipStream_t s);
 // Up to kGemvBatch GEMVs of one shape over one x in one launch (grid y =
 // entry): the per-block adaLN projections of a forward, each entry's bits
 // those of launch_gemv on it.
@@ -428,6 +431,8 @@ hipError_t launch_row_xa(const RowXaArgs& a, hipStream_t s);
 // d[m][n] = T[m] . B_a[n] in f32, a = rid[m]; -0 for rows without an adapter,
 // which any sum takes without a change. N % 4 == 0.
 hipError_t launch_row_delta(const RowAdapters& r, int M, int N, float* d, hipStream_t s);
+// A [rank][K] into the x.A kernels' operand order, ranks rounded up to 16.
+hipError_t launch_repack_adapter(const uint16_t* A, int rank, int K, uint16_t* out, hipStream_t s);
 // *flag = 1 where any of n bf16 values is not finite
 hipError_t launch_check_finite(const uint16_t* v, long long n, int* flag, hipStream_t s);
 hipError_t validate_adapter_kernels();

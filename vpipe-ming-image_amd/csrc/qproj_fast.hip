@@ -34,6 +34,7 @@
 #include "deq_frag.h"
 #include "kernels.h"
 #include "lds_ring.h"
+#include "row_adapters.h"
 
 namespace ming {
 namespace {
@@ -1118,14 +1119,17 @@ __global__ void lora_xa_reduce_kernel(const float* part, int kslices, int M,
     }
     const float co = a.ident ? 1.0f : a.coef[c >> 3];
     uint4 o = make_uint4(0, 0, 0, 0);
-    if (co != 0.0f && (a.bias || a.delta)) {
+    if (co != 0.0f && (a.bias || a.rows.rid)) {
       // the dense split-K GEMM with a bias or its rows' adapters (coef 1): one
       // rounding
       float r[8] = {co * s0.x, co * s0.y, co * s0.z, co * s0.w,
                     co * s1.x, co * s1.y, co * s1.z, co * s1.w};
+      if (a.bias) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        r[e] += a.bias ? bf16_to_f32(a.bias[c + e]) : a.delta[(size_t)m * n_cols + c + e];
+        for (int e = 0; e < 8; ++e) r[e] += bf16_to_f32(a.bias[c + e]);
+      } else {
+        add_row_adapter(a.rows, (int)m, (int)c, r);
+      }
       o.x = pack_bf16x2_rne(r[0], r[1]);
       o.y = pack_bf16x2_rne(r[2], r[3]);
       o.z = pack_bf16x2_rne(r[4], r[5]);

@@ -1026,15 +1026,12 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
           if (sg.slot[sl].rank > 0 && scales && scales[sl] != 0.0f) gemv = false;
     }
     if (gemv) {
-      float* plane = nullptr;
       if (rows) {
-        const size_t need = rows_need + Carve::aligned256((size_t)M * qs[0]->N * 4);
-        if (const int rc = rows_room(need)) return rc;
+        if (const int rc = rows_room(rows_need)) return rc;
         if (carve->measure) return ok();
         ra.rid = (const int32_t*)carve->take((size_t)M * 4);
         ra.t = (const uint16_t*)carve->take((size_t)(M + 1) * ra.ldt * 2);
-        plane = (float*)carve->take((size_t)M * qs[0]->N * 4);
-        if (const int rc = rows_launch(plane, qs[0]->N)) return rc;
+        if (const int rc = rows_launch(nullptr, qs[0]->N)) return rc;
       }
       for (int i = 0; i < n; ++i) {
         const ming_qweight* q = qs[i];
@@ -1045,7 +1042,7 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
                                   : (double)q->N * K * q->bits / 8 + 4.0 * q->N * (K / 64);
         MING_HIP(profiled(c, kBGemv, 2.0 * M * (double)q->N * K,
                           wbytes + 2.0 * M * K + 2.0 * M * q->N,
-                          [&] { return ming::launch_gemv_delta(q->bits, ga, plane, c->stream); }),
+                          [&] { return ming::launch_gemv_rows(q->bits, ga, rows ? &ra : nullptr, c->stream); }),
                  "gemv launch");
         if (q->bits == 4) c->eng.gemm_q4 += 1;
         else if (q->bits == 8) c->eng.gemm_q8 += 1;
@@ -1256,7 +1253,8 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
   const uint16_t* xh = xh_src;
   if (carve && rows) {
     // The tile kernels take the rows' adapters as a tail over lists of their
-    // chunks, one a row tile; the other launches an f32 plane.
+    // chunks, one a row tile; the dense split's sum adds them up itself; the other
+    // launches take an f32 plane.
     const bool tail = fast[0] || dense_rf[0] > 0;
     size_t plane_bytes = 0, list_bytes = 0, count_bytes = 0;
     if (tail) {
@@ -1274,7 +1272,7 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
       list_bytes = (size_t)tiles * xr.stride * sizeof(ming::RowChunk);
       xr.slices = fast[0] && split_ks[0] >= 2 ? split_ks[0] : 1;
       count_bytes = (size_t)tiles * xr.slices * 4;
-    } else {
+    } else if (dense_plan[0].slices < 2) {
       plane_bytes = (size_t)M * qs[0]->N * 4;
     }
     const size_t need = rows_need + Carve::aligned256(plane_bytes) +
@@ -1482,7 +1480,9 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
     if (dense_plan[i].slices > 0) {
       ming::LoraXaArgs da{};
       da.x = x; da.ldx = ldx; da.A[0] = q->w16; da.K = K; da.M = M;
-      da.n_cols = q->N; da.t = a.y; da.ldt = (int)a.ldy; da.bias = o.bias; da.delta = plane;
+      da.n_cols = q->N; da.t = a.y; da.ldt = (int)a.ldy; da.bias = o.bias;
+      da.delta = plane;
+      if (rows && !plane) da.rows = ra;
       da.ident = true; da.tile = dense_plan[i].tile;
       const int dks = dense_plan[i].slices;
       MING_HIP(profiled(c, bk, base_flops, 2.0 * M * K + wbytes + 2.0 * M * q->N,
@@ -1654,27 +1654,30 @@ int ming_adapters_set(ming_adapters* b, int id, int rank, const uint16_t* A, con
   LoraBind nb;
   nb.rank = rank; nb.rank8 = r8; nb.fold = fold;
   int* flag = nullptr;
+  uint16_t* stage = nullptr;   // A as it comes
   int bad = 0;
   auto drop = [&] {
     if (nb.A) (void)hipFree(nb.A);
     if (nb.B) (void)hipFree(nb.B);
     if (flag) (void)hipFree(flag);
+    if (stage) (void)hipFree(stage);
   };
-  if (hipMalloc(&nb.A, (size_t)r8 * K * 2) != hipSuccess ||
+  if (hipMalloc(&nb.A, (size_t)round_up(rank, 16) * K * 2) != hipSuccess ||
+      hipMalloc(&stage, (size_t)rank * K * 2) != hipSuccess ||
       hipMalloc(&nb.B, N * r8 * 2) != hipSuccess || hipMalloc(&flag, sizeof(int)) != hipSuccess) {
     (void)hipGetLastError();
     drop();
     return fail(MING_ERR_ALLOC, "ming_adapters_set: allocation failed");
   }
   const hipMemcpyKind kind = src_on_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice;
-  hipError_t e = hipMemsetAsync(nb.A, 0, (size_t)r8 * K * 2, c->stream);
-  if (e == hipSuccess) e = hipMemsetAsync(nb.B, 0, N * r8 * 2, c->stream);
+  hipError_t e = hipMemsetAsync(nb.B, 0, N * r8 * 2, c->stream);
   if (e == hipSuccess) e = hipMemsetAsync(flag, 0, sizeof(int), c->stream);
-  if (e == hipSuccess) e = hipMemcpyAsync(nb.A, A, (size_t)rank * K * 2, kind, c->stream);
+  if (e == hipSuccess) e = hipMemcpyAsync(stage, A, (size_t)rank * K * 2, kind, c->stream);
   if (e == hipSuccess)
     e = hipMemcpy2DAsync(nb.B, (size_t)r8 * 2, B, (size_t)rank * 2, (size_t)rank * 2, N, kind,
                          c->stream);
-  if (e == hipSuccess) e = ming::launch_check_finite(nb.A, (long long)(r8 * K), flag, c->stream);
+  if (e == hipSuccess) e = ming::launch_check_finite(stage, (long long)(rank * K), flag, c->stream);
+  if (e == hipSuccess) e = ming::launch_repack_adapter(stage, rank, (int)K, nb.A, c->stream);
   if (e == hipSuccess) e = ming::launch_check_finite(nb.B, (long long)(N * r8), flag, c->stream);
   if (e == hipSuccess) e = hipMemcpyAsync(&bad, flag, sizeof(int), hipMemcpyDeviceToHost, c->stream);
   if (e == hipSuccess) e = hipStreamSynchronize(c->stream);
@@ -1684,7 +1687,9 @@ int ming_adapters_set(ming_adapters* b, int id, int rank, const uint16_t* A, con
                            : fail(MING_ERR_RANGE, "ming_adapters_set: a factor is not finite");
   }
   (void)hipFree(flag);
+  (void)hipFree(stage);
   flag = nullptr;
+  stage = nullptr;
   const int rc = adapters_replace(b, id, nb);
   if (rc != MING_OK) {
     drop();
