@@ -4,57 +4,12 @@
 
 #include "common.h"
 #include "kernels.h"
+#include "row_xa.h"
 
 namespace ming {
 namespace {
 
-// T[m] = strength * fold * (x[m] . A_a^T), a = ids[m]. A block takes 16 or 32 rows;
-// the adapters among them (in any order) are found with ballots, and each
-// adapter's 16-rank chunks are v_mfma_f32_16x16x32_bf16 tiles over all the rows, of
-// which only that adapter's are stored: requests' rows lie together, so a block
-// has one or two adapters, and where every row has its own the time is that of
-// reading their A. K is shared out over the eight waves by 64-groups, the sums
-// meet in LDS and are added in wave order (no atomics). A is resident in the
-// operand's own order (launch_repack_adapter): a wave's load is one run of 1 KB, of
-// which lanes past the rank take no part.
-//
-// Two forms. Few rows (row_xa_kernel): 16 rows, a chunk a block and turn, operands
-// straight from memory, all of a chunk's at once; grid y shares out the chunks. Bound by three memory
-// latencies in a row (ids, table, A and x). Many rows (row_xa_many_kernel): x passes
-// through LDS in whole 1 KB row pieces, read from memory once for two (or four)
-// chunks and for the fp16 copy of x that a quantized projection multiplies. Bound by HBM, x
-// once and its copy once ([8704, 3840]: 79 us with x from memory a lane's 16 bytes
-// at a time).
 constexpr int XW = 8;
-
-__device__ __forceinline__ uint4 to_f16(const uint4& v, uint32_t& seen) {
-  seen = range_track4(seen, v);
-  uint4 f;
-  f.x = bf16x2_to_f16x2(v.x);
-  f.y = bf16x2_to_f16x2(v.y);
-  f.z = bf16x2_to_f16x2(v.z);
-  f.w = bf16x2_to_f16x2(v.w);
-  return f;
-}
-
-// The adapter of row m with its entry and the factor of its T; id -1 for none.
-struct RowOf {
-  int id;
-  float coef;
-  AdapterEntry e;
-};
-__device__ __forceinline__ RowOf resolve(const RowXaArgs& a, int m) {
-  RowOf r = {-1, 0.0f, {}};
-  if (m >= a.M) return r;
-  const int id = a.ids[m];
-  const float s = a.scale ? a.scale[m] : 1.0f;
-  if (id < 0 || id >= a.cap || s == 0.0f) return r;
-  r.e = a.table[id];
-  if (r.e.r8 == 0) return r;
-  r.id = id;
-  r.coef = s * r.e.fold;
-  return r;
-}
 
 // The chunk list of row tile `tile` (at most 256 rows, a thread each): the chunks
 // of each adapter where the tile's first row of it stands.
@@ -79,80 +34,25 @@ __device__ __forceinline__ void row_chunks(const RowXaArgs& a, int tile, int* id
   }
   const int chunks = first ? (e.r8 + 31) / 32 : 0;
   RowChunk* const out = reinterpret_cast<RowChunk*>(a.chunks) + (long long)tile * a.stride;
-  int base = 0;
-  for (int s = 0; s < a.slices; ++s) {     // chunk c of adapter id is slice (id + c) % slices'
-    const int c0 = (s + a.slices - (id < 0 ? 0 : id) % a.slices) % a.slices;
-    const int n = chunks > c0 ? (chunks - c0 + a.slices - 1) / a.slices : 0;
-    int run = n;
+  int run = chunks;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int v = __shfl_up(run, o, 64);
-      if (lane >= o) run += v;
-    }
-    __syncthreads();                       // the last slice's sums are read
-    if (lane == 63) sums[tid >> 6] = run;
-    __syncthreads();
-    int at = base + run - n;
-    for (int w = 0; w < 4; ++w) {
-      if (w < (tid >> 6)) at += sums[w];
-      base += sums[w];
-    }
-    for (int i = 0; i < n; ++i) {
-      const int c = c0 + i * a.slices;
-      const int groups = e.r8 - 32 * c >= 32 ? 4 : (e.r8 - 32 * c) / 8;
-      out[at + i] = RowChunk{e.B + 32 * c, id,
-                             (uint32_t)e.r8 | (uint32_t)c << 12 | (uint32_t)(groups - 1) << 20};
-    }
-    if (tid == 0) a.counts[tile * a.slices + s] = base;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int v = __shfl_up(run, o, 64);
+    if (lane >= o) run += v;
   }
+  if (lane == 63) sums[tid >> 6] = run;
+  __syncthreads();
+  int at = run - chunks;
+  for (int w = 0; w < (tid >> 6); ++w) at += sums[w];
+  for (int c = 0; c < chunks; ++c) {
+    const int groups = e.r8 - 32 * c >= 32 ? 4 : (e.r8 - 32 * c) / 8;
+    out[at + c] = RowChunk{e.B + 32 * c, id,
+                           (uint32_t)e.r8 | (uint32_t)c << 12 | (uint32_t)(groups - 1) << 20};
+  }
+  if (tid == 255) a.counts[tile] = at + chunks;
   // T's row of zeros
   if (tile == 0)
     for (int i = tid; i < a.ldt; i += 64 * XW) a.t[(long long)a.M * a.ldt + i] = 0;
-}
-
-// The 16-rank chunks of a block's rows in order: `visit(adapter, r8, A, first
-// rank)`, all wave-uniform, out of what the lanes hold (a table read an adapter would
-// be one memory latency each). T's columns past the rank, up to whole 32, are zeros:
-// `zero(adapter, r8, first rank)` for a chunk that lies there.
-template <class F, class Z>
-__device__ __forceinline__ void each_chunk(const RowOf& row, F&& visit, Z&& zero) {
-  uint64_t left = __ballot(row.id >= 0);
-  const uint64_t p = (uint64_t)(uintptr_t)row.e.A;
-  while (left) {
-    const int w = __builtin_ctzll(left);
-    const int cur = __builtin_amdgcn_readlane(row.id, w);
-    left &= ~__ballot(row.id == cur);
-    const int r8 = __builtin_amdgcn_readlane(row.e.r8, w);
-    const uint64_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)p, w);
-    const uint64_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(p >> 32), w);
-    const uint4* const A = reinterpret_cast<const uint4*>((uintptr_t)(hi << 32 | lo));
-    for (int ch = 0; ch < r8; ch += 16) visit(cur, r8, A, ch);
-    if ((r8 + 15 & ~15) & 16) zero(cur, r8, r8 + 15 & ~15);
-  }
-}
-
-// T's columns ch + 4g .. + 3 of row m from four sums.
-__device__ __forceinline__ void store_t(const RowXaArgs& a, int m, float coef, int r8, int r0,
-                                        const floatx4_t& v) {
-  uint2 o = make_uint2(0, 0);
-  if (r0 < r8) {                             // r8 is a multiple of 8, r0 of 4
-    o.x = pack_bf16x2_rne(coef * v[0], coef * v[1]);
-    o.y = pack_bf16x2_rne(coef * v[2], coef * v[3]);
-  }
-  *reinterpret_cast<uint2*>(a.t + (long long)m * a.ldt + r0) = o;
-}
-
-// Where a lane reads a chunk's operand (16-byte units of the resident order, half h
-// of 64-group kt at + 64 (2 kt + h)). Lanes past the rank read the last one's, which
-// costs no memory; store_t writes zeros for them.
-__device__ __forceinline__ const uint4* chunk_lane(const uint4* A, int r8, int K, int ch, int lane) {
-  const int c = lane & 15, last = r8 - 1 - ch;
-  return A + (long long)(ch / 16) * (K / 32) * 64 + (lane & 48) + (c < last ? c : last);
-}
-
-__device__ __forceinline__ floatx4_t mfma16(const uint4& w, const uint4& x, floatx4_t c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w),
-                                                 __builtin_bit_cast(bf16x8_t, x), c, 0, 0, 0);
 }
 
 __global__ __launch_bounds__(64 * XW) void row_xa_kernel(const RowXaArgs a) {
@@ -163,73 +63,7 @@ __global__ __launch_bounds__(64 * XW) void row_xa_kernel(const RowXaArgs a) {
     if (blockIdx.y == 0) row_chunks(a, (int)blockIdx.x - xtiles, ids, sums);
     return;
   }
-  const int lane = (int)threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int c = lane & 15, g = lane >> 4;
-  const int m0 = (int)blockIdx.x * 16, m = m0 + c;
-  const int KT = a.K / 64;
-  constexpr int U = 8;                       // 64-groups of a wave at once
-  const uint16_t* const xr = a.x + (long long)(m < a.M ? m : a.M - 1) * a.ldx + 8 * g;
-  uint4 xv[U][2];
-  auto load_x = [&](int k0) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int kt = k0 + XW * u < KT ? k0 + XW * u : KT - 1;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        xv[u][h] = *reinterpret_cast<const uint4*>(xr + 64 * kt + 32 * h);
-    }
-  };
-  const RowOf row = resolve(a, m);           // the wave's quarters hold the same rows
-  if (blockIdx.y == 0 && wave == 0 && lane < 16 && m < a.M) a.rid[m] = row.id;
-  if (a.xh) {
-    // the fp16 copy of the block's rows, grid y sharing out the columns
-    const int k8 = a.K / 8, c0 = k8 * (int)blockIdx.y / (int)gridDim.y;
-    const int c1 = k8 * ((int)blockIdx.y + 1) / (int)gridDim.y;
-    uint32_t seen = 0;
-    for (int r = wave; r < 16 && m0 + r < a.M; r += XW)
-      for (int k = c0 + lane; k < c1; k += 64) {
-        const uint4 v = *reinterpret_cast<const uint4*>(a.x + (long long)(m0 + r) * a.ldx + 8 * k);
-        *reinterpret_cast<uint4*>(a.xh + (long long)(m0 + r) * a.K + 8 * k) = to_f16(v, seen);
-      }
-    range_report(a.range, seen);
-  }
-  int turn = 0;
-  bool there = false;
-  each_chunk(row, [&](int cur, int r8, const uint4* A, int ch) {
-    if (turn++ % (int)gridDim.y != (int)blockIdx.y) return;
-    const uint4* const ar = chunk_lane(A, r8, a.K, ch, lane);
-    floatx4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k0 = wave; k0 < KT; k0 += XW * U) {
-      uint4 av[U][2];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int kt = k0 + XW * u < KT ? k0 + XW * u : KT - 1;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) av[u][h] = ar[64 * (2 * kt + h)];
-      }
-      if (!there) load_x(k0);
-      there = KT <= XW * U;
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (k0 + XW * u < KT) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) acc = mfma16(av[u][h], xv[u][h], acc);
-        }
-    }
-    red[wave][lane] = acc;
-    __syncthreads();
-    if (wave == 0) {
-      floatx4_t v = red[0][lane];
-#pragma unroll
-      for (int w = 1; w < XW; ++w) v += red[w][lane];
-      if (row.id == cur) store_t(a, m, row.coef, r8, ch + 4 * g, v);
-    }
-    __syncthreads();
-  }, [&](int cur, int r8, int ch) {
-    if (blockIdx.y == 0 && wave == 0 && row.id == cur)
-      store_t(a, m, 0.0f, r8, ch + 4 * g, floatx4_t{0.0f, 0.0f, 0.0f, 0.0f});
-  });
+  row_xa_block<XW>(a, (int)blockIdx.x, (int)blockIdx.y, (int)gridDim.y, red);
 }
 
 // Up to NC chunks a pass; a pass walks K in steps of 512 through two LDS buffers,
@@ -313,7 +147,7 @@ void row_xa_many_kernel(const RowXaArgs a) {
         for (int b = 0; b < 2; ++b) {
           const uint4 xv = buf[(16 * b + c) * (KS / 8) + ((8 * wave + 4 * h + g) ^ c)];
 #pragma unroll
-          for (int i = 0; i < C; ++i) acc[i][b] = mfma16(av[i][h], xv, acc[i][b]);
+          for (int i = 0; i < C; ++i) acc[i][b] = mfma_rows(av[i][h], xv, acc[i][b]);
         }
     };
     load(0, v0);
@@ -433,12 +267,9 @@ __global__ void check_finite_kernel(const uint16_t* v, long long n, int* flag) {
 
 }  // namespace
 
-// From these rows on x passes through LDS.
-constexpr int kRowXaMany = 768;
-
 hipError_t launch_row_xa(const RowXaArgs& a, hipStream_t s) {
   if (a.M <= 0) return hipSuccess;
-  if (a.K % 64 || a.ldt % 32 || (a.counts && (a.rows_main % 256 || a.rest < 1 || a.rest > 256 || a.slices < 1)))
+  if (a.K % 64 || a.ldt % 32 || (a.counts && (a.rows_main % 256 || a.rest < 1 || a.rest > 256)))
     return hipErrorInvalidValue;
   const int tiles = (a.M + 31) / 32;
   const int lists = a.counts ? row_tiles(a.M, a.rows_main, a.rest) : 0;

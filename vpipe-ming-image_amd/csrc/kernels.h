@@ -59,8 +59,8 @@ struct RowAdapters {
   int ldt;
   const AdapterEntry* table;
   // For the tile kernels' tails: per row tile the 32-rank chunks of the adapters
-  // its rows name (RowChunk, `stride` a tile), how many (split: where each slice's
-  // end), and T's row of zeros as a byte offset from t.
+  // its rows name (RowChunk, `stride` a tile), how many, and T's row of zeros as a
+  // byte offset from t.
   const uint4* chunks;
   const int32_t* counts;
   int stride;
@@ -72,6 +72,8 @@ struct RowChunk {
   int32_t id;
   uint32_t shape;       // r8 | chunk << 12 | (live 8-rank groups - 1) << 20
 };
+
+struct RowXaArgs;
 
 struct QprojArgs {
   const uint16_t* x;
@@ -120,8 +122,9 @@ struct QprojArgs {
   const uint16_t* bias;
   // optional f32 [M][N], added like the bias: what rows' own adapters add
   const float* delta;
-  // rows' own adapters as a tail of the tiles (launch_qproj_fast and
-  // launch_dense_fast; no segments' adapters then), counts NULL: none
+  // rows' own adapters (no segments' adapters then): as a tail of the tiles
+  // (launch_qproj_fast and launch_dense_fast) where counts is set, in the sum of a
+  // K split where rid alone is
   RowAdapters rows;
 };
 
@@ -330,7 +333,9 @@ hipError_t validate_gemv_kernels();
 
 // ---- the fast quantized route (qproj_fast.hip) --------------------------------
 // x is fp16 (carrying bf16 values), a.codes / a.sb the fast resident layout.
-hipError_t launch_qproj_fast(int bits, const QprojArgs& a, hipStream_t s);
+// xa (a K split only): the rows' x.A in the same launch (qproj_rows_beside).
+hipError_t launch_qproj_fast(int bits, const QprojArgs& a, hipStream_t s,
+                             const RowXaArgs* xa = nullptr);
 // Up to three projections over one x as one launch (the fields at QprojArgs::nw),
 // each one's bits those of its own: the same K slices, tiles by the rounds of
 // all. qproj_merge_pays: whether that is less time than one launch each.
@@ -379,8 +384,12 @@ struct DensePlan {
   int slices;
 };
 DensePlan dense_split_plan(int M, int N, int K);
+// Whether a split takes its rows' x.A beside its own blocks.
+bool qproj_rows_beside(int M, int N, int kslices, int rf);
+bool dense_rows_beside(int M, int N, const DensePlan& p);
+// xa: as launch_qproj_fast's, beside a dense weight's split.
 hipError_t launch_lora_xa_fast(const LoraXaArgs& a, float* part, int kslices,
-                               hipStream_t s);
+                               hipStream_t s, const RowXaArgs* xa = nullptr);
 hipError_t launch_bf16_to_f16(const uint16_t* x, long long ldx, uint16_t* y,
                               long long ldy, int rows, int K, hipStream_t s,
                               int* range = nullptr);
@@ -418,7 +427,6 @@ struct RowXaArgs {
   uint4* chunks;
   int32_t* counts;
   int stride, rows_main, rest;
-  int slices;           // of a split launch, else 1: counts [tiles][slices], where each ends
   // optional: the fp16 copy of x, [M][K], and the word it raises (QprojArgs::range)
   uint16_t* xh;
   int* range;
@@ -428,6 +436,9 @@ inline int row_tiles(int M, int rows_main, int rest) {
   return rows_main / 256 + (M > rows_main ? (M - rows_main + rest - 1) / rest : 0);
 }
 hipError_t launch_row_xa(const RowXaArgs& a, hipStream_t s);
+// Below these rows launch_row_xa's blocks are 16 rows each, which a split
+// projection can take beside its own.
+constexpr int kRowXaMany = 768;
 // d[m][n] = T[m] . B_a[n] in f32, a = rid[m]; -0 for rows without an adapter,
 // which any sum takes without a change. N % 4 == 0.
 hipError_t launch_row_delta(const RowAdapters& r, int M, int N, float* d, hipStream_t s);

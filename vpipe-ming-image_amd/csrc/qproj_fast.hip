@@ -35,6 +35,7 @@
 #include "kernels.h"
 #include "lds_ring.h"
 #include "row_adapters.h"
+#include "row_xa.h"
 
 namespace ming {
 namespace {
@@ -55,11 +56,9 @@ constexpr int BM = 256, BN = 256, BK = 64;
 //
 // ROWS (qproj_rows_kernel): instead of the segments' adapters the tail runs the
 // chunks of the adapters that the tile's rows name (a.rows), each over all its
-// rows: those with another adapter read T's row of zeros. Split, the slices share
-// them out by adapter and chunk alone, so that a row's sum does not depend on
-// which others are in its tile.
+// rows: those with another adapter read T's row of zeros.
 template <int BITS, bool SPLIT, bool PAIR, int RF, int NW, bool MULTI = false, bool ROWS = false>
-__device__ __forceinline__ void qproj_fast_body(const QprojArgs& a) {
+__device__ __forceinline__ void qproj_fast_body(const QprojArgs& a, int block) {
   constexpr int WCH = BITS == 4 ? 512 : 1024;    // 16-B code chunks per stage
   constexpr int CPR = BITS == 4 ? 2 : 4;         // code chunks per row
   constexpr int WDMA = WCH / (64 * NW);          // code DMAs per wave per stage
@@ -103,7 +102,7 @@ __device__ __forceinline__ void qproj_fast_body(const QprojArgs& a) {
 
   const int tiles_m = (a.M + BMT - 1) / BMT;
   const int tiles_n = (a.N + BNT - 1) / BNT;
-  int tm, tn, blk = (int)blockIdx.x, ks = 0, kt0 = 0;
+  int tm, tn, blk = block, ks = 0, kt0 = 0;
   int KT = a.K / BK;
   const int tiles_all = MULTI ? a.nw * tiles_n : tiles_n;
   if constexpr (SPLIT) {
@@ -365,14 +364,12 @@ __device__ __forceinline__ void qproj_fast_body(const QprojArgs& a) {
 
   if constexpr (ROWS) {
     const RowAdapters& ra = a.rows;
-    const int32_t* const ends = ra.counts + (SPLIT ? tm * a.kslices + ks : tm);
-    const int ch0 = SPLIT && ks > 0 ? ends[-1] : 0;
-    const int n = ends[0] - ch0;
+    const int n = ra.counts[tm];
     if (n > 0) {
       // uniform reads through the scalar cache: a vector load would count with
       // the DMAs
       typedef const __attribute__((address_space(4))) uint64_t* Const64;
-      const Const64 list = (Const64)(uintptr_t)(ra.chunks + (long long)tm * ra.stride + ch0);
+      const Const64 list = (Const64)(uintptr_t)(ra.chunks + (long long)tm * ra.stride);
       uint32_t trow[TD], bn[BD];
       int rid[TD], tc[TD], bc[BD];
 #pragma unroll
@@ -763,22 +760,38 @@ __device__ __forceinline__ void qproj_fast_body(const QprojArgs& a) {
 
 template <int BITS, bool SPLIT, int RF, int NW>
 __global__ __launch_bounds__(64 * NW, 1) void qproj_fast_kernel(const QprojArgs a) {
-  qproj_fast_body<BITS, SPLIT, false, RF, NW>(a);
+  qproj_fast_body<BITS, SPLIT, false, RF, NW>(a, (int)blockIdx.x);
 }
 
 template <int BITS, int RF, int NW>
 __global__ __launch_bounds__(64 * NW, 1) void qproj_pair_kernel(const QprojArgs a) {
-  qproj_fast_body<BITS, false, true, RF, NW>(a);
+  qproj_fast_body<BITS, false, true, RF, NW>(a, (int)blockIdx.x);
 }
 
 template <int BITS, bool SPLIT, int RF, int NW>
 __global__ __launch_bounds__(64 * NW, 1) void qproj_merged_kernel(const QprojArgs a) {
-  qproj_fast_body<BITS, SPLIT, false, RF, NW, true>(a);
+  qproj_fast_body<BITS, SPLIT, false, RF, NW, true>(a, (int)blockIdx.x);
 }
 
-template <int BITS, bool SPLIT, int RF, int NW>
+template <int BITS, int RF, int NW>
 __global__ __launch_bounds__(64 * NW, 1) void qproj_rows_kernel(const QprojArgs a) {
-  qproj_fast_body<BITS, SPLIT, false, RF, NW, false, true>(a);
+  qproj_fast_body<BITS, false, false, RF, NW, false, true>(a, (int)blockIdx.x);
+}
+
+// A split projection with its rows' x.A beside it: `first` blocks of that, their
+// latency under the projection's own; the sum of the slices adds what T brings.
+template <int BITS, int RF, int NW>
+__global__ __launch_bounds__(64 * NW, 1) void qproj_split_rows_kernel(const QprojArgs a,
+                                                                      const RowXaArgs r,
+                                                                      int first) {
+  __shared__ floatx4_t red[NW][64];
+  const int b = (int)blockIdx.x;
+  if (b < first) {
+    const int tiles = (r.M + 15) / 16;
+    row_xa_block<NW>(r, b % tiles, b / tiles, first / tiles, red);
+    return;
+  }
+  qproj_fast_body<BITS, true, false, RF, NW>(a, b - first);
 }
 
 // The split projection's end (grid y: the projection of a merged launch): y =
@@ -823,6 +836,64 @@ __global__ void qproj_split_reduce_kernel(const QprojArgs a) {
   range_report(a.range, seen);
 }
 
+// The same with what the rows' own adapters add: y = bf16(sum of the slices in
+// order + T . B_a^T). A wave takes 16 rows x 64 columns; each adapter among the rows
+// is v_mfma_f32_16x16x32_bf16 tiles over all of them, the others' T read as zeros,
+// so a request's B is read once for its rows (a thread's own dot products read it
+// once a row: [500, 3840] of ranks 16 to 64, 14.6 us).
+__global__ __launch_bounds__(256) void qproj_split_rows_reduce_kernel(const QprojArgs a) {
+  const int lane = (int)threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int n0 = (int)blockIdx.x * 64, m0 = (int)blockIdx.y * 64 + 16 * wave, m = m0 + c;
+  if (m0 >= a.M) return;                   // no barrier below
+  const bool row = m < a.M;
+  const int ms = row ? m : a.M - 1;
+  const int id = row ? a.rows.rid[ms] : -1;
+  floatx4_t acc[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) acc[t] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  const uint16_t* const tr = a.rows.t + (long long)ms * a.rows.ldt + 8 * g;
+  uint64_t left = __ballot(id >= 0);
+  while (left) {
+    const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+    left &= ~__ballot(id == cur);
+    const AdapterEntry e = a.rows.table[cur];
+    for (int k = 0; k < e.r8; k += 32) {
+      // past the rank T is zero: any of B's columns will do
+      const int kc = k + 8 * g < e.r8 ? k + 8 * g : e.r8 - 8;
+      uint4 tv = make_uint4(0, 0, 0, 0), bv[4];
+      if (id == cur) tv = *reinterpret_cast<const uint4*>(tr + k);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int n = n0 + 16 * t + c;
+        bv[t] = *reinterpret_cast<const uint4*>(e.B + (long long)(n < a.N ? n : a.N - 1) * e.r8 + kc);
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) acc[t] = mfma_rows(bv[t], tv, acc[t]);
+    }
+  }
+  // lane (row c, g): columns 4g + 0..3 of each 16
+  const size_t plane = (size_t)a.M * (size_t)a.N;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int n = n0 + 16 * t + 4 * g;
+    if (!row || n >= a.N) continue;
+    const float* p = a.part + (size_t)m * a.N + n;
+    float4 sum = *reinterpret_cast<const float4*>(p);
+    for (int k = 1; k < a.kslices; ++k) {
+      p += plane;
+      const float4 v = *reinterpret_cast<const float4*>(p);
+      sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+    }
+    if (id >= 0) {
+      sum.x += acc[t][0]; sum.y += acc[t][1]; sum.z += acc[t][2]; sum.w += acc[t][3];
+    }
+    *reinterpret_cast<uint2*>(a.y + (size_t)m * a.ldy + n) =
+        make_uint2(pack_bf16x2_rne(sum.x, sum.y), pack_bf16x2_rne(sum.z, sum.w));
+  }
+}
+
 // ---- T = x . A_live^T * coef: the adapters' stacked down-projection --------
 // Block tile 64*MR rows x 64*CJ stacked ranks. Four MFMA waves in 2 x 2, each
 // 32*MR rows x 32*CJ ranks (MR x CJ tiles of v_mfma_f32_32x32x16_bf16,
@@ -839,8 +910,8 @@ __global__ void qproj_split_reduce_kernel(const QprojArgs a) {
 // finished every read of stage t (steps 0-2 read it; step 3, after the barrier,
 // reads stage t + 1's first fragments).
 template <int MR, int CJ>
-__global__ __launch_bounds__(512, 1) void lora_xa_fast_kernel(const LoraXaArgs a, float* part,
-                                                              int kslices) {
+__device__ __forceinline__ void lora_xa_fast_body(const LoraXaArgs& a, float* part, int kslices,
+                                                  int block, int blocks) {
   constexpr int XR = 64 * MR, XC = 64 * CJ;      // rows and ranks of the tile
   constexpr int XCH = XR * 8;                    // 16-B chunks of the x tile
   constexpr int STG = XCH + XC * 8;              // x tile + A tile
@@ -856,9 +927,8 @@ __global__ __launch_bounds__(512, 1) void lora_xa_fast_kernel(const LoraXaArgs a
   int m0, c0, ks;
   {
     const int tiles_m = (a.M + XR - 1) / XR, tiles_c = (a.n_cols + XC - 1) / XC;
-    const int nb = (int)gridDim.x;
-    const int q = nb / 8, rem = nb % 8;
-    const int xcd = (int)blockIdx.x % 8, local = (int)blockIdx.x / 8;
+    const int q = blocks / 8, rem = blocks % 8;
+    const int xcd = block % 8, local = block / 8;
     const int v = xcd * q + (xcd < rem ? xcd : rem) + local;
     const int tc = v % tiles_c, rest = v / tiles_c;
     m0 = (rest % tiles_m) * XR;
@@ -1079,6 +1149,27 @@ __global__ __launch_bounds__(512, 1) void lora_xa_fast_kernel(const LoraXaArgs a
       }
     }
   }
+}
+
+template <int MR, int CJ>
+__global__ __launch_bounds__(512, 1) void lora_xa_fast_kernel(const LoraXaArgs a, float* part,
+                                                              int kslices) {
+  lora_xa_fast_body<MR, CJ>(a, part, kslices, (int)blockIdx.x, (int)gridDim.x);
+}
+
+// The dense split with its rows' x.A beside it (qproj_split_rows_kernel).
+template <int MR, int CJ>
+__global__ __launch_bounds__(512, 1) void lora_xa_rows_kernel(const LoraXaArgs a, float* part,
+                                                              int kslices, const RowXaArgs r,
+                                                              int first) {
+  __shared__ floatx4_t red[8][64];
+  const int b = (int)blockIdx.x;
+  if (b < first) {
+    const int tiles = (r.M + 15) / 16;
+    row_xa_block<8>(r, b % tiles, b / tiles, first / tiles, red);
+    return;
+  }
+  lora_xa_fast_body<MR, CJ>(a, part, kslices, b - first, (int)gridDim.x - first);
 }
 
 // T[m][c] = bf16(coef * sum_s P[s][m][c]), slices summed in order 0..S-1,
@@ -1398,14 +1489,46 @@ bool qproj_merge_pays(int M, int N, int K, int nw) {
          0.95 * nw * plan_rows(M, tiles_n, K / BK, false).us;
 }
 
+// Blocks of rows' x.A beside `blocks` of a projection, one a CU: the chip's CUs left
+// over in its last round. 0 where they are fewer than one for every 16 rows: a
+// round of their own takes longer than a launch ([500, 3840] x [3840, 3840] w4: 31.7
+// us beside, 13.4 and 25.5 apart with x's fp16 copy in the first, 5.1 by itself).
+static int row_xa_blocks(int M, int blocks) {
+  const int cus = device_cus(), tiles = (M + 15) / 16;
+  const int free = (blocks + cus - 1) / cus * cus - blocks;
+  const int ny = free / tiles;
+  return tiles * (ny < 32 ? ny : 32);
+}
+
+bool qproj_rows_beside(int M, int N, int kslices, int rf) {
+  return M < kRowXaMany &&
+         row_xa_blocks(M, (M + 32 * rf - 1) / (32 * rf) * ((N + BN - 1) / BN) * kslices) > 0;
+}
+
+bool dense_rows_beside(int M, int N, const DensePlan& p) {
+  const int xr = 64 * p.tile.mr, xc = 64 * p.tile.cj;
+  return M < kRowXaMany &&
+         row_xa_blocks(M, (M + xr - 1) / xr * ((N + xc - 1) / xc) * p.slices) > 0;
+}
+
 template <int BITS, bool SPLIT, int RF, int NW>
-static void launch_tiles(const QprojArgs& a, hipStream_t s) {
+static void launch_tiles(const QprojArgs& a, hipStream_t s, const RowXaArgs* xa = nullptr) {
   const int tiles = ((a.M + 32 * RF - 1) / (32 * RF)) * ((a.N + BN - 1) / BN);
-  const dim3 grid((unsigned)(SPLIT ? tiles * a.kslices : tiles));
-  if (a.rows.counts)
-    hipLaunchKernelGGL((qproj_rows_kernel<BITS, SPLIT, RF, NW>), grid, dim3(64 * NW), 0, s, a);
-  else
-    hipLaunchKernelGGL((qproj_fast_kernel<BITS, SPLIT, RF, NW>), grid, dim3(64 * NW), 0, s, a);
+  const int blocks = SPLIT ? tiles * a.kslices : tiles;
+  if constexpr (SPLIT) {
+    if (xa) {
+      const int first = row_xa_blocks(xa->M, blocks);
+      hipLaunchKernelGGL((qproj_split_rows_kernel<BITS, RF, NW>), dim3((unsigned)(blocks + first)),
+                         dim3(64 * NW), 0, s, a, *xa, first);
+      return;
+    }
+  } else if (a.rows.counts) {
+    hipLaunchKernelGGL((qproj_rows_kernel<BITS, RF, NW>), dim3((unsigned)blocks), dim3(64 * NW), 0,
+                       s, a);
+    return;
+  }
+  hipLaunchKernelGGL((qproj_fast_kernel<BITS, SPLIT, RF, NW>), dim3((unsigned)blocks),
+                     dim3(64 * NW), 0, s, a);
 }
 template <int BITS>
 static void launch_rows(const QprojArgs& a, int rf, hipStream_t s) {
@@ -1417,11 +1540,11 @@ static void launch_rows(const QprojArgs& a, int rf, hipStream_t s) {
   }
 }
 template <int BITS>
-static void launch_split(const QprojArgs& a, hipStream_t s) {
+static void launch_split(const QprojArgs& a, hipStream_t s, const RowXaArgs* xa) {
   switch (a.split_rf) {
-    case 2: launch_tiles<BITS, true, 2, 8>(a, s); break;
-    case 4: launch_tiles<BITS, true, 4, 8>(a, s); break;
-    default: launch_tiles<BITS, true, 8, 4>(a, s); break;
+    case 2: launch_tiles<BITS, true, 2, 8>(a, s, xa); break;
+    case 4: launch_tiles<BITS, true, 4, 8>(a, s, xa); break;
+    default: launch_tiles<BITS, true, 8, 4>(a, s, xa); break;
   }
 }
 template <int BITS, bool SPLIT, int RF, int NW>
@@ -1493,19 +1616,26 @@ static hipError_t launch_plan(const QprojArgs& a, const RowPlan& p, F&& rows) {
   return hipGetLastError();
 }
 
-hipError_t launch_qproj_fast(int bits, const QprojArgs& a, hipStream_t s) {
+hipError_t launch_qproj_fast(int bits, const QprojArgs& a, hipStream_t s, const RowXaArgs* xa) {
   if (a.M <= 0 || a.N <= 0) return hipSuccess;
-  if (bits != 4 && bits != 8) return hipErrorInvalidValue;
+  if ((bits != 4 && bits != 8) || (xa && (a.kslices <= 1 || xa->M != a.M || xa->M >= kRowXaMany)))
+    return hipErrorInvalidValue;
   if (a.kslices > 1) {
     if (!a.part || a.N % 4 != 0 || (long long)a.M * (a.N / 4) >= (1ll << 31) ||
         a.K / BK < a.kslices)
       return hipErrorInvalidValue;
     if (bits == 4)
-      launch_split<4>(a, s);
+      launch_split<4>(a, s, xa);
     else
-      launch_split<8>(a, s);
+      launch_split<8>(a, s, xa);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
+    if (a.rows.rid) {
+      hipLaunchKernelGGL(qproj_split_rows_reduce_kernel,
+                         dim3((unsigned)((a.N + 63) / 64), (unsigned)((a.M + 63) / 64)), dim3(256), 0,
+                         s, a);
+      return hipGetLastError();
+    }
     long long blocks = ((long long)a.M * (a.N / 4) + 255) / 256;
     if (blocks > 4096) blocks = 4096;
     hipLaunchKernelGGL(qproj_split_reduce_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a);
@@ -1678,14 +1808,22 @@ DensePlan dense_split_plan(int M, int N, int K) {
 }
 
 template <int MR, int CJ>
-static hipError_t launch_xa_tiles(const LoraXaArgs& a, float* part, int kslices, hipStream_t s) {
+static hipError_t launch_xa_tiles(const LoraXaArgs& a, float* part, int kslices, hipStream_t s,
+                                  const RowXaArgs* xa) {
   constexpr int XR = 64 * MR, XC = 64 * CJ;
   const long long tiles = (long long)((a.M + XR - 1) / XR) * ((a.n_cols + XC - 1) / XC);
   // the reduce's 32-bit indexing: one thread per two float4s of a slice
   const long long work = tiles * 1024 * MR * CJ;
   if (kslices > 1 && (a.n_cols % 8 != 0 || work >= (1ll << 31))) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((lora_xa_fast_kernel<MR, CJ>), dim3((unsigned)(tiles * kslices)), dim3(512),
-                     0, s, a, part, kslices);
+  const int nb = (int)(tiles * kslices);
+  if (xa) {
+    const int first = row_xa_blocks(xa->M, nb);
+    hipLaunchKernelGGL((lora_xa_rows_kernel<MR, CJ>), dim3((unsigned)(nb + first)), dim3(512), 0, s,
+                       a, part, kslices, *xa, first);
+  } else {
+    hipLaunchKernelGGL((lora_xa_fast_kernel<MR, CJ>), dim3((unsigned)nb), dim3(512), 0, s, a, part,
+                       kslices);
+  }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || kslices == 1) return e;
   long long blocks = (work / 2 + 255) / 256;
@@ -1696,15 +1834,17 @@ static hipError_t launch_xa_tiles(const LoraXaArgs& a, float* part, int kslices,
 }
 
 hipError_t launch_lora_xa_fast(const LoraXaArgs& a, float* part, int kslices,
-                               hipStream_t s) {
+                               hipStream_t s, const RowXaArgs* xa) {
   if (a.M <= 0 || a.n_cols <= 0) return hipSuccess;
+  if (xa && (kslices <= 1 || !a.ident || xa->M != a.M || xa->M >= kRowXaMany))
+    return hipErrorInvalidValue;
   const XaTile t = a.ident ? a.tile : xa_tile(a.M, a.n_cols, a.K, kslices);
   switch (10 * t.mr + t.cj) {
-    case 11: return launch_xa_tiles<1, 1>(a, part, kslices, s);
-    case 12: return launch_xa_tiles<1, 2>(a, part, kslices, s);
-    case 21: return launch_xa_tiles<2, 1>(a, part, kslices, s);
-    case 22: return launch_xa_tiles<2, 2>(a, part, kslices, s);
-    case 42: return launch_xa_tiles<4, 2>(a, part, kslices, s);
+    case 11: return launch_xa_tiles<1, 1>(a, part, kslices, s, xa);
+    case 12: return launch_xa_tiles<1, 2>(a, part, kslices, s, xa);
+    case 21: return launch_xa_tiles<2, 1>(a, part, kslices, s, xa);
+    case 22: return launch_xa_tiles<2, 2>(a, part, kslices, s, xa);
+    case 42: return launch_xa_tiles<4, 2>(a, part, kslices, s, xa);
     default: return hipErrorInvalidValue;
   }
 }
@@ -1767,22 +1907,28 @@ hipError_t validate_qproj_fast_kernels() {
                        reinterpret_cast<const void*>(&qproj_fast_kernel<8, true, 8, 4>),
                        reinterpret_cast<const void*>(&qproj_pair_kernel<8, 4, 8>),
                        reinterpret_cast<const void*>(&qproj_pair_kernel<8, 6, 8>),
-#define MING_QPROJ_ROWS(BITS)                                              \
-  reinterpret_cast<const void*>(&qproj_rows_kernel<BITS, false, 2, 8>),    \
-      reinterpret_cast<const void*>(&qproj_rows_kernel<BITS, false, 4, 8>), \
-      reinterpret_cast<const void*>(&qproj_rows_kernel<BITS, false, 6, 8>), \
-      reinterpret_cast<const void*>(&qproj_rows_kernel<BITS, false, 8, 4>), \
-      reinterpret_cast<const void*>(&qproj_rows_kernel<BITS, true, 2, 8>), \
-      reinterpret_cast<const void*>(&qproj_rows_kernel<BITS, true, 4, 8>), \
-      reinterpret_cast<const void*>(&qproj_rows_kernel<BITS, true, 8, 4>)
+#define MING_QPROJ_ROWS(BITS)                                             \
+  reinterpret_cast<const void*>(&qproj_rows_kernel<BITS, 2, 8>),          \
+      reinterpret_cast<const void*>(&qproj_rows_kernel<BITS, 4, 8>),      \
+      reinterpret_cast<const void*>(&qproj_rows_kernel<BITS, 6, 8>),      \
+      reinterpret_cast<const void*>(&qproj_rows_kernel<BITS, 8, 4>),      \
+      reinterpret_cast<const void*>(&qproj_split_rows_kernel<BITS, 2, 8>), \
+      reinterpret_cast<const void*>(&qproj_split_rows_kernel<BITS, 4, 8>), \
+      reinterpret_cast<const void*>(&qproj_split_rows_kernel<BITS, 8, 4>)
                        MING_QPROJ_ROWS(4), MING_QPROJ_ROWS(8),
 #undef MING_QPROJ_ROWS
                        reinterpret_cast<const void*>(&qproj_split_reduce_kernel),
+                       reinterpret_cast<const void*>(&qproj_split_rows_reduce_kernel),
                        reinterpret_cast<const void*>(&repack_fast_kernel),
                        reinterpret_cast<const void*>(&repack_sbf_kernel),
                        reinterpret_cast<const void*>(&bf16_to_f16_kernel),
                        reinterpret_cast<const void*>(&qproj_pair_kernel<4, 8, 4>),
                        reinterpret_cast<const void*>(&qproj_pair_kernel<8, 8, 4>),
+                       reinterpret_cast<const void*>(&lora_xa_rows_kernel<1, 1>),
+                       reinterpret_cast<const void*>(&lora_xa_rows_kernel<1, 2>),
+                       reinterpret_cast<const void*>(&lora_xa_rows_kernel<2, 1>),
+                       reinterpret_cast<const void*>(&lora_xa_rows_kernel<2, 2>),
+                       reinterpret_cast<const void*>(&lora_xa_rows_kernel<4, 2>),
                        reinterpret_cast<const void*>(&lora_xa_fast_kernel<1, 1>),
                        reinterpret_cast<const void*>(&lora_xa_reduce_kernel<1, 1>),
                        reinterpret_cast<const void*>(&lora_xa_fast_kernel<1, 2>),

@@ -995,16 +995,17 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
   };
   // T of every row's adapter, then (plane) the f32 plane; the projections follow
   ming::RowXaArgs xr{};
-  auto rows_launch = [&](float* plane, int N) {
+  auto rows_args = [&] {
     xr.x = x; xr.ldx = ldx; xr.M = M; xr.K = K;
     xr.ids = rows->ids; xr.scale = rows->scale;
     xr.table = ra.table; xr.cap = rows->bank->cap;
     xr.rid = const_cast<int32_t*>(ra.rid); xr.t = const_cast<uint16_t*>(ra.t); xr.ldt = ra.ldt;
+  };
+  auto rows_launch = [&](float* plane, int N) {
+    rows_args();
     MING_HIP(profiled(c, kBRowXa, 0.0, 2.0 * M * K,
                       [&] { return ming::launch_row_xa(xr, c->stream); }),
              "row adapters' x.A launch");
-    c->eng.lora_xa += 1;
-    c->eng.lora_proj += 1;
     if (plane)
       MING_HIP(profiled(c, kBRowXa, 0.0, 4.0 * M * N,
                         [&] { return ming::launch_row_delta(ra, M, N, plane, c->stream); }),
@@ -1032,6 +1033,8 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
         ra.rid = (const int32_t*)carve->take((size_t)M * 4);
         ra.t = (const uint16_t*)carve->take((size_t)(M + 1) * ra.ldt * 2);
         if (const int rc = rows_launch(nullptr, qs[0]->N)) return rc;
+        c->eng.lora_xa += 1;
+        c->eng.lora_proj += 1;
       }
       for (int i = 0; i < n; ++i) {
         const ming_qweight* q = qs[i];
@@ -1250,19 +1253,19 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
   float* part = nullptr;
   uint16_t* up = nullptr;
   float* plane = nullptr;
+  bool rows_beside = false;
   const uint16_t* xh = xh_src;
   if (carve && rows) {
     // The tile kernels take the rows' adapters as a tail over lists of their
-    // chunks, one a row tile; the dense split's sum adds them up itself; the other
-    // launches take an f32 plane.
-    const bool tail = fast[0] || dense_rf[0] > 0;
+    // chunks, one a row tile; the sum of a K split adds them up itself, with few
+    // rows after blocks for their x.A beside the split's own; the other launches
+    // take an f32 plane.
+    const bool split = fast[0] ? split_ks[0] >= 2 : dense_plan[0].slices >= 2;
+    const bool tail = !split && (fast[0] || dense_rf[0] > 0);
     size_t plane_bytes = 0, list_bytes = 0, count_bytes = 0;
     if (tail) {
       ming::RowPlan rp{0, 2 * dense_rf[0], 0.0};
-      if (fast[0])
-        rp = split_ks[0] >= 2
-                 ? ming::RowPlan{0, qa[0].split_rf, 0.0}
-                 : ming::plan_rows(M, (qs[0]->N + 255) / 256, K / 64, false);
+      if (fast[0]) rp = ming::plan_rows(M, (qs[0]->N + 255) / 256, K / 64, false);
       xr.rows_main = rp.rows_main / 256 * 256;
       xr.rest = 32 * rp.rf_rest;
       const int tiles = ming::row_tiles(M, xr.rows_main, xr.rest);
@@ -1270,9 +1273,8 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
       const int most = std::max(xr.rows_main > 0 ? 256 : 0, xr.rest);
       xr.stride = std::min({most, M, rows->bank->cap}) * (ra.ldt / 32);
       list_bytes = (size_t)tiles * xr.stride * sizeof(ming::RowChunk);
-      xr.slices = fast[0] && split_ks[0] >= 2 ? split_ks[0] : 1;
-      count_bytes = (size_t)tiles * xr.slices * 4;
-    } else if (dense_plan[0].slices < 2) {
+      count_bytes = (size_t)tiles * 4;
+    } else if (!split) {
       plane_bytes = (size_t)M * qs[0]->N * 4;
     }
     const size_t need = rows_need + Carve::aligned256(plane_bytes) +
@@ -1290,8 +1292,11 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
       ra.counts = xr.counts;
       ra.stride = xr.stride;
       ra.zero = (uint32_t)((size_t)M * ra.ldt * 2);
-      qa[0].rows = ra;
     }
+    rows_beside = split && (fast[0] ? ming::qproj_rows_beside(M, qs[0]->N, split_ks[0],
+                                                              qa[0].split_rf)
+                                    : ming::dense_rows_beside(M, qs[0]->N, dense_plan[0]));
+    if (!plane) qa[0].rows = ra;
     if (xh_bytes) xh = (const uint16_t*)carve->take(xh_bytes);
     if (part_bytes) part = (float*)carve->take(part_bytes);
   } else if (carve) {
@@ -1327,6 +1332,12 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
   // write the fp16 copy as they go, in place of the conversion launch.
   const bool xh_in_xa = need_xh && t_cols > 0 && xa_fast;
   if (rows) {
+    c->eng.lora_xa += 1;
+    c->eng.lora_proj += 1;
+  }
+  if (rows_beside) {
+    rows_args();
+  } else if (rows) {
     if (need_xh) {
       // the rows' x.A reads every element of x: it writes the fp16 copy too
       xr.xh = const_cast<uint16_t*>(xh);
@@ -1354,7 +1365,7 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
              "lora_xa launch");
     c->eng.lora_xa += 1;
   }
-  if (need_xh && !xh_in_xa && !rows) {
+  if (need_xh && !xh_in_xa && (!rows || rows_beside)) {
     uint16_t* dst = const_cast<uint16_t*>(xh);
     MING_HIP(profiled(c, kBCvt, 0.0, 4.0 * M * K,
                       [&] { return ming::launch_bf16_to_f16(x, ldx, dst, K, M, K,
@@ -1486,13 +1497,17 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
       da.ident = true; da.tile = dense_plan[i].tile;
       const int dks = dense_plan[i].slices;
       MING_HIP(profiled(c, bk, base_flops, 2.0 * M * K + wbytes + 2.0 * M * q->N,
-                        [&] { return ming::launch_lora_xa_fast(da, part, dks, c->stream); }),
+                        [&] {
+                          return ming::launch_lora_xa_fast(da, part, dks, c->stream,
+                                                           rows_beside ? &xr : nullptr);
+                        }),
                "dense split-K launch");
     } else {
       MING_HIP(profiled(c, bk, base_flops + tail_flops[i],
                         2.0 * M * K + wbytes + 2.0 * M * q->N,
                         [&] {
-                          return fast[i]       ? ming::launch_qproj_fast(q->bits, a, c->stream)
+                          return fast[i]       ? ming::launch_qproj_fast(q->bits, a, c->stream,
+                                                                         rows_beside ? &xr : nullptr)
                                  : dense_rf[i] ? ming::launch_dense_fast(a, dense_rf[i], c->stream)
                                                : ming::launch_qproj(q->bits, a, c->stream,
                                                                     c->route == MING_ROUTE_WIDE);
