@@ -909,7 +909,9 @@ __global__ __launch_bounds__(256) void qproj_split_rows_reduce_kernel(const Qpro
 // t - 1 left and wait until stage t + 1 has landed; the MFMA waves have then
 // finished every read of stage t (steps 0-2 read it; step 3, after the barrier,
 // reads stage t + 1's first fragments).
-template <int MR, int CJ>
+//
+// ROWS: the outputs also take a.delta (a dense weight's one slice).
+template <int MR, int CJ, bool ROWS>
 __device__ __forceinline__ void lora_xa_fast_body(const LoraXaArgs& a, float* part, int kslices,
                                                   int block, int blocks) {
   constexpr int XR = 64 * MR, XC = 64 * CJ;      // rows and ranks of the tile
@@ -1130,15 +1132,17 @@ __device__ __forceinline__ void lora_xa_fast_body(const LoraXaArgs& a, float* pa
         uint2 v;
         if (f == 0.0f) {
           v = make_uint2(0, 0);
-        } else if (a.bias || a.delta) {
-          // the dense split-K GEMM with a bias or its rows' adapters (coef 1):
-          // one rounding
+        } else if (ROWS && a.delta) {
+          // the dense split-K GEMM with its rows' adapters (coef 1): one rounding
+          const float4 d =
+              *reinterpret_cast<const float4*>(a.delta + (long long)m * a.n_cols + c);
+          v.x = pack_bf16x2_rne(acc[i][j][4 * q + 0] + d.x, acc[i][j][4 * q + 1] + d.y);
+          v.y = pack_bf16x2_rne(acc[i][j][4 * q + 2] + d.z, acc[i][j][4 * q + 3] + d.w);
+        } else if (a.bias) {
+          // the dense split-K GEMM with a bias (coef 1): one rounding
           float r[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            r[e] = f * acc[i][j][4 * q + e] +
-                   (a.bias ? bf16_to_f32(a.bias[c + e])
-                           : a.delta[(long long)m * a.n_cols + c + e]);
+          for (int e = 0; e < 4; ++e) r[e] = f * acc[i][j][4 * q + e] + bf16_to_f32(a.bias[c + e]);
           v.x = pack_bf16x2_rne(r[0], r[1]);
           v.y = pack_bf16x2_rne(r[2], r[3]);
         } else {
@@ -1154,10 +1158,11 @@ __device__ __forceinline__ void lora_xa_fast_body(const LoraXaArgs& a, float* pa
 template <int MR, int CJ>
 __global__ __launch_bounds__(512, 1) void lora_xa_fast_kernel(const LoraXaArgs a, float* part,
                                                               int kslices) {
-  lora_xa_fast_body<MR, CJ>(a, part, kslices, (int)blockIdx.x, (int)gridDim.x);
+  lora_xa_fast_body<MR, CJ, false>(a, part, kslices, (int)blockIdx.x, (int)gridDim.x);
 }
 
-// The dense split with its rows' x.A beside it (qproj_split_rows_kernel).
+// The dense split with what its rows' adapters add; several slices: their x.A beside
+// it, in the first `first` blocks (qproj_split_rows_kernel).
 template <int MR, int CJ>
 __global__ __launch_bounds__(512, 1) void lora_xa_rows_kernel(const LoraXaArgs a, float* part,
                                                               int kslices, const RowXaArgs r,
@@ -1169,7 +1174,7 @@ __global__ __launch_bounds__(512, 1) void lora_xa_rows_kernel(const LoraXaArgs a
     row_xa_block<8>(r, b % tiles, b / tiles, first / tiles, red);
     return;
   }
-  lora_xa_fast_body<MR, CJ>(a, part, kslices, b - first, (int)gridDim.x - first);
+  lora_xa_fast_body<MR, CJ, true>(a, part, kslices, b - first, (int)gridDim.x - first);
 }
 
 // T[m][c] = bf16(coef * sum_s P[s][m][c]), slices summed in order 0..S-1,
@@ -1180,7 +1185,8 @@ __global__ __launch_bounds__(512, 1) void lora_xa_rows_kernel(const LoraXaArgs a
 // coalesced), one 16-byte store of T. Positions of row tiles past M or
 // column blocks past n_cols are skipped. 32-bit indices (the host keeps a
 // slice's float4 count below 2^31).
-template <int MR, int CJ>
+// ROWS: plus what the rows' own adapters add (a dense weight's split).
+template <int MR, int CJ, bool ROWS>
 __global__ void lora_xa_reduce_kernel(const float* part, int kslices, int M,
                                       int n_cols, const LoraXaArgs a) {
   constexpr unsigned XR = 64 * MR, XC = 64 * CJ, FR = 4 * MR * CJ;
@@ -1210,16 +1216,16 @@ __global__ void lora_xa_reduce_kernel(const float* part, int kslices, int M,
     }
     const float co = a.ident ? 1.0f : a.coef[c >> 3];
     uint4 o = make_uint4(0, 0, 0, 0);
-    if (co != 0.0f && (a.bias || a.rows.rid)) {
+    if (ROWS || (co != 0.0f && a.bias)) {
       // the dense split-K GEMM with a bias or its rows' adapters (coef 1): one
       // rounding
       float r[8] = {co * s0.x, co * s0.y, co * s0.z, co * s0.w,
                     co * s1.x, co * s1.y, co * s1.z, co * s1.w};
-      if (a.bias) {
+      if constexpr (ROWS) {
+        add_row_adapter(a.rows, (int)m, (int)c, r);
+      } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) r[e] += bf16_to_f32(a.bias[c + e]);
-      } else {
-        add_row_adapter(a.rows, (int)m, (int)c, r);
       }
       o.x = pack_bf16x2_rne(r[0], r[1]);
       o.y = pack_bf16x2_rne(r[2], r[3]);
@@ -1816,10 +1822,10 @@ static hipError_t launch_xa_tiles(const LoraXaArgs& a, float* part, int kslices,
   const long long work = tiles * 1024 * MR * CJ;
   if (kslices > 1 && (a.n_cols % 8 != 0 || work >= (1ll << 31))) return hipErrorInvalidValue;
   const int nb = (int)(tiles * kslices);
-  if (xa) {
-    const int first = row_xa_blocks(xa->M, nb);
+  if (xa || a.delta) {
+    const int first = xa ? row_xa_blocks(xa->M, nb) : 0;
     hipLaunchKernelGGL((lora_xa_rows_kernel<MR, CJ>), dim3((unsigned)(nb + first)), dim3(512), 0, s,
-                       a, part, kslices, *xa, first);
+                       a, part, kslices, xa ? *xa : RowXaArgs{}, first);
   } else {
     hipLaunchKernelGGL((lora_xa_fast_kernel<MR, CJ>), dim3((unsigned)nb), dim3(512), 0, s, a, part,
                        kslices);
@@ -1828,8 +1834,12 @@ static hipError_t launch_xa_tiles(const LoraXaArgs& a, float* part, int kslices,
   if (e != hipSuccess || kslices == 1) return e;
   long long blocks = (work / 2 + 255) / 256;
   if (blocks > 4096) blocks = 4096;
-  hipLaunchKernelGGL((lora_xa_reduce_kernel<MR, CJ>), dim3((unsigned)blocks), dim3(256), 0, s,
-                     part, kslices, a.M, a.n_cols, a);
+  if (a.rows.rid)
+    hipLaunchKernelGGL((lora_xa_reduce_kernel<MR, CJ, true>), dim3((unsigned)blocks), dim3(256), 0, s,
+                       part, kslices, a.M, a.n_cols, a);
+  else
+    hipLaunchKernelGGL((lora_xa_reduce_kernel<MR, CJ, false>), dim3((unsigned)blocks), dim3(256), 0,
+                       s, part, kslices, a.M, a.n_cols, a);
   return hipGetLastError();
 }
 
@@ -1930,15 +1940,20 @@ hipError_t validate_qproj_fast_kernels() {
                        reinterpret_cast<const void*>(&lora_xa_rows_kernel<2, 2>),
                        reinterpret_cast<const void*>(&lora_xa_rows_kernel<4, 2>),
                        reinterpret_cast<const void*>(&lora_xa_fast_kernel<1, 1>),
-                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<1, 1>),
+                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<1, 1, false>),
+                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<1, 1, true>),
                        reinterpret_cast<const void*>(&lora_xa_fast_kernel<1, 2>),
-                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<1, 2>),
+                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<1, 2, false>),
+                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<1, 2, true>),
                        reinterpret_cast<const void*>(&lora_xa_fast_kernel<2, 1>),
-                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<2, 1>),
+                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<2, 1, false>),
+                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<2, 1, true>),
                        reinterpret_cast<const void*>(&lora_xa_fast_kernel<2, 2>),
-                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<2, 2>),
+                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<2, 2, false>),
+                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<2, 2, true>),
                        reinterpret_cast<const void*>(&lora_xa_fast_kernel<4, 2>),
-                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<4, 2>)};
+                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<4, 2, false>),
+                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<4, 2, true>)};
   for (const void* f : fns) {
     const hipError_t e = hipFuncGetAttributes(&fa, f);
     if (e != hipSuccess) return e;
