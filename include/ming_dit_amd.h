@@ -338,7 +338,8 @@ int ming_ln_modulate(ming_ctx* ctx, const uint16_t* x, int64_t ldx,
  * captured, and a replay takes the choices that are in memory then. Scratch is
  * the caller's (ws, 16-byte aligned, at least the bytes the size function
  * names; it holds nothing between calls, and calls or graphs that may run at
- * the same time need one each). Strides in elements.
+ * the same time need one each). Strides in elements. A call of no rows does
+ * nothing; one of more than a launch holds (2^32 threads) is MING_ERR_SHAPE.
  *
  * The router: per row of logits [rows][ld] (f32 when logits_f32, else bf16)
  * the scores s = softmax(l) or sigmoid(l) over n_experts, the keys s + bias
@@ -352,7 +353,7 @@ int ming_ln_modulate(ming_ctx* ctx, const uint16_t* x, int64_t ldx,
  * left ends in ids of -1 with weights of 0. A logit of +inf counts as the
  * largest finite one. Scores, keys and sums are in f64. n_experts <= 1024, a
  * multiple of n_groups <= 64; top_k <= 64 and <= the experts of top_groups
- * groups. */
+ * groups; rows below 2^26. ids and weights share memory with nothing else. */
 #define MING_SCORE_SOFTMAX 0
 #define MING_SCORE_SIGMOID 1
 int ming_topk_route(ming_ctx* ctx, const void* logits, int64_t ld, int logits_f32,
@@ -365,7 +366,8 @@ int ming_topk_route(ming_ctx* ctx, const void* logits, int64_t ld, int logits_f3
  * offsets [n_groups + 1]: group g is places offsets[g] .. offsets[g + 1] - 1;
  * order [n]: the entry at each place; place [n]: each entry's place. Entries
  * whose id is outside [0, n_groups) are in no group: their place is -1, and so
- * is order from offsets[n_groups] on. n_groups <= 1024, n <= 2^30. */
+ * is order from offsets[n_groups] on. n_groups <= 1024, n <= 2^30. No two of the
+ * arrays share memory. */
 size_t ming_group_rows_workspace_bytes(int n, int n_groups);
 int ming_group_rows(ming_ctx* ctx, const int32_t* ids, int n, int n_groups, int32_t* offsets,
                     int32_t* order, int32_t* place, void* ws, size_t ws_bytes);
@@ -394,8 +396,8 @@ int ming_experts_shape(const ming_experts* ex, int* n_experts, int* N, int* K, i
  * itself where order is NULL (x already in place order). Rows of y from
  * offsets[n_experts] on are left as they were. x [x_rows][ldx], 16-byte
  * aligned, ldx % 8 == 0, x_rows * ldx below 2^30; y [n][ldy], 16-byte aligned,
- * ldy % 8 == 0; they share no memory. Quantized stacks multiply fp16
- * activations from some rows an expert on, with ming_lin's range rule (see
+ * ldy % 8 == 0; none of x, order and offsets shares memory with y or ws, or y with
+ * ws. Quantized stacks multiply fp16 activations from some rows an expert on, with ming_lin's range rule (see
  * MING_ERR_RANGE); on the general and the wide route they take bf16 ones at
  * any size, and more time. */
 size_t ming_experts_workspace_bytes(const ming_experts* ex, int x_rows);
@@ -409,7 +411,8 @@ int ming_experts_swiglu(ming_ctx* ctx, const ming_experts* ex, const uint16_t* x
 /* The expert rows back to their tokens: out[t] = bf16(add[t] + sum over j <
  * top_k of weights[t][j] * y[place[t * top_k + j]]), f32, j in order, one
  * rounding. A place outside [0, n) adds nothing. add [tokens][ldadd] may be NULL
- * or out itself. N, strides multiples of 8, 16-byte aligned. */
+ * or out itself (with ldo), else nothing shares memory with out. N, strides
+ * multiples of 8, 16-byte aligned. */
 int ming_experts_combine(ming_ctx* ctx, const uint16_t* y, int64_t ldy, int n,
                          const int32_t* place, const float* weights, int tokens, int top_k,
                          const uint16_t* add, int64_t ldadd, uint16_t* out, int64_t ldo, int N);
@@ -437,7 +440,10 @@ int ming_adapters_rank(const ming_adapters* bank, int id);
  * is 0, is ming_lin's row without adapters. The adapters' sum joins the f32
  * result before the one rounding; a row's bits do not depend on the other rows'
  * adapters (but for the sign of a zero). Slots bound on the weight take no part.
- * x and y as ming_lin's; they share no memory. */
+ * x as ming_lin's, y 16-byte aligned with ldy % 8 == 0; none of x, row_adapter and
+ * row_scale shares memory with y or ws. The size is that of x rows beside each
+ * other; a dense projection of x rows that span more than 2 GiB may need more, and
+ * says how much (MING_ERR_SHAPE). */
 size_t ming_lin_adapters_workspace_bytes(ming_ctx* ctx, const ming_qweight* qw,
                                          const ming_adapters* bank, int M);
 int ming_lin_adapters(ming_ctx* ctx, const ming_qweight* qw, const ming_adapters* bank,

@@ -8,7 +8,8 @@ import torch
 
 import ming_dit_amd as m
 import rows_ref as ref
-from helpers import bf16, f32, from_dev, make_weight, randn, sync, to_dev
+from helpers import (bf16, dense_plan, f32, from_dev, make_weight, plan_rows, randn, split_plan,
+                     sync, to_dev)
 
 pytestmark = pytest.mark.gpu
 SENTINEL = 0x4242
@@ -289,6 +290,126 @@ def test_set_replaces_and_clear_empties(ctx):
     bank.set(1, to_dev(A), to_dev(B), 1.0, on_device=True)
     held[1] = (f32(A), f32(B), 1.0)
     check(call(ctx, qw, bank, x, ids, None), x, w, held, ids, None, 4)
+    bank.close()
+    qw.close()
+
+
+@pytest.mark.parametrize("bits", [4, 8, 16])
+@pytest.mark.parametrize("M,N,K,ranks", [
+    (900, 264, 320, (16, 4, 32, 8, 7)),              # x.A of two chunks a pass
+    (800, 136, 576, tuple(8 + i % 57 for i in range(70))),   # many adapters, many passes
+    (768, 72, 4160, RANKS), (767, 72, 4160, RANKS),  # many K steps, the last one short
+    (5, 72, 4160, RANKS), (40, 72, 4160, RANKS),
+    (900, 512, 4096, RANKS), (760, 512, 4096, RANKS), (60, 2048, 1088, (512, 130, 1))])
+def test_large_and_long(ctx, bits, M, N, K, ranks):
+    """Both forms of the down-projection with K past one reading of it, and with
+    more chunks than a pass holds; splits too wide for blocks beside them."""
+    qw, w = weight(ctx, 16300, N, K, bits)
+    bank, held = make_bank(ctx, 16400, N, K, ranks)
+    x = bf16(randn(16500 + M, (M, K)))
+    ids, s = requests(M, N, len(ranks), cuts=min(M, 2 * len(ranks)))
+    check(call(ctx, qw, bank, x, ids, s, padx=8), x, w, held, ids, s, bits)
+    bank.close()
+    qw.close()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("M,tiles,stages", [(3460, 41, 6), (6560, 22, 6)])
+def test_rows_in_two_heights(ctx, bits, M, tiles, stages):
+    """A plan of full tiles and a rest of lower ones: requests across the seam."""
+    N, K = 256 * tiles - 32, 64 * stages
+    p = plan_rows(M, tiles, stages, False)
+    assert 0 < p.rows_main < M and split_plan(M, N, K)[0] < 2
+    qw, w = weight(ctx, 16600, N, K, bits)
+    bank, held = make_bank(ctx, 16700, N, K, RANKS)
+    x = bf16(randn(16800, (M, K)))
+    ids, s = requests(M, 3, len(RANKS), cuts=9)
+    seam = p.rows_main
+    ids[seam - 20:seam + 30], s[seam - 20:seam + 30] = 4, 0.7
+    got = call(ctx, qw, bank, x, ids, s)
+    some = np.unique(np.concatenate([np.arange(0, M, 61), np.arange(seam - 40, seam + 50), [M - 1]]))
+    check(got[some], x[some], w, held, ids[some], s[some], bits)
+    bank.close()
+    qw.close()
+
+
+@pytest.mark.parametrize("M,N,K", [(40, 64, 64), (600, 128, 192), (1500, 192, 576),
+                                   (3000, 1024, 1024), (3000, 192, 4096), (1500, 320, 4096)])
+def test_dense_splits(ctx, M, N, K):
+    """Narrow dense weights: one slice takes what the adapters add as a plane,
+    several add it in their sum."""
+    qw, w = weight(ctx, 16900, N, K, 16)
+    assert dense_plan(M, N, K)[2] >= 1
+    bank, held = make_bank(ctx, 17000, N, K, RANKS)
+    x = bf16(randn(17100 + M, (M, K)))
+    ids, s = requests(M, 5, len(RANKS), cuts=12)
+    some = np.unique(np.concatenate([np.arange(0, M, 7), [M - 1]]))
+    got = call(ctx, qw, bank, x, ids, s)[some]
+    check(got, x[some], w, held, ids[some], s[some], 16)
+    bank.close()
+    qw.close()
+
+
+def test_two_contexts_at_once(ctx):
+    """Calls on two streams, a workspace each, over one x: the bits of one alone."""
+    N, K, M = 1024, 2048, 200
+    x = to_dev(bf16(randn(17200, (M, K))))
+    ids = torch.arange(M, dtype=torch.int32, device="cuda") % 3
+    got = []
+    held = []
+    for i in range(2):
+        s = torch.cuda.Stream()
+        c = m.Ctx(0, s.cuda_stream)
+        qw, _ = weight(c, 17300, N, K, 4)
+        bank, _ = make_bank(c, 17400, N, K, (16, 40, 8))
+        y = to_dev(np.zeros((M, N), np.uint16))
+        ws = torch.empty(c.lin_adapters_workspace_bytes(qw, bank, M), dtype=torch.uint8,
+                         device="cuda")
+        held.append((s, c, qw, bank, y, ws))
+    sync()
+    for _ in range(20):
+        for _, c, qw, bank, y, ws in held:
+            c.lin_adapters(qw, bank, x, y, M, ids, None, ws)
+    sync()
+    for _, c, qw, bank, y, ws in held:
+        got.append(from_dev(y))
+        y.zero_()
+    sync()
+    for i, (_, c, qw, bank, y, ws) in enumerate(held):
+        c.lin_adapters(qw, bank, x, y, M, ids, None, ws)
+        c.synchronize()
+        assert np.array_equal(from_dev(y), got[i])
+        bank.close()
+        qw.close()
+        c.close()
+    assert np.array_equal(got[0], got[1])
+
+
+def test_shared_memory_is_refused(ctx):
+    """Blocks resolve their rows by themselves while others store: what they read
+    may not be what they write. Columns beside each other are not shared."""
+    N, K, M = 64, 64, 20
+    qw, w = weight(ctx, 17500, N, K, 16)
+    bank, held = make_bank(ctx, 17600, N, K, (8, 24))
+    x = bf16(randn(17700, (M, K)))
+    both = np.zeros((M, K + N), np.uint16)
+    both[:, :K] = x
+    xy = to_dev(both)
+    ids, s = torch.arange(M, dtype=torch.int32, device="cuda") % 2, torch.ones(M, device="cuda")
+    need = ctx.lin_adapters_workspace_bytes(qw, bank, M)
+    ws = torch.zeros(need + 4096, dtype=torch.uint8, device="cuda")
+    ok = dict(qw=qw, bank=bank, x=xy, y=xy.data_ptr() + 2 * K, M=M, row_adapter=ids,
+              row_scale=s, ws=ws, ldx=K + N, ldy=K + N)
+    sync()
+    ctx.lin_adapters(**ok)
+    ctx.synchronize()
+    check(from_dev(xy)[:, K:], x, w, held, from_dev(ids), from_dev(s), 16)
+    inside = ws[256:256 + 4 * M].view(torch.int32)
+    for kw in ({"y": xy.data_ptr() + 2 * K - 16}, {"row_adapter": inside}, {"row_scale": inside},
+               {"y": ws}, {"x": ws}, {"y": ids, "ldy": N}, {"y": s, "ldy": N},
+               {"ldy": K + N + 4}, {"y": xy.data_ptr() + 2 * K + 8}):
+        with pytest.raises(m.MingError, match="share|16-byte"):
+            ctx.lin_adapters(**dict(ok, **kw))
     bank.close()
     qw.close()
 

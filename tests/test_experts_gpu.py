@@ -312,6 +312,44 @@ def test_products_refusals(ctx):
     ex.close()
 
 
+@pytest.mark.parametrize("bits,kernel", [(16, 0), (16, 2), (4, 2)])
+def test_shared_memory_and_sizes(ctx, cut, bits, kernel):
+    """What every block reads may not be what others write; columns beside each
+    other may. Calls of nothing, and of more than a launch holds."""
+    E, N, K, n = 2, 64, 64, 20
+    ex, w = ref.make_experts(ctx, 13200, E, N, K, bits)
+    cut(kernel)
+    offsets, order, src = ref.plan_of([12, 8], x_rows=n)
+    x = bf16(randn(13300, (n, K)))
+    both = np.zeros((n, K + N), np.uint16)
+    both[:, :K] = x
+    xy, od, fd = to_dev(both), to_dev(order), to_dev(offsets)
+    ws = torch.zeros(ex.workspace_bytes(n) + 4096, dtype=torch.uint8, device="cuda")
+    # 2^31 places of 2^16 columns: 2^32 tiles and more
+    wide, _ = ref.make_experts(ctx, 13400, 1, 1 << 16, 64, bits)
+    ok = dict(ex=ex, x=xy, x_rows=n, order=od, offsets=fd, n=n, y=xy.data_ptr() + 2 * K, ws=ws,
+              ldx=K + N, ldy=K + N)
+    sync()
+    ctx.experts_lin(**ok)
+    ctx.synchronize()
+    check(from_dev(xy)[:, K:], w, x, offsets, src, False, bits)
+    bad = [{"y": xy.data_ptr() + 2 * K - 16}, {"order": xy.data_ptr() + 2 * K},
+           {"offsets": xy.data_ptr() + 2 * K + 4}]
+    if ex.workspace_bytes(n):
+        bad += [{"order": ws}, {"offsets": ws}, {"y": ws}, {"x": ws}]
+    for kw in bad:
+        with pytest.raises(m.MingError, match="share"):
+            ctx.experts_lin(**dict(ok, **kw))
+    if kernel:
+        with pytest.raises(m.MingError, match="launch"):
+            ctx.experts_lin(**dict(ok, n=2 ** 31 - 1, y=1 << 60, ldy=1 << 20, ex=wide))
+    with pytest.raises(m.MingError, match="2\\^30"):
+        ctx.experts_lin(**dict(ok, ldx=1 << 62))
+    ctx.experts_lin(ex, None, 0, None, None, 0, None)
+    wide.close()
+    ex.close()
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 def test_create_refusals(ctx, bits):
     pack, _ = ref.stack(12800, 2, 16, 64, bits)

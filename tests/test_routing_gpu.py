@@ -116,6 +116,36 @@ def test_route_refusals(ctx):
     assert bool((ids == -7).all())
 
 
+def test_route_shared_memory_and_sizes(ctx):
+    l = to_dev(randn(9501, (16, 64)))
+    ids, w = _i32(64), torch.zeros(64, device="cuda")
+    sync()
+    for kw in ({"ids": l}, {"weights": l}, {"ids": w}, {"bias": w, "weights": w},
+               {"rows": 1 << 26}):
+        a = dict(logits=l, rows=16, n_experts=64, top_k=4, ids=ids, weights=w)
+        a.update(kw)
+        with pytest.raises(m.MingError, match="share|2\\^26"):
+            ctx.topk_route(**a)
+    none = torch.zeros((0, 64), device="cuda")            # has no address
+    ctx.topk_route(none, 0, 64, 4, none, none)
+
+
+@pytest.mark.parametrize("E,k", [(1024, 64), (1000, 64), (65, 64), (1, 1)])
+def test_route_largest_and_smallest(ctx, E, k):
+    """All of a wave's lanes hold a choice; scores that tie across registers."""
+    for rows, seed in ((1, 0), (5, 1)):
+        l = np.round(randn(9600 + E + seed, (rows, E), 3.0) * 4) / 4
+        l[:, ::7] = l[:, :1]
+        ids, w = _i32(rows * k), torch.zeros((rows, k), device="cuda")
+        ld = to_dev(l.astype(np.float32))
+        sync()
+        ctx.topk_route(ld, rows, E, k, ids, w)
+        ctx.synchronize()
+        wid, ww = ref.route(l.astype(np.float32), k)
+        assert np.array_equal(from_dev(ids).reshape(rows, k), wid)
+        assert np.allclose(from_dev(w), ww, rtol=ref.F32 * 2, atol=1e-30)
+
+
 # ---- grouping ------------------------------------------------------------------
 def _group(ctx, ids, G):
     n = ids.size
@@ -164,6 +194,21 @@ def test_group_rows_refusals(ctx):
         ctx.group_rows(None, 10, 64, off, o, p, ws)
 
 
+def test_group_rows_shared_memory(ctx):
+    buf = _i32(20000, 0)
+    off, o, p, ids = buf[:100], buf[100:5100], buf[5100:10100], buf[10100:15100]
+    ws = buf[15100:].view(torch.uint8)
+    ws = ws[(-ws.data_ptr()) % 16:]
+    ok = dict(ids=ids, n=5000, n_groups=64, offsets=off, order=o, place=p, ws=ws)
+    sync()
+    ctx.group_rows(**ok)
+    ctx.synchronize()
+    for kw in ({"order": p}, {"place": ids}, {"order": ids}, {"offsets": buf[60:160]},
+               {"ws": buf[(-buf.data_ptr()) % 16 // 4:].view(torch.uint8)}):
+        with pytest.raises(m.MingError, match="share"):
+            ctx.group_rows(**dict(ok, **kw))
+
+
 # ---- the weighted sum -------------------------------------------------------------
 @pytest.mark.parametrize("tokens,k,N,pad,add", [
     (1, 1, 8, 0, None), (1, 8, 2048, 0, "own"), (7, 3, 72, 16, "own"), (300, 9, 264, 8, "out"),
@@ -203,3 +248,19 @@ def test_combine_refusals(ctx):
         with pytest.raises(m.MingError):
             ctx.experts_combine(**dict(ok, **kw))
     ctx.experts_combine(**dict(ok, tokens=0))
+    ctx.experts_combine(None, 0, None, None, 0, 2, None, 64)
+
+
+def test_combine_shared_memory_and_sizes(ctx):
+    buf, w = empty_bf16(64, 128), torch.zeros(32, device="cuda")
+    y, out = buf.data_ptr(), buf.data_ptr() + 2 * 64      # columns beside each other
+    place = _i32(32, 0)
+    ok = dict(y=y, n=64, place=place, weights=w, tokens=16, top_k=2, out=out, N=64, ldy=128,
+              ldo=128)
+    sync()
+    ctx.experts_combine(**ok)
+    ctx.synchronize()
+    for kw in ({"out": out - 16}, {"place": out + 128}, {"weights": out}, {"add": out, "ldadd": 64},
+               {"add": out + 16, "ldadd": 128}, {"tokens": 2 ** 31 - 1}):
+        with pytest.raises(m.MingError, match="share|launch"):
+            ctx.experts_combine(**dict(ok, **kw))

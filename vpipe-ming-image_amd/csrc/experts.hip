@@ -185,18 +185,14 @@ __global__ __launch_bounds__(64 * WK) void experts_rows_kernel(const ExpertsArgs
   }
 }
 
-template <int BITS, bool GATED, int CO>
-void rows_wide(const ExpertsArgs& a, hipStream_t s) {
+template <int BITS, bool GATED>
+void rows_shape(const ExpertsArgs& a, hipStream_t s) {
+  constexpr int CO = GATED ? 1 : 2;
   const dim3 grid((unsigned)((a.N + 16 * CO - 1) / (16 * CO)), (unsigned)(a.n < a.E ? a.n : a.E));
   if (a.K <= 512)
     hipLaunchKernelGGL((experts_rows_kernel<BITS, GATED, 4, CO>), grid, dim3(256), 0, s, a);
   else
     hipLaunchKernelGGL((experts_rows_kernel<BITS, GATED, 8, CO>), grid, dim3(512), 0, s, a);
-}
-
-template <int BITS, bool GATED>
-void rows_shape(const ExpertsArgs& a, int co, hipStream_t s) {
-  co == 2 ? rows_wide<BITS, GATED, 2>(a, s) : rows_wide<BITS, GATED, 1>(a, s);
 }
 
 // w [NW][K] -> [K / 64][NW][64], 16 bytes a thread and step.
@@ -222,14 +218,14 @@ hipError_t launch_repack_dense(const uint16_t* w, int NW, int K, uint16_t* out, 
   return hipGetLastError();
 }
 
-hipError_t launch_experts_rows(int bits, bool gated, const ExpertsArgs& a, int co, hipStream_t s) {
+hipError_t launch_experts_rows(int bits, bool gated, const ExpertsArgs& a, hipStream_t s) {
   if (a.n <= 0 || a.N <= 0) return hipSuccess;
   if (a.K % 64 || a.N % 8 || a.NW != a.N * (gated ? 2 : 1) || a.E < 1 || a.fan < 1 || a.x_rows < 1)
     return hipErrorInvalidValue;
   switch (bits) {
-    case 4: gated ? rows_shape<4, true>(a, co, s) : rows_shape<4, false>(a, co, s); break;
-    case 8: gated ? rows_shape<8, true>(a, co, s) : rows_shape<8, false>(a, co, s); break;
-    case 16: gated ? rows_shape<16, true>(a, co, s) : rows_shape<16, false>(a, co, s); break;
+    case 4: gated ? rows_shape<4, true>(a, s) : rows_shape<4, false>(a, s); break;
+    case 8: gated ? rows_shape<8, true>(a, s) : rows_shape<8, false>(a, s); break;
+    case 16: gated ? rows_shape<16, true>(a, s) : rows_shape<16, false>(a, s); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
@@ -238,14 +234,13 @@ hipError_t launch_experts_rows(int bits, bool gated, const ExpertsArgs& a, int c
 hipError_t validate_experts_kernels() {
   hipFuncAttributes fa;
   const void* fns[] = {
-#define MING_EXPERTS_ROWS(BITS, CO)                                               \
-  reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 4, CO>),        \
-      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 8, CO>),    \
-      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 4, CO>),     \
-      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 8, CO>)
+#define MING_EXPERTS_ROWS(BITS)                                                \
+  reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 4, 2>),      \
+      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 8, 2>),  \
+      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 4, 1>),   \
+      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 8, 1>)
       reinterpret_cast<const void*>(&repack_dense_kernel),
-      MING_EXPERTS_ROWS(4, 1), MING_EXPERTS_ROWS(8, 1), MING_EXPERTS_ROWS(16, 1),
-      MING_EXPERTS_ROWS(4, 2), MING_EXPERTS_ROWS(8, 2), MING_EXPERTS_ROWS(16, 2)
+      MING_EXPERTS_ROWS(4), MING_EXPERTS_ROWS(8), MING_EXPERTS_ROWS(16)
 #undef MING_EXPERTS_ROWS
   };
   for (const void* f : fns) {

@@ -14,10 +14,10 @@
 // address of their own. Three LDS stages of 64 of K, one barrier a stage.
 //
 // The grid is an upper bound (the groups' sizes are on the device): a block
-// finds its tile by find_group, the rest leave. Groups are cut every 64 * places;
-// what is left of one runs at the height it needs. The lower cuts leave LDS and
-// registers for two or three blocks a CU, which hide each other's barriers and
-// starts and keep more of the weights in flight: see experts_plan for which cut.
+// finds its tile by find_group, the rest leave. Groups are cut every 64 to 256
+// places; what is left of one runs at the height it needs. The lower cuts leave LDS
+// and registers for two or three blocks a CU, which hide each other's barriers and
+// starts and keep more of the weights in flight: experts_cut says which cut.
 #include "common.h"
 #include "deq_frag.h"
 #include "kernels.h"
@@ -320,11 +320,7 @@ constexpr int tall(int bits) { return bits == 4 ? 4 : 8; }
 
 template <int BITS, bool GATED>
 void launch_max(const ExpertsArgs& a, int max, hipStream_t s) {
-  // every group ends in at most one partial tile
-  const int bn = GATED ? QBN / 2 : QBN;
-  const long long tiles = (long long)(a.n / (32 * max) + (a.n < a.E ? a.n : a.E)) *
-                          ((a.N + bn - 1) / bn);
-  const dim3 grid((unsigned)tiles);
+  const dim3 grid((unsigned)experts_tiles(BITS, GATED, max, a.n, a.E, a.N));
   if (max == 2)
     hipLaunchKernelGGL((experts_qtile_kernel<BITS, GATED, 2>), grid, dim3(64 * NW), 0, s, a);
   else

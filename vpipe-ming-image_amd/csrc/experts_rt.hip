@@ -80,14 +80,12 @@ bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
 int hip_fail(hipError_t e, const char* what) {
   return rt_fail(MING_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
 }
-// Two address ranges of rows x stride (the last row `width` wide), 2-byte elements.
-bool overlap(const void* a, int64_t ra, int64_t lda, int64_t wa, const void* b, int64_t rb,
-             int64_t ldb, int64_t wb) {
-  if (ra <= 0 || rb <= 0) return false;
-  const uint64_t a0 = (uint64_t)(uintptr_t)a, b0 = (uint64_t)(uintptr_t)b;
-  return a0 < b0 + 2 * (uint64_t)((rb - 1) * ldb + wb) &&
-         b0 < a0 + 2 * (uint64_t)((ra - 1) * lda + wa);
+ming::Span row_span(const void* p, int64_t rows, int64_t ld, int64_t width) {
+  return {p, rows, 2 * ld, 2 * width};
 }
+ming::Span flat_span(const void* p, int64_t bytes) { return {p, 1, bytes, bytes}; }
+// A launch holds 2^32 - 1 threads along x.
+bool one_launch(long long blocks, int threads) { return blocks <= 0xffffffffll / threads; }
 
 // One launch, timed when the context profiles.
 template <class F>
@@ -105,7 +103,7 @@ int products(const char* who, bool gated, ming_ctx* c, const ming_experts* ex, c
              int64_t ldx, int x_rows, const int32_t* order, int fan, const int32_t* offsets, int n,
              uint16_t* y, int64_t ldy, void* ws, size_t ws_bytes) {
   auto bad = [&](int code, const char* why) { return rt_fail(code, std::string(who) + ": " + why); };
-  if (!c || !ex || !x || !offsets || !y) return bad(MING_ERR_ARG, "null argument");
+  if (!c || !ex || (n > 0 && (!x || !offsets || !y))) return bad(MING_ERR_ARG, "null argument");
   if (ex->ctx != c) return bad(MING_ERR_ARG, "experts of another context");
   if (n < 0 || x_rows < 0 || fan < 1) return bad(MING_ERR_ARG, "a count out of range");
   const int N = gated ? ex->N / 2 : ex->N;
@@ -118,10 +116,8 @@ int products(const char* who, bool gated, ming_ctx* c, const ming_experts* ex, c
   if (n == 0) return rt_ok();
   if (x_rows == 0) return bad(MING_ERR_ARG, "places without rows of x");
   if (!order && x_rows < n) return bad(MING_ERR_SHAPE, "without an order x needs n rows");
-  if ((uint64_t)x_rows * (uint64_t)ldx >= (1ull << 30))
+  if (ldx > ((1ll << 30) - 1) / x_rows)
     return bad(MING_ERR_SHAPE, "x_rows * ldx must be below 2^30");
-  if (overlap(x, x_rows, ldx, ex->K, y, n, ldy, N))
-    return bad(MING_ERR_ARG, "x and y share memory");
   // the quantized tiles multiply fp16, which the other routes are chosen against
   const int cut = ex->bits != 16 && ming::rt_route(c) != MING_ROUTE_AUTO ? 0
                   : ming::rt_experts_cut(c) >= 0
@@ -134,6 +130,17 @@ int products(const char* who, bool gated, ming_ctx* c, const ming_experts* ex, c
     return rt_fail(MING_ERR_SHAPE, std::string(who) + ": the call needs " +
                                        std::to_string(xh_bytes) + " bytes of workspace, " +
                                        std::to_string(ws_bytes) + " given");
+  if (cut && !one_launch(ming::experts_tiles(ex->bits, gated, cut, n, ex->E, N),
+                         ex->bits == 16 ? 512 : 256))
+    return bad(MING_ERR_SHAPE, "more places times columns than one launch holds");
+  // every block reads the plan and the rows by itself, while others store
+  const ming::Span xs = row_span(x, x_rows, ldx, ex->K), ys = row_span(y, n, ldy, N);
+  const ming::Span os = flat_span(order, order ? 4ll * n : 0), fs = flat_span(offsets, 4ll * (ex->E + 1));
+  const ming::Span sc = flat_span(ws, (int64_t)xh_bytes);
+  for (const ming::Span& in : {xs, os, fs})
+    if (ming::spans_meet(in, ys) || ming::spans_meet(in, sc))
+      return bad(MING_ERR_ARG, "x, order or offsets share memory with y or ws");
+  if (ming::spans_meet(ys, sc)) return bad(MING_ERR_ARG, "y and ws share memory");
   DeviceGuard g(ming::rt_device(c));
   ming::ExpertsArgs a{};
   a.x = x; a.ldx = ldx;
@@ -149,7 +156,7 @@ int products(const char* who, bool gated, ming_ctx* c, const ming_experts* ex, c
       c, ming::kRtExperts, flops, wb * std::min(n, ex->E) + 2.0 * x_rows * ex->K + 2.0 * n * N, who,
       [&] {
         if (cut == 0)
-          return ming::launch_experts_rows(ex->bits, gated, a, gated ? 1 : 2, stream_of(c));
+          return ming::launch_experts_rows(ex->bits, gated, a, stream_of(c));
         if (ex->bits == 16) return ming::launch_experts_tile(gated, a, cut, stream_of(c));
         // one conversion of x to fp16 for all experts' rows
         auto* xh = static_cast<uint16_t*>(ws);
@@ -196,8 +203,10 @@ int ming_topk_route(ming_ctx* c, const void* logits, int64_t ld, int logits_f32,
   auto bad = [](int code, const char* why) {
     return rt_fail(code, std::string("ming_topk_route: ") + why);
   };
-  if (!c || !logits || !ids || !weights) return bad(MING_ERR_ARG, "null argument");
+  if (!c || (rows > 0 && (!logits || !ids || !weights)))
+    return bad(MING_ERR_ARG, "null argument");
   if (rows < 0) return bad(MING_ERR_ARG, "rows < 0");
+  if (rows >= 1 << 26) return bad(MING_ERR_SHAPE, "rows must be below 2^26");
   if (score != MING_SCORE_SOFTMAX && score != MING_SCORE_SIGMOID)
     return bad(MING_ERR_ARG, "no such score");
   if (n_experts < 1 || n_experts > ming::kRouteMaxExperts || n_groups < 1 || n_groups > 64 ||
@@ -212,6 +221,13 @@ int ming_topk_route(ming_ctx* c, const void* logits, int64_t ld, int logits_f32,
       !aligned(weights, 4))
     return bad(MING_ERR_ARG, "a misaligned pointer");
   if (rows == 0) return rt_ok();
+  const int64_t el = logits_f32 ? 4 : 2;
+  const ming::Span ls = {logits, rows, el * ld, el * n_experts};
+  const ming::Span bs = flat_span(bias, bias ? 4ll * n_experts : 0);
+  const ming::Span is = flat_span(ids, 4ll * rows * top_k), wt = flat_span(weights, 4ll * rows * top_k);
+  if (ming::spans_meet(is, wt) || ming::spans_meet(ls, is) || ming::spans_meet(ls, wt) ||
+      ming::spans_meet(bs, is) || ming::spans_meet(bs, wt))
+    return bad(MING_ERR_ARG, "logits, bias, ids and weights must not share memory");
   DeviceGuard g(ming::rt_device(c));
   ming::RouteArgs a{};
   a.logits = logits; a.ld = ld; a.f32 = logits_f32 != 0; a.bias = bias;
@@ -249,6 +265,13 @@ int ming_group_rows(ming_ctx* c, const int32_t* ids, int n, int n_groups, int32_
     return rt_fail(MING_ERR_SHAPE, "ming_group_rows: the call needs " + std::to_string(need) +
                                        " bytes of workspace, " + std::to_string(ws_bytes) +
                                        " given");
+  const ming::Span all[5] = {flat_span(ids, 4ll * n), flat_span(offsets, 4ll * (n_groups + 1)),
+                             flat_span(order, 4ll * n), flat_span(place, 4ll * n),
+                             flat_span(ws, (int64_t)need)};
+  for (int i = 0; i < 5; ++i)
+    for (int j = 0; j < i; ++j)
+      if (ming::spans_meet(all[i], all[j]))
+        return bad(MING_ERR_ARG, "ids, offsets, order, place and ws must not share memory");
   DeviceGuard g(ming::rt_device(c));
   ming::GroupRowsArgs a{};
   a.ids = ids; a.n = n; a.G = n_groups;
@@ -396,7 +419,8 @@ int ming_experts_combine(ming_ctx* c, const uint16_t* y, int64_t ldy, int n, con
   auto bad = [](int code, const char* why) {
     return rt_fail(code, std::string("ming_experts_combine: ") + why);
   };
-  if (!c || !out || !place || !weights || (n > 0 && !y)) return bad(MING_ERR_ARG, "null argument");
+  if (!c || (tokens > 0 && (!out || !place || !weights || (n > 0 && !y))))
+    return bad(MING_ERR_ARG, "null argument");
   if (n < 0 || tokens < 0 || top_k < 1) return bad(MING_ERR_ARG, "a count out of range");
   if (N <= 0 || N % 8 != 0 || (n > 0 && ldy < N) || ldo < N || (add && ldadd < N) ||
       ldy % 8 != 0 || ldo % 8 != 0 || (add && ldadd % 8 != 0))
@@ -405,9 +429,15 @@ int ming_experts_combine(ming_ctx* c, const uint16_t* y, int64_t ldy, int n, con
       !aligned(weights, 4))
     return bad(MING_ERR_ARG, "y, add and out must be 16-byte, place and weights 4-byte aligned");
   if (tokens == 0) return rt_ok();
-  if (n > 0 && overlap(y, n, ldy, N, out, tokens, ldo, N))
+  if (!one_launch(ming::combine_blocks(tokens, N), 256))
+    return bad(MING_ERR_SHAPE, "more tokens than one launch holds");
+  const ming::Span outs = row_span(out, tokens, ldo, N);
+  if (ming::spans_meet(row_span(y, n, ldy, N), outs))
     return bad(MING_ERR_ARG, "y and out share memory");
-  if (add && !(add == out && ldadd == ldo) && overlap(add, tokens, ldadd, N, out, tokens, ldo, N))
+  if (ming::spans_meet(flat_span(place, 4ll * tokens * top_k), outs) ||
+      ming::spans_meet(flat_span(weights, 4ll * tokens * top_k), outs))
+    return bad(MING_ERR_ARG, "place or weights share memory with out");
+  if (add && !(add == out && ldadd == ldo) && ming::spans_meet(row_span(add, tokens, ldadd, N), outs))
     return bad(MING_ERR_ARG, "add and out share memory but are not the same rows");
   DeviceGuard g(ming::rt_device(c));
   ming::CombineArgs a{};

@@ -250,11 +250,7 @@ __global__ __launch_bounds__(64 * NW, 1) void experts_tile_kernel(const ExpertsA
 
 template <int MAX>
 void launch_max(bool gated, const ExpertsArgs& a, hipStream_t s) {
-  // every group ends in at most one partial tile
-  const int bn = gated ? TBN / 2 : TBN;
-  const long long tiles = (long long)(a.n / (64 * MAX) + (a.n < a.E ? a.n : a.E)) *
-                          ((a.N + bn - 1) / bn);
-  const dim3 grid((unsigned)tiles);
+  const dim3 grid((unsigned)experts_tiles(16, gated, MAX, a.n, a.E, a.N));
   if (gated)
     hipLaunchKernelGGL((experts_tile_kernel<MAX, true>), grid, dim3(64 * NW), 0, s, a);
   else

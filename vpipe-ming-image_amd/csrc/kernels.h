@@ -491,6 +491,7 @@ struct CombineArgs {
   int tpr;              // set by the launch
 };
 hipError_t launch_combine(CombineArgs a, hipStream_t s);
+long long combine_blocks(long long tokens, int N);
 hipError_t validate_routing_kernels();
 
 // ---- the experts' ragged products (experts.hip) ---------------------------------
@@ -498,8 +499,8 @@ hipError_t validate_routing_kernels();
 // W_e^T with row(p) = order ? order[p] / fan : p, kept inside [0, x_rows). W is
 // a stack of E projections of NW rows: NW = N, or gated 2 N, the gate's N rows
 // before the up projection's, y = bf16(silu(gate) * up) of the f32 results.
-// Weights: bits 16 w16 [E][K / 64][NW][64] (launch_repack_dense); bits 4 / 8 the fast resident layout
-// (launch_repack_fast) an expert after another.
+// Weights: bits 16 w16 [E][K / 64][NW][64] (launch_repack_dense); bits 4 / 8 the fast
+// resident layout (launch_repack_fast) an expert after another.
 struct ExpertsArgs {
   const uint16_t* x;
   long long ldx;
@@ -518,9 +519,8 @@ struct ExpertsArgs {
 // few of the memory's channels ([64][2048, 2048], 512 rows: 128.7 us by rows, 96.5
 // with K = 2112).
 hipError_t launch_repack_dense(const uint16_t* w, int NW, int K, uint16_t* out, hipStream_t s);
-// few rows an expert, any weights: 16 rows and 16 * co columns (co 1, 2) a block
-// (experts.hip)
-hipError_t launch_experts_rows(int bits, bool gated, const ExpertsArgs& a, int co, hipStream_t s);
+// few rows an expert, any weights (experts.hip)
+hipError_t launch_experts_rows(int bits, bool gated, const ExpertsArgs& a, hipStream_t s);
 hipError_t validate_experts_kernels();
 // dense weights, tiles (experts_tile.hip): groups cut every 64 * max places, max 2
 // or 4; x_rows * ldx and NW * K below 2^30, y 16-byte aligned with ldy % 8 == 0
@@ -531,6 +531,11 @@ hipError_t validate_experts_tile_kernels();
 hipError_t launch_experts_qtile(int bits, bool gated, const ExpertsArgs& a, int max,
                                 hipStream_t s);
 hipError_t validate_experts_qtile_kernels();
+// Blocks of the tiles: every group ends in at most one partial one.
+inline long long experts_tiles(int bits, bool gated, int max, int n, int E, int N) {
+  const int cut = (bits == 16 ? 64 : 32) * max, bn = gated ? 128 : 256;
+  return (long long)(n / cut + (n < E ? n : E)) * ((N + bn - 1) / bn);
+}
 // Which of them takes n places of a stack of N weight rows: 0 the few-row kernel,
 // else the tiles' cut (`max`).
 int experts_cut(int E, int N, int K, int bits, int n);

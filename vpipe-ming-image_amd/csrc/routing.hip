@@ -164,6 +164,7 @@ __global__ __launch_bounds__(256) void topk_route_kernel(const RouteArgs a) {
   }
 #pragma unroll
   for (int i = 0; i < P; ++i) mine[64 * i + lane] = s[i];
+  __builtin_amdgcn_wave_barrier();
   uint64_t u[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) u[i] = key[i] > none ? ordered(key[i]) : 0;
@@ -442,13 +443,22 @@ hipError_t launch_group_rows(GroupRowsArgs a, hipStream_t s) {
   return hipGetLastError();
 }
 
+static int combine_threads(int N) {
+  int tpr = 1;
+  while (tpr < 256 && tpr * 8 < N) tpr *= 2;
+  return tpr;
+}
+
+long long combine_blocks(long long tokens, int N) {
+  const int rpb = 256 / combine_threads(N);
+  return (tokens + rpb - 1) / rpb;
+}
+
 hipError_t launch_combine(CombineArgs a, hipStream_t s) {
   if (a.tokens <= 0 || a.N <= 0) return hipSuccess;
   if (a.N % 8 || a.k < 1) return hipErrorInvalidValue;
-  a.tpr = 1;
-  while (a.tpr < 256 && a.tpr * 8 < a.N) a.tpr *= 2;
-  const int rpb = 256 / a.tpr;
-  hipLaunchKernelGGL(combine_kernel, dim3((unsigned)((a.tokens + rpb - 1) / rpb)), dim3(256), 0, s,
+  a.tpr = combine_threads(a.N);
+  hipLaunchKernelGGL(combine_kernel, dim3((unsigned)combine_blocks(a.tokens, a.N)), dim3(256), 0, s,
                      a);
   return hipGetLastError();
 }

@@ -11,6 +11,25 @@
 #include "../../include/ming_dit_amd.h"
 
 namespace ming {
+// Memory of a call: `rows` rows of `width` bytes, `ld` bytes apart.
+struct Span {
+  const void* p;
+  int64_t rows, ld, width;
+};
+// Whether they share a byte. Rows of one stride may lie beside each other; of two
+// strides, ranges that meet count as shared.
+inline bool spans_meet(const Span& a, const Span& b) {
+  if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return false;
+  const auto end = [](const Span& s) {
+    return (__uint128_t)(uintptr_t)s.p + (__uint128_t)(s.rows - 1) * (uint64_t)s.ld +
+           (uint64_t)s.width;
+  };
+  if (end(a) <= (uintptr_t)b.p || end(b) <= (uintptr_t)a.p) return false;
+  if (a.ld != b.ld || a.ld <= 0) return true;
+  const uint64_t ld = (uint64_t)a.ld, a0 = (uintptr_t)a.p, b0 = (uintptr_t)b.p;
+  const uint64_t d = b0 >= a0 ? (b0 - a0) % ld : (ld - (a0 - b0) % ld) % ld;
+  return d < (uint64_t)a.width || d + (uint64_t)b.width > ld;
+}
 int rt_fail(int code, const std::string& why);
 int rt_ok();
 int rt_device(const ming_ctx* c);

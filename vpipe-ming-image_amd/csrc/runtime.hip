@@ -1606,7 +1606,12 @@ int ming_adapters_create(ming_ctx* c, int N, int K, int capacity, int max_rank,
   if (!b) return fail(MING_ERR_ALLOC, "ming_adapters_create: out of memory");
   b->ctx = c; b->N = N; b->K = K; b->cap = capacity; b->max_rank = max_rank;
   b->ldt = round_up(max_rank, 32);
-  b->bound.resize(capacity);
+  try {
+    b->bound.resize(capacity);
+  } catch (const std::bad_alloc&) {
+    delete b;
+    return fail(MING_ERR_ALLOC, "ming_adapters_create: out of memory");
+  }
   c->live_weights += 1;
   const size_t bytes = (size_t)capacity * sizeof(ming::AdapterEntry);
   if (hipMalloc(&b->table, bytes) != hipSuccess) {
@@ -1763,9 +1768,23 @@ int ming_lin_adapters(ming_ctx* c, const ming_qweight* qw, const ming_adapters* 
   if (!aligned(ws, 16) || !aligned(row_adapter, 4) || !aligned(row_scale, 4))
     return fail(MING_ERR_ARG,
                 "ming_lin_adapters: ws must be 16-byte, ids and strengths 4-byte aligned");
-  if (qw && x && y && M > 0 && ldx >= qw->K && ldy >= qw->N &&
-      overlap(x, ldx, qw->K, y, ldy, qw->N, M))
-    return fail(MING_ERR_ARG, "ming_lin_adapters: x and y share memory");
+  // rows of y that do not take 16-byte stores would have a plan of their own, with
+  // another workspace
+  if (!aligned(y, 16) || ldy % 8 != 0)
+    return fail(MING_ERR_ARG, "ming_lin_adapters: y must be 16-byte aligned, ldy a multiple of 8");
+  if (qw && x && y && M > 0 && ldx >= qw->K && ldy >= qw->N) {
+    // every block resolves its rows' adapters by itself, while others store
+    const ming::Span xs = {x, M, 2 * ldx, 2ll * qw->K}, ys = {y, M, 2 * ldy, 2ll * qw->N};
+    const ming::Span is = {row_adapter, 1, 4ll * M, 4ll * M};
+    const ming::Span ss = {row_scale, 1, 4ll * M, 4ll * M};
+    const ming::Span sc = {ws, 1, (int64_t)ws_bytes, (int64_t)ws_bytes};
+    for (const ming::Span& in : {xs, is, ss})
+      if (ming::spans_meet(in, ys) || ming::spans_meet(in, sc))
+        return fail(MING_ERR_ARG,
+                    "ming_lin_adapters: x, row_adapter or row_scale share memory with y or ws");
+    if (ming::spans_meet(ys, sc))
+      return fail(MING_ERR_ARG, "ming_lin_adapters: y and ws share memory");
+  }
   Carve cv;
   cv.base = static_cast<char*>(ws);
   cv.cap = ws_bytes;
