@@ -282,7 +282,7 @@ __device__ __forceinline__ void experts_qtile(const ExpertsArgs& a, uint4* const
   }
 }
 
-// Groups are cut every 32 * MAX places.
+// Groups of more than 32 * MAX places are cut into the fewest tiles that hold them.
 template <int BITS, bool GATED, int MAX>
 __global__ __launch_bounds__(64 * NW, MAX == 8 ? 1 : MAX == 2 && BITS == 4 ? 3 : 2)
 void experts_qtile_kernel(const ExpertsArgs a) {
@@ -304,14 +304,19 @@ void experts_qtile_kernel(const ExpertsArgs a) {
   if (rg.e < 0) return;
   const int tiles_m = (rg.rows + CUT - 1) / CUT;
   const int tn = rg.index / tiles_m, tm = rg.index - tn * tiles_m;
-  const int p0 = rg.p0 + tm * CUT, n0 = tn * BNT;
-  const int rows = rg.rows - tm * CUT < CUT ? rg.rows - tm * CUT : CUT;
+  const RowTile rt = row_tile<MAX == 8 ? 64 : 32>(rg.rows, tiles_m, tm);
+  const int p0 = rg.p0 + rt.first, rows = rt.rows, n0 = tn * BNT;
   if constexpr (MAX >= 8)
     if (rows > 192) return experts_qtile<BITS, GATED, 8, PP>(a, st0, st1, st2, rg.e, p0, rows, n0);
   if constexpr (MAX >= 8)
     if (rows > 128) return experts_qtile<BITS, GATED, 6, PP>(a, st0, st1, st2, rg.e, p0, rows, n0);
   if constexpr (MAX >= 4)
-    if (rows > 64) return experts_qtile<BITS, GATED, 4, PP>(a, st0, st1, st2, rg.e, p0, rows, n0);
+    if (rows > (MAX == 8 ? 64 : 96))
+      return experts_qtile<BITS, GATED, 4, PP>(a, st0, st1, st2, rg.e, p0, rows, n0);
+  if constexpr (MAX == 4)
+    if (rows > 64) return experts_qtile<BITS, GATED, 3, PP>(a, st0, st1, st2, rg.e, p0, rows, n0);
+  if constexpr (MAX < 8)
+    if (rows <= 32) return experts_qtile<BITS, GATED, 1, PP>(a, st0, st1, st2, rg.e, p0, rows, n0);
   experts_qtile<BITS, GATED, 2, PP>(a, st0, st1, st2, rg.e, p0, rows, n0);
 }
 

@@ -25,24 +25,27 @@ namespace ming {
 // Which kernel takes n places: 0 the few-row one, else the tiles, cut every
 // 64 (dense) or 32 (quantized) * max places. The groups' sizes are on the device,
 // so it goes by what an even router gives: live experts, rows of each. Of both the
-// times below are fits (us) to [8 to 256][256 to 4096, 512 to 4096] at 2 to 34816
+// times below are fits (us) to [16 to 256][1024 to 4096, 1024 to 4096] at 8 to 384
 // places; where they are close, so are the kernels.
 //   few rows, dense: 2.5 + bytes / 5.9 TB/s, longer by the rows' own reads (swiglu
-//     of [64][2048, 2048], 8 places: 13.7, the tiles 17.0); w4 and w8: the codes'
-//     conversion, 2.8 and 3.9 weights a ps ([128][1024, 2048] w8 gated, 32 places:
-//     19.2, the tiles 25); 16 rows a pass over the weights.
-//   tiles: a start and the K stages of one, then the weights at 6.1 TB/s, a round
-//     of the chip (one dense block a CU) at least that again (the same, 64 places:
-//     62.0, few rows 56.2; 128: 80.2 and 83.2). Out of cold caches the tiles lose a
-//     little more: they have to win by 8%.
-// Cuts: dense, 128 rows up to 192 an expert, then 256 ([64][2048, 2048] gated at
-// 128 rows 121 us, 147 cut at 256; at 544 rows 317 and 359). w4, 64 rows, three
-// blocks a CU, then 128, two ([128][1024, 2048] gated at 128 rows 102 both, at 272
-// 186 and 166); w8, 64 rows, then 256 (at 64 rows 75, at 272 214 and 202).
+//     of [64][2048, 2048], 8 places: 14.1, the tiles 17.3); w4 and w8: the codes'
+//     conversion, 3.3 and 4.6 weights a ps ([60][2048, 1024] w8, 16 places: 11.5, the
+//     tiles 16.0), and a start a block; 16 rows a pass over the weights.
+//   tiles: a start and the K stages of one, then the weights at 5.6 to 6.1 TB/s, a
+//     round of the chip (one dense block a CU) at least that again (dense as above, 64
+//     places: 68.8, few rows 66.0; 128: 85.3 and 89.9; w8 as above, 64: 23.6 and 28.8).
+//     Out of cold caches the tiles lose more (the 64 places: 71.6 and 61.2): they have
+//     to win by 8%.
+// Cuts (low / tall, us): more rows a tile read the weights less often and, quantized,
+// convert them less often; fewer fill the chip where there are few tiles. Dense, 128
+// or 256 rows ([64][2048, 2048] gated, 96 rows an expert 99 / 103, 128: 125 / 110, 544:
+// 311 / 283; [16][2048, 4096], 192 rows, 128 tall tiles: 65 / 94); w4, 64 rows and three
+// blocks a CU or 128 and two ([128][1024, 2048] gated, 32 rows 41 / 43, 78: 70 / 57); w8, 64
+// or 256 ([60][2048, 1024], 160 rows 63 / 62, all groups of 256: 86 / 74).
 int experts_cut(int E, int N, int K, int bits, int n) {
   const double live = E * (1.0 - std::exp(-(double)n / E)), rows = n / live;
   const double weights = live * N * (double)K, stages = K / 64.0;
-  const double passes = rows > 16.0 ? rows / 16.0 : 1.0;
+  const double passes = rows > 8.0 ? rows / 16.0 + 0.5 : 1.0;
   double few, tile;
   if (bits == 16) {
     const double one = 256.0 * K * 2 / 6.1e6;            // a tile's weights, us
@@ -50,13 +53,15 @@ int experts_cut(int E, int N, int K, int bits, int n) {
     few = 2.5 + weights * 2 / 5.9e6 * (1.0 + rows / 40.0) * passes;
     tile = round * one + std::max(4.0 + 0.4 * stages, 2.5 + (all - round) * one);
   } else {
-    few = 3.0 + weights / (bits == 4 ? 2.8e6 : 3.9e6) * passes;
-    tile = 2.5 + std::max(4.6 + 0.5 * stages, 2.5 + weights * bits / 8 / 4.5e6);
+    few = 3.0 + weights / (bits == 4 ? 3.3e6 : 4.6e6) * passes + 0.0035 * live * (N / 32.0);
+    tile = std::max(5.5 + 0.6 * stages, 7.0 + weights * (bits / 8.0 + 1.0 / 16) / 5.6e6);
   }
   if (few < 1.08 * tile) return 0;
-  if (bits == 16) return rows < 192.0 ? 2 : 4;
-  if (bits == 4) return rows < 160.0 ? 2 : 4;
-  return rows < 200.0 ? 2 : 8;
+  const int low = 2, tall = bits == 8 ? 8 : 4;
+  const double from = bits == 16 ? 112.0 : bits == 4 ? 60.0 : 240.0;
+  // tiles of the tall cut, of which every group ends in half a one on average
+  const double each = std::max(1.0, rows / ((bits == 16 ? 64 : 32) * tall) + 0.5);
+  return rows < from || live * each * ((N + 255) / 256) < 180.0 ? low : tall;
 }
 
 }  // namespace ming

@@ -219,8 +219,7 @@ __device__ __forceinline__ void experts_tile(const ExpertsArgs& a, uint4* const 
   }
 }
 
-// Groups are cut every 64 * MAX places; what is left of one runs at the height
-// it needs.
+// Groups of more than 64 * MAX places are cut into the fewest tiles that hold them.
 template <int MAX, bool GATED>
 __global__ __launch_bounds__(64 * NW, 1) void experts_tile_kernel(const ExpertsArgs a) {
   constexpr int CUT = 64 * MAX;
@@ -236,8 +235,8 @@ __global__ __launch_bounds__(64 * NW, 1) void experts_tile_kernel(const ExpertsA
   if (rg.e < 0) return;
   const int tiles_m = (rg.rows + CUT - 1) / CUT;
   const int tn = rg.index / tiles_m, tm = rg.index - tn * tiles_m;
-  const int p0 = rg.p0 + tm * CUT, n0 = tn * BNT;
-  const int rows = rg.rows - tm * CUT < CUT ? rg.rows - tm * CUT : CUT;
+  const RowTile rt = row_tile<64>(rg.rows, tiles_m, tm);
+  const int p0 = rg.p0 + rt.first, rows = rt.rows, n0 = tn * BNT;
   if constexpr (MAX >= 4)
     if (rows > 192) return experts_tile<4, GATED>(a, ring, rg.e, p0, rows, n0);
   if constexpr (MAX >= 3)

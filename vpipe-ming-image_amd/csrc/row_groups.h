@@ -66,4 +66,18 @@ __device__ __forceinline__ RowGroup find_group(const int32_t* __restrict__ offse
   return g;
 }
 
+// Tile tm of a group of `rows` that takes `tiles` of them, in units of U rows spread
+// over the tiles as evenly as they go: heights differ by a unit at most, so no block
+// is left with the sliver of a group, whose stages cost nearly a full tile's.
+struct RowTile {
+  int first, rows;
+};
+template <int U>
+__device__ __forceinline__ RowTile row_tile(int rows, int tiles, int tm) {
+  const int units = (rows + U - 1) / U, each = units / tiles, more = units - each * tiles;
+  const int first = U * (each * tm + (tm < more ? tm : more));
+  const int h = U * (each + (tm < more ? 1 : 0));
+  return {first, rows - first < h ? rows - first : h};
+}
+
 }  // namespace ming
