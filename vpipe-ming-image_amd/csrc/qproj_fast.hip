@@ -34,7 +34,6 @@
 #include "deq_frag.h"
 #include "kernels.h"
 #include "lds_ring.h"
-#include "row_adapters.h"
 #include "row_xa.h"
 
 namespace ming {
@@ -836,64 +835,6 @@ __global__ void qproj_split_reduce_kernel(const QprojArgs a) {
   range_report(a.range, seen);
 }
 
-// The same with what the rows' own adapters add: y = bf16(sum of the slices in
-// order + T . B_a^T). A wave takes 16 rows x 64 columns; each adapter among the rows
-// is v_mfma_f32_16x16x32_bf16 tiles over all of them, the others' T read as zeros,
-// so a request's B is read once for its rows (a thread's own dot products read it
-// once a row: [500, 3840] of ranks 16 to 64, 14.6 us).
-__global__ __launch_bounds__(256) void qproj_split_rows_reduce_kernel(const QprojArgs a) {
-  const int lane = (int)threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int c = lane & 15, g = lane >> 4;
-  const int n0 = (int)blockIdx.x * 64, m0 = (int)blockIdx.y * 64 + 16 * wave, m = m0 + c;
-  if (m0 >= a.M) return;                   // no barrier below
-  const bool row = m < a.M;
-  const int ms = row ? m : a.M - 1;
-  const int id = row ? a.rows.rid[ms] : -1;
-  floatx4_t acc[4];
-#pragma unroll
-  for (int t = 0; t < 4; ++t) acc[t] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  const uint16_t* const tr = a.rows.t + (long long)ms * a.rows.ldt + 8 * g;
-  uint64_t left = __ballot(id >= 0);
-  while (left) {
-    const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-    left &= ~__ballot(id == cur);
-    const AdapterEntry e = a.rows.table[cur];
-    for (int k = 0; k < e.r8; k += 32) {
-      // past the rank T is zero: any of B's columns will do
-      const int kc = k + 8 * g < e.r8 ? k + 8 * g : e.r8 - 8;
-      uint4 tv = make_uint4(0, 0, 0, 0), bv[4];
-      if (id == cur) tv = *reinterpret_cast<const uint4*>(tr + k);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int n = n0 + 16 * t + c;
-        bv[t] = *reinterpret_cast<const uint4*>(e.B + (long long)(n < a.N ? n : a.N - 1) * e.r8 + kc);
-      }
-#pragma unroll
-      for (int t = 0; t < 4; ++t) acc[t] = mfma_rows(bv[t], tv, acc[t]);
-    }
-  }
-  // lane (row c, g): columns 4g + 0..3 of each 16
-  const size_t plane = (size_t)a.M * (size_t)a.N;
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int n = n0 + 16 * t + 4 * g;
-    if (!row || n >= a.N) continue;
-    const float* p = a.part + (size_t)m * a.N + n;
-    float4 sum = *reinterpret_cast<const float4*>(p);
-    for (int k = 1; k < a.kslices; ++k) {
-      p += plane;
-      const float4 v = *reinterpret_cast<const float4*>(p);
-      sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
-    }
-    if (id >= 0) {
-      sum.x += acc[t][0]; sum.y += acc[t][1]; sum.z += acc[t][2]; sum.w += acc[t][3];
-    }
-    *reinterpret_cast<uint2*>(a.y + (size_t)m * a.ldy + n) =
-        make_uint2(pack_bf16x2_rne(sum.x, sum.y), pack_bf16x2_rne(sum.z, sum.w));
-  }
-}
-
 // ---- T = x . A_live^T * coef: the adapters' stacked down-projection --------
 // Block tile 64*MR rows x 64*CJ stacked ranks. Four MFMA waves in 2 x 2, each
 // 32*MR rows x 32*CJ ranks (MR x CJ tiles of v_mfma_f32_32x32x16_bf16,
@@ -1185,8 +1126,7 @@ __global__ __launch_bounds__(512, 1) void lora_xa_rows_kernel(const LoraXaArgs a
 // coalesced), one 16-byte store of T. Positions of row tiles past M or
 // column blocks past n_cols are skipped. 32-bit indices (the host keeps a
 // slice's float4 count below 2^31).
-// ROWS: plus what the rows' own adapters add (a dense weight's split).
-template <int MR, int CJ, bool ROWS>
+template <int MR, int CJ>
 __global__ void lora_xa_reduce_kernel(const float* part, int kslices, int M,
                                       int n_cols, const LoraXaArgs a) {
   constexpr unsigned XR = 64 * MR, XC = 64 * CJ, FR = 4 * MR * CJ;
@@ -1216,17 +1156,12 @@ __global__ void lora_xa_reduce_kernel(const float* part, int kslices, int M,
     }
     const float co = a.ident ? 1.0f : a.coef[c >> 3];
     uint4 o = make_uint4(0, 0, 0, 0);
-    if (ROWS || (co != 0.0f && a.bias)) {
-      // the dense split-K GEMM with a bias or its rows' adapters (coef 1): one
-      // rounding
+    if (co != 0.0f && a.bias) {
+      // the dense split-K GEMM with a bias (coef 1): one rounding
       float r[8] = {co * s0.x, co * s0.y, co * s0.z, co * s0.w,
                     co * s1.x, co * s1.y, co * s1.z, co * s1.w};
-      if constexpr (ROWS) {
-        add_row_adapter(a.rows, (int)m, (int)c, r);
-      } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) r[e] += bf16_to_f32(a.bias[c + e]);
-      }
+      for (int e = 0; e < 8; ++e) r[e] += bf16_to_f32(a.bias[c + e]);
       o.x = pack_bf16x2_rne(r[0], r[1]);
       o.y = pack_bf16x2_rne(r[2], r[3]);
       o.z = pack_bf16x2_rne(r[4], r[5]);
@@ -1244,6 +1179,117 @@ __global__ void lora_xa_reduce_kernel(const float* part, int kslices, int M,
       reinterpret_cast<uint2*>(tp)[0] = make_uint2(o.x, o.y);
       reinterpret_cast<uint2*>(tp)[1] = make_uint2(o.z, o.w);
     }
+  }
+}
+
+// ---- a K split's end with what the rows' own adapters add --------------------
+// y = bf16(sum of the slices in order + T . B_a^T), the slices of a quantized
+// projection as planes [M][N] (MR 0), a dense one's in lora_xa_fast_kernel's order. A
+// wave takes 16 rows x 16 CT columns; each adapter among the rows is
+// v_mfma_f32_16x16x32_bf16 tiles over all of them, the others' T read as zeros, so a
+// request's B is read once for its rows (a thread's own dot products read it once a
+// row: [500, 3840] dense of 32 adapters, 63 us). Bound by memory latency where rows
+// bring many adapters: their entries are held by the lanes and the operands of NB
+// 32-rank chunks are in flight together (one at a time 18.8 us at 16 rows of 16).
+struct RowsSum {
+  const float* part;
+  int kslices, M, N;
+  uint16_t* y;
+  long long ldy;
+  RowAdapters rows;
+};
+template <int MR, int CJ, int CT>
+__global__ __launch_bounds__(256) void split_rows_sum_kernel(const RowsSum a) {
+  constexpr int NB = CT == 1 ? 8 : 4;
+  const int lane = (int)threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int n0 = ((int)blockIdx.x * 4 + wave) * 16 * CT, m = (int)blockIdx.y * 16 + c;
+  if (n0 >= a.N) return;                   // no barrier below
+  const bool row = m < a.M;
+  const int ms = row ? m : a.M - 1;
+  const int id = row ? a.rows.rid[ms] : -1;
+  // the slices' sums: lane (row c, g): columns 4g + 0..3 of each 16
+  float4 sum[CT];
+#pragma unroll
+  for (int t = 0; t < CT; ++t) {
+    const int n = n0 + 16 * t + 4 * g < a.N ? n0 + 16 * t + 4 * g : a.N - 4;
+    size_t at, plane;                      // in float4s
+    if constexpr (MR == 0) {
+      at = ((size_t)ms * a.N + n) / 4;
+      plane = (size_t)a.M * a.N / 4;
+    } else {
+      // ((tile * 4 + wave) * FR + f) * 64 + fr + 32 half, f = (CJ fi + fj) 4 + fq
+      constexpr unsigned XR = 64 * (MR ? MR : 1), XC = 64 * (CJ ? CJ : 1), FR = 4 * MR * CJ;
+      const unsigned um = (unsigned)ms, un = (unsigned)n;
+      const unsigned tiles_c = ((unsigned)a.N + XC - 1) / XC, tm = um / XR, tc = un / XC;
+      const unsigned r = um % XR, q = un % XC;
+      const unsigned w = r / (XR / 2) + 2 * (q / (XC / 2));
+      const unsigned f = (CJ * (r / 32 % MR) + q / 32 % CJ) * 4 + q / 8 % 4;
+      at = (((size_t)(tm * tiles_c + tc) * 4 + w) * FR + f) * 64 + r % 32 + 8 * (q & 4);
+      plane = (size_t)((((unsigned)a.M + XR - 1) / XR) * tiles_c) * (256u * FR);
+    }
+    const float4* p = reinterpret_cast<const float4*>(a.part) + at;
+    sum[t] = *p;
+    for (int k = 1; k < a.kslices; ++k) {
+      p += plane;
+      const float4 v = *p;
+      sum[t].x += v.x; sum[t].y += v.y; sum[t].z += v.z; sum[t].w += v.w;
+    }
+  }
+  AdapterEntry e = {};
+  if (id >= 0) e = a.rows.table[id];
+  const uint64_t ptr = (uint64_t)(uintptr_t)e.B;
+  floatx4_t acc[CT];
+#pragma unroll
+  for (int t = 0; t < CT; ++t) acc[t] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  const uint16_t* const tr = a.rows.t + (long long)ms * a.rows.ldt + 8 * g;
+  uint64_t left = __ballot(id >= 0);
+  int k = 0;
+  while (left) {
+    uint4 tv[NB], bv[NB][CT];
+    int held = 0;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      if (!left) break;
+      const int w = __builtin_ctzll(left);
+      const int cur = __builtin_amdgcn_readlane(id, w);
+      const int r8 = __builtin_amdgcn_readlane(e.r8, w);
+      const uint64_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)ptr, w);
+      const uint64_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(ptr >> 32), w);
+      const uint16_t* const B = reinterpret_cast<const uint16_t*>((uintptr_t)(hi << 32 | lo));
+      // past the rank T is zero: any of B's columns will do
+      const int kc = k + 8 * g < r8 ? k + 8 * g : r8 - 8;
+      tv[b] = make_uint4(0, 0, 0, 0);
+      if (id == cur) tv[b] = *reinterpret_cast<const uint4*>(tr + k);
+#pragma unroll
+      for (int t = 0; t < CT; ++t) {
+        const int n = n0 + 16 * t + c;
+        bv[b][t] = *reinterpret_cast<const uint4*>(B + (long long)(n < a.N ? n : a.N - 1) * r8 + kc);
+      }
+      k += 32;
+      if (k >= r8) {
+        left &= ~__ballot(id == cur);
+        k = 0;
+      }
+      held = b + 1;
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+      if (b < held) {
+#pragma unroll
+        for (int t = 0; t < CT; ++t) acc[t] = mfma_rows(bv[b][t], tv[b], acc[t]);
+      }
+  }
+#pragma unroll
+  for (int t = 0; t < CT; ++t) {
+    const int n = n0 + 16 * t + 4 * g;
+    if (!row || n >= a.N) continue;
+    if (id >= 0) {
+      sum[t].x += acc[t][0]; sum[t].y += acc[t][1]; sum[t].z += acc[t][2]; sum[t].w += acc[t][3];
+    }
+    *reinterpret_cast<uint2*>(a.y + (long long)m * a.ldy + n) =
+        make_uint2(pack_bf16x2_rne(sum[t].x, sum[t].y), pack_bf16x2_rne(sum[t].z, sum[t].w));
   }
 }
 
@@ -1622,6 +1668,18 @@ static hipError_t launch_plan(const QprojArgs& a, const RowPlan& p, F&& rows) {
   return hipGetLastError();
 }
 
+// 64 columns a wave reuse T, 16 fill the chip with waves where there are few.
+template <int MR, int CJ>
+static void launch_rows_sum(const RowsSum& a, hipStream_t s) {
+  const int low = (a.M + 15) / 16;
+  if ((long long)low * ((a.N + 255) / 256) < 512)
+    hipLaunchKernelGGL((split_rows_sum_kernel<MR, CJ, 1>), dim3((unsigned)((a.N + 63) / 64), (unsigned)low),
+                       dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((split_rows_sum_kernel<MR, CJ, 4>),
+                       dim3((unsigned)((a.N + 255) / 256), (unsigned)low), dim3(256), 0, s, a);
+}
+
 hipError_t launch_qproj_fast(int bits, const QprojArgs& a, hipStream_t s, const RowXaArgs* xa) {
   if (a.M <= 0 || a.N <= 0) return hipSuccess;
   if ((bits != 4 && bits != 8) || (xa && (a.kslices <= 1 || xa->M != a.M || xa->M >= kRowXaMany)))
@@ -1637,9 +1695,7 @@ hipError_t launch_qproj_fast(int bits, const QprojArgs& a, hipStream_t s, const 
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (a.rows.rid) {
-      hipLaunchKernelGGL(qproj_split_rows_reduce_kernel,
-                         dim3((unsigned)((a.N + 63) / 64), (unsigned)((a.M + 63) / 64)), dim3(256), 0,
-                         s, a);
+      launch_rows_sum<0, 0>({a.part, a.kslices, a.M, a.N, a.y, a.ldy, a.rows}, s);
       return hipGetLastError();
     }
     long long blocks = ((long long)a.M * (a.N / 4) + 255) / 256;
@@ -1835,11 +1891,10 @@ static hipError_t launch_xa_tiles(const LoraXaArgs& a, float* part, int kslices,
   long long blocks = (work / 2 + 255) / 256;
   if (blocks > 4096) blocks = 4096;
   if (a.rows.rid)
-    hipLaunchKernelGGL((lora_xa_reduce_kernel<MR, CJ, true>), dim3((unsigned)blocks), dim3(256), 0, s,
-                       part, kslices, a.M, a.n_cols, a);
+    launch_rows_sum<MR, CJ>({part, kslices, a.M, a.n_cols, a.t, a.ldt, a.rows}, s);
   else
-    hipLaunchKernelGGL((lora_xa_reduce_kernel<MR, CJ, false>), dim3((unsigned)blocks), dim3(256), 0,
-                       s, part, kslices, a.M, a.n_cols, a);
+    hipLaunchKernelGGL((lora_xa_reduce_kernel<MR, CJ>), dim3((unsigned)blocks), dim3(256), 0, s,
+                       part, kslices, a.M, a.n_cols, a);
   return hipGetLastError();
 }
 
@@ -1928,7 +1983,8 @@ hipError_t validate_qproj_fast_kernels() {
                        MING_QPROJ_ROWS(4), MING_QPROJ_ROWS(8),
 #undef MING_QPROJ_ROWS
                        reinterpret_cast<const void*>(&qproj_split_reduce_kernel),
-                       reinterpret_cast<const void*>(&qproj_split_rows_reduce_kernel),
+                       reinterpret_cast<const void*>(&split_rows_sum_kernel<0, 0, 1>),
+                       reinterpret_cast<const void*>(&split_rows_sum_kernel<0, 0, 4>),
                        reinterpret_cast<const void*>(&repack_fast_kernel),
                        reinterpret_cast<const void*>(&repack_sbf_kernel),
                        reinterpret_cast<const void*>(&bf16_to_f16_kernel),
@@ -1940,20 +1996,25 @@ hipError_t validate_qproj_fast_kernels() {
                        reinterpret_cast<const void*>(&lora_xa_rows_kernel<2, 2>),
                        reinterpret_cast<const void*>(&lora_xa_rows_kernel<4, 2>),
                        reinterpret_cast<const void*>(&lora_xa_fast_kernel<1, 1>),
-                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<1, 1, false>),
-                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<1, 1, true>),
+                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<1, 1>),
+                       reinterpret_cast<const void*>(&split_rows_sum_kernel<1, 1, 1>),
+                       reinterpret_cast<const void*>(&split_rows_sum_kernel<1, 1, 4>),
                        reinterpret_cast<const void*>(&lora_xa_fast_kernel<1, 2>),
-                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<1, 2, false>),
-                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<1, 2, true>),
+                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<1, 2>),
+                       reinterpret_cast<const void*>(&split_rows_sum_kernel<1, 2, 1>),
+                       reinterpret_cast<const void*>(&split_rows_sum_kernel<1, 2, 4>),
                        reinterpret_cast<const void*>(&lora_xa_fast_kernel<2, 1>),
-                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<2, 1, false>),
-                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<2, 1, true>),
+                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<2, 1>),
+                       reinterpret_cast<const void*>(&split_rows_sum_kernel<2, 1, 1>),
+                       reinterpret_cast<const void*>(&split_rows_sum_kernel<2, 1, 4>),
                        reinterpret_cast<const void*>(&lora_xa_fast_kernel<2, 2>),
-                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<2, 2, false>),
-                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<2, 2, true>),
+                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<2, 2>),
+                       reinterpret_cast<const void*>(&split_rows_sum_kernel<2, 2, 1>),
+                       reinterpret_cast<const void*>(&split_rows_sum_kernel<2, 2, 4>),
                        reinterpret_cast<const void*>(&lora_xa_fast_kernel<4, 2>),
-                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<4, 2, false>),
-                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<4, 2, true>)};
+                       reinterpret_cast<const void*>(&lora_xa_reduce_kernel<4, 2>),
+                       reinterpret_cast<const void*>(&split_rows_sum_kernel<4, 2, 1>),
+                       reinterpret_cast<const void*>(&split_rows_sum_kernel<4, 2, 4>)};
   for (const void* f : fns) {
     const hipError_t e = hipFuncGetAttributes(&fa, f);
     if (e != hipSuccess) return e;

@@ -18,8 +18,9 @@ namespace ming {
 //
 // Two forms. Few rows (row_xa_block; also beside a split projection's own blocks,
 // which need T in their sum alone): 16 rows, a chunk a block and turn, operands
-// straight from memory, all of a chunk's at once; `ny` blocks share out the chunks. Bound by three memory
-// latencies in a row (ids, table, A and x). Many rows (row_xa_many_kernel): x passes
+// straight from memory, all of a chunk's at once and under the chunk before it;
+// `ny` blocks share out the chunks. Bound by three memory latencies in a row (ids, table, A)
+// and, where every row brings its own adapter, by a chunk's own. Many rows (row_xa_many_kernel): x passes
 // through LDS in whole 1 KB row pieces, read from memory once for two (or four)
 // chunks and for the fp16 copy of x that a quantized projection multiplies. Bound by HBM, x
 // once and its copy once ([8704, 3840]: 79 us with x from memory a lane's 16 bytes
@@ -119,6 +120,8 @@ __device__ __forceinline__ void row_xa_block(const RowXaArgs& a, int bx, int by,
         xv[u][h] = *reinterpret_cast<const uint4*>(xr + 64 * kt + 32 * h);
     }
   };
+  const bool whole = KT <= XW * U;           // x fits the registers
+  if (whole) load_x(wave);                   // (while the adapters are looked up)
   const RowOf row = resolve(a, m);           // the wave's quarters hold the same rows
   if (by == 0 && wave == 0 && lane < 16 && m < a.M) a.rid[m] = row.id;
   if (a.xh) {
@@ -133,42 +136,98 @@ __device__ __forceinline__ void row_xa_block(const RowXaArgs& a, int bx, int by,
       }
     range_report(a.range, seen);
   }
-  int turn = 0;
-  bool there = false;
-  each_chunk(row, [&](int cur, int r8, const uint4* A, int ch) {
-    if (turn++ % ny != by) return;
-    const uint4* const ar = chunk_lane(A, r8, a.K, ch, lane);
-    floatx4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k0 = wave; k0 < KT; k0 += XW * U) {
-      uint4 av[U][2];
+  struct Held {
+    int id, r8, ch;
+  };
+  auto load_a = [&](uint4 (&av)[U][2], const uint4* ar, int k0) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int kt = k0 + XW * u < KT ? k0 + XW * u : KT - 1;
+    for (int u = 0; u < U; ++u) {
+      const int kt = k0 + XW * u < KT ? k0 + XW * u : KT - 1;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) av[u][h] = ar[64 * (2 * kt + h)];
-      }
-      if (!there) load_x(k0);
-      there = KT <= XW * U;
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (k0 + XW * u < KT) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) acc = mfma_rows(av[u][h], xv[u][h], acc);
-        }
+      for (int h = 0; h < 2; ++h) av[u][h] = ar[64 * (2 * kt + h)];
     }
+  };
+  auto sums = [&](const uint4 (&av)[U][2], int k0, floatx4_t& acc) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k0 + XW * u < KT) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) acc = mfma_rows(av[u][h], xv[u][h], acc);
+      }
+  };
+  // barriers for LDS alone: the next chunk's operands stay in flight over them
+  auto join = [&](const floatx4_t& acc, const Held& q) {
     red[wave][lane] = acc;
-    __syncthreads();
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (wave == 0) {
       floatx4_t v = red[0][lane];
 #pragma unroll
       for (int w = 1; w < XW; ++w) v += red[w][lane];
-      if (row.id == cur) store_t(a, m, row.coef, r8, ch + 4 * g, v);
+      if (row.id == q.id) store_t(a, m, row.coef, q.r8, q.ch + 4 * g, v);
     }
-    __syncthreads();
-  }, [&](int cur, int r8, int ch) {
-    if (by == 0 && wave == 0 && row.id == cur)
-      store_t(a, m, 0.0f, r8, ch + 4 * g, floatx4_t{0.0f, 0.0f, 0.0f, 0.0f});
-  });
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
+  auto finish = [&](const uint4 (&av)[U][2], const Held& q) {
+    floatx4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    sums(av, wave, acc);
+    join(acc, q);
+  };
+  // T's columns past the rank, up to whole 32
+  const int r16 = (row.e.r8 + 15) & ~15;
+  if (by == 0 && wave == 0 && row.id >= 0 && (r16 & 16))
+    store_t(a, m, 0.0f, row.e.r8, r16 + 4 * g, floatx4_t{0.0f, 0.0f, 0.0f, 0.0f});
+  // this block's next chunk and where its operand lies
+  uint64_t left = __ballot(row.id >= 0);
+  const uint64_t p = (uint64_t)(uintptr_t)row.e.A;
+  int turn = 0, at = 0;
+  auto next = [&](Held& q, const uint4*& ar) {
+    bool mine = false;
+    while (left && !mine) {
+      const int w = __builtin_ctzll(left);
+      q.id = __builtin_amdgcn_readlane(row.id, w);
+      q.r8 = __builtin_amdgcn_readlane(row.e.r8, w);
+      q.ch = at;
+      const uint64_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)p, w);
+      const uint64_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(p >> 32), w);
+      ar = chunk_lane(reinterpret_cast<const uint4*>((uintptr_t)(hi << 32 | lo)), q.r8, a.K, at, lane);
+      at += 16;
+      if (at >= q.r8) {
+        left &= ~__ballot(row.id == q.id);
+        at = 0;
+      }
+      mine = turn++ % ny == by;
+    }
+    return mine;
+  };
+  uint4 a0[U][2];
+  Held q0, q1;
+  const uint4* ar;
+  if (!whole) {
+    while (next(q0, ar)) {
+      floatx4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int k0 = wave; k0 < KT; k0 += XW * U) {
+        load_a(a0, ar, k0);
+        load_x(k0);
+        sums(a0, k0, acc);
+      }
+      join(acc, q0);
+    }
+    return;
+  }
+  // a chunk's operands in flight over the one before it
+  if (!next(q0, ar)) return;
+  load_a(a0, ar, wave);
+  uint4 a1[U][2];
+  while (true) {
+    const bool more = next(q1, ar);
+    if (more) load_a(a1, ar, wave);
+    finish(a0, q0);
+    if (!more) return;
+    const bool again = next(q0, ar);
+    if (again) load_a(a0, ar, wave);
+    finish(a1, q1);
+    if (!again) return;
+  }
 }
 
 }  // namespace ming
