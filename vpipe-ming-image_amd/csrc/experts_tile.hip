@@ -15,6 +15,8 @@
 // The grid is an upper bound (the groups' sizes are on the device): a block
 // finds its tile by find_group, the rest leave. An XCD takes a contiguous range
 // of tiles, an expert's columns outermost, so its L2 holds the weights in use.
+// [64][2048, 2048] gated: 32768 places in groups of 512, 234 us (1177 TFLOP/s); 34816
+// in uneven ones, 295 (matrix pipes 52% busy, 1.0 GB past the L2s).
 #include <type_traits>
 
 #include "common.h"

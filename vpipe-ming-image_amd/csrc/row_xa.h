@@ -19,12 +19,14 @@ namespace ming {
 // Two forms. Few rows (row_xa_block; also beside a split projection's own blocks,
 // which need T in their sum alone): 16 rows, a chunk a block and turn, operands
 // straight from memory, all of a chunk's at once and under the chunk before it;
-// `ny` blocks share out the chunks. Bound by three memory latencies in a row (ids, table, A)
-// and, where every row brings its own adapter, by a chunk's own. Many rows (row_xa_many_kernel): x passes
-// through LDS in whole 1 KB row pieces, read from memory once for two (or four)
-// chunks and for the fp16 copy of x that a quantized projection multiplies. Bound by HBM, x
-// once and its copy once ([8704, 3840]: 79 us with x from memory a lane's 16 bytes
-// at a time).
+// `ny` blocks share out the chunks. Bound by three memory latencies in a row (ids,
+// table, A) and, where every row brings its own adapter, by a chunk's bytes at a CU's
+// rate (7 us from 1 to 37 rows of [3840], as many adapters). Many rows
+// (row_xa_many_kernel): x passes through LDS in whole 1 KB row pieces, read from memory
+// once for two (or four) chunks and for the fp16 copy of x that a quantized projection
+// multiplies. Bound by HBM, x once and its copy once ([8704, 3840] with the copy: 38 to
+// 45 us, 79 with x from memory a lane's 16 bytes at a time).
+
 __device__ __forceinline__ uint4 to_f16(const uint4& v, uint32_t& seen) {
   seen = range_track4(seen, v);
   uint4 f;
