@@ -384,9 +384,9 @@ struct DensePlan {
   int slices;
 };
 DensePlan dense_split_plan(int M, int N, int K);
-// Whether a split takes its rows' x.A beside its own blocks.
-bool qproj_rows_beside(int M, int N, int kslices, int rf);
-bool dense_rows_beside(int M, int N, const DensePlan& p);
+// Blocks for 16 rows' x.A that a split can take beside its own; 0: none.
+int qproj_rows_beside(int M, int N, int kslices, int rf);
+int dense_rows_beside(int M, int N, const DensePlan& p);
 // xa: as launch_qproj_fast's, beside a dense weight's split.
 hipError_t launch_lora_xa_fast(const LoraXaArgs& a, float* part, int kslices,
                                hipStream_t s, const RowXaArgs* xa = nullptr);

@@ -1544,7 +1544,7 @@ bool qproj_merge_pays(int M, int N, int K, int nw) {
 // Blocks of rows' x.A beside `blocks` of a projection, one a CU: the chip's CUs left
 // over in its last round. 0 where they are fewer than one for every 16 rows: a
 // round of their own takes longer than a launch ([500, 3840] x [3840, 3840] w4: 31.7
-// us beside, 13.4 and 25.5 apart with x's fp16 copy in the first, 5.1 by itself).
+// us beside and 4.4 for x's fp16 copy, 24.5 and, with the copy, 9.0 apart).
 static int row_xa_blocks(int M, int blocks) {
   const int cus = device_cus(), tiles = (M + 15) / 16;
   const int free = (blocks + cus - 1) / cus * cus - blocks;
@@ -1552,32 +1552,36 @@ static int row_xa_blocks(int M, int blocks) {
   return tiles * (ny < 32 ? ny : 32);
 }
 
-bool qproj_rows_beside(int M, int N, int kslices, int rf) {
-  return M < kRowXaMany &&
-         row_xa_blocks(M, (M + 32 * rf - 1) / (32 * rf) * ((N + BN - 1) / BN) * kslices) > 0;
+// (the 256-row tiles' four waves would add T's sums in another order)
+int qproj_rows_beside(int M, int N, int kslices, int rf) {
+  if (M >= kRowXaMany || rf > 4) return 0;
+  return row_xa_blocks(M, (M + 32 * rf - 1) / (32 * rf) * ((N + BN - 1) / BN) * kslices) /
+         ((M + 15) / 16);
 }
 
-bool dense_rows_beside(int M, int N, const DensePlan& p) {
+int dense_rows_beside(int M, int N, const DensePlan& p) {
   const int xr = 64 * p.tile.mr, xc = 64 * p.tile.cj;
-  return M < kRowXaMany &&
-         row_xa_blocks(M, (M + xr - 1) / xr * ((N + xc - 1) / xc) * p.slices) > 0;
+  if (M >= kRowXaMany) return 0;
+  return row_xa_blocks(M, (M + xr - 1) / xr * ((N + xc - 1) / xc) * p.slices) / ((M + 15) / 16);
 }
 
 template <int BITS, bool SPLIT, int RF, int NW>
 static void launch_tiles(const QprojArgs& a, hipStream_t s, const RowXaArgs* xa = nullptr) {
   const int tiles = ((a.M + 32 * RF - 1) / (32 * RF)) * ((a.N + BN - 1) / BN);
   const int blocks = SPLIT ? tiles * a.kslices : tiles;
-  if constexpr (SPLIT) {
+  if constexpr (SPLIT && RF <= 4) {
     if (xa) {
       const int first = row_xa_blocks(xa->M, blocks);
       hipLaunchKernelGGL((qproj_split_rows_kernel<BITS, RF, NW>), dim3((unsigned)(blocks + first)),
                          dim3(64 * NW), 0, s, a, *xa, first);
       return;
     }
-  } else if (a.rows.counts) {
-    hipLaunchKernelGGL((qproj_rows_kernel<BITS, RF, NW>), dim3((unsigned)blocks), dim3(64 * NW), 0,
-                       s, a);
-    return;
+  } else if constexpr (!SPLIT) {
+    if (a.rows.counts) {
+      hipLaunchKernelGGL((qproj_rows_kernel<BITS, RF, NW>), dim3((unsigned)blocks), dim3(64 * NW), 0,
+                         s, a);
+      return;
+    }
   }
   hipLaunchKernelGGL((qproj_fast_kernel<BITS, SPLIT, RF, NW>), dim3((unsigned)blocks),
                      dim3(64 * NW), 0, s, a);
@@ -1682,7 +1686,7 @@ static void launch_rows_sum(const RowsSum& a, hipStream_t s) {
 
 hipError_t launch_qproj_fast(int bits, const QprojArgs& a, hipStream_t s, const RowXaArgs* xa) {
   if (a.M <= 0 || a.N <= 0) return hipSuccess;
-  if ((bits != 4 && bits != 8) || (xa && (a.kslices <= 1 || xa->M != a.M || xa->M >= kRowXaMany)))
+  if ((bits != 4 && bits != 8) || (xa && (a.kslices <= 1 || xa->M != a.M || !qproj_rows_beside(a.M, a.N, a.kslices, a.split_rf))))
     return hipErrorInvalidValue;
   if (a.kslices > 1) {
     if (!a.part || a.N % 4 != 0 || (long long)a.M * (a.N / 4) >= (1ll << 31) ||
@@ -1978,8 +1982,7 @@ hipError_t validate_qproj_fast_kernels() {
       reinterpret_cast<const void*>(&qproj_rows_kernel<BITS, 6, 8>),      \
       reinterpret_cast<const void*>(&qproj_rows_kernel<BITS, 8, 4>),      \
       reinterpret_cast<const void*>(&qproj_split_rows_kernel<BITS, 2, 8>), \
-      reinterpret_cast<const void*>(&qproj_split_rows_kernel<BITS, 4, 8>), \
-      reinterpret_cast<const void*>(&qproj_split_rows_kernel<BITS, 8, 4>)
+      reinterpret_cast<const void*>(&qproj_split_rows_kernel<BITS, 4, 8>)
                        MING_QPROJ_ROWS(4), MING_QPROJ_ROWS(8),
 #undef MING_QPROJ_ROWS
                        reinterpret_cast<const void*>(&qproj_split_reduce_kernel),

@@ -21,7 +21,7 @@ namespace ming {
 // straight from memory, all of a chunk's at once and under the chunk before it;
 // `ny` blocks share out the chunks. Bound by three memory latencies in a row (ids,
 // table, A) and, where every row brings its own adapter, by a chunk's bytes at a CU's
-// rate (7 us from 1 to 37 rows of [3840], as many adapters). Many rows
+// rate (4.8 us at 4 rows of [3840], 8.7 at 37, as many adapters). Many rows
 // (row_xa_many_kernel): x passes through LDS in whole 1 KB row pieces, read from memory
 // once for two (or four) chunks and for the fp16 copy of x that a quantized projection
 // multiplies. Bound by HBM, x once and its copy once ([8704, 3840] with the copy: 38 to
@@ -181,25 +181,29 @@ __device__ __forceinline__ void row_xa_block(const RowXaArgs& a, int bx, int by,
   // this block's next chunk and where its operand lies
   uint64_t left = __ballot(row.id >= 0);
   const uint64_t p = (uint64_t)(uintptr_t)row.e.A;
-  int turn = 0, at = 0;
+  int skip = by, at = 0;                     // chunks of other blocks, then this adapter's
   auto next = [&](Held& q, const uint4*& ar) {
-    bool mine = false;
-    while (left && !mine) {
+    while (left) {
       const int w = __builtin_ctzll(left);
       q.id = __builtin_amdgcn_readlane(row.id, w);
       q.r8 = __builtin_amdgcn_readlane(row.e.r8, w);
-      q.ch = at;
+      const int n = (q.r8 + 15) / 16;
+      if (at + skip >= n) {
+        skip -= n - at;
+        at = 0;
+        left &= ~__ballot(row.id == q.id);
+        continue;
+      }
+      q.ch = 16 * (at + skip);
+      at += skip + 1;
+      skip = ny - 1;
       const uint64_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)p, w);
       const uint64_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(p >> 32), w);
-      ar = chunk_lane(reinterpret_cast<const uint4*>((uintptr_t)(hi << 32 | lo)), q.r8, a.K, at, lane);
-      at += 16;
-      if (at >= q.r8) {
-        left &= ~__ballot(row.id == q.id);
-        at = 0;
-      }
-      mine = turn++ % ny == by;
+      ar = chunk_lane(reinterpret_cast<const uint4*>((uintptr_t)(hi << 32 | lo)), q.r8, a.K, q.ch,
+                      lane);
+      return true;
     }
-    return mine;
+    return false;
   };
   uint4 a0[U][2];
   Held q0, q1;

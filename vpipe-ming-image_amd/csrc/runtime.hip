@@ -199,6 +199,7 @@ struct ming_adapters {
   ming_ctx* ctx = nullptr;
   int N = 0, K = 0, cap = 0, max_rank = 0, ldt = 0;
   std::vector<LoraBind> bound;
+  int held = 0, chunks = 0;              // adapters bound, their 16-rank chunks
   ming::AdapterEntry* table = nullptr;   // [cap], device
 };
 
@@ -1293,9 +1294,16 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
       ra.stride = xr.stride;
       ra.zero = (uint32_t)((size_t)M * ra.ldt * 2);
     }
-    rows_beside = split && (fast[0] ? ming::qproj_rows_beside(M, qs[0]->N, split_ks[0],
-                                                              qa[0].split_rf)
-                                    : ming::dense_rows_beside(M, qs[0]->N, dense_plan[0]));
+    // Beside the split where its blocks have at most five 16-rank chunks each, were
+    // every row of a tile its own request: they pass at 2 us a chunk, a launch of its
+    // own takes 5 to 9 ([3840, 3840] dense, 37 rows of as many adapters of 16 to 64
+    // ranks: 26.2 us beside, 10.8 and 8.7 apart; 700 rows of 32 in turn: 83, 31 and 20;
+    // 37 rows of five requests, w4: 11.5 beside, 9.6 and 6 apart).
+    const int ny = !split    ? 0
+                   : fast[0] ? ming::qproj_rows_beside(M, qs[0]->N, split_ks[0], qa[0].split_rf)
+                             : ming::dense_rows_beside(M, qs[0]->N, dense_plan[0]);
+    const double held = std::max(rows->bank->held, 1);
+    rows_beside = ny > 0 && std::min({16.0, held, (double)M}) * rows->bank->chunks / held <= 5.0 * ny;
     if (!plane) qa[0].rows = ra;
     if (xh_bytes) xh = (const uint16_t*)carve->take(xh_bytes);
     if (part_bytes) part = (float*)carve->take(part_bytes);
@@ -1656,6 +1664,8 @@ static int adapters_replace(ming_adapters* b, int id, const LoraBind& nb) {
   LoraBind& old = b->bound[id];
   if (old.A) (void)hipFree(old.A);
   if (old.B) (void)hipFree(old.B);
+  b->held += (nb.rank > 0) - (old.rank > 0);
+  b->chunks += (nb.rank8 + 15) / 16 - (old.rank8 + 15) / 16;
   old = nb;
   return MING_OK;
 }
