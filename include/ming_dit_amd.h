@@ -440,7 +440,7 @@ int ming_adapters_rank(const ming_adapters* bank, int id);
  * is 0, is ming_lin's row without adapters. The adapters' sum joins the f32
  * result before the one rounding; a row's bits do not depend on the other rows'
  * adapters (but for the sign of a zero). Slots bound on the weight take no part.
- * x as ming_lin's, y 16-byte aligned with ldy % 8 == 0; none of x, row_adapter and
+ * M below 2^28. x as ming_lin's, y 16-byte aligned with ldy % 8 == 0; none of x, row_adapter and
  * row_scale shares memory with y or ws. The size is that of x rows beside each
  * other; a dense projection of x rows that span more than 2 GiB may need more, and
  * says how much (MING_ERR_SHAPE). */

@@ -350,6 +350,40 @@ def test_dense_splits(ctx, M, N, K):
     qw.close()
 
 
+@pytest.mark.parametrize("bits,M,N,K", [(4, 1500, 2040, 1088), (8, 1500, 2040, 1088),
+                                        (16, 3000, 1024, 4096)])
+def test_sums_of_many_rows(ctx, bits, M, N, K):
+    """A split whose sum has work for the chip in its widest blocks."""
+    assert (split_plan(M, N, K)[0] if bits != 16 else dense_plan(M, N, K)[2]) >= 2
+    assert (M + 15) // 16 * ((N + 255) // 256) >= 512
+    qw, w = weight(ctx, 17800, N, K, bits)
+    bank, held = make_bank(ctx, 17900, N, K, RANKS)
+    x = bf16(randn(18000, (M, K)))
+    ids, s = requests(M, 6, len(RANKS), cuts=30)
+    ids[100:140] = np.arange(40) % len(RANKS)             # a row its own, in turn
+    some = np.unique(np.concatenate([np.arange(0, M, 13), np.arange(96, 144), [M - 1]]))
+    got = call(ctx, qw, bank, x, ids, s)[some]
+    check(got, x[some], w, held, ids[some], s[some], bits)
+    bank.close()
+    qw.close()
+
+
+@pytest.mark.parametrize("bits,M,N,K", [(4, 37, 1024, 2048), (8, 64, 2048, 1088),
+                                        (16, 37, 1024, 2048), (16, 130, 512, 4096)])
+def test_bits_do_not_depend_on_the_bank(ctx, bits, M, N, K):
+    """A bank of two adapters and one of forty run other launches to the same bits."""
+    qw, w = weight(ctx, 18100, N, K, bits)
+    few, held = make_bank(ctx, 18200, N, K, (24, 64), cap=40, max_rank=64)
+    many, _ = make_bank(ctx, 18200, N, K, (24, 64) + (64,) * 38)
+    x = bf16(randn(18300 + M, (M, K)))
+    ids, s = np.arange(M) % 3 - 1, np.linspace(-1, 1, M).astype(np.float32)
+    a = call(ctx, qw, few, x, ids, s)
+    check(a, x, w, held, ids, s, bits)
+    assert np.array_equal(call(ctx, qw, many, x, ids, s), a)
+    for h in (few, many, qw):
+        h.close()
+
+
 def test_two_contexts_at_once(ctx):
     """Calls on two streams, a workspace each, over one x: the bits of one alone."""
     N, K, M = 1024, 2048, 200
@@ -450,6 +484,9 @@ def test_refusals(ctx):
                {"ws": ws[4:]}):
         with pytest.raises(m.MingError):
             ctx.lin_adapters(**dict(ok, **kw))
+    with pytest.raises(m.MingError, match="2\\^28"):
+        ctx.lin_adapters(**dict(ok, M=1 << 28, row_adapter=1 << 50, y=1 << 56))
+    assert ctx.lin_adapters_workspace_bytes(qw, bank, 2 ** 31 - 1) == 0
     ctx.lin_adapters(**dict(ok, M=0))
     wide, _ = make_bank(ctx, 16200, 72, K, (8,))
     with pytest.raises(m.MingError, match="shape"):

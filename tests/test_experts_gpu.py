@@ -350,6 +350,32 @@ def test_shared_memory_and_sizes(ctx, cut, bits, kernel):
     ex.close()
 
 
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("offsets", [[0, 300, 0, 300, 0, 300, 0], [300, 200, 100, 0, -5, 7, 9],
+                                     [-9, 400, 2 ** 31 - 1, -2 ** 31, 50, 60, 2 ** 31 - 1],
+                                     [7, 7, 7, 7, 7, 7, 7]])
+def test_what_is_no_plan_stays_inside(ctx, cut, bits, offsets):
+    """Offsets that descend or leave the places, an order out of range: some rows of y,
+    none outside, and the context goes on."""
+    E, N, K, n = 6, 272, 128, 300
+    ex, w = ref.make_experts(ctx, 13500, E, N, K, bits)
+    x = bf16(randn(13600, (20, K)))
+    order = np.random.default_rng(1).integers(-2 ** 31, 2 ** 31, n).astype(np.int32)
+    xd, offd, od = to_dev(x), to_dev(np.array(offsets, np.int32)), to_dev(order)
+    ws = torch.empty(max(1, ex.workspace_bytes(20)), dtype=torch.uint8, device="cuda")
+    for c in ref.CUTS[bits]:
+        cut(c)
+        y = torch.full(((n + 4) * N,), SENTINEL, dtype=torch.int16, device="cuda")
+        sync()
+        ctx.experts_lin(ex, xd, 20, od, offd, n, y[2 * N:], fan=1, ws=ws)
+        ctx.synchronize()
+        assert bool((y[:2 * N] == SENTINEL).all()) and bool((y[(n + 2) * N:] == SENTINEL).all())
+    good, order, src = ref.plan_of([40, 0, 60, 0, 0, 200], x_rows=20)
+    cut(-1)
+    check(run(ctx, ex, False, x, good, order, order.size), w, x, good, src, False, bits)
+    ex.close()
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 def test_create_refusals(ctx, bits):
     pack, _ = ref.stack(12800, 2, 16, 64, bits)

@@ -36,6 +36,9 @@ __device__ __forceinline__ RowGroup find_group(const int32_t* __restrict__ offse
     sum += count(lo, hi);
     lo = hi;
   }
+  // A launch holds fewer units than 2^24 and no group of a plan more; the lanes of
+  // what is no plan are cut so that their total stays an int.
+  sum = sum < (1 << 25) - 1 ? sum : (1 << 25) - 1;
   int run = sum;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {

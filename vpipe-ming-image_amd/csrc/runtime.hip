@@ -1740,6 +1740,8 @@ int ming_adapters_rank(const ming_adapters* b, int id) {
   return b && id >= 0 && id < b->cap ? b->bound[id].rank : 0;
 }
 
+constexpr int kRowsMax = 1 << 28;   // the x.A's 32-row tiles in one launch
+
 // Shared by the call and its size: the projection planned with its rows'
 // adapters, its scratch from `cv`.
 static int lin_adapters(ming_ctx* c, const ming_qweight* qw, const ming_adapters* bank,
@@ -1760,7 +1762,7 @@ static int lin_adapters(ming_ctx* c, const ming_qweight* qw, const ming_adapters
 
 size_t ming_lin_adapters_workspace_bytes(ming_ctx* c, const ming_qweight* qw,
                                          const ming_adapters* bank, int M) {
-  if (!c || !qw || !bank || M <= 0) return 0;
+  if (!c || !qw || !bank || M <= 0 || M >= kRowsMax) return 0;
   Carve cv;
   cv.measure = true;
   cv.cap = SIZE_MAX;
@@ -1778,6 +1780,7 @@ int ming_lin_adapters(ming_ctx* c, const ming_qweight* qw, const ming_adapters* 
   if (!aligned(ws, 16) || !aligned(row_adapter, 4) || !aligned(row_scale, 4))
     return fail(MING_ERR_ARG,
                 "ming_lin_adapters: ws must be 16-byte, ids and strengths 4-byte aligned");
+  if (M >= kRowsMax) return fail(MING_ERR_SHAPE, "ming_lin_adapters: M must be below 2^28");
   // rows of y that do not take 16-byte stores would have a plan of their own, with
   // another workspace
   if (!aligned(y, 16) || ldy % 8 != 0)
