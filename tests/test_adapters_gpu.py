@@ -384,6 +384,30 @@ def test_bits_do_not_depend_on_the_bank(ctx, bits, M, N, K):
         h.close()
 
 
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("M,N,K", [(6, 64, 128), (200, 264, 128), (300, 1024, 2048)])
+def test_outputs_past_32_bits(ctx, bits, M, N, K):
+    """Rows of y more than 2^32 bytes apart: the bits of rows beside each other."""
+    ld = 1 << 30 if M == 6 else 1 << 24
+    qw, _ = weight(ctx, 18400, N, K, bits)
+    bank, _ = make_bank(ctx, 18500, N, K, RANKS)
+    x = bf16(randn(18600, (M, K)))
+    ids, s = requests(M, 8, len(RANKS))
+    want = call(ctx, qw, bank, x, ids, s)
+    y = torch.empty((M, ld), dtype=torch.int16, device="cuda")
+    xd, idd, sd = to_dev(x), to_dev(ids.astype(np.int32)), to_dev(s)
+    ws = torch.empty(ctx.lin_adapters_workspace_bytes(qw, bank, M), dtype=torch.uint8,
+                     device="cuda")
+    sync()
+    ctx.lin_adapters(qw, bank, xd, y, M, idd, sd, ws, ldy=ld)
+    ctx.synchronize()
+    assert np.array_equal(from_dev(y[:, :N].contiguous()), want)
+    del y
+    torch.cuda.empty_cache()
+    bank.close()
+    qw.close()
+
+
 def test_two_contexts_at_once(ctx):
     """Calls on two streams, a workspace each, over one x: the bits of one alone."""
     N, K, M = 1024, 2048, 200

@@ -350,6 +350,38 @@ def test_shared_memory_and_sizes(ctx, cut, bits, kernel):
     ex.close()
 
 
+@pytest.mark.parametrize("bits", [4, 8, 16])
+def test_outputs_past_32_bits(ctx, cut, bits):
+    """Rows of y more than 2^32 bytes apart, and their sum from there."""
+    E, N, K, n, ld = 3, 272, 128, 200, 1 << 24
+    ex, w = ref.make_experts(ctx, 13700, E, N, K, bits)
+    offsets, order, src = ref.plan_of([90, 0, 110], x_rows=40)
+    x = bf16(randn(13800, (40, K)))
+    xd, offd, od = to_dev(x), to_dev(offsets), to_dev(order)
+    ws = torch.empty(max(1, ex.workspace_bytes(40)), dtype=torch.uint8, device="cuda")
+    y = torch.empty((n, ld), dtype=torch.int16, device="cuda")
+    for c in ref.CUTS[bits]:
+        cut(c)
+        y[:, :N + 8] = SENTINEL
+        sync()
+        ctx.experts_lin(ex, xd, 40, od, offd, n, y, ws=ws, ldy=ld)
+        ctx.synchronize()
+        got = from_dev(y[:, :N + 8].contiguous())
+        assert np.all(got[:, N:] == SENTINEL)
+        check(got[:, :N], w, x, offsets, src, False, bits)
+    place = np.random.default_rng(2).permutation(n).astype(np.int32).reshape(n // 2, 2)
+    wt = np.linspace(-1, 1, n, dtype=np.float32).reshape(n // 2, 2)
+    pd, wd, out = to_dev(place), to_dev(wt), to_dev(np.zeros((n // 2, N), np.uint16))
+    sync()
+    ctx.experts_combine(y, n, pd, wd, n // 2, 2, out, N, ldy=ld)
+    ctx.synchronize()
+    want, bound = ref.combine(f32(got[:, :N]), place, wt, None, n)
+    assert np.all(np.abs(f32(from_dev(out)) - want) <= bound)
+    del y
+    torch.cuda.empty_cache()
+    ex.close()
+
+
 @pytest.mark.parametrize("bits", [4, 16])
 @pytest.mark.parametrize("offsets", [[0, 300, 0, 300, 0, 300, 0], [300, 200, 100, 0, -5, 7, 9],
                                      [-9, 400, 2 ** 31 - 1, -2 ** 31, 50, 60, 2 ** 31 - 1],
