@@ -85,11 +85,14 @@ __device__ __forceinline__ void operands(const Raw<BITS>& r, uint4& w0, uint4& w
 // the weights of the experts that have rows, once (w4 and w8, by the codes'
 // conversion: 3.3 and 4.6 weights a ps). Blocks of 16 (gated) or 32 columns leave
 // thousands of them, so loads of many are in flight: [64][2048, 2048] dense, gated,
-// 64 places 59 us, 303 MB at 5.1 TB/s; [60][2048, 1024] w8, 16 places 13.0.
-template <int BITS, bool GATED, int WK, int CO>
+// 64 places 59 us, 303 MB at 5.1 TB/s; [60][2048, 1024] w8, 16 places 10.9.
+//
+// WK waves with U groups in flight, by K: 8 with 2 (4 cost registers, so waves: 20 to
+// 55% longer), to K = 1024 with 1 ([60][2048, 1024] w8, 64 places 31.1 -> 26.0 us; K 7168
+// 8% slower), to 512 4 waves ([64][2048, 512] w8 gated, 64 places 14.1, eight 19.4).
+template <int BITS, bool GATED, int WK, int U, int CO>
 __global__ __launch_bounds__(64 * WK) void experts_rows_kernel(const ExpertsArgs a) {
   constexpr int CT = GATED ? 2 * CO : CO;  // column tiles: the outputs', then the up rows'
-  constexpr int U = WK == 4 || CT > 4 ? 1 : 4 / CT;   // groups of a wave in flight
   const RowGroup rg =
       find_group(a.offsets, a.E, a.n, [](int) { return 1; }, [](int) { return (int)blockIdx.y; });
   if (rg.e < 0) return;
@@ -193,9 +196,11 @@ void rows_shape(const ExpertsArgs& a, hipStream_t s) {
   constexpr int CO = GATED ? 1 : 2;
   const dim3 grid((unsigned)((a.N + 16 * CO - 1) / (16 * CO)), (unsigned)(a.n < a.E ? a.n : a.E));
   if (a.K <= 512)
-    hipLaunchKernelGGL((experts_rows_kernel<BITS, GATED, 4, CO>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((experts_rows_kernel<BITS, GATED, 4, 1, CO>), grid, dim3(256), 0, s, a);
+  else if (a.K <= 1024)
+    hipLaunchKernelGGL((experts_rows_kernel<BITS, GATED, 8, 1, CO>), grid, dim3(512), 0, s, a);
   else
-    hipLaunchKernelGGL((experts_rows_kernel<BITS, GATED, 8, CO>), grid, dim3(512), 0, s, a);
+    hipLaunchKernelGGL((experts_rows_kernel<BITS, GATED, 8, 2, CO>), grid, dim3(512), 0, s, a);
 }
 
 // w [NW][K] -> [K / 64][NW][64], 16 bytes a thread and step.
@@ -237,11 +242,13 @@ hipError_t launch_experts_rows(int bits, bool gated, const ExpertsArgs& a, hipSt
 hipError_t validate_experts_kernels() {
   hipFuncAttributes fa;
   const void* fns[] = {
-#define MING_EXPERTS_ROWS(BITS)                                                \
-  reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 4, 2>),      \
-      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 8, 2>),  \
-      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 4, 1>),   \
-      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 8, 1>)
+#define MING_EXPERTS_ROWS(BITS)                                                   \
+  reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 4, 1, 2>),      \
+      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 8, 1, 2>),  \
+      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 8, 2, 2>),  \
+      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 4, 1, 1>),   \
+      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 8, 1, 1>),   \
+      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 8, 2, 1>)
       reinterpret_cast<const void*>(&repack_dense_kernel),
       MING_EXPERTS_ROWS(4), MING_EXPERTS_ROWS(8), MING_EXPERTS_ROWS(16)
 #undef MING_EXPERTS_ROWS

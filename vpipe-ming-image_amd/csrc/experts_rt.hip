@@ -29,11 +29,11 @@ namespace ming {
 // places out of cold caches; where they are close, so are the kernels.
 //   few rows, dense: 2.5 + bytes / 5.9 TB/s, longer by the rows' own reads (swiglu
 //     of [64][2048, 2048], 8 places: 14.6, the tiles 17.5); w4 and w8: the codes'
-//     conversion, 3.3 and 4.6 weights a ps ([60][2048, 1024] w8, 16 places: 13.0, the
+//     conversion, 3.3 and 4.6 weights a ps ([60][2048, 1024] w8, 16 places: 10.9, the
 //     tiles 15.4); a start a block; 16 rows a pass over the weights.
 //   tiles: a start and the K stages of one, then the weights at 5.6 to 6.1 TB/s, a
 //     round of the chip (one dense block a CU) at least that again (dense as above, 64
-//     places: 74.1, few rows 68.8; 128: 85.4 and 89.6; w8 as above, 64: 25.0 and 33.8).
+//     places: 74.1, few rows 68.8; 128: 85.4 and 89.6; w8 as above, 64: 25.0 and 27.9).
 //     They have to win by 8%: x's fp16 copy grows with x.
 // Cuts (low / tall, us): more rows a tile read the weights less often and, quantized,
 // convert them less often; fewer fill the chip where there are few tiles. Dense, 128
