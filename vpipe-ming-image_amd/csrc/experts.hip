@@ -19,9 +19,13 @@ __device__ __forceinline__ float f16_hi(uint32_t u) {
   return (float)__builtin_bit_cast(_Float16, (uint16_t)(u >> 16));
 }
 
-// One 64-group of weight row n, the 16 values k 16g..16g+15, as the A operands
-// of two v_mfma_f32_16x16x32_bf16: dense weights as they are, codes as the
-// integers they hold (exact in bf16).
+// One 64-group of weight row n, lane quarter g's 16 values as the A operands of two
+// v_mfma_f32_16x16x32_bf16: dense weights as they are, w8 codes as the integers they
+// hold, w4 codes as 128 more (0x43 over a code is that in bf16, so two codes are a
+// v_perm; the group's bias takes the 128 scales off again). Which k a quarter has is
+// free as long as x's agree (x_at): they are what one wide load brings, with the lanes
+// of a row side by side (w4 as two 4-byte loads a lane: [64][2048, 2048] gated, 8 places
+// 13.9 us, 8.5 so).
 template <int BITS>
 struct Raw {
   uint4 v[BITS == 16 ? 2 : 1];
@@ -31,28 +35,36 @@ __device__ __forceinline__ void load_group(const ExpertsArgs& a, const void* w, 
                                            int g, Raw<BITS>& r) {
   if constexpr (BITS == 16) {
     const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(w) +
-                                                    ((long long)kt * a.NW + n) * 64 + 16 * g);
+                                                    ((long long)kt * a.NW + n) * 64 + 8 * g);
     r.v[0] = p[0];
-    r.v[1] = p[1];
+    r.v[1] = p[4];
   } else {
-    // [kt][n][fk][kk] words: k 16 kk + 8 fk + 0..7
-    const uint32_t* p = static_cast<const uint32_t*>(w) + ((long long)kt * a.NW + n) * (2 * BITS);
+    // [kt][n][fk][kk] (w8: two words each): k 16 kk + 8 fk + 0..7, a quarter's kk 2 (g & 1)
+    // and the next of fk g >> 1 in one load
+    const uint32_t* p =
+        static_cast<const uint32_t*>(w) + ((long long)kt * a.NW + n) * (2 * BITS) + BITS / 2 * g;
     if constexpr (BITS == 4) {
-      r.v[0] = make_uint4(p[g], p[4 + g], 0, 0);
+      const uint2 c = *reinterpret_cast<const uint2*>(p);
+      r.v[0] = make_uint4(c.x, c.y, 0, 0);
     } else {
-      const uint2 c = *reinterpret_cast<const uint2*>(p + 2 * g);
-      const uint2 d = *reinterpret_cast<const uint2*>(p + 8 + 2 * g);
-      r.v[0] = make_uint4(c.x, c.y, d.x, d.y);
+      r.v[0] = *reinterpret_cast<const uint4*>(p);
     }
   }
 }
+// k of quarter g's two 8-value pieces of x: the first, and how far the second.
+template <int BITS>
+__device__ __forceinline__ int x_at(int g) {
+  return BITS == 16 ? 8 * g : 32 * (g & 1) + 8 * (g >> 1);
+}
+template <int BITS>
+constexpr int kXStep = BITS == 16 ? 32 : 16;
 template <int BITS>
 __device__ __forceinline__ void operands(const Raw<BITS>& r, uint4& w0, uint4& w1) {
   if constexpr (BITS == 16) {
     w0 = r.v[0];
     w1 = r.v[1];
   } else {
-    auto bytes = [](uint32_t c, uint32_t d) {
+    [[maybe_unused]] auto bytes = [](uint32_t c, uint32_t d) {
       uint4 o;
       o.x = pack_bf16x2_rne(byte_f(c, 0), byte_f(c, 1));
       o.y = pack_bf16x2_rne(byte_f(c, 2), byte_f(c, 3));
@@ -62,10 +74,12 @@ __device__ __forceinline__ void operands(const Raw<BITS>& r, uint4& w0, uint4& w
     };
     if constexpr (BITS == 4) {
       // nibbles {k0,k4,k1,k5,k2,k6,k3,k7}: the even ones are k0..k3 by byte
-      auto word = [&](uint32_t c) {
-        uint32_t lo = c & 0x0F0F0F0Fu, hi = (c >> 4) & 0x0F0F0F0Fu;
-        asm("" : "+v"(lo), "+v"(hi));   // kept as two masks, a conversion a byte
-        return bytes(lo, hi);
+      auto word = [](uint32_t c) {
+        const uint32_t lo = c & 0x0F0F0F0Fu, hi = (c >> 4) & 0x0F0F0F0Fu;
+        return make_uint4(__builtin_amdgcn_perm(0x43434343u, lo, 0x05010400u),
+                          __builtin_amdgcn_perm(0x43434343u, lo, 0x05030402u),
+                          __builtin_amdgcn_perm(0x43434343u, hi, 0x05010400u),
+                          __builtin_amdgcn_perm(0x43434343u, hi, 0x05030402u));
       };
       w0 = word(r.v[0].x);
       w1 = word(r.v[0].y);
@@ -116,7 +130,7 @@ __global__ __launch_bounds__(64 * WK) void experts_rows_kernel(const ExpertsArgs
       src = a.order[p] / a.fan;
       src = src < 0 ? 0 : src < a.x_rows ? src : a.x_rows - 1;
     }
-    const uint16_t* const xr = a.x + (long long)src * a.ldx + 16 * g;
+    const uint16_t* const xr = a.x + (long long)src * a.ldx + x_at<BITS>(g);
     floatx4_t acc[CT];
 #pragma unroll
     for (int t = 0; t < CT; ++t) acc[t] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
@@ -130,7 +144,7 @@ __global__ __launch_bounds__(64 * WK) void experts_rows_kernel(const ExpertsArgs
         if (kt < KT) {
           const uint4* xp = reinterpret_cast<const uint4*>(xr + 64 * kt);
           x[u][0] = xp[0];
-          x[u][1] = xp[1];
+          x[u][1] = xp[kXStep<BITS> / 8];
 #pragma unroll
           for (int t = 0; t < CT; ++t) {
             // columns past N (a multiple of 8) compute the last ones, never store
@@ -161,8 +175,11 @@ __global__ __launch_bounds__(64 * WK) void experts_rows_kernel(const ExpertsArgs
               const floatx4_t d = mfma16(w1, x[u][1], mfma16(w0, x[u][0], zero));
               const uint32_t* sp = &sb[u][t].x;
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                acc[t][r] += __builtin_fmaf(f16_lo(sp[r]), d[r], f16_hi(sp[r]) * sx[r]);
+              for (int r = 0; r < 4; ++r) {
+                const float s = f16_lo(sp[r]);
+                const float b = BITS == 4 ? __builtin_fmaf(-128.0f, s, f16_hi(sp[r])) : f16_hi(sp[r]);
+                acc[t][r] += __builtin_fmaf(s, d[r], b * sx[r]);
+              }
             }
           }
         }

@@ -33,7 +33,7 @@ namespace ming {
 //     tiles 15.4); a start a block; 16 rows a pass over the weights.
 //   tiles: a start and the K stages of one, then the weights at 5.6 to 6.1 TB/s, a
 //     round of the chip (one dense block a CU) at least that again (dense as above, 64
-//     places: 74.1, few rows 68.8; 128: 85.4 and 89.6; w8 as above, 64: 25.0 and 27.9).
+//     places: 74.1, few rows 68.8; 128: 85.4 and 89.6; w8 as above, 64: 25.0 and 26.1).
 //     They have to win by 8%: x's fp16 copy grows with x.
 // Cuts (low / tall, us): more rows a tile read the weights less often and, quantized,
 // convert them less often; fewer fill the chip where there are few tiles. Dense, 128
