@@ -96,8 +96,8 @@ __device__ __forceinline__ void operands(const Raw<BITS>& r, uint4& w0, uint4& w
 // LDS and are added in class order, so the bits depend on K alone. Quantized
 // weights multiply as integers: scale * sum(q x) + bias * sum(x) a group, in
 // f32, the activations as the bf16 they are (no range limit). Bound by HBM:
-// the weights of the experts that have rows, once (w4 and w8, by the codes'
-// conversion: 3.3 and 4.6 weights a ps). Blocks of 16 (gated) or 32 columns leave
+// the weights of the experts that have rows, once (w4 and w8, by the loads beside
+// them, x and scales: 6 and 5 weights a ps). Blocks of 16 (gated) or 32 columns leave
 // thousands of them, so loads of many are in flight: [64][2048, 2048] dense, gated,
 // 64 places 59 us, 303 MB at 5.1 TB/s; [60][2048, 1024] w8, 16 places 10.9.
 //

@@ -28,12 +28,13 @@ namespace ming {
 // times below are fits (us) to [16 to 256][1024 to 4096, 1024 to 4096] at 8 to 384
 // places out of cold caches; where they are close, so are the kernels.
 //   few rows, dense: 2.5 + bytes / 5.9 TB/s, longer by the rows' own reads (swiglu
-//     of [64][2048, 2048], 8 places: 14.6, the tiles 17.5); w4 and w8: the codes'
-//     conversion, 3.3 and 4.6 weights a ps ([60][2048, 1024] w8, 16 places: 10.9, the
-//     tiles 15.4); a start a block; 16 rows a pass over the weights.
+//     of [64][2048, 2048], 8 places: 14.6, the tiles 17.5); w4 and w8: 6 and 5
+//     weights a ps ([60][2048, 1024], 16 places: 9.7 and 11.0, the tiles 13.6 and
+//     15.4); a start a block; 16 rows a pass over the weights.
 //   tiles: a start and the K stages of one, then the weights at 5.6 to 6.1 TB/s, a
 //     round of the chip (one dense block a CU) at least that again (dense as above, 64
-//     places: 74.1, few rows 68.8; 128: 85.4 and 89.6; w8 as above, 64: 25.0 and 26.1).
+//     places: 74.1, few rows 68.8; 128: 85.4 and 89.6; w8 as above, 64: 25.0 and 26.3,
+//     w4 19.7 and 23.3).
 //     They have to win by 8%: x's fp16 copy grows with x.
 // Cuts (low / tall, us): more rows a tile read the weights less often and, quantized,
 // convert them less often; fewer fill the chip where there are few tiles. Dense, 128
@@ -50,9 +51,9 @@ int experts_cut(int E, int N, int K, int bits, int n) {
     const double one = 256.0 * K * 2 / 6.1e6;            // a tile's weights, us
     const double all = live * ((N + 255) / 256), round = std::floor(all / 256.0) * 256.0;
     few = 2.5 + weights * 2 / 5.9e6 * (1.0 + rows / 40.0) * passes + 0.002 * blocks;
-    tile = round * one + std::max(4.0 + 0.6 * stages, 2.5 + (all - round) * one);
+    tile = round * one + std::max(4.0 + 0.75 * stages, 2.5 + (all - round) * one);
   } else {
-    few = 3.0 + weights / (bits == 4 ? 3.3e6 : 4.6e6) * passes + 0.0035 * blocks;
+    few = 3.0 + weights / (bits == 4 ? 6.0e6 : 5.0e6) * passes + 0.0035 * blocks;
     tile = std::max(5.5 + 0.5 * stages, 7.0 + weights * (bits / 8.0 + 1.0 / 16) / 5.6e6);
   }
   if (few < 1.08 * tile) return 0;
