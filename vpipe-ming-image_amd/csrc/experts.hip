@@ -103,7 +103,11 @@ __device__ __forceinline__ void operands(const Raw<BITS>& r, uint4& w0, uint4& w
 //
 // WK waves with U groups in flight, by K: 8 with 2 (4 cost registers, so waves: 20 to
 // 55% longer), to K = 1024 with 1 ([60][2048, 1024] w8, 64 places 31.1 -> 26.0 us; K 7168
-// 8% slower), to 512 4 waves ([64][2048, 512] w8 gated, 64 places 14.1, eight 19.4).
+// 8% slower), to 512 4 waves ([64][2048, 512] w8 gated, 64 places 14.1, eight 19.4). CO
+// 16-column tiles of the output, 2 plain (1 is 7 to 30% longer, 4 as much), 1 gated and,
+// with dense weights past K = 1024, plain ([16][2048, 4096], one place 11.1 -> 7.5, 16 36.3
+// -> 31.2).
+constexpr int rows_long_co(int bits, bool gated) { return gated || bits == 16 ? 1 : 2; }
 template <int BITS, bool GATED, int WK, int U, int CO>
 __global__ __launch_bounds__(64 * WK) void experts_rows_kernel(const ExpertsArgs a) {
   constexpr int CT = GATED ? 2 * CO : CO;  // column tiles: the outputs', then the up rows'
@@ -208,16 +212,21 @@ __global__ __launch_bounds__(64 * WK) void experts_rows_kernel(const ExpertsArgs
   }
 }
 
+template <int BITS, bool GATED, int WK, int U, int CO>
+void rows_launch(const ExpertsArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)((a.N + 16 * CO - 1) / (16 * CO)), (unsigned)(a.n < a.E ? a.n : a.E));
+  hipLaunchKernelGGL((experts_rows_kernel<BITS, GATED, WK, U, CO>), grid, dim3(64 * WK), 0, s, a);
+}
+
 template <int BITS, bool GATED>
 void rows_shape(const ExpertsArgs& a, hipStream_t s) {
   constexpr int CO = GATED ? 1 : 2;
-  const dim3 grid((unsigned)((a.N + 16 * CO - 1) / (16 * CO)), (unsigned)(a.n < a.E ? a.n : a.E));
   if (a.K <= 512)
-    hipLaunchKernelGGL((experts_rows_kernel<BITS, GATED, 4, 1, CO>), grid, dim3(256), 0, s, a);
+    rows_launch<BITS, GATED, 4, 1, CO>(a, s);
   else if (a.K <= 1024)
-    hipLaunchKernelGGL((experts_rows_kernel<BITS, GATED, 8, 1, CO>), grid, dim3(512), 0, s, a);
+    rows_launch<BITS, GATED, 8, 1, CO>(a, s);
   else
-    hipLaunchKernelGGL((experts_rows_kernel<BITS, GATED, 8, 2, CO>), grid, dim3(512), 0, s, a);
+    rows_launch<BITS, GATED, 8, 2, rows_long_co(BITS, GATED)>(a, s);
 }
 
 // w [NW][K] -> [K / 64][NW][64], 16 bytes a thread and step.
@@ -262,7 +271,8 @@ hipError_t validate_experts_kernels() {
 #define MING_EXPERTS_ROWS(BITS)                                                   \
   reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 4, 1, 2>),      \
       reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 8, 1, 2>),  \
-      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 8, 2, 2>),  \
+      reinterpret_cast<const void*>(                                              \
+          &experts_rows_kernel<BITS, false, 8, 2, rows_long_co(BITS, false)>),    \
       reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 4, 1, 1>),   \
       reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 8, 1, 1>),   \
       reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 8, 2, 1>)
