@@ -223,7 +223,7 @@ __global__ __launch_bounds__(256) void topk_route_kernel(const RouteArgs a) {
 // launch that counts each block's groups and one that places: there each block
 // adds up the counts of the blocks before it itself, which is less than a
 // launch of its own. Bound by the launches and the chain inside them: 64 ids 3.8 us,
-// 34816 of 64 groups 2.9 and 6.4.
+// 34816 of 64 groups 7.6 in two launches, 262144 10.0, of 1024 groups 30.
 constexpr int GT = 1024, GW = GT / 64, GBINS = 1024 + 1;
 
 __device__ __forceinline__ uint64_t lanes_with(int v, int bits, uint64_t active) {
@@ -253,11 +253,35 @@ __global__ __launch_bounds__(GT) void group_rows_kernel(const GroupRowsArgs a) {
     return id >= 0 && id < a.G ? id : a.G;
   };
   auto cnt = [&](int w, int g) -> uint32_t& { return counts[w * bins + g]; };
+  // the wave's first batch, read once (while the counts of the blocks come in)
+  const int first = w0 + lane < w1 ? bin_of(w0 + lane) : 0;
   for (int i = tid; i < GW * bins; i += GT) counts[i] = 0;
   if constexpr (MODE == 2)
     for (int g = tid; g < bins; g += GT) tot[g] = pre[g] = 0;
   __syncthreads();
-  for (long long i = w0 + lane; i < w1; i += 64) atomicAdd(&cnt(wave, bin_of(i)), 1u);
+  if constexpr (MODE == 2) {
+    // the blocks' counts, one run of memory: all of them, and those before this one's;
+    // eight reads of a thread at a time ([34816] of 1024 groups: 26.4 us a block's row
+    // after the other)
+    constexpr int UN = 8;
+    const int total = (int)gridDim.x * bins, before = (int)blockIdx.x * bins;
+    const int step = GT % bins;
+    int g = tid % bins;
+    for (int i = tid; i < total; i += GT * UN) {
+      uint32_t v[UN];
+#pragma unroll
+      for (int u = 0; u < UN; ++u) v[u] = i + GT * u < total ? a.counts[i + GT * u] : 0;
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        if (v[u]) atomicAdd(&tot[g], v[u]);
+        if (v[u] && i + GT * u < before) atomicAdd(&pre[g], v[u]);
+        g += step;
+        g = g >= bins ? g - bins : g;
+      }
+    }
+  }
+  if (w0 + lane < w1) atomicAdd(&cnt(wave, first), 1u);
+  for (long long i = w0 + lane + 64; i < w1; i += 64) atomicAdd(&cnt(wave, bin_of(i)), 1u);
   __syncthreads();
   if constexpr (MODE == 1) {
     for (int g = tid; g < bins; g += GT) {
@@ -275,18 +299,8 @@ __global__ __launch_bounds__(GT) void group_rows_kernel(const GroupRowsArgs a) {
       for (int w = 0; w < GW; ++w) t += cnt(w, g);
       tot[g] = t;
     }
-  } else {
-    // the blocks' counts, a wave every 16th block's: all of them, and those before
-    // this one
-#pragma unroll 4
-    for (int b = wave; b < (int)gridDim.x; b += GW)
-      for (int g = lane; g < bins; g += 64) {
-        const uint32_t v = a.counts[(long long)b * bins + g];
-        if (v) atomicAdd(&tot[g], v);
-        if (v && b < (int)blockIdx.x) atomicAdd(&pre[g], v);
-      }
+    __syncthreads();
   }
-  __syncthreads();
   if (wave == 0) {                         // exclusive scan, a lane's bins in a row
     const int per = (bins + 63) / 64;
     uint32_t sum = 0;
@@ -323,7 +337,7 @@ __global__ __launch_bounds__(GT) void group_rows_kernel(const GroupRowsArgs a) {
   for (long long i0 = w0; i0 < w1; i0 += 64) {
     const long long i = i0 + lane;
     const bool live = i < w1;
-    const int g = live ? bin_of(i) : 0;
+    const int g = !live ? 0 : i0 == w0 ? first : bin_of(i);
     const uint64_t peers = lanes_with(g, a.bits, __ballot(live));
     if (live) {
       const int rank = __popcll(peers & ((1ull << lane) - 1));
@@ -418,7 +432,7 @@ hipError_t launch_topk_route(const RouteArgs& a, hipStream_t s) {
 
 // The blocks of n entries: one up to kGroupOne, else a batch of 64 a wave each as
 // long as that is at most 128 blocks (each reads every block's counts). 34816 ids of
-// 64 groups: 11.4 us in nine blocks of 4096.
+// 64 groups: 11.4 us in nine blocks of 4096, 7.6 in 34.
 constexpr int kGroupOne = 4096;
 static int group_chunk(long long n) {
   if (n <= kGroupOne) return (int)(n > 0 ? n : 1);
