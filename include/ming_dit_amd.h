@@ -397,9 +397,10 @@ int ming_experts_shape(const ming_experts* ex, int* n_experts, int* N, int* K, i
  * offsets[n_experts] on are left as they were. x [x_rows][ldx], 16-byte
  * aligned, ldx % 8 == 0, x_rows * ldx below 2^30; y [n][ldy], 16-byte aligned,
  * ldy % 8 == 0; none of x, order and offsets shares memory with y or ws, or y with
- * ws. Quantized stacks multiply fp16 activations from some rows an expert on, with ming_lin's range rule (see
- * MING_ERR_RANGE); on the general and the wide route they take bf16 ones at
- * any size, and more time. */
+ * ws. Quantized stacks multiply fp16 activations from some rows an expert on, with
+ * ming_lin's range rule (see MING_ERR_RANGE) for the rows that some place names: the
+ * others may hold anything, as y's rows behind the last group do. On the general and
+ * the wide route they take bf16 ones at any size, and more time. */
 size_t ming_experts_workspace_bytes(const ming_experts* ex, int x_rows);
 int ming_experts_lin(ming_ctx* ctx, const ming_experts* ex, const uint16_t* x, int64_t ldx,
                      int x_rows, const int32_t* order, int fan, const int32_t* offsets, int n,

@@ -424,3 +424,65 @@ def test_create_refusals(ctx, bits):
         m.Experts.dense(ctx, np.zeros((2, 12, 64), np.uint16))
     with pytest.raises(m.MingError):
         m.Experts.dense(ctx, np.zeros((2, 16, 72), np.uint16))
+
+
+@pytest.mark.parametrize("bits,kernel", [(4, 2), (4, 4), (8, 2), (8, 8)])
+def test_rows_that_no_place_names_may_hold_anything(ctx, cut, bits, kernel):
+    """Choices that were dropped leave rows of h unwritten and tokens unread: what lies
+    there is no range fault, in the gathered product or in the one after it."""
+    E, k, T, H, F = 6, 3, 260, 192, 320
+    n = T * k
+    gu, wgu = ref.make_experts(ctx, 18700, E, 2 * F, H, bits)
+    dn, wdn = ref.make_experts(ctx, 18750, E, H, F, bits)
+    rng = np.random.default_rng(kernel)
+    ids = rng.integers(0, E, (T, k)).astype(np.int32)
+    ids[rng.random((T, k)) < 0.3] = -1
+    away = rng.permutation(T)[:25]
+    ids[away] = E + 3
+    x = bf16(randn(18800, (T, H)))
+    x[away, rng.integers(0, H, 25)] = np.resize(np.uint16([0x7f80, 0x7fc0, 0xff80, 0x4780, 0xc7ff]), 25)
+    offsets, order, _ = ref.group(ids.reshape(-1), E)
+    held = int(offsets[-1])
+    assert 0 < held < n - 75
+    h = np.resize(np.uint16([0x7f80, 0x7fc0, 0x4780]), (n, F))
+    xd, hd, yd = to_dev(x), to_dev(h), to_dev(np.full((n, H), SENTINEL, np.uint16))
+    ws = torch.empty(max(gu.workspace_bytes(T), dn.workspace_bytes(n)), dtype=torch.uint8, device="cuda")
+    od, fd = to_dev(order), to_dev(offsets)
+    cut(kernel)
+    sync()
+    ctx.experts_swiglu(gu, xd, T, od, fd, n, hd, fan=k, ws=ws)
+    ctx.synchronize()
+    ctx.experts_lin(dn, hd, n, None, fd, n, yd, ws=ws)
+    ctx.synchronize()
+    hh, y = from_dev(hd), from_dev(yd)
+    check(hh[:held], wgu, x, offsets, order[:held] // k, True, bits)
+    check(y[:held], wdn, hh, offsets, np.arange(held), False, bits)
+    assert np.array_equal(hh[held:], h[held:]) and np.all(y[held:] == SENTINEL)
+    gu.close()
+    dn.close()
+
+
+@pytest.mark.parametrize("bits,kernel", [(4, 2), (4, 4), (8, 2), (8, 8)])
+def test_a_row_that_a_place_names_is_reported(ctx, cut, bits, kernel):
+    """Wherever it stands among the places: first and last of a group and of its tiles."""
+    E, N, K, counts = 3, 560, 128, [300, 0, 517]
+    ex, _ = ref.make_experts(ctx, 18900, E, N, K, bits)
+    offsets, _, _ = ref.plan_of(counts)
+    n = sum(counts)
+    x, fd = to_dev(bf16(randn(18950, (n, K)))), to_dev(offsets)
+    y = to_dev(np.zeros((n, N), np.uint16))
+    ws = torch.empty(ex.workspace_bytes(n), dtype=torch.uint8, device="cuda")
+    cut(kernel)
+    for at in (0, 31, 64, 150, 299, 300, 558, n - 1):
+        was = x[at, K - 1].clone()
+        x[at, K - 1] = 0x4780
+        sync()
+        ctx.experts_lin(ex, x, n, None, fd, n, y, ws=ws)
+        with pytest.raises(m.MingError) as e:
+            ctx.synchronize()
+        assert e.value.code == m.ERR_RANGE
+        x[at, K - 1] = was
+        sync()
+        ctx.experts_lin(ex, x, n, None, fd, n, y, ws=ws)
+        ctx.synchronize()
+    ex.close()

@@ -85,11 +85,14 @@ __device__ __forceinline__ uint32_t range_track4(uint32_t seen, const uint4& v) 
   seen = range_track(seen, v.z);
   return range_track(seen, v.w);
 }
+__device__ __forceinline__ bool range_beyond(uint32_t seen) {
+  return (seen & 0xffffu) >= 0x4780u || (seen >> 16) >= 0x4780u;
+}
 // Raises *flag (a plain store of 1; concurrent writers store the same value)
 // when a tracked magnitude is 2^16 or more, inf or NaN: a value the fp16
 // copy does not hold. Only lanes that saw one store.
 __device__ __forceinline__ void range_report(int* flag, uint32_t seen) {
-  if (flag && ((seen & 0xffffu) >= 0x4780u || (seen >> 16) >= 0x4780u)) *flag = 1;
+  if (flag && range_beyond(seen)) *flag = 1;
 }
 
 // Two f32 -> two fp16, round to nearest even.

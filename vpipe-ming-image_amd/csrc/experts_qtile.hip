@@ -1,7 +1,8 @@
 // The experts' products over many rows, w4 and w8 stacks: y[p] = x[row(p)] .
 // W_e^T for the places p of every expert's group, plain or SwiGLU-gated, x as
-// fp16 carrying bf16 values (exact inside fp16's range; the copy reports what it
-// cannot hold) and every scale and bias exact in fp16.
+// fp16 carrying bf16 values (exact inside fp16's range; rows that it cannot hold are
+// marked, and reported by the tiles whose places name them) and every scale and bias
+// exact in fp16.
 //
 // MFMA-bound over many rows an expert, HBM-bound (the weights, once) over few. A
 // block is a tile of up to 256 places of one expert x 256 rows of its weights, 4
@@ -30,6 +31,12 @@ namespace ming {
 namespace {
 
 constexpr int QBN = 256, QBK = 64, NW = 4, JT = 2;
+
+// The row of x at a place, inside x whatever the order says.
+__device__ __forceinline__ int source_row(const ExpertsArgs& a, int place) {
+  const int src = a.order ? a.order[place] / a.fan : place;
+  return src < 0 ? 0 : src < a.x_rows ? src : a.x_rows - 1;
+}
 
 // One tile: places p0 .. p0 + rows - 1 of expert e, output columns from n0;
 // st0..st2 the ring's stages.
@@ -66,9 +73,7 @@ __device__ __forceinline__ void experts_qtile(const ExpertsArgs& a, uint4* const
     const int p = 64 * (XD * wave + i) + lane;
     const int row = p >> 3;
     const int c = (p & 7) ^ ((row >> 1) & 7);
-    int src = p0 + (row < rows ? row : rows - 1);
-    if (a.order) src = a.order[src] / a.fan;
-    src = src < 0 ? 0 : src < a.x_rows ? src : a.x_rows - 1;
+    const int src = source_row(a, p0 + (row < rows ? row : rows - 1));
     xoff[i] = (uint32_t)(((long long)src * a.ldx + 8 * c) * 2);
   }
 #pragma unroll
@@ -308,18 +313,55 @@ void experts_qtile_kernel(const ExpertsArgs a) {
   const int tn = rg.index / tiles_m, tm = rg.index - tn * tiles_m;
   const RowTile rt = row_tile<MAX == 8 ? 64 : 32>(rg.rows, tiles_m, tm);
   const int p0 = rg.p0 + rt.first, rows = rt.rows, n0 = tn * BNT;
-  if constexpr (MAX >= 8)
-    if (rows > 192) return experts_qtile<BITS, GATED, 8, PP>(a, st0, st1, st2, rg.e, p0, rows, n0);
-  if constexpr (MAX >= 8)
-    if (rows > 128) return experts_qtile<BITS, GATED, 6, PP>(a, st0, st1, st2, rg.e, p0, rows, n0);
-  if constexpr (MAX >= 4)
-    if (rows > (MAX == 8 ? 64 : 96))
-      return experts_qtile<BITS, GATED, 4, PP>(a, st0, st1, st2, rg.e, p0, rows, n0);
-  if constexpr (MAX == 4)
-    if (rows > 64) return experts_qtile<BITS, GATED, 3, PP>(a, st0, st1, st2, rg.e, p0, rows, n0);
-  if constexpr (MAX < 8)
-    if (rows <= 32) return experts_qtile<BITS, GATED, 1, PP>(a, st0, st1, st2, rg.e, p0, rows, n0);
-  experts_qtile<BITS, GATED, 2, PP>(a, st0, st1, st2, rg.e, p0, rows, n0);
+  [&] {
+    if constexpr (MAX >= 8)
+      if (rows > 192) return experts_qtile<BITS, GATED, 8, PP>(a, st0, st1, st2, rg.e, p0, rows, n0);
+    if constexpr (MAX >= 8)
+      if (rows > 128) return experts_qtile<BITS, GATED, 6, PP>(a, st0, st1, st2, rg.e, p0, rows, n0);
+    if constexpr (MAX >= 4)
+      if (rows > (MAX == 8 ? 64 : 96))
+        return experts_qtile<BITS, GATED, 4, PP>(a, st0, st1, st2, rg.e, p0, rows, n0);
+    if constexpr (MAX == 4)
+      if (rows > 64) return experts_qtile<BITS, GATED, 3, PP>(a, st0, st1, st2, rg.e, p0, rows, n0);
+    if constexpr (MAX < 8)
+      if (rows <= 32) return experts_qtile<BITS, GATED, 1, PP>(a, st0, st1, st2, rg.e, p0, rows, n0);
+    experts_qtile<BITS, GATED, 2, PP>(a, st0, st1, st2, rg.e, p0, rows, n0);
+  }();
+  // Rows of x that no place names may hold anything: a row is reported by the tiles
+  // that multiply it, one in each row of them (a tile has at most a place a thread).
+  const int place = (int)threadIdx.x;
+  if (tn == 0 && place < rows && a.beyond[source_row(a, p0 + place)] && a.range) *a.range = 1;
+}
+
+// x as fp16, and a byte a row: whether it holds a magnitude of 2^16 or more, inf or
+// NaN. L lanes (a power of two, at most a wave) a row, 16 bytes a lane and step.
+__global__ __launch_bounds__(256) void experts_f16_kernel(const uint16_t* __restrict__ x,
+                                                          long long ldx, int rows, int K, int L,
+                                                          uint16_t* __restrict__ y,
+                                                          uint8_t* __restrict__ beyond) {
+  const int lane = (int)threadIdx.x & 63, sub = lane & (L - 1);
+  const long long r = (long long)blockIdx.x * (256 / L) + (int)threadIdx.x / L;
+  if (r >= rows) return;
+  uint32_t seen = 0;
+  for (int k0 = 8 * sub; k0 < K; k0 += 32 * L) {
+    uint4 v[4];                              // in flight together
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int k = k0 + 8 * L * u;
+      if (k < K) v[u] = *reinterpret_cast<const uint4*>(x + r * ldx + k);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int k = k0 + 8 * L * u;
+      if (k >= K) continue;
+      seen = range_track4(seen, v[u]);
+      *reinterpret_cast<uint4*>(y + r * K + k) =
+          make_uint4(bf16x2_to_f16x2(v[u].x), bf16x2_to_f16x2(v[u].y), bf16x2_to_f16x2(v[u].z),
+                     bf16x2_to_f16x2(v[u].w));
+    }
+  }
+  const uint64_t all = __ballot(range_beyond(seen)) >> (lane & ~(L - 1));
+  if (sub == 0) beyond[r] = (all & (~0ull >> (64 - L))) != 0;
 }
 
 // The taller cut of each type.
@@ -341,7 +383,7 @@ hipError_t launch_experts_qtile(int bits, bool gated, const ExpertsArgs& a, int 
                                 hipStream_t s) {
   if (a.n <= 0 || a.N <= 0) return hipSuccess;
   if (a.K % 64 || a.N % 8 || a.NW != a.N * (gated ? 2 : 1) || a.E < 1 || a.fan < 1 ||
-      a.x_rows < 1 || a.ldy % 8 || (bits != 4 && bits != 8) || (max != 2 && max != tall(bits)))
+      a.x_rows < 1 || a.ldy % 8 || !a.beyond || (bits != 4 && bits != 8) || (max != 2 && max != tall(bits)))
     return hipErrorInvalidValue;
   if (bits == 4)
     gated ? launch_max<4, true>(a, max, s) : launch_max<4, false>(a, max, s);
@@ -350,9 +392,22 @@ hipError_t launch_experts_qtile(int bits, bool gated, const ExpertsArgs& a, int 
   return hipGetLastError();
 }
 
+hipError_t launch_experts_f16(const uint16_t* x, long long ldx, int rows, int K, uint16_t* y,
+                              uint8_t* beyond, hipStream_t s) {
+  if (rows <= 0) return hipSuccess;
+  if (K < 64 || K % 64 || ldx % 8) return hipErrorInvalidValue;
+  int L = 8;
+  while (L < 64 && 16 * L <= K) L *= 2;
+  const int rpb = 256 / L;
+  hipLaunchKernelGGL(experts_f16_kernel, dim3((unsigned)((rows + (long long)rpb - 1) / rpb)),
+                     dim3(256), 0, s, x, ldx, rows, K, L, y, beyond);
+  return hipGetLastError();
+}
+
 hipError_t validate_experts_qtile_kernels() {
   hipFuncAttributes fa;
-  const void* fns[] = {reinterpret_cast<const void*>(&experts_qtile_kernel<4, false, 2>),
+  const void* fns[] = {reinterpret_cast<const void*>(&experts_f16_kernel),
+                       reinterpret_cast<const void*>(&experts_qtile_kernel<4, false, 2>),
                        reinterpret_cast<const void*>(&experts_qtile_kernel<4, true, 2>),
                        reinterpret_cast<const void*>(&experts_qtile_kernel<8, false, 2>),
                        reinterpret_cast<const void*>(&experts_qtile_kernel<8, true, 2>),

@@ -128,7 +128,7 @@ int products(const char* who, bool gated, ming_ctx* c, const ming_experts* ex, c
                   : ming::rt_experts_cut(c) >= 0
                       ? ming::rt_experts_cut(c)
                       : ming::experts_cut(ex->E, ex->N, ex->K, ex->bits, n);
-  const size_t xh_bytes = cut && ex->bits != 16 ? (size_t)x_rows * ex->K * 2 : 0;
+  const size_t xh_bytes = cut ? ming_experts_workspace_bytes(ex, x_rows) : 0;
   if (xh_bytes > 0 && (!ws || !aligned(ws, 16)))
     return bad(MING_ERR_ARG, "ws must be given, 16-byte aligned");
   if (ws_bytes < xh_bytes)
@@ -165,11 +165,14 @@ int products(const char* who, bool gated, ming_ctx* c, const ming_experts* ex, c
         if (ex->bits == 16) return ming::launch_experts_tile(gated, a, cut, stream_of(c));
         // one conversion of x to fp16 for all experts' rows
         auto* xh = static_cast<uint16_t*>(ws);
-        const hipError_t e = ming::launch_bf16_to_f16(x, ldx, xh, ex->K, x_rows, ex->K,
-                                                      stream_of(c), ming::rt_range_word(c));
+        auto* beyond = static_cast<uint8_t*>(ws) + (size_t)x_rows * ex->K * 2;
+        const hipError_t e =
+            ming::launch_experts_f16(x, ldx, x_rows, ex->K, xh, beyond, stream_of(c));
         if (e != hipSuccess) return e;
         a.x = xh;
         a.ldx = ex->K;
+        a.beyond = beyond;
+        a.range = ming::rt_range_word(c);
         return ming::launch_experts_qtile(ex->bits, gated, a, cut, stream_of(c));
       });
   if (rc != MING_OK) return rc;
@@ -399,9 +402,10 @@ int ming_experts_shape(const ming_experts* ex, int* n_experts, int* N, int* K, i
 }
 
 size_t ming_experts_workspace_bytes(const ming_experts* ex, int x_rows) {
-  // the fp16 copy of x that the tiles of a quantized stack multiply
+  // the fp16 copy of x that the tiles of a quantized stack multiply, a byte a row for
+  // what it does not hold
   if (!ex || x_rows <= 0 || ex->bits == 16) return 0;
-  return (size_t)x_rows * ex->K * 2;
+  return (size_t)x_rows * ex->K * 2 + ((size_t)x_rows + 15) / 16 * 16;
 }
 
 int ming_experts_lin(ming_ctx* c, const ming_experts* ex, const uint16_t* x, int64_t ldx,

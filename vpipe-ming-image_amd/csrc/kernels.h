@@ -513,6 +513,10 @@ struct ExpertsArgs {
   int N, NW, K;
   uint16_t* y;
   long long ldy;
+  // tiles of quantized stacks: a byte a row of x, 1 where its fp16 copy does not hold
+  // it (launch_experts_f16), and the word raised for such a row that a place names
+  const uint8_t* beyond;
+  int* range;
 };
 // One projection [NW][K] into [K / 64][NW][64]: a stage of a tile is then one run
 // of memory. In rows of a power of two the same 128 bytes of every row lie on a
@@ -530,6 +534,9 @@ hipError_t validate_experts_tile_kernels();
 // every 32 * max places, max 2 or, of w4, 4, of w8, 8
 hipError_t launch_experts_qtile(int bits, bool gated, const ExpertsArgs& a, int max,
                                 hipStream_t s);
+// That copy, y [rows][K], with ExpertsArgs::beyond.
+hipError_t launch_experts_f16(const uint16_t* x, long long ldx, int rows, int K, uint16_t* y,
+                              uint8_t* beyond, hipStream_t s);
 hipError_t validate_experts_qtile_kernels();
 // Blocks of the tiles: every group ends in at most one partial one.
 inline long long experts_tiles(int bits, bool gated, int max, int n, int E, int N) {
