@@ -521,3 +521,30 @@ def test_refusals(ctx):
     other.close()
     for h in (bank, wide, qw):
         h.close()
+
+
+@pytest.mark.parametrize("bits,M,N,K", [(16, 200, 3840, 3840), (16, 700, 3840, 3840),
+                                        (16, 300, 1024, 2048), (4, 200, 3840, 3840),
+                                        (8, 700, 3840, 3840)])
+def test_beside_and_apart_give_the_same_bits(ctx, bits, M, N, K):
+    """A bank of two adapters runs its x.A beside the split's blocks, one of forty in a
+    launch of its own (the profile says so): the same rows, the same bits."""
+    qw, w = weight(ctx, 19000, N, K, bits)
+    few, held = make_bank(ctx, 19100, N, K, (8, 24), cap=40, max_rank=64)
+    many, _ = make_bank(ctx, 19100, N, K, (8, 24) + (64,) * 38)
+    x = bf16(randn(19300 + M, (M, K)))
+    ids, s = np.arange(M) % 3 - 1, np.linspace(-1, 1, M).astype(np.float32)
+    got = []
+    for bank, apart in ((few, 0), (many, 1)):
+        ctx.profile_collect()
+        ctx.set_profiling(True)
+        try:
+            got.append(call(ctx, qw, bank, x, ids, s))
+            assert ctx.profile_collect().get("row_adapters", {"launches": 0})["launches"] == apart
+        finally:
+            ctx.set_profiling(False)
+    some = np.unique(np.concatenate([np.arange(0, M, 9), [M - 1]]))
+    check(got[0][some], x[some], w, held, ids[some], s[some], bits)
+    assert np.array_equal(got[1], got[0])
+    for h in (few, many, qw):
+        h.close()

@@ -1,6 +1,8 @@
 """The launch plans, which choose tile heights and K slices by size alone: on the
 CPU (without a device they count the MI355X's 256 CUs), through the library's
 own symbols."""
+import ctypes as C
+
 import pytest
 
 from helpers import dense_plan, plan_rows, xa_tile
@@ -52,3 +54,14 @@ def test_xa_tiles_at_half_a_chip():
     assert xa_tile(16640, 256, 3840, 1) == (64, 128)
     assert xa_tile(16384, 256, 10240, 1) == (64, 128)
     assert xa_tile(4352, 64, 3840, 3) == (64, 64)
+
+
+def test_a_banks_size_says_where_its_rows_run():
+    """The rows' x.A beside a split: a few adapters' chunks, not forty's; none bound
+    always, no blocks to spare never."""
+    import ming_dit_amd as m
+    f = m.lib()._ZN4ming13row_xa_besideEiiiii
+    f.restype = C.c_bool
+    for ny, M, K in ((5, 200, 3840), (1, 700, 3840), (3, 300, 2048)):
+        assert f(ny, M, K, 2, 3) and not f(ny, M, K, 40, 2 + 38 * 4)
+        assert f(ny, M, K, 0, 0) and not f(0, M, K, 2, 3)

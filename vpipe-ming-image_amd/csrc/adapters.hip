@@ -1,5 +1,6 @@
 // Low-rank adapters that rows choose: the down-projection T = x . A^T of every
 // row's own adapter. The up-projection runs in the projection's own launch.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -288,6 +289,22 @@ hipError_t launch_row_xa(const RowXaArgs& a, hipStream_t s) {
   hipLaunchKernelGGL(row_xa_kernel, dim3((unsigned)(low + lists), (unsigned)y), dim3(64 * XW), 0, s,
                      a);
   return hipGetLastError();
+}
+
+// Beside the split where its blocks have at most 10 us of 16-rank chunks each, were
+// every row of a tile its own request: a chunk of K = 3840 takes 2 us, past 4096
+// (where x is read again for each) half as long again; a launch of its own takes 5
+// to 20 ([3840, 3840] dense, 37 rows of as many adapters of 16 to 64
+// ranks: 26.2 us beside, 10.8 and 8.7 apart; 700 rows of 32 in turn: 83, 31 and 20;
+// 37 rows of five requests, w4: 11.5 beside, 9.6 and 6 apart; [3840, 10240], 18 rows
+// of six adapters of 64 and 128 ranks: 76.6 beside, 11.0 and 18.7 apart). Either way
+// T has the same bits.
+bool row_xa_beside(int ny, int M, int K, int held, int chunks) {
+  if (ny <= 0) return false;
+  if (held < 1) return true;
+  const double chunk_us = K / 1920.0 * (K > 4096 ? 1.5 : 1.0);
+  const double requests = std::min({16.0, (double)held, (double)M});
+  return requests * chunks / held * chunk_us <= 10.0 * ny;
 }
 
 hipError_t launch_row_delta(const RowAdapters& r, int M, int N, float* d, hipStream_t s) {

@@ -439,6 +439,9 @@ hipError_t launch_row_xa(const RowXaArgs& a, hipStream_t s);
 // Below these rows launch_row_xa's blocks are 16 rows each, which a split
 // projection can take beside its own.
 constexpr int kRowXaMany = 768;
+// Whether it does, with ny blocks for 16 rows, over a bank of `held` adapters of
+// `chunks` 16-rank chunks.
+bool row_xa_beside(int ny, int M, int K, int held, int chunks);
 // d[m][n] = T[m] . B_a[n] in f32, a = rid[m]; -0 for rows without an adapter,
 // which any sum takes without a change. N % 4 == 0.
 hipError_t launch_row_delta(const RowAdapters& r, int M, int N, float* d, hipStream_t s);

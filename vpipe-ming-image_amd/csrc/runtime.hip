@@ -1294,20 +1294,10 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
       ra.stride = xr.stride;
       ra.zero = (uint32_t)((size_t)M * ra.ldt * 2);
     }
-    // Beside the split where its blocks have at most 10 us of 16-rank chunks each, were
-    // every row of a tile its own request: a chunk of K = 3840 takes 2 us, past 4096
-    // (where x is read again for each) half as long again; a launch of its own takes 5
-    // to 20 ([3840, 3840] dense, 37 rows of as many adapters of 16 to 64
-    // ranks: 26.2 us beside, 10.8 and 8.7 apart; 700 rows of 32 in turn: 83, 31 and 20;
-    // 37 rows of five requests, w4: 11.5 beside, 9.6 and 6 apart; [3840, 10240], 18 rows
-    // of six adapters of 64 and 128 ranks: 76.6 beside, 11.0 and 18.7 apart).
     const int ny = !split    ? 0
                    : fast[0] ? ming::qproj_rows_beside(M, qs[0]->N, split_ks[0], qa[0].split_rf)
                              : ming::dense_rows_beside(M, qs[0]->N, dense_plan[0]);
-    const double held = std::max(rows->bank->held, 1);
-    const double chunk_us = K / 1920.0 * (K > 4096 ? 1.5 : 1.0);
-    rows_beside = ny > 0 && std::min({16.0, held, (double)M}) * rows->bank->chunks / held *
-                                    chunk_us <= 10.0 * ny;
+    rows_beside = ming::row_xa_beside(ny, M, K, rows->bank->held, rows->bank->chunks);
     if (!plane) qa[0].rows = ra;
     if (xh_bytes) xh = (const uint16_t*)carve->take(xh_bytes);
     if (part_bytes) part = (float*)carve->take(part_bytes);
