@@ -339,7 +339,8 @@ int ming_ln_modulate(ming_ctx* ctx, const uint16_t* x, int64_t ldx,
  * the caller's (ws, 16-byte aligned, at least the bytes the size function
  * names; it holds nothing between calls, and calls or graphs that may run at
  * the same time need one each). Strides in elements. A call of no rows does
- * nothing; one of more than a launch holds (2^32 threads) is MING_ERR_SHAPE.
+ * nothing (ming_group_rows of no entries writes its offsets) and takes NULL
+ * arrays; one of more than a launch holds (2^32 threads) is MING_ERR_SHAPE.
  *
  * The router: per row of logits [rows][ld] (f32 when logits_f32, else bf16)
  * the scores s = softmax(l) or sigmoid(l) over n_experts, the keys s + bias

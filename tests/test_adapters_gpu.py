@@ -548,3 +548,25 @@ def test_beside_and_apart_give_the_same_bits(ctx, bits, M, N, K):
     assert np.array_equal(got[1], got[0])
     for h in (few, many, qw):
         h.close()
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_an_empty_batch(ctx, bits):
+    """No rows: nothing runs, and empty tensors, which have no address, will do. What is
+    no call of this bank and weight is refused all the same."""
+    N, K = 64, 128
+    qw, _ = weight(ctx, 19400, N, K, bits)
+    bank, _ = make_bank(ctx, 19500, N, K, (8,))
+    none = torch.empty(0, dtype=torch.int16, device="cuda")
+    ids = torch.empty(0, dtype=torch.int32, device="cuda")
+    assert none.data_ptr() == 0 and ctx.lin_adapters_workspace_bytes(qw, bank, 0) == 0
+    ctx.lin_adapters(qw, bank, none, none, 0, ids, None, none)
+    ctx.lin_adapters(qw, bank, None, None, 0, None, None, None)
+    ctx.synchronize()
+    wide, _ = make_bank(ctx, 19600, 72, K, (8,))
+    with pytest.raises(m.MingError, match="shape"):
+        ctx.lin_adapters(qw, wide, None, None, 0, None, None, None)
+    with pytest.raises(m.MingError):
+        ctx.lin_adapters(qw, bank, None, None, -1, None, None, None)
+    for h in (bank, wide, qw):
+        h.close()

@@ -264,3 +264,16 @@ def test_combine_shared_memory_and_sizes(ctx):
                {"add": out + 16, "ldadd": 128}, {"tokens": 2 ** 31 - 1}):
         with pytest.raises(m.MingError, match="share|launch"):
             ctx.experts_combine(**dict(ok, **kw))
+
+
+def test_empty_arrays(ctx):
+    """Calls of no rows take tensors without an address; a grouping of no entries says
+    that every group is empty."""
+    e = torch.empty(0, dtype=torch.int32, device="cuda")
+    off = torch.full((6,), 7, dtype=torch.int32, device="cuda")
+    sync()
+    ctx.topk_route(e, 0, 8, 2, e, e)
+    ctx.group_rows(e, 0, 5, off, e, e)
+    ctx.experts_combine(e, 0, e, e, 0, 2, e, 64)
+    ctx.synchronize()
+    assert not from_dev(off).any()

@@ -1736,15 +1736,22 @@ int ming_adapters_rank(const ming_adapters* b, int id) {
 
 constexpr int kRowsMax = 1 << 28;   // the x.A's 32-row tiles in one launch
 
+// The handles of a call, before any array is looked at.
+static int check_rows_call(ming_ctx* c, const ming_qweight* qw, const ming_adapters* bank, int M) {
+  if (!c || !qw || !bank) return fail(MING_ERR_ARG, "ming_lin_adapters: null argument");
+  if (bank->ctx != c) return fail(MING_ERR_ARG, "ming_lin_adapters: bank of another context");
+  if (qw->ctx != c) return fail(MING_ERR_ARG, "ming_lin_adapters: weight of another context");
+  if (bank->N != qw->N || bank->K != qw->K)
+    return fail(MING_ERR_SHAPE, "ming_lin_adapters: the bank's shape is not the weight's");
+  if (M < 0) return fail(MING_ERR_ARG, "ming_lin_adapters: M < 0");
+  return MING_OK;
+}
+
 // Shared by the call and its size: the projection planned with its rows'
 // adapters, its scratch from `cv`.
 static int lin_adapters(ming_ctx* c, const ming_qweight* qw, const ming_adapters* bank,
                         const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, int M,
                         const int32_t* ids, const float* scale, Carve* cv) {
-  if (!c || !qw || !bank) return fail(MING_ERR_ARG, "ming_lin_adapters: null argument");
-  if (bank->ctx != c) return fail(MING_ERR_ARG, "ming_lin_adapters: bank of another context");
-  if (bank->N != qw->N || bank->K != qw->K)
-    return fail(MING_ERR_SHAPE, "ming_lin_adapters: the bank's shape is not the weight's");
   cv->who = "ming_lin_adapters";
   cv->what = "the workspace";
   LinOut o;
@@ -1756,7 +1763,7 @@ static int lin_adapters(ming_ctx* c, const ming_qweight* qw, const ming_adapters
 
 size_t ming_lin_adapters_workspace_bytes(ming_ctx* c, const ming_qweight* qw,
                                          const ming_adapters* bank, int M) {
-  if (!c || !qw || !bank || M <= 0 || M >= kRowsMax) return 0;
+  if (M <= 0 || M >= kRowsMax || check_rows_call(c, qw, bank, M) != MING_OK) return 0;
   Carve cv;
   cv.measure = true;
   cv.cap = SIZE_MAX;
@@ -1770,6 +1777,8 @@ int ming_lin_adapters(ming_ctx* c, const ming_qweight* qw, const ming_adapters* 
                       const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, int M,
                       const int32_t* row_adapter, const float* row_scale, void* ws,
                       size_t ws_bytes) {
+  if (const int rc = check_rows_call(c, qw, bank, M)) return rc;
+  if (M == 0) return ok();               // (empty arrays have no address)
   if (!row_adapter || !ws) return fail(MING_ERR_ARG, "ming_lin_adapters: null argument");
   if (!aligned(ws, 16) || !aligned(row_adapter, 4) || !aligned(row_scale, 4))
     return fail(MING_ERR_ARG,
@@ -1779,7 +1788,7 @@ int ming_lin_adapters(ming_ctx* c, const ming_qweight* qw, const ming_adapters* 
   // another workspace
   if (!aligned(y, 16) || ldy % 8 != 0)
     return fail(MING_ERR_ARG, "ming_lin_adapters: y must be 16-byte aligned, ldy a multiple of 8");
-  if (qw && x && y && M > 0 && ldx >= qw->K && ldy >= qw->N) {
+  if (x && y && ldx >= qw->K && ldy >= qw->N) {
     // every block resolves its rows' adapters by itself, while others store
     const ming::Span xs = {x, M, 2 * ldx, 2ll * qw->K}, ys = {y, M, 2 * ldy, 2ll * qw->N};
     const ming::Span is = {row_adapter, 1, 4ll * M, 4ll * M};
