@@ -354,7 +354,7 @@ int ming_ln_modulate(ming_ctx* ctx, const uint16_t* x, int64_t ldx,
  * left ends in ids of -1 with weights of 0. A logit of +inf counts as the
  * largest finite one. Scores, keys and sums are in f64. n_experts <= 1024, a
  * multiple of n_groups <= 64; top_k <= 64 and <= the experts of top_groups
- * groups; rows below 2^26. ids and weights share memory with nothing else. */
+ * groups; rows up to 2^26 - 4. ids and weights share memory with nothing else. */
 #define MING_SCORE_SOFTMAX 0
 #define MING_SCORE_SIGMOID 1
 int ming_topk_route(ming_ctx* ctx, const void* logits, int64_t ld, int logits_f32,
@@ -442,7 +442,7 @@ int ming_adapters_rank(const ming_adapters* bank, int id);
  * is 0, is ming_lin's row without adapters. The adapters' sum joins the f32
  * result before the one rounding; a row's bits do not depend on the other rows'
  * adapters (but for the sign of a zero). Slots bound on the weight take no part.
- * M below 2^28. x as ming_lin's, y 16-byte aligned with ldy % 8 == 0; none of x, row_adapter and
+ * M up to 2^28 - 32. x as ming_lin's, y 16-byte aligned with ldy % 8 == 0; none of x, row_adapter and
  * row_scale shares memory with y or ws. The size is that of x rows beside each
  * other; a dense projection of x rows that span more than 2 GiB may need more, and
  * says how much (MING_ERR_SHAPE). */

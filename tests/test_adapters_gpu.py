@@ -570,3 +570,17 @@ def test_an_empty_batch(ctx, bits):
         ctx.lin_adapters(qw, bank, None, None, -1, None, None, None)
     for h in (bank, wide, qw):
         h.close()
+
+
+@pytest.mark.parametrize("M", [2 ** 28 - 31, 2 ** 28 - 1, 2 ** 31 - 1])
+def test_more_rows_than_a_launch_holds(ctx, M):
+    N, K = 64, 128
+    qw, _ = weight(ctx, 19700, N, K, 16)
+    bank, _ = make_bank(ctx, 19800, N, K, (8,))
+    far = 1 << 56
+    with pytest.raises(m.MingError, match="2\\^28") as e:
+        ctx.lin_adapters(qw, bank, far, far << 1, M, far << 2, None,
+                         torch.empty(4096, dtype=torch.uint8, device="cuda"))
+    assert e.value.code == 2 and ctx.lin_adapters_workspace_bytes(qw, bank, M) == 0
+    bank.close()
+    qw.close()

@@ -65,3 +65,13 @@ def test_a_banks_size_says_where_its_rows_run():
     for ny, M, K in ((5, 200, 3840), (1, 700, 3840), (3, 300, 2048)):
         assert f(ny, M, K, 2, 3) and not f(ny, M, K, 40, 2 + 38 * 4)
         assert f(ny, M, K, 0, 0) and not f(0, M, K, 2, 3)
+
+
+def test_the_last_rows_that_one_launch_holds():
+    """2^32 - 1 threads: a block more than that is refused before it is launched."""
+    import ming_dit_amd as m
+    route, xa = m.lib()._ZN4ming10route_fitsEx, m.lib()._ZN4ming11row_xa_fitsEii
+    route.argtypes, route.restype, xa.restype = [C.c_longlong], C.c_bool, C.c_bool
+    assert route(2 ** 26 - 4) and not route(2 ** 26 - 3) and not route(2 ** 31 - 1)
+    assert xa(2 ** 28 - 32, 0) and not xa(2 ** 28 - 31, 0) and not xa(2 ** 28 - 32, 1)
+    assert xa(767, 100) and not xa(2 ** 31 - 1, 0)

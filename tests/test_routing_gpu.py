@@ -277,3 +277,13 @@ def test_empty_arrays(ctx):
     ctx.experts_combine(e, 0, e, e, 0, 2, e, 64)
     ctx.synchronize()
     assert not from_dev(off).any()
+
+
+@pytest.mark.parametrize("rows", [2 ** 26 - 3, 2 ** 26 - 1, 2 ** 31 - 1])
+def test_route_of_more_rows_than_a_launch_holds(ctx, rows):
+    """Refused by their count, before any array is looked at."""
+    far = 1 << 56
+    with pytest.raises(m.MingError, match="2\\^26") as e:
+        m._check(m.lib().ming_topk_route(ctx.h, far, 8, 1, None, rows, 8, 2, 1, 1, 0, 1, 1.0,
+                                         far << 1, far << 2))
+    assert e.value.code == 2

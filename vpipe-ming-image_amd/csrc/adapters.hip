@@ -268,11 +268,21 @@ __global__ void check_finite_kernel(const uint16_t* v, long long n, int* flag) {
 
 }  // namespace
 
+// The x.A's row tiles: of 32 rows, or of 16 where there are few.
+static int row_xa_tiles(int M) {
+  const int rows = M >= kRowXaMany ? 32 : 16;
+  return (int)(((long long)M + rows - 1) / rows);
+}
+
+bool row_xa_fits(int M, int lists) {
+  return one_launch((long long)row_xa_tiles(M) + lists, 64 * XW);
+}
+
 hipError_t launch_row_xa(const RowXaArgs& a, hipStream_t s) {
   if (a.M <= 0) return hipSuccess;
   if (a.K % 64 || a.ldt % 32 || (a.counts && (a.rows_main % 256 || a.rest < 1 || a.rest > 256)))
     return hipErrorInvalidValue;
-  const int tiles = (a.M + 31) / 32;
+  const int tiles = row_xa_tiles(a.M);
   const int lists = a.counts ? row_tiles(a.M, a.rows_main, a.rest) : 0;
   if (a.M >= kRowXaMany) {
     // ranks past 32 make it more than one pass over x: four chunks a pass then
@@ -283,10 +293,9 @@ hipError_t launch_row_xa(const RowXaArgs& a, hipStream_t s) {
       hipLaunchKernelGGL(row_xa_many_kernel<4>, grid, dim3(64 * XW), 0, s, a);
     return hipGetLastError();
   }
-  const int low = (a.M + 15) / 16;
   // a block a CU (two rounds of them, [500, 3840]: 14.6 us, one 9.0)
-  const int y = low < 256 / 64 ? 64 : low < 256 ? 256 / low : 1;
-  hipLaunchKernelGGL(row_xa_kernel, dim3((unsigned)(low + lists), (unsigned)y), dim3(64 * XW), 0, s,
+  const int y = tiles < 256 / 64 ? 64 : tiles < 256 ? 256 / tiles : 1;
+  hipLaunchKernelGGL(row_xa_kernel, dim3((unsigned)(tiles + lists), (unsigned)y), dim3(64 * XW), 0, s,
                      a);
   return hipGetLastError();
 }

@@ -89,8 +89,6 @@ ming::Span row_span(const void* p, int64_t rows, int64_t ld, int64_t width) {
   return {p, rows, 2 * ld, 2 * width};
 }
 ming::Span flat_span(const void* p, int64_t bytes) { return {p, 1, bytes, bytes}; }
-// A launch holds 2^32 - 1 threads along x.
-bool one_launch(long long blocks, int threads) { return blocks <= 0xffffffffll / threads; }
 
 // One launch, timed when the context profiles.
 template <class F>
@@ -135,7 +133,7 @@ int products(const char* who, bool gated, ming_ctx* c, const ming_experts* ex, c
     return rt_fail(MING_ERR_SHAPE, std::string(who) + ": the call needs " +
                                        std::to_string(xh_bytes) + " bytes of workspace, " +
                                        std::to_string(ws_bytes) + " given");
-  if (cut && !one_launch(ming::experts_tiles(ex->bits, gated, cut, n, ex->E, N),
+  if (cut && !ming::one_launch(ming::experts_tiles(ex->bits, gated, cut, n, ex->E, N),
                          ex->bits == 16 ? 512 : 256))
     return bad(MING_ERR_SHAPE, "more places times columns than one launch holds");
   // every block reads the plan and the rows by itself, while others store
@@ -214,7 +212,7 @@ int ming_topk_route(ming_ctx* c, const void* logits, int64_t ld, int logits_f32,
   if (!c || (rows > 0 && (!logits || !ids || !weights)))
     return bad(MING_ERR_ARG, "null argument");
   if (rows < 0) return bad(MING_ERR_ARG, "rows < 0");
-  if (rows >= 1 << 26) return bad(MING_ERR_SHAPE, "rows must be below 2^26");
+  if (!ming::route_fits(rows)) return bad(MING_ERR_SHAPE, "rows must be at most 2^26 - 4");
   if (score != MING_SCORE_SOFTMAX && score != MING_SCORE_SIGMOID)
     return bad(MING_ERR_ARG, "no such score");
   if (n_experts < 1 || n_experts > ming::kRouteMaxExperts || n_groups < 1 || n_groups > 64 ||
@@ -438,7 +436,7 @@ int ming_experts_combine(ming_ctx* c, const uint16_t* y, int64_t ldy, int n, con
       !aligned(weights, 4))
     return bad(MING_ERR_ARG, "y, add and out must be 16-byte, place and weights 4-byte aligned");
   if (tokens == 0) return rt_ok();
-  if (!one_launch(ming::combine_blocks(tokens, N), 256))
+  if (!ming::one_launch(ming::combine_blocks(tokens, N), 256))
     return bad(MING_ERR_SHAPE, "more tokens than one launch holds");
   const ming::Span outs = row_span(out, tokens, ldo, N);
   if (ming::spans_meet(row_span(y, n, ldy, N), outs))

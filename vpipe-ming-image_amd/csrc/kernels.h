@@ -8,6 +8,9 @@
 
 namespace ming {
 
+// A launch holds 2^32 - 1 threads along x.
+inline bool one_launch(long long blocks, int threads) { return blocks <= 0xffffffffll / threads; }
+
 // ---- quantized / dense projection GEMM with the LoRA tail ------------------
 //
 // y[m][n] = sum_k x[m][k] W[n][k]  (+ sum_r T[m][seg.t_col0 + r] B[n][r])
@@ -436,6 +439,8 @@ inline int row_tiles(int M, int rows_main, int rest) {
   return rows_main / 256 + (M > rows_main ? (M - rows_main + rest - 1) / rest : 0);
 }
 hipError_t launch_row_xa(const RowXaArgs& a, hipStream_t s);
+// Whether its blocks, with `lists` of row tiles beside them, fit one launch.
+bool row_xa_fits(int M, int lists);
 // Below these rows launch_row_xa's blocks are 16 rows each, which a split
 // projection can take beside its own.
 constexpr int kRowXaMany = 768;
@@ -453,6 +458,8 @@ hipError_t validate_adapter_kernels();
 
 // ---- a mixture's router, grouping and weighted sum (routing.hip) ---------------
 constexpr int kRouteMaxExperts = 1024;
+// Whether the router's blocks for them fit one launch: up to 2^26 - 4.
+bool route_fits(long long rows);
 struct RouteArgs {
   const void* logits;   // [rows][ld], f32 or bf16
   long long ld;

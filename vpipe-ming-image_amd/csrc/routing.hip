@@ -411,12 +411,16 @@ __global__ __launch_bounds__(256) void combine_kernel(const CombineArgs a) {
 
 }  // namespace
 
+static long long route_blocks(long long rows) { return (rows + 3) / 4; }
+
+bool route_fits(long long rows) { return one_launch(route_blocks(rows), 256); }
+
 hipError_t launch_topk_route(const RouteArgs& a, hipStream_t s) {
   if (a.rows <= 0) return hipSuccess;
   if (a.E < 1 || a.E > kRouteMaxExperts || a.G < 1 || a.G > 64 || a.E % a.G || a.k < 1 ||
       a.k > 64)
     return hipErrorInvalidValue;
-  const dim3 grid((unsigned)((a.rows + 3) / 4));
+  const dim3 grid((unsigned)route_blocks(a.rows));
   if (a.E <= 64)
     hipLaunchKernelGGL(topk_route_kernel<1>, grid, dim3(256), 0, s, a);
   else if (a.E <= 128)

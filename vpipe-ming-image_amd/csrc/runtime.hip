@@ -1734,8 +1734,6 @@ int ming_adapters_rank(const ming_adapters* b, int id) {
   return b && id >= 0 && id < b->cap ? b->bound[id].rank : 0;
 }
 
-constexpr int kRowsMax = 1 << 28;   // the x.A's 32-row tiles in one launch
-
 // The handles of a call, before any array is looked at.
 static int check_rows_call(ming_ctx* c, const ming_qweight* qw, const ming_adapters* bank, int M) {
   if (!c || !qw || !bank) return fail(MING_ERR_ARG, "ming_lin_adapters: null argument");
@@ -1744,6 +1742,9 @@ static int check_rows_call(ming_ctx* c, const ming_qweight* qw, const ming_adapt
   if (bank->N != qw->N || bank->K != qw->K)
     return fail(MING_ERR_SHAPE, "ming_lin_adapters: the bank's shape is not the weight's");
   if (M < 0) return fail(MING_ERR_ARG, "ming_lin_adapters: M < 0");
+  // (the lists of row tiles come with fewer rows than that)
+  if (!ming::row_xa_fits(M, 0))
+    return fail(MING_ERR_SHAPE, "ming_lin_adapters: M must be at most 2^28 - 32");
   return MING_OK;
 }
 
@@ -1763,7 +1764,7 @@ static int lin_adapters(ming_ctx* c, const ming_qweight* qw, const ming_adapters
 
 size_t ming_lin_adapters_workspace_bytes(ming_ctx* c, const ming_qweight* qw,
                                          const ming_adapters* bank, int M) {
-  if (M <= 0 || M >= kRowsMax || check_rows_call(c, qw, bank, M) != MING_OK) return 0;
+  if (M <= 0 || check_rows_call(c, qw, bank, M) != MING_OK) return 0;
   Carve cv;
   cv.measure = true;
   cv.cap = SIZE_MAX;
@@ -1783,7 +1784,6 @@ int ming_lin_adapters(ming_ctx* c, const ming_qweight* qw, const ming_adapters* 
   if (!aligned(ws, 16) || !aligned(row_adapter, 4) || !aligned(row_scale, 4))
     return fail(MING_ERR_ARG,
                 "ming_lin_adapters: ws must be 16-byte, ids and strengths 4-byte aligned");
-  if (M >= kRowsMax) return fail(MING_ERR_SHAPE, "ming_lin_adapters: M must be below 2^28");
   // rows of y that do not take 16-byte stores would have a plan of their own, with
   // another workspace
   if (!aligned(y, 16) || ldy % 8 != 0)
