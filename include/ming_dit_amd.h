@@ -395,7 +395,7 @@ int ming_experts_shape(const ming_experts* ex, int* n_experts, int* N, int* K, i
  *                         wide, the products stay in f32 up to the one rounding
  * with r = order[p] / fan (a token's row for each of its fan choices), or p
  * itself where order is NULL (x already in place order). Rows of y from
- * offsets[n_experts] on are left as they were. x [x_rows][ldx], 16-byte
+ * offsets[n_experts] on are left as they were. n <= 2^30. x [x_rows][ldx], 16-byte
  * aligned, ldx % 8 == 0, x_rows * ldx below 2^30; y [n][ldy], 16-byte aligned,
  * ldy % 8 == 0; none of x, order and offsets shares memory with y or ws, or y with
  * ws. Quantized stacks multiply fp16 activations from some rows an expert on, with
@@ -414,7 +414,7 @@ int ming_experts_swiglu(ming_ctx* ctx, const ming_experts* ex, const uint16_t* x
  * top_k of weights[t][j] * y[place[t * top_k + j]]), f32, j in order, one
  * rounding. A place outside [0, n) adds nothing. add [tokens][ldadd] may be NULL
  * or out itself (with ldo), else nothing shares memory with out. N, strides
- * multiples of 8, 16-byte aligned. */
+ * multiples of 8, 16-byte aligned; top_k <= 2^30. */
 int ming_experts_combine(ming_ctx* ctx, const uint16_t* y, int64_t ldy, int n,
                          const int32_t* place, const float* weights, int tokens, int top_k,
                          const uint16_t* add, int64_t ldadd, uint16_t* out, int64_t ldo, int N);

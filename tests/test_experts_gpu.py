@@ -486,3 +486,24 @@ def test_a_row_that_a_place_names_is_reported(ctx, cut, bits, kernel):
         ctx.experts_lin(ex, x, n, None, fd, n, y, ws=ws)
         ctx.synchronize()
     ex.close()
+
+
+@pytest.mark.parametrize("bits,kernel", [(4, 0), (16, 0), (4, 2), (16, 4)])
+def test_counts_past_an_int(ctx, cut, bits, kernel):
+    """Places and choices whose counts pass 2^31 before they end are refused by their
+    number alone: the arrays are small."""
+    ex, _ = ref.make_experts(ctx, 19900, 1, 16, 64, bits)
+    x, y = to_dev(np.zeros((8, 64), np.uint16)), to_dev(np.zeros((8, 16), np.uint16))
+    i = torch.zeros(8, dtype=torch.int32, device="cuda")
+    w = torch.zeros(8, device="cuda")
+    ws = torch.empty(4096, dtype=torch.uint8, device="cuda")
+    cut(kernel)
+    for n in ((1 << 30) + 1, 2 ** 31 - 16, 2 ** 31 - 1):
+        with pytest.raises(m.MingError, match="2\\^30") as e:
+            ctx.experts_lin(ex, x, 8, i, i, n, 1 << 56, ws=ws)
+        assert e.value.code == 2
+        with pytest.raises(m.MingError, match="2\\^30"):
+            ctx.experts_swiglu(ex, x, 8, i, i, n, 1 << 56, ws=ws)
+        with pytest.raises(m.MingError, match="2\\^30"):
+            ctx.experts_combine(y, 8, i, w, 1, n, 1 << 56, 16)
+    ex.close()

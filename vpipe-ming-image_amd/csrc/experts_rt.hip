@@ -109,6 +109,8 @@ int products(const char* who, bool gated, ming_ctx* c, const ming_experts* ex, c
   if (!c || !ex || (n > 0 && (!x || !offsets || !y))) return bad(MING_ERR_ARG, "null argument");
   if (ex->ctx != c) return bad(MING_ERR_ARG, "experts of another context");
   if (n < 0 || x_rows < 0 || fan < 1) return bad(MING_ERR_ARG, "a count out of range");
+  // a group's rows are counted in ints, up to a tile past its end
+  if (n > 1 << 30) return bad(MING_ERR_SHAPE, "n past 2^30, more places than a launch takes");
   const int N = gated ? ex->N / 2 : ex->N;
   if (gated && ex->N % 16 != 0)
     return bad(MING_ERR_SHAPE, "gate and up rows need N % 16 == 0");
@@ -429,6 +431,8 @@ int ming_experts_combine(ming_ctx* c, const uint16_t* y, int64_t ldy, int n, con
   if (!c || (tokens > 0 && (!out || !place || !weights || (n > 0 && !y))))
     return bad(MING_ERR_ARG, "null argument");
   if (n < 0 || tokens < 0 || top_k < 1) return bad(MING_ERR_ARG, "a count out of range");
+  // choices are counted in ints, four at a time
+  if (top_k > 1 << 30) return bad(MING_ERR_SHAPE, "top_k must be at most 2^30");
   if (N <= 0 || N % 8 != 0 || (n > 0 && ldy < N) || ldo < N || (add && ldadd < N) ||
       ldy % 8 != 0 || ldo % 8 != 0 || (add && ldadd % 8 != 0))
     return bad(MING_ERR_SHAPE, "N and the strides must be multiples of 8, strides >= N");
