@@ -507,3 +507,43 @@ def test_counts_past_an_int(ctx, cut, bits, kernel):
         with pytest.raises(m.MingError, match="2\\^30"):
             ctx.experts_combine(y, 8, i, w, 1, n, 1 << 56, 16)
     ex.close()
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("K", [64, 512, 1024, 2112])
+def test_w4_sums_of_few_rows_are_exact_where_f32_is(ctx, cut, gated, K):
+    """Whole numbers whose sums with codes of up to 31 stay below 2^24: every f32 sum is
+    exact, in any order, and what is left of them after the bias is a small number. Sums
+    of 128 more than the codes would pass 2^25 and lose it."""
+    E, N, T = 2, 32, 5
+    rng = np.random.default_rng(K)
+    # a group: one x of 1 under a code of its own, the others large under 8
+    x = (rng.integers(129, 256, (T, K)) * 32).astype(np.float32)
+    at = 64 * np.arange(K // 64) + rng.integers(0, 64, K // 64)
+    x[:, at] = 1.0
+    assert 31 * x.reshape(T, -1, 64).sum(-1).max() < 2 ** 24
+    assert 136 * x.reshape(T, -1, 64).sum(-1).min() > 2 ** 25
+    q = np.full((E, 2 * N if gated else N, K), 8, np.uint32)
+    q[:, :, at] = rng.integers(1, 16, q[:, :, at].shape)
+    if gated:                                   # the gates' sums 32 a group, so silu is them
+        q[:, :N, at] = 8 + 7
+        extra = 64 * np.arange(K // 64) + (at + 1) % 64
+        x[:, extra] = 8.0
+        q[:, :N, extra] = 8 + 4
+    codes = (q.reshape(*q.shape[:2], K // 8, 8) << (4 * np.arange(8, dtype=np.uint32))).sum(-1)
+    ones = np.full(q.shape[:2] + (K // 64,), 0x3f80, np.uint16)
+    ex = m.Experts.quantized(ctx, codes.astype(np.uint32), ones, np.full_like(ones, 0xc100), 4)
+    offsets, order, src = ref.plan_of([3, 40], x_rows=T)
+    cut(0)
+    got = f32(run(ctx, ex, gated, bf16(x), offsets, order, order.size)).astype(np.float64)
+    e = np.repeat([0, 1], [3, 40])
+    t = np.einsum("pk,pnk->pn", x[src].astype(np.float64), q[e].astype(np.float64) - 8.0)
+    if gated:
+        assert (t[:, :N] == 39 * (K // 64)).all()
+        want = t[:, :N] * t[:, N:]
+        # silu(g) is g but for 2 of its own steps and e^-39: one rounding to bf16
+        assert np.all(np.abs(got - want) <= (ref.BF16 + 4 * ref.F32) * np.abs(want))
+    else:
+        assert np.abs(t).max() <= 256            # exact in bf16
+        assert np.array_equal(got, t)
+    ex.close()

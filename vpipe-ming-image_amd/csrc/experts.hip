@@ -21,11 +21,12 @@ __device__ __forceinline__ float f16_hi(uint32_t u) {
 
 // One 64-group of weight row n, lane quarter g's 16 values as the A operands of two
 // v_mfma_f32_16x16x32_bf16: dense weights as they are, w8 codes as the integers they
-// hold, w4 codes as 128 more (0x43 over a code is that in bf16, so two codes are a
-// v_perm; the group's bias takes the 128 scales off again). Which k a quarter has is
-// free as long as x's agree (x_at): they are what one wide load brings, with the lanes
-// of a row side by side (w4 as two 4-byte loads a lane: [64][2048, 2048] gated, 8 places
-// 13.9 us, 8.5 so).
+// hold, w4 codes as 16 more (0x4180 with the code in the upper four bits of its mantissa
+// is that in bf16, so two codes are a v_perm; the group's bias takes the 16 scales off
+// again, at sums of three times the codes' own: two bits of the f32 sums' 24, where the
+// output keeps eight). Which k a quarter has is free as long as x's agree (x_at): they
+// are what one wide load brings, with the lanes of a row side by side (w4 as two 4-byte
+// loads a lane: [64][2048, 2048] gated, 8 places 13.9 us, 8.5 so).
 template <int BITS>
 struct Raw {
   uint4 v[BITS == 16 ? 2 : 1];
@@ -75,11 +76,12 @@ __device__ __forceinline__ void operands(const Raw<BITS>& r, uint4& w0, uint4& w
     if constexpr (BITS == 4) {
       // nibbles {k0,k4,k1,k5,k2,k6,k3,k7}: the even ones are k0..k3 by byte
       auto word = [](uint32_t c) {
-        const uint32_t lo = c & 0x0F0F0F0Fu, hi = (c >> 4) & 0x0F0F0F0Fu;
-        return make_uint4(__builtin_amdgcn_perm(0x43434343u, lo, 0x05010400u),
-                          __builtin_amdgcn_perm(0x43434343u, lo, 0x05030402u),
-                          __builtin_amdgcn_perm(0x43434343u, hi, 0x05010400u),
-                          __builtin_amdgcn_perm(0x43434343u, hi, 0x05030402u));
+        const uint32_t lo = ((c << 3) & 0x78787878u) | 0x80808080u;
+        const uint32_t hi = ((c >> 1) & 0x78787878u) | 0x80808080u;
+        return make_uint4(__builtin_amdgcn_perm(0x41414141u, lo, 0x05010400u),
+                          __builtin_amdgcn_perm(0x41414141u, lo, 0x05030402u),
+                          __builtin_amdgcn_perm(0x41414141u, hi, 0x05010400u),
+                          __builtin_amdgcn_perm(0x41414141u, hi, 0x05030402u));
       };
       w0 = word(r.v[0].x);
       w1 = word(r.v[0].y);
@@ -181,7 +183,7 @@ __global__ __launch_bounds__(64 * WK) void experts_rows_kernel(const ExpertsArgs
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
                 const float s = f16_lo(sp[r]);
-                const float b = BITS == 4 ? __builtin_fmaf(-128.0f, s, f16_hi(sp[r])) : f16_hi(sp[r]);
+                const float b = BITS == 4 ? __builtin_fmaf(-16.0f, s, f16_hi(sp[r])) : f16_hi(sp[r]);
                 acc[t][r] += __builtin_fmaf(s, d[r], b * sx[r]);
               }
             }
