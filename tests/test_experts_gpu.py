@@ -547,3 +547,63 @@ def test_w4_sums_of_few_rows_are_exact_where_f32_is(ctx, cut, gated, K):
         assert np.abs(t).max() <= 256            # exact in bf16
         assert np.array_equal(got, t)
     ex.close()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_sources_on_the_host_and_on_the_device(ctx, bits):
+    """The same stack from host arrays, in more than one piece, from device arrays, and
+    from device arrays that start beside a word."""
+    E, N, K = 6, 2048, 8192 if bits == 8 else 16384      # 16 MiB of codes an expert
+    rng = np.random.default_rng(bits)
+    codes = rng.integers(0, 2 ** 32, (E, N, K * bits // 32), dtype=np.uint32)
+    sc = bf16(rng.choice([0.5, 0.25, 2.0], (E, N, K // 64)).astype(np.float32) / 1024)
+    bi = bf16(rng.choice([-0.5, -0.25, 1.0], (E, N, K // 64)).astype(np.float32) / 16)
+    dev = [to_dev(a.view(np.int32) if a is codes else a) for a in (codes, sc, bi)]
+    odd = []
+    for t in dev:
+        b = torch.empty(t.numel() * t.element_size() + 1, dtype=torch.uint8, device="cuda")
+        b[1:] = t.reshape(-1).view(torch.uint8)
+        odd.append(b[1:])
+    n = 8
+    x, y = to_dev(bf16(randn(20000, (n, K)))), to_dev(np.zeros((n, N), np.uint16))
+    off = to_dev(np.minimum(np.arange(E + 1) * 2, n).astype(np.int32))
+    got = []
+    sync()
+    for src in (None, dev, odd):
+        if src is None:
+            ex = m.Experts.quantized(ctx, codes, sc, bi, bits)
+        else:
+            h = m.C.c_void_p()
+            m._check(m.lib().ming_experts_create(ctx.h, E, N, K, bits, 64, *map(m._ptr, src), 1,
+                                                 m.C.byref(h)))
+            ex = m.Experts(ctx, h)
+        for shift in (0, 4):                             # two rows to each of four experts
+            o = torch.zeros_like(off)
+            o[shift // 2:] = off[:E + 1 - shift // 2]
+            sync()
+            ctx.experts_lin(ex, x, n, None, o, n, y)
+            ctx.synchronize()
+            got.append(from_dev(y))
+        ex.close()
+    assert np.array_equal(got[0], got[2]) and np.array_equal(got[0], got[4])
+    assert np.array_equal(got[1], got[3]) and np.array_equal(got[1], got[5])
+    assert not np.array_equal(got[0], got[1])
+
+
+@pytest.mark.parametrize("on_device", [True, False])
+def test_a_stack_needs_its_own_memory_and_little_more(ctx, on_device):
+    """Created where three quarters of its size again are free, beside its sources."""
+    E, N, K = 16, 8192, 16384                            # 2 GiB of w8 codes
+    codes = torch.zeros((E, N, K // 4), dtype=torch.int32, device="cuda" if on_device else "cpu")
+    sc = torch.full((E, N, K // 64), 0x3f80, dtype=torch.int16, device=codes.device)
+    size = codes.numel() * 4 + sc.numel() * 4
+    torch.cuda.empty_cache()
+    free = torch.cuda.mem_get_info()[0]
+    fill = torch.empty(free - size * 7 // 4, dtype=torch.uint8, device="cuda")
+    try:
+        ex = m.Experts.quantized(ctx, codes, sc, sc, 8, on_device=on_device)
+        assert (ex.n_experts, ex.N, ex.K) == (E, N, K)
+        ex.close()
+    finally:
+        del fill, codes, sc
+        torch.cuda.empty_cache()

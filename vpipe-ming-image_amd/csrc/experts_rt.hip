@@ -192,14 +192,9 @@ int check_stack(ming_ctx* c, int E, int N, int K) {
   return MING_OK;
 }
 
-// Host or device memory copied to a new device buffer on the context's stream.
-hipError_t copy_in(ming_ctx* c, void** dst, const void* src, size_t bytes, int on_device) {
-  hipError_t e = hipMalloc(dst, bytes);
-  if (e == hipSuccess)
-    e = hipMemcpyAsync(*dst, src, bytes, on_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice,
-                       stream_of(c));
-  return e;
-}
+// Source memory that a stack's creation has on the device at a time where it has to
+// bring it there: some experts, so that a stack can be as large as the memory.
+constexpr size_t kStageBytes = 64u << 20;
 
 }  // namespace
 
@@ -360,22 +355,40 @@ int ming_experts_create(ming_ctx* c, int n_experts, int N, int K, int bits, int 
   const size_t words = (size_t)N * K * bits / 32, pairs = (size_t)N * (K / 64);
   const size_t E = (size_t)n_experts;
   hipStream_t s = stream_of(c);
-  void *dc = nullptr, *ds = nullptr, *db = nullptr;
+  // device arrays that the repack can read are read where they are
+  const bool direct =
+      src_on_device && aligned(codes, 4) && aligned(scales, 2) && aligned(biases, 2);
+  const size_t some =
+      direct ? E : std::clamp<size_t>(kStageBytes / (words * 4 + pairs * 4), 1, E);
+  const hipMemcpyKind kind = src_on_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice;
+  uint32_t* dc = nullptr;
+  uint16_t *ds = nullptr, *db = nullptr;
   int *flag = nullptr, inexact = 0;
-  hipError_t e = copy_in(c, &dc, codes, E * words * 4, src_on_device);
-  if (e == hipSuccess) e = copy_in(c, &ds, scales, E * pairs * 2, src_on_device);
-  if (e == hipSuccess) e = copy_in(c, &db, biases, E * pairs * 2, src_on_device);
-  if (e == hipSuccess) e = hipMalloc(&ex->codes, E * words * 4);
+  hipError_t e = hipMalloc(&ex->codes, E * words * 4);
   if (e == hipSuccess) e = hipMalloc(&ex->sb, E * pairs * 4);
   if (e == hipSuccess) e = hipMalloc(&flag, sizeof(int));
+  if (e == hipSuccess && !direct) e = hipMalloc(&dc, some * words * 4);
+  if (e == hipSuccess && !direct) e = hipMalloc(&ds, some * pairs * 2);
+  if (e == hipSuccess && !direct) e = hipMalloc(&db, some * pairs * 2);
   if (e == hipSuccess) e = hipMemsetAsync(flag, 0, sizeof(int), s);
-  for (size_t i = 0; i < E && e == hipSuccess; ++i)
-    e = ming::launch_repack_fast(bits, (const uint32_t*)dc + i * words,
-                                 (const uint16_t*)ds + i * pairs, (const uint16_t*)db + i * pairs,
-                                 N, K, ex->codes + i * words, ex->sb + i * pairs, flag, s);
+  for (size_t i0 = 0; i0 < E && e == hipSuccess; i0 += some) {
+    const size_t n = std::min(some, E - i0);
+    const uint32_t* sc = codes + i0 * words;
+    const uint16_t *ss = scales + i0 * pairs, *sb = biases + i0 * pairs;
+    if (!direct) {                         // (behind the repack of those before, in order)
+      e = hipMemcpyAsync(dc, sc, n * words * 4, kind, s);
+      if (e == hipSuccess) e = hipMemcpyAsync(ds, ss, n * pairs * 2, kind, s);
+      if (e == hipSuccess) e = hipMemcpyAsync(db, sb, n * pairs * 2, kind, s);
+      sc = dc; ss = ds; sb = db;
+    }
+    for (size_t i = 0; i < n && e == hipSuccess; ++i)
+      e = ming::launch_repack_fast(bits, sc + i * words, ss + i * pairs, sb + i * pairs, N, K,
+                                   ex->codes + (i0 + i) * words, ex->sb + (i0 + i) * pairs, flag,
+                                   s);
+  }
   if (e == hipSuccess) e = hipMemcpyAsync(&inexact, flag, sizeof(int), hipMemcpyDeviceToHost, s);
   if (e == hipSuccess) e = hipStreamSynchronize(s);
-  for (void* p : {dc, ds, db, (void*)flag})
+  for (void* p : {(void*)dc, (void*)ds, (void*)db, (void*)flag})
     if (p) (void)hipFree(p);
   if (e != hipSuccess || inexact) {
     (void)hipGetLastError();
