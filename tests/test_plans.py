@@ -2,6 +2,7 @@
 CPU (without a device they count the MI355X's 256 CUs), through the library's
 own symbols."""
 import ctypes as C
+import random
 
 import pytest
 
@@ -75,3 +76,21 @@ def test_the_last_rows_that_one_launch_holds():
     assert route(2 ** 26 - 4) and not route(2 ** 26 - 3) and not route(2 ** 31 - 1)
     assert xa(2 ** 28 - 32, 0) and not xa(2 ** 28 - 31, 0) and not xa(2 ** 28 - 32, 1)
     assert xa(767, 100) and not xa(2 ** 31 - 1, 0)
+
+
+@pytest.mark.parametrize("rows_main,rest", [(0, 64), (0, 256), (256, 128), (2048, 64), (2048, 192)])
+def test_a_tiles_list_holds_every_row_its_own_adapter(rows_main, rest):
+    """The bound the lists' blocks write under, against tiles counted row by row."""
+    import ming_dit_amd as m
+    f = m.lib()._ZN4ming15row_tile_chunksEiiiii
+    rng = random.Random(rest)
+    for M in (rows_main + 1, rows_main + rest - 1, rows_main + rest, rows_main + 5 * rest + 3,
+              max(rows_main, 1)):
+        for cap, max_rank in ((1, 512), (40, 17), (4096, 64)):
+            ldt = (max_rank + 31) // 32 * 32
+            ids = [rng.randrange(cap) for _ in range(M)]
+            for own in (ids, [i % cap for i in range(M)]):
+                edges = list(range(0, rows_main, 256)) + list(range(rows_main, M, rest)) + [M]
+                most = max(len(set(own[a:b])) for a, b in zip(edges, edges[1:]))
+                assert most * ((max_rank + 31) // 32) <= f(M, rows_main, rest, cap, ldt)
+            assert f(M, rows_main, rest, cap, ldt) <= 256 * (ldt // 32)

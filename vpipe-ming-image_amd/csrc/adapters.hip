@@ -13,7 +13,7 @@ namespace {
 constexpr int XW = 8;
 
 // The chunk list of row tile `tile` (at most 256 rows, a thread each): the chunks
-// of each adapter where the tile's first row of it stands.
+// of each adapter where the tile's first row of it stands, row_tile_chunks at most.
 __device__ __forceinline__ void row_chunks(const RowXaArgs& a, int tile, int* ids, int* sums) {
   const int tid = (int)threadIdx.x, lane = tid & 63;
   const int mains = a.rows_main / 256;
@@ -267,6 +267,11 @@ __global__ void check_finite_kernel(const uint16_t* v, long long n, int* flag) {
 }
 
 }  // namespace
+
+int row_tile_chunks(int M, int rows_main, int rest, int cap, int ldt) {
+  const int tallest = std::max(rows_main > 0 ? 256 : 0, M > rows_main ? rest : 0);
+  return std::min({tallest, M, cap}) * (ldt / 32);
+}
 
 // The x.A's row tiles: of 32 rows, or of 16 where there are few.
 static int row_xa_tiles(int M) {

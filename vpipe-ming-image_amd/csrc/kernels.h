@@ -434,10 +434,14 @@ struct RowXaArgs {
   uint16_t* xh;
   int* range;
 };
-// Row tiles of the lists, and chunks a tile may need.
+// Row tiles of the lists.
 inline int row_tiles(int M, int rows_main, int rest) {
   return rows_main / 256 + (M > rows_main ? (M - rows_main + rest - 1) / rest : 0);
 }
+// Chunks a tile may need, RowXaArgs::stride: an adapter a row of the tallest tile at
+// most, no more than the bank's `cap`, each of as many chunks as ldt holds. The lists'
+// blocks write up to that many and rely on it.
+int row_tile_chunks(int M, int rows_main, int rest, int cap, int ldt);
 hipError_t launch_row_xa(const RowXaArgs& a, hipStream_t s);
 // Whether its blocks, with `lists` of row tiles beside them, fit one launch.
 bool row_xa_fits(int M, int lists);

@@ -1270,9 +1270,7 @@ static int lin_multi(ming_ctx* c, int n, const ming_qweight* const* qs, const Li
       xr.rows_main = rp.rows_main / 256 * 256;
       xr.rest = 32 * rp.rf_rest;
       const int tiles = ming::row_tiles(M, xr.rows_main, xr.rest);
-      // at most an adapter a row of the tile
-      const int most = std::max(xr.rows_main > 0 ? 256 : 0, xr.rest);
-      xr.stride = std::min({most, M, rows->bank->cap}) * (ra.ldt / 32);
+      xr.stride = ming::row_tile_chunks(M, xr.rows_main, xr.rest, rows->bank->cap, ra.ldt);
       list_bytes = (size_t)tiles * xr.stride * sizeof(ming::RowChunk);
       count_bytes = (size_t)tiles * 4;
     } else if (!split) {
