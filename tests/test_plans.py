@@ -94,3 +94,16 @@ def test_a_tiles_list_holds_every_row_its_own_adapter(rows_main, rest):
                 most = max(len(set(own[a:b])) for a, b in zip(edges, edges[1:]))
                 assert most * ((max_rank + 31) // 32) <= f(M, rows_main, rest, cap, ldt)
             assert f(M, rows_main, rest, cap, ldt) <= 256 * (ldt // 32)
+
+
+@pytest.mark.parametrize("bits", [4, 8, 16])
+def test_the_experts_plan_counts_the_cus(bits):
+    """An eighth of a chip is full of tall tiles at an eighth of the groups; 256 CUs are
+    what a host without a device plans for."""
+    import ming_dit_amd as m
+    on, here = m.lib()._ZN4ming14experts_cut_onEiiiiii, m.lib()._ZN4ming11experts_cutEiiiii
+    for E in (8, 16, 64, 128):
+        for n in (1, 64, 1000, 300 * E, 600 * E):
+            assert on(256, E, 2048, 2048, bits, n) == here(E, 2048, 2048, bits, n)
+    tall = 8 if bits == 8 else 4
+    assert on(256, 2, 2048, 2048, bits, 600) == 2 and on(32, 2, 2048, 2048, bits, 600) == tall

@@ -287,11 +287,11 @@ hipError_t launch_row_xa(const RowXaArgs& a, hipStream_t s) {
   if (a.M <= 0) return hipSuccess;
   if (a.K % 64 || a.ldt % 32 || (a.counts && (a.rows_main % 256 || a.rest < 1 || a.rest > 256)))
     return hipErrorInvalidValue;
-  const int tiles = row_xa_tiles(a.M);
+  const int tiles = row_xa_tiles(a.M), cus = device_cus();
   const int lists = a.counts ? row_tiles(a.M, a.rows_main, a.rest) : 0;
   if (a.M >= kRowXaMany) {
     // ranks past 32 make it more than one pass over x: four chunks a pass then
-    const dim3 grid((unsigned)(tiles + lists), tiles < 128 ? 4u : tiles < 256 ? 2u : 1u);
+    const dim3 grid((unsigned)(tiles + lists), tiles < cus / 2 ? 4u : tiles < cus ? 2u : 1u);
     if (a.ldt <= 32)
       hipLaunchKernelGGL(row_xa_many_kernel<2>, grid, dim3(64 * XW), 0, s, a);
     else
@@ -299,7 +299,7 @@ hipError_t launch_row_xa(const RowXaArgs& a, hipStream_t s) {
     return hipGetLastError();
   }
   // a block a CU (two rounds of them, [500, 3840]: 14.6 us, one 9.0)
-  const int y = tiles < 256 / 64 ? 64 : tiles < 256 ? 256 / tiles : 1;
+  const int y = tiles < cus / 64 ? 64 : tiles < cus ? cus / tiles : 1;
   hipLaunchKernelGGL(row_xa_kernel, dim3((unsigned)(tiles + lists), (unsigned)y), dim3(64 * XW), 0, s,
                      a);
   return hipGetLastError();

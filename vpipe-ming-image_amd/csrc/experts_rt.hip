@@ -43,13 +43,16 @@ namespace ming {
 // blocks a CU or 128 and two ([128][1024, 2048] gated, 32 rows 41 / 43, 78: 70 / 57); w8, 64
 // or 256 ([60][2048, 1024], 160 rows 63 / 62, all groups of 256: 86 / 74).
 int experts_cut(int E, int N, int K, int bits, int n) {
+  return experts_cut_on(device_cus(), E, N, K, bits, n);
+}
+int experts_cut_on(int cus, int E, int N, int K, int bits, int n) {
   const double live = E * (1.0 - std::exp(-(double)n / E)), rows = n / live;
   const double weights = live * N * (double)K, stages = K / 64.0, blocks = live * (N / 32.0);
   const double passes = rows > 8.0 ? rows / 16.0 + 0.5 : 1.0;
   double few, tile;
   if (bits == 16) {
     const double one = 256.0 * K * 2 / 6.1e6;            // a tile's weights, us
-    const double all = live * ((N + 255) / 256), round = std::floor(all / 256.0) * 256.0;
+    const double all = live * ((N + 255) / 256), round = std::floor(all / cus) * cus;
     few = 2.5 + weights * 2 / 5.9e6 * (1.0 + rows / 40.0) * passes + 0.002 * blocks;
     tile = round * one + std::max(4.0 + 0.75 * stages, 2.5 + (all - round) * one);
   } else {
@@ -61,7 +64,7 @@ int experts_cut(int E, int N, int K, int bits, int n) {
   const double from = bits == 16 ? 112.0 : bits == 4 ? 60.0 : 240.0;
   // tiles of the tall cut, of which every group ends in half a one on average
   const double each = std::max(1.0, rows / ((bits == 16 ? 64 : 32) * tall) + 0.5);
-  return rows < from || live * each * ((N + 255) / 256) < 180.0 ? low : tall;
+  return rows < from || live * each * ((N + 255) / 256) < cus * (180.0 / 256.0) ? low : tall;
 }
 
 }  // namespace ming
@@ -123,6 +126,7 @@ int products(const char* who, bool gated, ming_ctx* c, const ming_experts* ex, c
   if (!order && x_rows < n) return bad(MING_ERR_SHAPE, "without an order x needs n rows");
   if (ldx > ((1ll << 30) - 1) / x_rows)
     return bad(MING_ERR_SHAPE, "x_rows * ldx must be below 2^30");
+  DeviceGuard g(ming::rt_device(c));       // (the plan counts its CUs)
   // the quantized tiles multiply fp16, which the other routes are chosen against
   const int cut = ex->bits != 16 && ming::rt_route(c) != MING_ROUTE_AUTO ? 0
                   : ming::rt_experts_cut(c) >= 0
@@ -146,7 +150,6 @@ int products(const char* who, bool gated, ming_ctx* c, const ming_experts* ex, c
     if (ming::spans_meet(in, ys) || ming::spans_meet(in, sc))
       return bad(MING_ERR_ARG, "x, order or offsets share memory with y or ws");
   if (ming::spans_meet(ys, sc)) return bad(MING_ERR_ARG, "y and ws share memory");
-  DeviceGuard g(ming::rt_device(c));
   ming::ExpertsArgs a{};
   a.x = x; a.ldx = ldx;
   a.codes = ex->codes; a.sb = ex->sb; a.w16 = ex->w16;

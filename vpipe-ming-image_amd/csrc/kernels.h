@@ -558,8 +558,9 @@ inline long long experts_tiles(int bits, bool gated, int max, int n, int E, int 
   return (long long)(n / cut + (n < E ? n : E)) * ((N + bn - 1) / bn);
 }
 // Which of them takes n places of a stack of N weight rows: 0 the few-row kernel,
-// else the tiles' cut (`max`).
+// else the tiles' cut (`max`). On the current device, or on a chip of `cus`.
 int experts_cut(int E, int N, int K, int bits, int n);
+int experts_cut_on(int cus, int E, int N, int K, int bits, int n);
 
 hipError_t validate_qproj_kernels();
 hipError_t validate_qproj_fast_kernels();
