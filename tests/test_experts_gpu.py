@@ -607,3 +607,23 @@ def test_a_stack_needs_its_own_memory_and_little_more(ctx, on_device):
     finally:
         del fill, codes, sc
         torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("K", [1088, 2048, 4160])
+@pytest.mark.parametrize("counts", [[0, 1, 0, 2], [17, 1, 40, 3]])
+def test_wide_and_narrow_few_row_blocks(ctx, cut, counts, K):
+    """Dense plain products past K = 1024, few places and many: blocks of 16 columns and
+    of 32, a row's bits its own whichever ran."""
+    E, N = 4, 4104
+    ex, w = ref.make_experts(ctx, 20100, E, N, K, 16)
+    offsets, order, src = ref.plan_of(counts, x_rows=9)
+    x = bf16(randn(20200, (9, K)))
+    cut(0)
+    got = run(ctx, ex, False, x, offsets, order, order.size)
+    check(got, w, x, offsets, src, False, 16)
+    one = np.zeros(E + 1, np.int32)
+    one[2:] = 1                                          # the first place of expert 1 alone
+    at = int(offsets[1])
+    alone = run(ctx, ex, False, x, one, order[at:at + 1], 1)
+    assert np.array_equal(alone[0], got[at])
+    ex.close()

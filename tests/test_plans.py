@@ -107,3 +107,14 @@ def test_the_experts_plan_counts_the_cus(bits):
             assert on(256, E, 2048, 2048, bits, n) == here(E, 2048, 2048, bits, n)
     tall = 8 if bits == 8 else 4
     assert on(256, 2, 2048, 2048, bits, 600) == 2 and on(32, 2, 2048, 2048, bits, 600) == tall
+
+
+def test_few_row_blocks_of_the_experts():
+    """Dense plain ones are narrow where wide ones would leave CUs idle, or K is long."""
+    import ming_dit_amd as m
+    f = m.lib()._ZN4ming18experts_rows_tilesEiibiiii
+    for n, K, co in ((1, 1088, 1), (7, 1472, 1), (8, 1472, 2), (64, 1088, 2), (64, 1536, 1),
+                     (1, 1024, 2)):
+        assert f(256, 16, False, 64, 1024, K, n) == co, (n, K)
+        assert f(256, 4, False, 64, 1024, K, n) == 2 and f(256, 8, True, 64, 1024, K, n) == 1
+    assert f(32, 16, False, 64, 1024, 1088, 1) == 2

@@ -106,10 +106,7 @@ __device__ __forceinline__ void operands(const Raw<BITS>& r, uint4& w0, uint4& w
 // WK waves with U groups in flight, by K: 8 with 2 (4 cost registers, so waves: 20 to
 // 55% longer), to K = 1024 with 1 ([60][2048, 1024] w8, 64 places 31.1 -> 26.0 us; K 7168
 // 8% slower), to 512 4 waves ([64][2048, 512] w8 gated, 64 places 14.1, eight 19.4). CO
-// 16-column tiles of the output, 2 plain (1 is 7 to 30% longer, 4 as much), 1 gated and,
-// with dense weights past K = 1024, plain ([16][2048, 4096], one place 11.1 -> 7.5, 16 36.3
-// -> 31.2).
-constexpr int rows_long_co(int bits, bool gated) { return gated || bits == 16 ? 1 : 2; }
+// 16-column tiles of the output by experts_rows_tiles.
 template <int BITS, bool GATED, int WK, int U, int CO>
 __global__ __launch_bounds__(64 * WK) void experts_rows_kernel(const ExpertsArgs a) {
   constexpr int CT = GATED ? 2 * CO : CO;  // column tiles: the outputs', then the up rows'
@@ -227,8 +224,10 @@ void rows_shape(const ExpertsArgs& a, hipStream_t s) {
     rows_launch<BITS, GATED, 4, 1, CO>(a, s);
   else if (a.K <= 1024)
     rows_launch<BITS, GATED, 8, 1, CO>(a, s);
-  else
-    rows_launch<BITS, GATED, 8, 2, rows_long_co(BITS, GATED)>(a, s);
+  else if (experts_rows_tiles(device_cus(), BITS, GATED, a.E, a.N, a.K, a.n) == CO)
+    rows_launch<BITS, GATED, 8, 2, CO>(a, s);
+  else if constexpr (BITS == 16)
+    rows_launch<BITS, GATED, 8, 2, 1>(a, s);
 }
 
 // w [NW][K] -> [K / 64][NW][64], 16 bytes a thread and step.
@@ -245,6 +244,21 @@ __global__ void repack_dense_kernel(const uint16_t* w, int NW, int K, uint16_t* 
 }
 
 }  // namespace
+
+// One gated (the up rows are a second one), 2 plain (1 is 7 to 30% longer up to K = 1024
+// and with quantized weights, 4 as much). Dense plain ones past K = 1024 are 1 where
+// blocks of 2 would leave CUs idle, and from K = 1536 on. Microseconds of 2 and 1:
+// [64][1024, 1088 to 2048], one and 4 places (32 and 128 blocks of 2) 5.3 to 7.5 and 4.5 to
+// 6.2; with more blocks, [64][1024, 1088], 16 places 8.8 and 9.4, [60][2048, 1088] 14.8 and
+// 16.4, [60][2048, 1408] 18.8 and 20.2; [16][2048, 1536], 32 places 17.8 and 16.4, 64 21.5 and
+// 23.1; [64][1024, 1792], 16 places 11.7 and 10.3; [128][512, 2048], 16 places 8.6 and 9.2;
+// [16][2048, 4096], 16 places 36.3 and 31.0; [16][1024, 7168], 8 places 18.7 and 20.0, 16 38.9
+// and 32.0.
+int experts_rows_tiles(int cus, int bits, bool gated, int E, int N, int K, int n) {
+  if (gated) return 1;
+  if (bits != 16 || K <= 1024) return 2;
+  return K >= 1536 || (long long)(n < E ? n : E) * ((N + 31) / 32) < cus ? 1 : 2;
+}
 
 hipError_t launch_repack_dense(const uint16_t* w, int NW, int K, uint16_t* out, hipStream_t s) {
   if (NW <= 0 || K <= 0 || K % 64) return hipErrorInvalidValue;
@@ -273,12 +287,12 @@ hipError_t validate_experts_kernels() {
 #define MING_EXPERTS_ROWS(BITS)                                                   \
   reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 4, 1, 2>),      \
       reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 8, 1, 2>),  \
-      reinterpret_cast<const void*>(                                              \
-          &experts_rows_kernel<BITS, false, 8, 2, rows_long_co(BITS, false)>),    \
+      reinterpret_cast<const void*>(&experts_rows_kernel<BITS, false, 8, 2, 2>),  \
       reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 4, 1, 1>),   \
       reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 8, 1, 1>),   \
       reinterpret_cast<const void*>(&experts_rows_kernel<BITS, true, 8, 2, 1>)
       reinterpret_cast<const void*>(&repack_dense_kernel),
+      reinterpret_cast<const void*>(&experts_rows_kernel<16, false, 8, 2, 1>),
       MING_EXPERTS_ROWS(4), MING_EXPERTS_ROWS(8), MING_EXPERTS_ROWS(16)
 #undef MING_EXPERTS_ROWS
   };

@@ -539,6 +539,9 @@ struct ExpertsArgs {
 hipError_t launch_repack_dense(const uint16_t* w, int NW, int K, uint16_t* out, hipStream_t s);
 // few rows an expert, any weights (experts.hip)
 hipError_t launch_experts_rows(int bits, bool gated, const ExpertsArgs& a, hipStream_t s);
+// 16-column tiles of its blocks on a chip of `cus`, for n places of a stack of outputs
+// N wide. The bits are the same.
+int experts_rows_tiles(int cus, int bits, bool gated, int E, int N, int K, int n);
 hipError_t validate_experts_kernels();
 // dense weights, tiles (experts_tile.hip): groups cut every 64 * max places, max 2
 // or 4; x_rows * ldx and NW * K below 2^30, y 16-byte aligned with ldy % 8 == 0
