@@ -58,7 +58,8 @@ __device__ __forceinline__ void row_chunks(const RowXaArgs& a, int tile, int* id
 
 __global__ __launch_bounds__(64 * XW) void row_xa_kernel(const RowXaArgs a) {
   __shared__ floatx4_t red[XW][64];
-  __shared__ int ids[256], sums[XW];
+  __shared__ alignas(16) int ids[256];       // row_chunks reads four at a time
+  __shared__ int sums[XW];
   const int xtiles = (a.M + 15) / 16;
   if ((int)blockIdx.x >= xtiles) {           // the lists' blocks
     if (blockIdx.y == 0) row_chunks(a, (int)blockIdx.x - xtiles, ids, sums);
