@@ -401,7 +401,8 @@ int ming_experts_shape(const ming_experts* ex, int* n_experts, int* N, int* K, i
  * ws. Quantized stacks multiply fp16 activations from some rows an expert on, with
  * ming_lin's range rule (see MING_ERR_RANGE) for the rows that some place names: the
  * others may hold anything, as y's rows behind the last group do. On the general and
- * the wide route they take bf16 ones at any size, and more time. */
+ * the wide route they take bf16 ones at any size, and more time. Sums are f32; the
+ * fp16 tiles round each dequantized weight to fp16, as ming_lin's do. */
 size_t ming_experts_workspace_bytes(const ming_experts* ex, int x_rows);
 int ming_experts_lin(ming_ctx* ctx, const ming_experts* ex, const uint16_t* x, int64_t ldx,
                      int x_rows, const int32_t* order, int fan, const int32_t* offsets, int n,
@@ -439,10 +440,11 @@ int ming_adapters_rank(const ming_adapters* bank, int id);
 /* ming_lin with an adapter a row: y[m] = x[m] . W^T + row_scale[m] * fold_a *
  * B_a (A_a x[m]), a = row_adapter[m] (device int32 [M]; row_scale device f32
  * [M], NULL: all 1). A row whose id names no bound adapter, or whose strength
- * is 0, is ming_lin's row without adapters. The adapters' sum joins the f32
- * result before the one rounding; a row's bits do not depend on the other rows'
- * adapters (but for the sign of a zero). Slots bound on the weight take no part.
- * M up to 2^28 - 32. x as ming_lin's, y 16-byte aligned with ldy % 8 == 0; none of x, row_adapter and
+ * is 0, is ming_lin's row without adapters. A row's scaled A_a x[m] is rounded to
+ * bf16, as ming_lin's is; the adapters' sum joins the f32 result before the one
+ * rounding; a row's bits do not depend on the other rows' adapters (but for the
+ * sign of a zero). Slots bound on the weight take no part. M up to 2^28 - 32. x as
+ * ming_lin's, y 16-byte aligned with ldy % 8 == 0; none of x, row_adapter and
  * row_scale shares memory with y or ws. The size is that of x rows beside each
  * other; a dense projection of x rows that span more than 2 GiB may need more, and
  * says how much (MING_ERR_SHAPE). */

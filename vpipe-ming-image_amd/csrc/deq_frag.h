@@ -1,5 +1,11 @@
 // Codes of the fast resident layout to fp16 MFMA fragments (qproj_fast.hip says
 // how the layout is built), and where a code tile's chunks lie in LDS.
+//
+// A weight, code * scale + bias, is rounded here once to fp16, at most 2^-11 of it: the
+// matrix operand's type, three bits more than the output keeps. Against weights in f32
+// sums move by 2e-4 (w8) and 4e-5 (w4, where code * scale has four bits less) of
+// themselves: bf16 outputs then differ by 9e-4 and 3e-4 in the 2-norm, where a value
+// falls to the other side, and their error against 64 bits stays at 1.7e-3, bf16's own.
 #pragma once
 
 #include "common.h"

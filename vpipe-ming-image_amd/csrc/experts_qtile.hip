@@ -19,8 +19,8 @@
 // places; what is left of one runs at the height it needs. The lower cuts leave LDS
 // and registers for two or three blocks a CU, which hide each other's barriers and
 // starts and keep more of the weights in flight: experts_cut says which cut.
-// [128][1024, 2048] w4 gated, 16384 places in uneven groups 85.9 us, in groups of 128
-// 61; [60][2048, 1024] w8, 1218 places 25.2, its weights at 5.6 TB/s.
+// [128][1024, 2048] w4 gated, 16384 places in uneven groups 85 to 95 us, by the card, groups
+// of 128 61 to 65; [60][2048, 1024] w8, 1218 places 25.2, its weights at 5.6 TB/s.
 #include "common.h"
 #include "deq_frag.h"
 #include "kernels.h"

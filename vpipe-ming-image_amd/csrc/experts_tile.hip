@@ -16,7 +16,7 @@
 // finds its tile by find_group, the rest leave. An XCD takes a contiguous range
 // of tiles, an expert's columns outermost, so its L2 holds the weights in use.
 // [64][2048, 2048] gated: 32768 places in groups of 512, 234 us (1177 TFLOP/s); 34816
-// in uneven ones, 295 (matrix pipes 52% busy, 1.0 GB past the L2s).
+// in uneven ones 294 to 308, by the card (matrix pipes 53% busy, 1.0 GB past the L2s).
 #include <type_traits>
 
 #include "common.h"
