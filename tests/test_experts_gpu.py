@@ -627,3 +627,26 @@ def test_wide_and_narrow_few_row_blocks(ctx, cut, counts, K):
     alone = run(ctx, ex, False, x, one, order[at:at + 1], 1)
     assert np.array_equal(alone[0], got[at])
     ex.close()
+
+
+@pytest.mark.parametrize("bits", [4, 8, 16])
+@pytest.mark.parametrize("where", ["pinned", "other device"])
+def test_sources_that_are_not_the_devices_own(ctx, bits, where):
+    """Arrays said to be on the device that lie in host memory the device can reach, or
+    on another device, come over by copies."""
+    if where == "other device" and torch.cuda.device_count() < 2:
+        pytest.skip("one device")
+    E, N, K = 3, 48, 192
+    pack, w = ref.stack(20300, E, N, K, bits)
+    there = []
+    for a in pack.values():
+        t = torch.from_numpy(np.ascontiguousarray(a).view(np.int32 if a.dtype == np.uint32 else np.int16))
+        there.append(t.pin_memory() if where == "pinned" else t.to("cuda:1"))
+    if bits == 16:
+        ex = m.Experts.dense(ctx, there[0], on_device=True)
+    else:
+        ex = m.Experts.quantized(ctx, *there, bits, on_device=True)
+    offsets, order, src = ref.plan_of([5, 0, 9], x_rows=20)
+    x = bf16(randn(20400, (20, K)))
+    check(run(ctx, ex, False, x, offsets, order, order.size), w, x, offsets, src, False, bits)
+    ex.close()

@@ -195,6 +195,17 @@ int check_stack(ming_ctx* c, int E, int N, int K) {
   return MING_OK;
 }
 
+// Whether the context's kernels can read p where it is: its own device's memory. That
+// of another device comes over by copies, which need no access from here.
+bool own_memory(const ming_ctx* c, const void* p) {
+  hipPointerAttribute_t at{};
+  if (hipPointerGetAttributes(&at, p) != hipSuccess) {
+    (void)hipGetLastError();
+    return false;
+  }
+  return at.type == hipMemoryTypeDevice && at.device == ming::rt_device(c);
+}
+
 // Source memory that a stack's creation has on the device at a time where it has to
 // bring it there: some experts, so that a stack can be as large as the memory.
 constexpr size_t kStageBytes = 64u << 20;
@@ -316,13 +327,15 @@ int ming_experts_create_dense(ming_ctx* c, int n_experts, int N, int K, const ui
   ming::rt_retain(c);
   const size_t one = (size_t)N * K;
   hipStream_t s = stream_of(c);
-  void* stage = nullptr;                 // an expert's source, where it is on the host
+  void* stage = nullptr;                 // an expert's source, where it is elsewhere
+  const bool direct = src_on_device && own_memory(c, w);
+  const hipMemcpyKind kind = src_on_device ? hipMemcpyDefault : hipMemcpyHostToDevice;
   hipError_t e = hipMalloc(&ex->w16, (size_t)n_experts * one * 2);
-  if (e == hipSuccess && !src_on_device) e = hipMalloc(&stage, one * 2);
+  if (e == hipSuccess && !direct) e = hipMalloc(&stage, one * 2);
   for (int i = 0; i < n_experts && e == hipSuccess; ++i) {
     const uint16_t* src = w + i * one;
     if (stage) {
-      e = hipMemcpyAsync(stage, src, one * 2, hipMemcpyHostToDevice, s);
+      e = hipMemcpyAsync(stage, src, one * 2, kind, s);
       src = static_cast<const uint16_t*>(stage);
     }
     if (e == hipSuccess) e = ming::launch_repack_dense(src, N, K, ex->w16 + i * one, s);
@@ -358,12 +371,13 @@ int ming_experts_create(ming_ctx* c, int n_experts, int N, int K, int bits, int 
   const size_t words = (size_t)N * K * bits / 32, pairs = (size_t)N * (K / 64);
   const size_t E = (size_t)n_experts;
   hipStream_t s = stream_of(c);
-  // device arrays that the repack can read are read where they are
-  const bool direct =
-      src_on_device && aligned(codes, 4) && aligned(scales, 2) && aligned(biases, 2);
+  // arrays that the repack can read are read where they are
+  const bool direct = src_on_device && aligned(codes, 4) && aligned(scales, 2) &&
+                      aligned(biases, 2) && own_memory(c, codes) && own_memory(c, scales) &&
+                      own_memory(c, biases);
   const size_t some =
       direct ? E : std::clamp<size_t>(kStageBytes / (words * 4 + pairs * 4), 1, E);
-  const hipMemcpyKind kind = src_on_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice;
+  const hipMemcpyKind kind = src_on_device ? hipMemcpyDefault : hipMemcpyHostToDevice;
   uint32_t* dc = nullptr;
   uint16_t *ds = nullptr, *db = nullptr;
   int *flag = nullptr, inexact = 0;
