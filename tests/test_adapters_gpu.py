@@ -2,6 +2,8 @@
 requests, against 64-bit arithmetic: every weight type and route, from one row
 to many tiles, requests that end inside tiles, rows without an adapter, ranks
 that are no multiple of 8, strengths, strides, captured calls."""
+import re
+
 import numpy as np
 import pytest
 import torch
@@ -582,5 +584,37 @@ def test_more_rows_than_a_launch_holds(ctx, M):
         ctx.lin_adapters(qw, bank, far, far << 1, M, far << 2, None,
                          torch.empty(4096, dtype=torch.uint8, device="cuda"))
     assert e.value.code == 2 and ctx.lin_adapters_workspace_bytes(qw, bank, M) == 0
+    bank.close()
+    qw.close()
+
+
+@pytest.mark.parametrize("bits", [4, 8, 16])
+@pytest.mark.parametrize("M", [6, 40, 300])
+def test_inputs_past_32_bits(ctx, bits, M):
+    """Rows of x that span more than 4 GiB. A dense projection takes another launch for
+    them and says what it needs."""
+    N, K, ld = 1032, 1024, 1 << 29 if M == 6 else 1 << 26 if M == 40 else 1 << 23
+    qw, w = weight(ctx, 20700, N, K, bits)
+    bank, held = make_bank(ctx, 20800, N, K, RANKS)
+    x = bf16(randn(20900, (M, K)))
+    ids, s = requests(M, 8, len(RANKS))
+    far = torch.empty((M, ld), dtype=torch.int16, device="cuda")
+    far[:, :K] = to_dev(x)
+    y = to_dev(np.zeros((M, N), np.uint16))
+    idd, sd = to_dev(ids.astype(np.int32)), to_dev(s)
+    need = ctx.lin_adapters_workspace_bytes(qw, bank, M)
+    sync()
+    for _ in range(2):
+        ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+        try:
+            ctx.lin_adapters(qw, bank, far, y, M, idd, sd, ws, ldx=ld)
+            break
+        except m.MingError as e:
+            assert bits == 16 and e.code == 2
+            need = int(re.search(r"needs (\d+) bytes", str(e)).group(1))
+    ctx.synchronize()
+    check(from_dev(y), x, w, held, ids, s, bits)
+    del far
+    torch.cuda.empty_cache()
     bank.close()
     qw.close()

@@ -650,3 +650,31 @@ def test_sources_that_are_not_the_devices_own(ctx, bits, where):
     x = bf16(randn(20400, (20, K)))
     check(run(ctx, ex, False, x, offsets, order, order.size), w, x, offsets, src, False, bits)
     ex.close()
+
+
+@pytest.mark.parametrize("bits", [4, 8, 16])
+def test_inputs_as_far_apart_as_they_may_be(ctx, cut, bits):
+    """Rows of x whose last lies 2 GiB from the first: the bits of rows side by side."""
+    E, N, K, T = 3, 272, 128, 64
+    ld = ((1 << 30) - 1) // T // 8 * 8
+    ex, w = ref.make_experts(ctx, 20500, E, N, K, bits)
+    offsets, order, src = ref.plan_of([90, 0, 110], x_rows=T)
+    order[5], src[5] = T - 1, T - 1
+    n = order.size
+    x = bf16(randn(20600, (T, K)))
+    far = torch.empty((T, ld), dtype=torch.int16, device="cuda")
+    far[:, :K] = to_dev(x)
+    od, fd, y = to_dev(order), to_dev(offsets), to_dev(np.zeros((n, N), np.uint16))
+    ws = torch.empty(max(1, ex.workspace_bytes(T)), dtype=torch.uint8, device="cuda")
+    for c in ref.CUTS[bits]:
+        cut(c)
+        near = run(ctx, ex, False, x, offsets, order, n)
+        check(near, w, x, offsets, src, False, bits)
+        y.zero_()
+        sync()
+        ctx.experts_lin(ex, far, T, od, fd, n, y, ws=ws, ldx=ld)
+        ctx.synchronize()
+        assert np.array_equal(from_dev(y), near)
+    del far
+    torch.cuda.empty_cache()
+    ex.close()

@@ -383,7 +383,8 @@ hipError_t launch_experts_qtile(int bits, bool gated, const ExpertsArgs& a, int 
                                 hipStream_t s) {
   if (a.n <= 0 || a.N <= 0) return hipSuccess;
   if (a.K % 64 || a.N % 8 || a.NW != a.N * (gated ? 2 : 1) || a.E < 1 || a.fan < 1 ||
-      a.x_rows < 1 || a.ldy % 8 || !a.beyond || (bits != 4 && bits != 8) || (max != 2 && max != tall(bits)))
+      a.x_rows < 1 || a.ldy % 8 || !a.beyond || (bits != 4 && bits != 8) ||
+      (max != 2 && max != tall(bits)))
     return hipErrorInvalidValue;
   if (bits == 4)
     gated ? launch_max<4, true>(a, max, s) : launch_max<4, false>(a, max, s);

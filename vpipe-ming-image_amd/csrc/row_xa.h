@@ -11,11 +11,11 @@ namespace ming {
 // whose T is bf16 too. Outputs of rows whose adapters add a third as much as the weight
 // move by 3e-4 before their own rounding, their error against 64 bits stays at 1.7e-3.
 // A block takes 16 or 32 rows; the adapters among them (in any order) are found with
-// ballots, and each adapter's 16-rank chunks are v_mfma_f32_16x16x32_bf16 tiles over all the rows, of
-// which only that adapter's are stored: requests' rows lie together, so a block
-// has one or two adapters, and where every row has its own the time is that of
-// reading their A. K is shared out over the eight waves by 64-groups, the sums
-// meet in LDS and are added in wave order (no atomics). A is resident in the
+// ballots, and each adapter's 16-rank chunks are v_mfma_f32_16x16x32_bf16 tiles over
+// all the rows, of which only that adapter's are stored: requests' rows lie together,
+// so a block has one or two adapters, and where every row has its own the time is
+// that of reading their A. K is shared out over the eight waves by 64-groups, the
+// sums meet in LDS and are added in wave order (no atomics). A is resident in the
 // operand's own order (launch_repack_adapter): a wave's load is one run of 1 KB, of
 // which lanes past the rank take no part.
 //
