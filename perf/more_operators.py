@@ -1,5 +1,5 @@
 """The operators of projections in 8-bit floating point (e4m3) with a scale for
-each block of 128, as cases that can be timed and checked: the quantizer of rows,
+each block of 128 (bf16 beside rows, f32 beside weights as checkpoints hold them), as cases that can be timed and checked: the quantizer of rows,
 the RMSNorm with the residual's addition whose output is in 8 bits, the product,
 the gated product whose result is in 8 bits again, and both products over the
 groups of a mixture of experts.
@@ -119,17 +119,20 @@ def _blocks(n):
     return (n + 127) // 128
 
 
-def _codes_of_rows(t, factor=None):
-    """[rows][D] -> codes [rows][D] and scales [blocks][rows], as the quantizer has them, of
-    t or of t times a factor a row [rows][1]. In 64 bits: values lie on the border of two
-    codes (448 times an 8-bit ratio often does), which a rounded factor would move."""
+def _scale_up(t):
+    """The least bf16 value of at least t (64-bit, positive)."""
+    s = t.float().to(torch.bfloat16)
+    return torch.where(s.double() < t, (s.view(torch.int16) + 1).view(torch.bfloat16), s)
+
+
+def _codes_of_rows(t):
+    """[rows][D] -> codes [rows][D] and bf16 scales [blocks][rows], as the quantizer has them.
+    In 64 bits: values often lie on the border of two codes (a ratio of 8-bit values)."""
     rows, D = t.shape
     p = torch.nn.functional.pad(t.double(), (0, _blocks(D) * 128 - D)).view(rows, -1, 128)
-    top = p.abs().amax(-1)
-    top = top.clamp(min=TINY) if factor is None else torch.maximum(top, TINY / factor)
-    q = (p * MOST / top[..., None]).float().to(F8).view(rows, -1)
-    s = (top if factor is None else top * factor) / MOST
-    return q[:, :D].contiguous(), s.float().t().contiguous()
+    s = _scale_up(p.abs().amax(-1).clamp(min=TINY) / MOST)
+    q = (p / s.double()[..., None]).float().to(F8).view(rows, -1)
+    return q[:, :D].contiguous(), s.t().contiguous()
 
 
 def _weight(seed, tag, shape, halves):
@@ -242,7 +245,7 @@ def _handles(st):
         st.y = _empty(rows, wide)
     else:
         st.codes = _empty(rows, wide, dtype=F8)
-        st.scales = _empty(_blocks(wide), rows, dtype=torch.float32)
+        st.scales = _empty(_blocks(wide), rows)
     ctx.synchronize()
 
 
@@ -280,7 +283,7 @@ def _own(st):
 # ---- the plain forms ------------------------------------------------------------------
 def _f32(x, xs):
     """Rows in 32 bits: code * scale."""
-    return x.float() * xs.t().repeat_interleave(128, 1)[:, :x.shape[1]]
+    return x.float() * xs.float().t().repeat_interleave(128, 1)[:, :x.shape[1]]
 
 
 def _w32(w):
@@ -300,10 +303,8 @@ def _norm(c, d):
     if c["add"]:
         h = (h.float() + d["sub"].float()).to(torch.bfloat16)
     v = h.float()
-    factor = torch.rsqrt((v * v).mean(1, keepdim=True) + EPS)
-    v = v * d["w"].float()            # 8 bits times 8 bits: exact
-    return [h if c["add"] else None, (v * factor).to(torch.bfloat16) if c["y"] else None,
-            *_codes_of_rows(v, factor.double())]
+    v = v * torch.rsqrt((v * v).mean(1, keepdim=True) + EPS) * d["w"].float()
+    return [h if c["add"] else None, v.to(torch.bfloat16) if c["y"] else None, *_codes_of_rows(v)]
 
 
 def _lin(c, d):
@@ -339,7 +340,7 @@ def work(case):
     if op in ("quantize", "norm"):
         n = float(c["rows"]) * c["D"]
         each = 3.0 if op == "quantize" else 3.0 + (4.0 if c["add"] else 0.0) + (2.0 if c["y"] else 0.0)
-        return {"bytes": each * n + 4.0 * c["rows"] * _blocks(c["D"]) + 2.0 * c["D"] * (op == "norm"),
+        return {"bytes": each * n + 2.0 * c["rows"] * _blocks(c["D"]) + 2.0 * c["D"] * (op == "norm"),
                 "flops": (4.0 if op == "quantize" else 8.0) * n}
     gated = op in ("swiglu", "experts_swiglu")
     N, K = c["N"], c["K"]
@@ -348,8 +349,8 @@ def work(case):
     rows = c["tokens"] if op == "experts_swiglu" else n
     E = c.get("experts", 1)
     live = E * (1.0 - (1.0 - 1.0 / E) ** n) if E > 1 else 1.0     # experts with a row, about
-    out = n * (N + 4.0 * _blocks(N)) if gated else 2.0 * n * N
-    return {"bytes": live * (wide * K + wide / 32.0 * _blocks(K)) + rows * (K + 4.0 * _blocks(K))
+    out = n * (N + 2.0 * _blocks(N)) if gated else 2.0 * n * N
+    return {"bytes": live * (wide * K + wide / 32.0 * _blocks(K)) + rows * (K + 2.0 * _blocks(K))
             + out + (2.0 * N if c.get("bias") else 0.0) + (4.0 * n if E > 1 else 0.0),
             "flops": 2.0 * n * wide * K}
 
@@ -358,21 +359,22 @@ def work(case):
 def _e4m3_64(v):
     """The nearest e4m3 value of |v| <= 448 in 64 bits, ties to even: steps of 2^(e - 3) in
     [2^e, 2^(e + 1)), of 2^-9 below 2^-6."""
-    e = torch.frexp(v.abs().clamp(min=2.0 ** -6))[1] - 1
-    step = torch.ldexp(torch.ones_like(v), e - 3)
+    a = v.abs().clamp(min=2.0 ** -6)
+    step = a / torch.frexp(a)[0] / 16.0           # 2^(e + 1) / 16
     return torch.round(v / step) * step
 
 
-def _quantize64(v, norm=1.0):
-    """Codes and scales of 64-bit rows over `norm`, block by block (the codes go by the
-    ratio of two values, in which norm has no part)."""
+def _quantize64(v):
+    """Codes and scales of 64-bit rows, block by block. The codes go by the scale as it is
+    stored, in bf16 and not below the largest value's 448th; that 448th is returned."""
     codes, scales = torch.empty_like(v), []
     for a in range(0, v.shape[1], 128):
         b = v[:, a:a + 128]
-        top = torch.maximum(b.abs().max(1, keepdim=True).values,
-                            torch.full_like(b[:, :1], TINY) * norm)
-        codes[:, a:a + 128] = _e4m3_64(448.0 * b / top)
-        scales.append((top / norm)[:, 0] / 448.0)
+        s = torch.clamp(b.abs().max(1, keepdim=True).values, min=TINY) / 448.0
+        m = torch.frexp(s)[0]
+        kept = torch.ceil(m * 256.0) / 256.0 * (s / m)            # 8 bits
+        codes[:, a:a + 128] = _e4m3_64(b / kept)
+        scales.append(s[:, 0])
     return [codes, torch.stack(scales)]
 
 
@@ -400,8 +402,8 @@ def exact(case, seed):
             h = (h + d["sub"].double())
         # the sum that goes on is the stored one
         kept = h.to(torch.bfloat16).double() if c["add"] else h
-        v, norm = kept * d["w"].double(), torch.sqrt(kept.square().mean(1, keepdim=True) + EPS)
-        return [h if c["add"] else None, v / norm if c["y"] else None, *_quantize64(v, norm)]
+        v = kept / torch.sqrt(kept.square().mean(1, keepdim=True) + EPS) * d["w"].double()
+        return [h if c["add"] else None, v if c["y"] else None, *_quantize64(v)]
     gated = op in ("swiglu", "experts_swiglu")
     if op in ("lin", "swiglu"):
         y = _product64(d["x"], d["xs"], d["w"], 0, 0)
