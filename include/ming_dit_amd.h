@@ -455,6 +455,92 @@ int ming_lin_adapters(ming_ctx* ctx, const ming_qweight* qw, const ming_adapters
                       const int32_t* row_adapter, const float* row_scale, void* ws,
                       size_t ws_bytes);
 
+/* ---- projections in 8-bit floating point, a scale a block of 128 ----------------
+ * Beside the w4, w8 and dense projections: weights and activations as OCP e4m3
+ * codes (one byte: largest value 448, NaN 0x7f and 0xff, no inf) with scales,
+ * multiplied on the 8-bit matrix cores. An activation [rows][ld] bytes has a bf16
+ * scale for each 128 columns of a row, held by blocks: scales[b * lds + row], lds
+ * >= rows; a weight [N][K] an f32 one for each 128 x 128 block, [ceil(N / 128)]
+ * [ceil(K / 128)], as checkpoints have them. A last block may be short. What a code
+ * stands for is code * scale.
+ *
+ * Quantized rows: of a block of 128 columns with largest magnitude a (2^-100 at
+ * least) the scale is the least bf16 of at least a / 448, a code the nearest e4m3
+ * of v / scale, ties to even. A block that holds inf or NaN has codes of NaN and a
+ * scale of NaN, and no other.
+ * Nothing here waits for the GPU or allocates but _create and _destroy, and
+ * every other call can be captured. Calls of no rows do nothing and take NULL
+ * arrays. Inputs, outputs and ws share no memory but where it says so.
+ *
+ * The rows of x [rows][ldx] bf16. D % 16 == 0; x and codes 16-byte aligned,
+ * ldx % 8 == 0, ldc % 16 == 0. */
+int ming_f8_quantize(ming_ctx* ctx, const uint16_t* x, int64_t ldx, int rows, int D,
+                     uint8_t* codes, int64_t ldc, uint16_t* scales, int64_t lds);
+/* RMSNorm with the residual's addition before it and 8-bit rows after it: h =
+ * bf16(x + sub), v = h * rsqrt(mean(h^2) + eps) * w, codes and scales of v, quantized
+ * without a rounding before it; with y not NULL also y = bf16(v). Without sub (NULL, and h
+ * NULL) h is x and not written; h may be x itself or sub itself, with its stride. A
+ * row whose mean square is inf or NaN in f32 has codes and scales of NaN. D % 16
+ * == 0, D <= 8192, eps 1e-12 to 1; pointers 16-byte aligned, strides multiples of
+ * 8, ldc of 16. */
+int ming_f8_rmsnorm(ming_ctx* ctx, const uint16_t* x, int64_t ldx, const uint16_t* sub,
+                    int64_t ldsub, uint16_t* h, int64_t ldh, const uint16_t* w, uint16_t* y,
+                    int64_t ldy, uint8_t* codes, int64_t ldc, uint16_t* scales, int64_t lds,
+                    int rows, int D, float eps);
+/* A weight w [N][K] bf16 (device) into the codes and scales that ming_f8_create
+ * takes: of a block of 128 x 128 the scale is f32(a / 448), a code the nearest
+ * e4m3 of 448 v / a. K % 16 == 0; w and codes 16-byte aligned. */
+int ming_f8_quantize_weight(ming_ctx* ctx, const uint16_t* w, int N, int K, uint8_t* codes,
+                            float* scales);
+
+/* A resident projection, or a stack of n_experts of one shape (1 to 1024): codes
+ * [n_experts][N][K] and scales [n_experts][ceil(N/128)][ceil(K/128)]. gated: a
+ * SwiGLU's two projections, codes [n_experts][2 N][K] with the gate's N rows
+ * before the up projection's, and scales [n_experts][2 ceil(N/128)][...] likewise,
+ * each half's blocks by itself. K % 16 == 0, N % 8 == 0, gated N % 16 == 0; an
+ * expert's weights, padded to 128 rows and columns, below 2 GiB. The sources may
+ * be freed when the call returns. */
+typedef struct ming_f8 ming_f8;
+int ming_f8_create(ming_ctx* ctx, int n_experts, int N, int K, int gated, const uint8_t* codes,
+                   const float* scales, int src_on_device, ming_f8** out);
+int ming_f8_destroy(ming_f8* w);
+int ming_f8_shape(const ming_f8* w, int* n_experts, int* N, int* K, int* gated);
+
+/* The products from rows x [M][ldx] of codes with scales xs [ceil(K/128)][ldxs].
+ * Sums over blocks of 128 are the 8-bit matrix instruction's (it cuts what lies 13
+ * bits below the largest of 8 products: 1.3e-5 of a block's sum in the 2-norm,
+ * beside 1.6e-3 of a result's rounding to bf16); they are added up in f32, times
+ * both scales.
+ *   ming_f8_lin:     y[m] = bf16(x[m] . W^T + bias), bias [N] bf16 or NULL
+ *   ming_f8_swiglu:  silu(x[m] . G^T) * (x[m] . U^T) of gated weights, in f32 and
+ *                    quantized like ming_f8_quantize's rows: codes h [M][ldh],
+ *                    scales hs [ceil(N/128)][ldhs], as the next product takes them
+ * x and h 16-byte aligned with strides multiples of 16, y 16-byte aligned with
+ * ldy % 8 == 0, bias 8-byte aligned; ldx below 2^22, M up to 2^28. ws 16-byte
+ * aligned, at least the bytes that ming_f8_workspace_bytes names for M rows (NULL
+ * where that is 0); it holds nothing between calls, and calls or graphs that may
+ * run at the same time need one each. */
+size_t ming_f8_workspace_bytes(const ming_f8* w, int rows);
+int ming_f8_lin(ming_ctx* ctx, const ming_f8* w, const uint8_t* x, int64_t ldx, const uint16_t* xs,
+                int64_t ldxs, uint16_t* y, int64_t ldy, int M, const uint16_t* bias, void* ws,
+                size_t ws_bytes);
+int ming_f8_swiglu(ming_ctx* ctx, const ming_f8* w, const uint8_t* x, int64_t ldx,
+                   const uint16_t* xs, int64_t ldxs, uint8_t* h, int64_t ldh, uint16_t* hs,
+                   int64_t ldhs, int M, void* ws, size_t ws_bytes);
+/* The same over a mixture's groups, with ming_experts_lin's plan (order, fan,
+ * offsets, n of ming_group_rows; order NULL: x in place order): place p of expert
+ * e's group has x row order[p] / fan and e's weights. x [x_rows][ldx], x_rows * ldx
+ * below 2^31; ws by ming_f8_workspace_bytes for n rows. Rows of the outputs (and of
+ * hs) from offsets[n_experts] on are left as they were. */
+int ming_f8_experts_lin(ming_ctx* ctx, const ming_f8* w, const uint8_t* x, int64_t ldx,
+                        const uint16_t* xs, int64_t ldxs, int x_rows, const int32_t* order,
+                        int fan, const int32_t* offsets, int n, uint16_t* y, int64_t ldy,
+                        void* ws, size_t ws_bytes);
+int ming_f8_experts_swiglu(ming_ctx* ctx, const ming_f8* w, const uint8_t* x, int64_t ldx,
+                           const uint16_t* xs, int64_t ldxs, int x_rows, const int32_t* order,
+                           int fan, const int32_t* offsets, int n, uint8_t* h, int64_t ldh,
+                           uint16_t* hs, int64_t ldhs, void* ws, size_t ws_bytes);
+
 /* ---- the pack quantizer (ming-quant-family.cc:31-59's recipe target) -----------
  * Device f32 w [N, K] -> the pack layout ming_qweight_create reads: bits 8
  * symmetric (s = bf16(max|w|/127), code = clamp(rint(w/s), -127, 127) +

@@ -1,0 +1,171 @@
+"""Plain 64-bit forms of the operators in 8-bit floating point (e4m3 codes, a scale
+a block of 128), and the bounds their rounding gives (numpy, on the CPU)."""
+import numpy as np
+
+from rows_ref import BF16, F32, silu
+
+E4M3 = 2.0 ** -4              # half a step of a rounding to e4m3, relative
+LEAST = 2.0 ** -100           # a block's largest magnitude counts as this at least
+NAN = 0x7f
+# the values of the codes 0 .. 0x7e
+_POS = np.array([(c & 7) * 2.0 ** -9 if c < 8 else (1 + (c & 7) / 8.0) * 2.0 ** ((c >> 3) - 7)
+                 for c in range(127)])
+VALUES = np.concatenate([_POS, [np.nan], -_POS, [np.nan]])
+
+
+def blocks(n):
+    return -(-n // 128)
+
+
+def decode(codes):
+    return VALUES[codes]
+
+
+def encode(v):
+    """Codes of 64-bit |v| < 464: the nearest e4m3 value, ties to the even code."""
+    a = np.abs(v)
+    hi = np.clip(np.searchsorted(_POS, a), 1, 126)
+    lo = hi - 1
+    dl, dh = a - _POS[lo], _POS[hi] - a          # exact: neighbours in 53 bits
+    pick = np.where(dl < dh, lo, np.where(dl > dh, hi, np.where(lo % 2 == 0, lo, hi)))
+    return (pick + 128 * np.signbit(v)).astype(np.uint8)
+
+
+def rows_of(x, xs):
+    """What rows of codes [M][K] with scales [blocks][M] (bf16 bits) stand for."""
+    from helpers import f32
+    return decode(x) * np.repeat(f32(xs).astype(np.float64).T, 128, 1)[:, :x.shape[1]]
+
+
+def weights_of(codes, scales):
+    """The same of a weight [N][K] with scales [blocks of N][blocks of K]."""
+    s = np.repeat(np.repeat(scales.astype(np.float64), 128, 0), 128, 1)
+    return decode(codes) * s[:codes.shape[0], :codes.shape[1]]
+
+
+def scale_up(t):
+    """bf16 bits of the least bf16 value of at least t (64-bit, normal, positive)."""
+    m, e = np.frexp(t)
+    s = np.ldexp(np.ceil(m * 256.0) / 256.0, e).astype(np.float32)
+    return (s.view(np.uint32) >> 16).astype(np.uint16)
+
+
+def quantize(v):
+    """(codes [rows][D], scales [blocks][rows] as bf16 bits) of 64-bit rows."""
+    from helpers import f32
+    rows, D = v.shape
+    codes, scales = np.zeros((rows, D), np.uint8), np.zeros((blocks(D), rows), np.uint16)
+    for b in range(blocks(D)):
+        t = v[:, 128 * b:128 * b + 128]
+        scales[b] = scale_up(np.maximum(np.abs(t).max(1), LEAST) / 448.0)
+        codes[:, 128 * b:128 * b + 128] = encode(t / f32(scales[b]).astype(np.float64)[:, None])
+    return codes, scales
+
+
+def quantize_weight(w):
+    """(codes [N][K], scales f32 [blocks of N][blocks of K])."""
+    N, K = w.shape
+    codes, scales = np.zeros((N, K), np.uint8), np.zeros((blocks(N), blocks(K)), np.float32)
+    for i in range(blocks(N)):
+        for j in range(blocks(K)):
+            at = np.s_[128 * i:128 * i + 128, 128 * j:128 * j + 128]
+            top = max(np.abs(w[at]).max(), LEAST)
+            codes[at] = encode(448.0 * w[at].astype(np.float64) / top)
+            scales[i, j] = np.float32(top) / np.float32(448.0)
+    return codes, scales
+
+
+def most8(a):
+    """The largest magnitude of each 8 columns (K is a multiple of 16)."""
+    return np.abs(a).reshape(a.shape[0], -1, 8).max(-1)
+
+
+def products(x, xs, codes, scales, offsets=None, src=None, gated=False, bias=None):
+    """(v, bound): 64-bit results (gated ones before they are quantized) and how far
+    the library's may be. x, xs rows of codes; codes [E][halves N][K], scales [E][halves
+    blocks of N][blocks of K]. Of each 8 products the matrix cores cut those but the
+    largest (no larger than the largest |x| times the largest |w|) below 2^-13 of it; the
+    rest are f32 sums, K + blocks + 8 roundings of the terms' magnitudes, each of a whole
+    step (cut, not rounded)."""
+    E, rows, K = codes.shape
+    halves = 2 if gated else 1
+    N, nb = rows // halves, blocks(rows // halves)
+    if offsets is None:
+        offsets, src = np.array([0, x.shape[0]]), np.arange(x.shape[0])
+    n = int(offsets[-1])
+    X = rows_of(x, xs)
+    v, d = np.zeros((n, N)), np.zeros((n, N))
+    per = (K + blocks(K) + 8) * 2 * F32
+    for e in range(E):
+        r = slice(int(offsets[e]), int(offsets[e + 1]))
+        if r.stop <= r.start:
+            continue
+        xr = X[src[r]]
+        parts = []
+        for h in range(halves):
+            w = weights_of(codes[e, h * N:(h + 1) * N], scales[e, h * nb:(h + 1) * nb])
+            cut = most8(xr) @ most8(w).T * (7 * 2.0 ** -13)
+            parts.append((xr @ w.T, np.abs(xr) @ np.abs(w).T * per + cut))
+        if gated:
+            (g, dg), (u, du) = parts
+            v[r] = silu(g) * u
+            # |silu'| <= 1.1; the two base-2 functions of silu are good to 2 steps
+            d[r] = 1.1 * dg * (np.abs(u) + du) + np.abs(silu(g)) * (du + 8 * F32 * np.abs(u))
+        else:
+            v[r], d[r] = parts[0]
+    if bias is not None:
+        v, d = v + bias, d + F32 * (np.abs(v) + np.abs(bias))
+    return v, d
+
+
+def bf16_bound(v, d):
+    return d * (1 + BF16) + BF16 * np.abs(v) + 1e-30
+
+
+def check_quantized(codes, scales, v, d):
+    """Codes and bf16 scales of values within d of v: each scale the least bf16 of its
+    block's largest over 448, each code within half a step of the value it rounds
+    (2^-10 scales below the smallest normal)."""
+    from helpers import f32
+    n, N = v.shape
+    for b in range(blocks(N)):
+        at = np.s_[:, 128 * b:128 * b + 128]
+        top, off = np.maximum(np.abs(v[at]).max(1), LEAST), d[at].max(1)
+        s = f32(scales[b, :n]).astype(np.float64)
+        lo, hi = (top - off) * (1 - 4 * F32) / 448.0, (top + off) * (1 + 4 * F32) / 448.0
+        # a step of bf16 is at most 2^-7 of its value
+        assert np.all(s >= lo) and np.all(s <= hi * (1 + 2.0 ** -7)), (s / lo, s / hi)
+        got = decode(codes[at])
+        assert np.all(np.abs(got) <= 448.0)
+        err = np.abs(got * s[:, None] - v[at])
+        bound = d[at] + E4M3 * (np.abs(v[at]) + d[at]) * (1 + 8 * F32) \
+            + 2.0 ** -10 * s[:, None] + 8 * F32 * np.abs(v[at]) + 1e-40
+        assert np.all(err <= bound), np.max(err / bound)
+    if v.size > 1000:
+        got = decode(codes) * np.repeat(f32(scales[:, :n]).astype(np.float64).T, 128, 1)[:, :N]
+        # errors spread evenly over half a step have a root mean square of it over sqrt 3
+        assert np.linalg.norm(got - v) <= E4M3 / np.sqrt(3.0) * 1.02 * np.linalg.norm(v)
+
+
+def make_rows(seed, rows, D):
+    """Codes and scales [blocks][rows] as a quantizer leaves activations."""
+    from helpers import bf16, f32, randn
+    return quantize(f32(bf16(randn(seed, (rows, D)))).astype(np.float64))
+
+
+def make_weight(seed, E, N, K, gated=False):
+    """A stack's codes [E][halves N][K] and scales, of blocks of unequal size."""
+    from helpers import randn
+    halves = 2 if gated else 1
+    rng = np.random.default_rng(seed)
+    codes, scales = [], []
+    for e in range(E):
+        c, s = [], []
+        for h in range(halves):
+            w = randn(seed + 10 * e + h, (N, K), 1.0 / np.sqrt(K))
+            one = quantize_weight(w)
+            c.append(one[0])
+            s.append(one[1] * np.exp(rng.normal(0.0, 0.5, one[1].shape)).astype(np.float32))
+        codes.append(np.concatenate(c))
+        scales.append(np.concatenate(s))
+    return np.stack(codes), np.stack(scales)

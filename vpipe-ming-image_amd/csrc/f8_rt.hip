@@ -1,0 +1,427 @@
+// Host side of the 8-bit floating-point operators: the quantizers, the norm, the
+// resident projections and their products.
+#include <algorithm>
+#include <initializer_list>
+#include <new>
+#include <string>
+
+#include "../../include/ming_dit_amd.h"
+#include "kernels.h"
+#include "rt.h"
+
+using ming::rt_fail;
+using ming::rt_ok;
+using ming::Span;
+
+struct ming_f8 {
+  ming_ctx* ctx = nullptr;
+  int E = 0, N = 0, K = 0, halves = 0;
+  int KB = 0, NR = 0, NB = 0;      // blocks of K, resident rows and scales a block of K
+  uint8_t* codes = nullptr;        // [E][KB][NR][128]
+  float* scales = nullptr;         // [E][KB][NB]
+};
+
+namespace {
+
+struct DeviceGuard {
+  int prev = -1;
+  explicit DeviceGuard(int dev) {
+    if (hipGetDevice(&prev) != hipSuccess) prev = -1;
+    if (prev != dev) (void)hipSetDevice(dev);
+  }
+  ~DeviceGuard() {
+    int cur = -1;
+    if (prev >= 0 && hipGetDevice(&cur) == hipSuccess && cur != prev) (void)hipSetDevice(prev);
+  }
+};
+
+hipStream_t stream_of(const ming_ctx* c) { return (hipStream_t)ming_ctx_stream(c); }
+bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
+int hip_fail(hipError_t e, const char* what) {
+  return rt_fail(MING_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
+}
+int blocks_of(int n) { return n / 128 + (n % 128 != 0); }
+Span bf16_rows(const void* p, int64_t rows, int64_t ld, int64_t width) {
+  return {p, rows, 2 * ld, 2 * width};
+}
+Span byte_rows(const void* p, int64_t rows, int64_t ld, int64_t width) { return {p, rows, ld, width}; }
+Span flat(const void* p, int64_t bytes) { return {p, 1, bytes, bytes}; }
+// Whether an output shares memory with another output or with an input.
+bool shared(std::initializer_list<Span> ins, std::initializer_list<Span> outs) {
+  for (const Span* o = outs.begin(); o != outs.end(); ++o) {
+    for (const Span& i : ins)
+      if (ming::spans_meet(i, *o)) return true;
+    for (const Span* q = outs.begin(); q != o; ++q)
+      if (ming::spans_meet(*q, *o)) return true;
+  }
+  return false;
+}
+
+// A stride in elements of b bytes whose rows' last byte 64 bits hold.
+bool stride_fits(int64_t ld) { return ld < (1ll << 30); }
+
+// One launch (or a call's few), timed when the context profiles.
+template <class F>
+int run(ming_ctx* c, ming::RtBucket b, double flops, double bytes, const char* what, F&& launch) {
+  void* ev = nullptr;
+  if (!ming::rt_profile_begin(c, &ev)) return hip_fail(hipErrorOutOfMemory, what);
+  const hipError_t e = launch();
+  const bool timed = ming::rt_profile_end(c, ev, b, flops, bytes);
+  if (e != hipSuccess) return hip_fail(e, what);
+  if (!timed) return hip_fail(hipErrorOutOfMemory, what);
+  return MING_OK;
+}
+
+// Whether the context's kernels can read p where it is: its own device's memory.
+bool own_memory(const ming_ctx* c, const void* p) {
+  hipPointerAttribute_t at{};
+  if (hipPointerGetAttributes(&at, p) != hipSuccess) {
+    (void)hipGetLastError();
+    return false;
+  }
+  return at.type == hipMemoryTypeDevice && at.device == ming::rt_device(c);
+}
+
+// What a product's call brings.
+struct Product {
+  const char* who;
+  bool gated, grouped;
+  const uint8_t* x;
+  int64_t ldx;
+  const uint16_t* xs;
+  int64_t ldxs;
+  int x_rows;
+  const int32_t* order;
+  int fan;
+  const int32_t* offsets;
+  int n;
+  const uint16_t* bias;
+  uint16_t* y;           // plain
+  int64_t ldy;
+  uint8_t* h;            // gated
+  int64_t ldh;
+  uint16_t* hs;
+  int64_t ldhs;
+  void* ws;
+  size_t ws_bytes;
+};
+
+int product(ming_ctx* c, const ming_f8* w, const Product& p) {
+  auto bad = [&](int code, const char* why) {
+    return rt_fail(code, std::string(p.who) + ": " + why);
+  };
+  if (!c || !w) return bad(MING_ERR_ARG, "null argument");
+  if (w->ctx != c) return bad(MING_ERR_ARG, "weights of another context");
+  if (p.n < 0 || p.x_rows < 0 || p.fan < 1) return bad(MING_ERR_ARG, "a count out of range");
+  if ((w->halves == 2) != p.gated)
+    return bad(MING_ERR_ARG, p.gated ? "the weights are not gated" : "the weights are gated");
+  if (!p.grouped && w->E != 1) return bad(MING_ERR_ARG, "the weights are a stack of experts");
+  if (p.n == 0) return rt_ok();
+  if (!p.x || !p.xs || (p.grouped && !p.offsets) || (p.gated ? !p.h || !p.hs : !p.y))
+    return bad(MING_ERR_ARG, "null argument");
+  if (p.n > 1 << 28 || p.x_rows > 1 << 28)
+    return bad(MING_ERR_SHAPE, "at most 2^28 rows");
+  if (p.x_rows == 0) return bad(MING_ERR_ARG, "places without rows of x");
+  if (p.grouped && !p.order && p.x_rows < p.n)
+    return bad(MING_ERR_SHAPE, "without an order x needs n rows");
+  if (p.ldx < w->K || p.ldx % 16 != 0 || p.ldxs < p.x_rows)
+    return bad(MING_ERR_SHAPE, "need ldx >= K, a multiple of 16, and ldxs >= the rows of x");
+  // rows are addressed in 32 bits from the first (of a tile, where they lie in order)
+  if (!stride_fits(p.ldxs) || p.ldx >= 1 << 22 ||
+      (p.grouped && p.ldx > ((1ll << 31) - 1) / p.x_rows))
+    return bad(MING_ERR_SHAPE, "need ldx below 2^22, ldxs below 2^30, and over groups x_rows * ldx "
+                               "below 2^31");
+  if (!aligned(p.x, 16) || !aligned(p.xs, 2) || !aligned(p.order, 4) || !aligned(p.offsets, 4))
+    return bad(MING_ERR_ARG, "x must be 16-byte, its scales 2-byte, order and offsets 4-byte aligned");
+  if (p.gated) {
+    if (p.ldh < w->N || p.ldh % 16 != 0 || p.ldhs < p.n || !stride_fits(p.ldh) || !stride_fits(p.ldhs))
+      return bad(MING_ERR_SHAPE, "need ldh >= N, a multiple of 16, and ldhs >= the rows, below 2^30");
+    if (!aligned(p.h, 16) || !aligned(p.hs, 2))
+      return bad(MING_ERR_ARG, "h must be 16-byte, its scales 2-byte aligned");
+  } else {
+    if (p.ldy < w->N || p.ldy % 8 != 0 || !stride_fits(p.ldy))
+      return bad(MING_ERR_SHAPE, "need ldy >= N, a multiple of 8, below 2^30");
+    if (!aligned(p.y, 16) || !aligned(p.bias, 8))
+      return bad(MING_ERR_ARG, "y must be 16-byte, bias 8-byte aligned");
+  }
+  DeviceGuard g(ming::rt_device(c));       // (the plan counts its CUs)
+  const size_t need = ming_f8_workspace_bytes(w, p.n);
+  if (need > 0 && (!p.ws || !aligned(p.ws, 16)))
+    return bad(MING_ERR_ARG, "ws must be given, 16-byte aligned");
+  if (p.ws_bytes < need)
+    return rt_fail(MING_ERR_SHAPE, std::string(p.who) + ": the call needs " + std::to_string(need) +
+                                       " bytes of workspace, " + std::to_string(p.ws_bytes) +
+                                       " given");
+  if (!ming::one_launch(ming::f8_rows_blocks(16, 16, p.grouped, p.n, w->E, w->N), 512) ||
+      !ming::one_launch(ming::f8_finish_blocks(p.n, w->N), 256))
+    return bad(MING_ERR_SHAPE, "more rows times columns than one launch holds");
+  const Span out = p.gated ? byte_rows(p.h, p.n, p.ldh, w->N) : bf16_rows(p.y, p.n, p.ldy, w->N);
+  const Span outs = bf16_rows(p.hs, p.gated ? blocks_of(w->N) : 0, p.ldhs, p.n);
+  if (shared({byte_rows(p.x, p.x_rows, p.ldx, w->K), bf16_rows(p.xs, w->KB, p.ldxs, p.x_rows),
+              flat(p.order, p.order ? 4ll * p.n : 0), flat(p.offsets, p.offsets ? 4ll * (w->E + 1) : 0),
+              flat(p.bias, p.bias ? 2ll * w->N : 0)},
+             {out, outs, flat(p.ws, (int64_t)need)}))
+    return bad(MING_ERR_ARG, "inputs, outputs and ws must not share memory");
+  ming::F8Args a{};
+  a.x = p.x; a.ldx = p.ldx; a.xs = p.xs; a.ldxs = p.ldxs;
+  a.w = w->codes; a.ws = w->scales;
+  a.w_expert = (long long)w->KB * w->NR * 128;
+  a.s_expert = (long long)w->KB * w->NB;
+  a.N = w->N; a.K = w->K; a.KB = w->KB; a.NR = w->NR; a.NB = w->NB;
+  a.n = p.n;
+  a.offsets = p.offsets; a.order = p.order;
+  a.E = w->E; a.fan = p.fan; a.x_rows = p.x_rows;
+  a.bias = p.bias; a.y = p.y; a.ldy = p.ldy;
+  a.h = p.h; a.ldh = p.ldh; a.hs = p.hs; a.ldhs = p.ldhs;
+  a.part = static_cast<float*>(p.ws);
+  const double wide = (double)w->N * w->halves, flops = 2.0 * p.n * wide * w->K;
+  const double bytes = wide * w->K * std::min(p.n, w->E) + (double)p.x_rows * w->K +
+                       (p.gated ? 1.0 : 2.0) * p.n * w->N;
+  const int rc = run(c, p.gated ? ming::kRtF8Swiglu : ming::kRtF8Lin, flops, bytes, p.who, [&] {
+    return ming::launch_f8_rows(p.gated, p.grouped, a, stream_of(c));
+  });
+  if (rc != MING_OK) return rc;
+  ming::rt_note_rows(c, 8, 2ull * (uint64_t)p.n * (uint64_t)w->N * w->halves * (uint64_t)w->K);
+  return rt_ok();
+}
+
+// Source memory that a creation has on the device at a time where it has to bring
+// it there.
+constexpr size_t kStageBytes = 64u << 20;
+
+}  // namespace
+
+extern "C" {
+
+int ming_f8_quantize(ming_ctx* c, const uint16_t* x, int64_t ldx, int rows, int D, uint8_t* codes,
+                     int64_t ldc, uint16_t* scales, int64_t lds) {
+  auto bad = [](int code, const char* why) {
+    return rt_fail(code, std::string("ming_f8_quantize: ") + why);
+  };
+  if (!c || (rows > 0 && (!x || !codes || !scales))) return bad(MING_ERR_ARG, "null argument");
+  if (rows < 0) return bad(MING_ERR_ARG, "rows < 0");
+  if (D <= 0 || D % 16 != 0) return bad(MING_ERR_SHAPE, "need D % 16 == 0");
+  if (rows == 0) return rt_ok();
+  if (ldx < D || ldx % 8 != 0 || ldc < D || ldc % 16 != 0 || lds < rows || !stride_fits(ldx) ||
+      !stride_fits(ldc) || !stride_fits(lds))
+    return bad(MING_ERR_SHAPE, "need ldx >= D, a multiple of 8, ldc >= D, a multiple of 16, and "
+                               "lds >= rows, below 2^30");
+  if (!aligned(x, 16) || !aligned(codes, 16) || !aligned(scales, 2))
+    return bad(MING_ERR_ARG, "x and codes must be 16-byte, scales 2-byte aligned");
+  if (!ming::one_launch(ming::f8_quantize_blocks(rows, D), 256))
+    return bad(MING_ERR_SHAPE, "more rows than one launch holds");
+  if (shared({bf16_rows(x, rows, ldx, D)},
+             {byte_rows(codes, rows, ldc, D), bf16_rows(scales, blocks_of(D), lds, rows)}))
+    return bad(MING_ERR_ARG, "x, codes and scales must not share memory");
+  DeviceGuard g(ming::rt_device(c));
+  const ming::F8QuantArgs a = {x, ldx, rows, D, codes, ldc, scales, lds};
+  const int rc = run(c, ming::kRtF8Quant, 0.0, 3.0 * rows * D, "ming_f8_quantize",
+                     [&] { return ming::launch_f8_quantize(a, stream_of(c)); });
+  if (rc != MING_OK) return rc;
+  ming::rt_note_rows(c, 0, 0);
+  return rt_ok();
+}
+
+int ming_f8_rmsnorm(ming_ctx* c, const uint16_t* x, int64_t ldx, const uint16_t* sub, int64_t ldsub,
+                    uint16_t* h, int64_t ldh, const uint16_t* w, uint16_t* y, int64_t ldy,
+                    uint8_t* codes, int64_t ldc, uint16_t* scales, int64_t lds, int rows, int D,
+                    float eps) {
+  auto bad = [](int code, const char* why) {
+    return rt_fail(code, std::string("ming_f8_rmsnorm: ") + why);
+  };
+  if (!c || (rows > 0 && (!x || !w || !codes || !scales))) return bad(MING_ERR_ARG, "null argument");
+  if (rows < 0) return bad(MING_ERR_ARG, "rows < 0");
+  if ((sub != nullptr) != (h != nullptr))
+    return bad(MING_ERR_ARG, "sub and h are given together");
+  if (D <= 0 || D % 16 != 0 || D > 8192) return bad(MING_ERR_SHAPE, "need D % 16 == 0 and D <= 8192");
+  if (!(eps >= 1e-12f) || !(eps <= 1.0f)) return bad(MING_ERR_ARG, "eps must be 1e-12 to 1");
+  if (rows == 0) return rt_ok();
+  auto odd = [&](int64_t ld, int of) { return ld < D || ld % of != 0 || !stride_fits(ld); };
+  if (odd(ldx, 8) || (sub && (odd(ldsub, 8) || odd(ldh, 8))) || (y && odd(ldy, 8)) || odd(ldc, 16) ||
+      lds < rows || !stride_fits(lds))
+    return bad(MING_ERR_SHAPE, "strides must be D at least, multiples of 8 (of codes 16), lds >= "
+                               "rows, below 2^30");
+  if (!aligned(x, 16) || !aligned(sub, 16) || !aligned(h, 16) || !aligned(w, 16) || !aligned(y, 16) ||
+      !aligned(codes, 16) || !aligned(scales, 2))
+    return bad(MING_ERR_ARG, "pointers must be 16-byte, scales 2-byte aligned");
+  if (!ming::one_launch(rows, 512)) return bad(MING_ERR_SHAPE, "more rows than one launch holds");
+  const Span xs = bf16_rows(x, rows, ldx, D), ss = bf16_rows(sub, rows, ldsub, D);
+  const Span hs = bf16_rows(h, rows, ldh, D), ws = bf16_rows(w, 1, D, D);
+  const Span ys = bf16_rows(y, rows, ldy, D), cs = byte_rows(codes, rows, ldc, D);
+  const Span sc = bf16_rows(scales, blocks_of(D), lds, rows);
+  // h may be x itself or sub itself: a thread reads both where it then writes
+  const bool over_x = h == x && ldh == ldx, over_sub = h == sub && ldh == ldsub;
+  if (shared({xs, ss, ws}, {ys, cs, sc}) || shared({ws}, {hs, ys, cs, sc}) ||
+      (!over_x && ming::spans_meet(xs, hs)) || (!over_sub && ming::spans_meet(ss, hs)))
+    return bad(MING_ERR_ARG, "inputs and outputs must not share memory (but h may be x or sub)");
+  DeviceGuard g(ming::rt_device(c));
+  const ming::F8NormArgs a = {x, ldx, sub, ldsub, h,   ldh,    w,   y,    ldy, codes,
+                              ldc, scales, lds, rows, D, eps};
+  const int rc = run(c, ming::kRtF8Norm, 0.0, (3.0 + (sub ? 4.0 : 0.0) + (y ? 2.0 : 0.0)) * rows * D,
+                     "ming_f8_rmsnorm", [&] { return ming::launch_f8_norm(a, stream_of(c)); });
+  if (rc != MING_OK) return rc;
+  ming::rt_note_norm(c);
+  return rt_ok();
+}
+
+int ming_f8_quantize_weight(ming_ctx* c, const uint16_t* w, int N, int K, uint8_t* codes,
+                            float* scales) {
+  auto bad = [](int code, const char* why) {
+    return rt_fail(code, std::string("ming_f8_quantize_weight: ") + why);
+  };
+  if (!c || !w || !codes || !scales) return bad(MING_ERR_ARG, "null argument");
+  if (N <= 0 || K <= 0 || K % 16 != 0) return bad(MING_ERR_SHAPE, "need K % 16 == 0");
+  if (blocks_of(N) > 65535) return bad(MING_ERR_SHAPE, "N must be at most 65535 * 128");
+  if (!aligned(w, 16) || !aligned(codes, 16) || !aligned(scales, 4))
+    return bad(MING_ERR_ARG, "w and codes must be 16-byte, scales 4-byte aligned");
+  if (shared({bf16_rows(w, N, K, K)},
+             {byte_rows(codes, N, K, K), flat(scales, 4ll * blocks_of(N) * blocks_of(K))}))
+    return bad(MING_ERR_ARG, "w, codes and scales must not share memory");
+  DeviceGuard g(ming::rt_device(c));
+  const int rc = run(c, ming::kRtF8Quant, 0.0, 3.0 * N * K, "ming_f8_quantize_weight",
+                     [&] { return ming::launch_f8_weight(w, N, K, codes, scales, stream_of(c)); });
+  if (rc != MING_OK) return rc;
+  ming::rt_note_rows(c, 0, 0);
+  return rt_ok();
+}
+
+int ming_f8_destroy(ming_f8* w) {
+  if (!w) return rt_ok();
+  DeviceGuard g(ming::rt_device(w->ctx));
+  (void)hipStreamSynchronize(stream_of(w->ctx));
+  if (w->codes) (void)hipFree(w->codes);
+  if (w->scales) (void)hipFree(w->scales);
+  ming::rt_release(w->ctx);
+  delete w;
+  return rt_ok();
+}
+
+int ming_f8_create(ming_ctx* c, int n_experts, int N, int K, int gated, const uint8_t* codes,
+                   const float* scales, int src_on_device, ming_f8** out) {
+  auto bad = [](int code, const char* why) {
+    return rt_fail(code, std::string("ming_f8_create: ") + why);
+  };
+  if (out) *out = nullptr;
+  if (!c || !out || !codes || !scales) return bad(MING_ERR_ARG, "null argument");
+  if (n_experts < 1 || n_experts > ming::kGroupMax) return bad(MING_ERR_SHAPE, "1 to 1024 experts");
+  if (N <= 0 || K <= 0 || K % 16 != 0 || N % (gated ? 16 : 8) != 0)
+    return bad(MING_ERR_SHAPE, "need K % 16 == 0 and N % 8 == 0, gated N % 16 == 0");
+  const int halves = gated ? 2 : 1, nb = blocks_of(N), KB = blocks_of(K);
+  if ((uint64_t)halves * nb * KB >= (1ull << 31) / (128 * 128))
+    return bad(MING_ERR_SHAPE, "an expert's weights, padded to 128 rows and columns, must be below "
+                               "2 GiB");
+  DeviceGuard g(ming::rt_device(c));
+  auto* w = new (std::nothrow) ming_f8();
+  if (!w) return bad(MING_ERR_ALLOC, "out of memory");
+  w->ctx = c; w->E = n_experts; w->N = N; w->K = K; w->halves = halves;
+  w->KB = KB; w->NR = halves * nb * 128; w->NB = halves * nb;
+  ming::rt_retain(c);
+  const size_t E = (size_t)n_experts, one = (size_t)halves * N * K, ones = (size_t)halves * nb * KB;
+  const size_t kept = (size_t)KB * w->NR * 128;
+  hipStream_t s = stream_of(c);
+  // arrays that the repack can read are read where they are
+  const bool direct = src_on_device && aligned(codes, 16) && aligned(scales, 4) &&
+                      own_memory(c, codes) && own_memory(c, scales);
+  const size_t some = direct ? E : std::clamp<size_t>(kStageBytes / (one + 4 * ones), 1, E);
+  const hipMemcpyKind kind = src_on_device ? hipMemcpyDefault : hipMemcpyHostToDevice;
+  uint8_t* dc = nullptr;
+  float* ds = nullptr;
+  hipError_t e = hipMalloc(&w->codes, E * kept);
+  if (e == hipSuccess) e = hipMalloc(&w->scales, E * ones * 4);
+  if (e == hipSuccess && !direct) e = hipMalloc(&dc, some * one);
+  if (e == hipSuccess && !direct) e = hipMalloc(&ds, some * ones * 4);
+  for (size_t i0 = 0; i0 < E && e == hipSuccess; i0 += some) {
+    const size_t n = std::min(some, E - i0);
+    const uint8_t* sc = codes + i0 * one;
+    const float* ss = scales + i0 * ones;
+    if (!direct) {                         // (behind the repack of those before, in order)
+      e = hipMemcpyAsync(dc, sc, n * one, kind, s);
+      if (e == hipSuccess) e = hipMemcpyAsync(ds, ss, n * ones * 4, kind, s);
+      sc = dc;
+      ss = ds;
+    }
+    for (size_t i = 0; i < n && e == hipSuccess; ++i)
+      e = ming::launch_f8_repack(sc + i * one, ss + i * ones, N, K, halves,
+                                 w->codes + (i0 + i) * kept, w->scales + (i0 + i) * ones, s);
+  }
+  if (e == hipSuccess) e = hipStreamSynchronize(s);
+  if (dc) (void)hipFree(dc);
+  if (ds) (void)hipFree(ds);
+  if (e != hipSuccess) {
+    (void)hipGetLastError();
+    ming_f8_destroy(w);
+    return e == hipErrorOutOfMemory ? bad(MING_ERR_ALLOC, "device allocation failed")
+                                    : hip_fail(e, "ming_f8_create");
+  }
+  *out = w;
+  return rt_ok();
+}
+
+int ming_f8_shape(const ming_f8* w, int* n_experts, int* N, int* K, int* gated) {
+  if (!w) return rt_fail(MING_ERR_ARG, "ming_f8_shape: null argument");
+  if (n_experts) *n_experts = w->E;
+  if (N) *N = w->N;
+  if (K) *K = w->K;
+  if (gated) *gated = w->halves == 2;
+  return rt_ok();
+}
+
+size_t ming_f8_workspace_bytes(const ming_f8* w, int rows) {
+  if (!w || rows <= 0 || w->halves != 2) return 0;
+  return (size_t)rows * w->N * 4;
+}
+
+int ming_f8_lin(ming_ctx* c, const ming_f8* w, const uint8_t* x, int64_t ldx, const uint16_t* xs,
+                int64_t ldxs, uint16_t* y, int64_t ldy, int M, const uint16_t* bias, void* ws,
+                size_t ws_bytes) {
+  Product p{};
+  p.who = "ming_f8_lin";
+  p.x = x; p.ldx = ldx; p.xs = xs; p.ldxs = ldxs;
+  p.x_rows = p.n = M; p.fan = 1;
+  p.bias = bias; p.y = y; p.ldy = ldy;
+  p.ws = ws; p.ws_bytes = ws_bytes;
+  return product(c, w, p);
+}
+
+int ming_f8_swiglu(ming_ctx* c, const ming_f8* w, const uint8_t* x, int64_t ldx, const uint16_t* xs,
+                   int64_t ldxs, uint8_t* h, int64_t ldh, uint16_t* hs, int64_t ldhs, int M, void* ws,
+                   size_t ws_bytes) {
+  Product p{};
+  p.who = "ming_f8_swiglu";
+  p.gated = true;
+  p.x = x; p.ldx = ldx; p.xs = xs; p.ldxs = ldxs;
+  p.x_rows = p.n = M; p.fan = 1;
+  p.h = h; p.ldh = ldh; p.hs = hs; p.ldhs = ldhs;
+  p.ws = ws; p.ws_bytes = ws_bytes;
+  return product(c, w, p);
+}
+
+int ming_f8_experts_lin(ming_ctx* c, const ming_f8* w, const uint8_t* x, int64_t ldx, const uint16_t* xs,
+                        int64_t ldxs, int x_rows, const int32_t* order, int fan,
+                        const int32_t* offsets, int n, uint16_t* y, int64_t ldy, void* ws,
+                        size_t ws_bytes) {
+  Product p{};
+  p.who = "ming_f8_experts_lin";
+  p.grouped = true;
+  p.x = x; p.ldx = ldx; p.xs = xs; p.ldxs = ldxs;
+  p.x_rows = x_rows; p.order = order; p.fan = fan; p.offsets = offsets; p.n = n;
+  p.y = y; p.ldy = ldy;
+  p.ws = ws; p.ws_bytes = ws_bytes;
+  return product(c, w, p);
+}
+
+int ming_f8_experts_swiglu(ming_ctx* c, const ming_f8* w, const uint8_t* x, int64_t ldx,
+                           const uint16_t* xs, int64_t ldxs, int x_rows, const int32_t* order, int fan,
+                           const int32_t* offsets, int n, uint8_t* h, int64_t ldh, uint16_t* hs,
+                           int64_t ldhs, void* ws, size_t ws_bytes) {
+  Product p{};
+  p.who = "ming_f8_experts_swiglu";
+  p.gated = p.grouped = true;
+  p.x = x; p.ldx = ldx; p.xs = xs; p.ldxs = ldxs;
+  p.x_rows = x_rows; p.order = order; p.fan = fan; p.offsets = offsets; p.n = n;
+  p.h = h; p.ldh = ldh; p.hs = hs; p.ldhs = ldhs;
+  p.ws = ws; p.ws_bytes = ws_bytes;
+  return product(c, w, p);
+}
+
+}  // extern "C"

@@ -565,6 +565,88 @@ inline long long experts_tiles(int bits, bool gated, int max, int n, int E, int 
 int experts_cut(int E, int N, int K, int bits, int n);
 int experts_cut_on(int cus, int E, int N, int K, int bits, int n);
 
+// ---- 8-bit floating point with a scale a block of 128 (f8_quant.hip) --------------
+// Rows of bf16 into e4m3 codes, and scales [blocks of D][lds >= rows] in bf16.
+// D % 16 == 0; x and codes 16-byte aligned, ldx % 8 == 0, ldc % 16 == 0.
+struct F8QuantArgs {
+  const uint16_t* x;
+  long long ldx;
+  int rows, D;
+  uint8_t* codes;
+  long long ldc;
+  uint16_t* scales;
+  long long lds;
+};
+hipError_t launch_f8_quantize(const F8QuantArgs& a, hipStream_t s);
+long long f8_quantize_blocks(long long rows, int D);
+// h = bf16(x + sub) where sub is given (h may be x), else x; the codes and scales of
+// v = h * rsqrt(mean(h^2) + eps) * w, and bf16(v) where y is given. D <= 8192.
+struct F8NormArgs {
+  const uint16_t* x;
+  long long ldx;
+  const uint16_t* sub;    // optional
+  long long ldsub;
+  uint16_t* h;            // with sub
+  long long ldh;
+  const uint16_t* w;
+  uint16_t* y;            // optional
+  long long ldy;
+  uint8_t* codes;
+  long long ldc;
+  uint16_t* scales;
+  long long lds;
+  int rows, D;
+  float eps;
+};
+hipError_t launch_f8_norm(const F8NormArgs& a, hipStream_t s);
+// w [N][K] bf16 into codes [N][K] and f32 scales [blocks of N][blocks of K].
+hipError_t launch_f8_weight(const uint16_t* w, int N, int K, uint8_t* codes, float* scales,
+                            hipStream_t s);
+hipError_t validate_f8_quant_kernels();
+
+// ---- their products (f8_rows.hip) ------------------------------------------------------
+// Row p of the output is x row p, or of a grouped call x row order[p] / fan (p itself
+// without an order; kept inside [0, x_rows)) times the weights of p's group. w is
+// resident as f8_repack leaves it, an expert after another: [KB][NR][128] bytes, NR
+// rows padded to 128 a half, with scales [KB][NB].
+struct F8Args {
+  const uint8_t* x;
+  long long ldx;
+  const uint16_t* xs;     // [KB][ldxs]
+  long long ldxs;
+  const uint8_t* w;
+  const float* ws;
+  long long w_expert, s_expert;   // bytes and scales an expert
+  int N, K, KB, NR, NB;
+  int n;                  // rows, or places
+  // grouped
+  const int32_t* offsets;
+  const int32_t* order;   // optional
+  int E, fan, x_rows;
+  // plain
+  const uint16_t* bias;   // optional
+  uint16_t* y;
+  long long ldy;
+  // gated: codes and scales out, and [n][N] f32 for the few-row kernel
+  uint8_t* h;
+  long long ldh;
+  uint16_t* hs;           // [blocks of N][ldhs]
+  long long ldhs;
+  float* part;
+};
+hipError_t launch_f8_repack(const uint8_t* codes, const float* scales, int N, int K, int halves,
+                            uint8_t* out, float* souts, hipStream_t s);
+hipError_t launch_f8_rows(bool gated, bool grouped, const F8Args& a, hipStream_t s);
+// Blocks of tiles of tm rows x tn columns: every group ends in at most one partial one.
+inline long long f8_rows_blocks(int tm, int tn, bool grouped, int n, int E, int N) {
+  const long long tiles_m = grouped ? n / tm + (n < E ? n : E) : ((long long)n + tm - 1) / tm;
+  return tiles_m * ((N + tn - 1) / tn);
+}
+inline long long f8_finish_blocks(int n, int N) {
+  return ((long long)n * ((N + 127) / 128) + 7) / 8;
+}
+hipError_t validate_f8_rows_kernels();
+
 hipError_t validate_qproj_kernels();
 hipError_t validate_qproj_fast_kernels();
 hipError_t validate_norm_kernels();

@@ -65,12 +65,15 @@ int rt_experts_cut(const ming_ctx* c);
 int* rt_range_word(const ming_ctx* c);
 // Event timing around one launch of a family (ming_ctx_set_profiling): begin
 // before it, end after; false where an event could not be had.
-enum RtBucket { kRtRoute, kRtGroup, kRtExperts, kRtCombine };
+enum RtBucket {
+  kRtRoute, kRtGroup, kRtExperts, kRtCombine, kRtF8Quant, kRtF8Norm, kRtF8Lin, kRtF8Swiglu
+};
 bool rt_profile_begin(ming_ctx* c, void** ev);
 bool rt_profile_end(ming_ctx* c, void* ev, RtBucket b, double flops, double bytes);
 // counts what was dispatched: a grouped product of `bits` weights, or one of the
 // small kernels (bits 0)
 void rt_note_rows(ming_ctx* c, int bits, uint64_t flops);
+void rt_note_norm(ming_ctx* c);
 
 // Fused forms the block driver uses (same bits as the public calls they
 // replace):

@@ -108,7 +108,7 @@ namespace {
 enum Bucket {
   kBQ4, kBQ8, kBDense, kBF4, kBF8, kBCvt, kBXa, kBRms, kBQkRope, kBRopeTab, kBSwiglu, kBResid,
   kBModulate, kBBias, kBLn, kBQuant, kBAttn, kBNormRes, kBGemv, kBP4, kBP8, kBRowXa, kBRoute,
-  kBGroup, kBExperts, kBCombine, kBCount
+  kBGroup, kBExperts, kBCombine, kBF8Quant, kBF8Norm, kBF8Lin, kBF8Swiglu, kBCount
 };
 const char* const kBucketName[kBCount] = {
     "qproj.w4", "qproj.w8", "qproj.dense", "qproj_fast.w4", "qproj_fast.w8",
@@ -116,7 +116,7 @@ const char* const kBucketName[kBCount] = {
     "qk_norm_rope", "rope_table", "swiglu", "residual", "modulate",
     "bias_act", "ln_modulate", "quantize", "attention", "norm_residual", "gemv",
     "qproj_pair.w4", "qproj_pair.w8", "row_adapters", "topk_route", "group_rows", "experts",
-    "experts_combine"};
+    "experts_combine", "f8_quantize", "f8_rmsnorm", "f8_lin", "f8_swiglu"};
 
 hipEvent_t take_event(ming_ctx* c) {
   if (!c->pool.empty()) {
@@ -454,6 +454,8 @@ hipError_t validate_kernels(int device) {
   if (e == hipSuccess) e = ming::validate_experts_kernels();
   if (e == hipSuccess) e = ming::validate_experts_tile_kernels();
   if (e == hipSuccess) e = ming::validate_experts_qtile_kernels();
+  if (e == hipSuccess) e = ming::validate_f8_quant_kernels();
+  if (e == hipSuccess) e = ming::validate_f8_rows_kernels();
   if (known) done[device] = e == hipSuccess;
   return e;
 }
@@ -2266,6 +2268,7 @@ void rt_note_rows(ming_ctx* c, int bits, uint64_t flops) {
   else c->eng.elementwise += 1;
   c->eng.gemm_flops += flops;
 }
+void rt_note_norm(ming_ctx* c) { c->eng.rmsnorm += 1; }
 
 int rt_fail(int code, const std::string& why) { return fail(code, why); }
 int rt_ok() { return ok(); }

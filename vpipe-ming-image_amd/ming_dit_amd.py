@@ -42,7 +42,7 @@ def close_all():
     weights before their contexts. Registered with atexit when the first
     handle opens; safe to call at any time."""
     objs = list(_open)
-    for kind in (Model, Experts, Adapters, QWeight, Pack, Ctx):
+    for kind in (Model, F8, Experts, Adapters, QWeight, Pack, Ctx):
         for o in objs:
             if isinstance(o, kind):
                 try:
@@ -287,6 +287,20 @@ def lib():
         "ming_adapters_rank": ([vp, i32], i32),
         "ming_lin_adapters_workspace_bytes": ([vp, vp, vp, i32], C.c_size_t),
         "ming_lin_adapters": ([vp, vp, vp, vp, i64, vp, i64, i32, vp, vp, vp, C.c_size_t], i32),
+        "ming_f8_quantize": ([vp, vp, i64, i32, i32, vp, i64, vp, i64], i32),
+        "ming_f8_rmsnorm": ([vp, vp, i64, vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, i64, i32,
+                             i32, f32], i32),
+        "ming_f8_quantize_weight": ([vp, vp, i32, i32, vp, vp], i32),
+        "ming_f8_create": ([vp, i32, i32, i32, i32, vp, vp, i32, C.POINTER(vp)], i32),
+        "ming_f8_destroy": ([vp], i32),
+        "ming_f8_shape": ([vp] + [C.POINTER(i32)] * 4, i32),
+        "ming_f8_workspace_bytes": ([vp, i32], C.c_size_t),
+        "ming_f8_lin": ([vp, vp, vp, i64, vp, i64, vp, i64, i32, vp, vp, C.c_size_t], i32),
+        "ming_f8_swiglu": ([vp, vp, vp, i64, vp, i64, vp, i64, vp, i64, i32, vp, C.c_size_t], i32),
+        "ming_f8_experts_lin": ([vp, vp, vp, i64, vp, i64, i32, vp, i32, vp, i32, vp, i64, vp,
+                                 C.c_size_t], i32),
+        "ming_f8_experts_swiglu": ([vp, vp, vp, i64, vp, i64, i32, vp, i32, vp, i32, vp, i64, vp,
+                                    i64, vp, C.c_size_t], i32),
         "ming_schedule_sigmas": ([i32, f32, C.POINTER(f32)], i32),
         "ming_model_denoise": ([vp, C.POINTER(DenoiseArgs), C.POINTER(f32), STEP_FN,
                                 vp], i32),
@@ -573,6 +587,58 @@ class Ctx:
     def lin_adapters_workspace_bytes(self, qw: "QWeight", bank: "Adapters", M: int) -> int:
         return int(lib().ming_lin_adapters_workspace_bytes(self.h, qw.h, bank.h, M))
 
+    def f8_quantize(self, x, rows: int, D: int, codes, scales, ldx=None, ldc=None, lds=None):
+        """bf16 rows into e4m3 codes [rows][D] and bf16 scales [ceil(D / 128)][rows]."""
+        _check(lib().ming_f8_quantize(self.h, _ptr(x), D if ldx is None else ldx, rows, D,
+                                      _ptr(codes), D if ldc is None else ldc, _ptr(scales),
+                                      rows if lds is None else lds))
+
+    def f8_rmsnorm(self, x, w, rows: int, D: int, codes, scales, sub=None, h=None, y=None,
+                   eps: float = 1e-6, ldx=None, ldsub=None, ldh=None, ldy=None, ldc=None,
+                   lds=None):
+        """h = x + sub, then its RMSNorm as e4m3 codes and scales (and bf16 y)."""
+        def at(v):
+            return D if v is None else v
+        _check(lib().ming_f8_rmsnorm(self.h, _ptr(x), at(ldx), _ptr(sub), at(ldsub), _ptr(h),
+                                     at(ldh), _ptr(w), _ptr(y), at(ldy), _ptr(codes), at(ldc),
+                                     _ptr(scales), rows if lds is None else lds, rows, D, eps))
+
+    def f8_quantize_weight(self, w, N: int, K: int, codes, scales):
+        """bf16 w [N][K] into codes [N][K] and scales [ceil(N / 128)][ceil(K / 128)]."""
+        _check(lib().ming_f8_quantize_weight(self.h, _ptr(w), N, K, _ptr(codes), _ptr(scales)))
+
+    def f8_lin(self, w: "F8", x, xs, y, M: int, bias=None, ws=None, ldx=None, ldxs=None, ldy=None):
+        """y = x . W^T + bias of e4m3 rows x with scales xs [ceil(K / 128)][M]."""
+        _check(lib().ming_f8_lin(self.h, w.h, _ptr(x), w.K if ldx is None else ldx, _ptr(xs),
+                                 M if ldxs is None else ldxs, _ptr(y),
+                                 w.N if ldy is None else ldy, M, _ptr(bias), _ptr(ws),
+                                 _nbytes(ws)))
+
+    def f8_swiglu(self, w: "F8", x, xs, h, hs, M: int, ws=None, ldx=None, ldxs=None, ldh=None,
+                  ldhs=None):
+        """Codes h and scales hs of silu(gate) * up over gated weights."""
+        _check(lib().ming_f8_swiglu(self.h, w.h, _ptr(x), w.K if ldx is None else ldx, _ptr(xs),
+                                    M if ldxs is None else ldxs, _ptr(h),
+                                    w.N if ldh is None else ldh, _ptr(hs),
+                                    M if ldhs is None else ldhs, M, _ptr(ws), _nbytes(ws)))
+
+    def f8_experts_lin(self, w: "F8", x, xs, x_rows: int, order, offsets, n: int, y, fan: int = 1,
+                       ws=None, ldx=None, ldxs=None, ldy=None):
+        """y[p] = x[order[p] / fan] . W_e^T for the places p of expert e's group."""
+        _check(lib().ming_f8_experts_lin(self.h, w.h, _ptr(x), w.K if ldx is None else ldx,
+                                         _ptr(xs), x_rows if ldxs is None else ldxs, x_rows,
+                                         _ptr(order), fan, _ptr(offsets), n, _ptr(y),
+                                         w.N if ldy is None else ldy, _ptr(ws), _nbytes(ws)))
+
+    def f8_experts_swiglu(self, w: "F8", x, xs, x_rows: int, order, offsets, n: int, h, hs,
+                          fan: int = 1, ws=None, ldx=None, ldxs=None, ldh=None, ldhs=None):
+        """Codes h and scales hs of silu(gate) * up, each place by its expert's weights."""
+        _check(lib().ming_f8_experts_swiglu(self.h, w.h, _ptr(x), w.K if ldx is None else ldx,
+                                            _ptr(xs), x_rows if ldxs is None else ldxs, x_rows,
+                                            _ptr(order), fan, _ptr(offsets), n, _ptr(h),
+                                            w.N if ldh is None else ldh, _ptr(hs),
+                                            n if ldhs is None else ldhs, _ptr(ws), _nbytes(ws)))
+
 
 SCORES = {"softmax": 0, "sigmoid": 1}
 
@@ -693,6 +759,41 @@ class Experts:
     def close(self):
         if self.h:
             lib().ming_experts_destroy(self.h)
+            self.h = None
+
+    def __del__(self, _fin=_finalize):
+        _fin(self)
+
+
+class F8:
+    """A resident e4m3 projection, or a stack of them (ming_f8)."""
+
+    def __init__(self, ctx: Ctx, codes, scales, N: int, gated: bool = False,
+                 on_device: bool = False):
+        """codes [E][N][K] (gated: [E][2 N][K], gate rows first), or without the E, of one
+        byte each; scales f32 [E][ceil(N / 128)][ceil(K / 128)] (gated: each half's)."""
+        shape = [int(v) for v in codes.shape]
+        rows, K = shape[-2:]
+        if _itemsize(codes) != 1 or _itemsize(scales) != 4 or rows != (2 * N if gated else N):
+            raise ValueError("codes of one byte over N (gated 2 N) rows, scales of f32")
+        E = shape[0] if len(shape) == 3 else 1
+        blocks = (2 if gated else 1) * -(-N // 128) * -(-K // 128)
+        if _nbytes(scales) != 4 * E * blocks:
+            raise ValueError("a scale for each block of 128 x 128")
+        h = C.c_void_p()
+        _check(lib().ming_f8_create(ctx.h, E, N, K, int(gated), _ptr(codes), _ptr(scales),
+                                    int(on_device), C.byref(h)))
+        self.ctx, self.h = ctx, h
+        self.n_experts, self.N, self.K, self.gated = E, N, K, gated
+        ctx._weights.add(self)
+        _track(self)
+
+    def workspace_bytes(self, rows: int) -> int:
+        return int(lib().ming_f8_workspace_bytes(self.h, rows))
+
+    def close(self):
+        if self.h:
+            lib().ming_f8_destroy(self.h)
             self.h = None
 
     def __del__(self, _fin=_finalize):
