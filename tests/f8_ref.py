@@ -169,3 +169,14 @@ def make_weight(seed, E, N, K, gated=False):
         codes.append(np.concatenate(c))
         scales.append(np.concatenate(s))
     return np.stack(codes), np.stack(scales)
+
+
+def set_plan(ctx, plan):
+    """The 8-bit products on ctx run this kernel (0 the few-row one, else tiles of 64 * plan
+    rows, 2 or 4 over groups); -1 the plan's."""
+    import ctypes as C
+
+    import ming_dit_amd as m
+    f = m.lib()._ZN4ming14rt_set_f8_planEP8ming_ctxi
+    f.argtypes, f.restype = [C.c_void_p, C.c_int], None
+    f(ctx.h, plan)

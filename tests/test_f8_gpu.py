@@ -329,6 +329,57 @@ def test_experts_in_place_order(ctx, gated, N, K, counts):
     W.w.close()
 
 
+@pytest.fixture()
+def plan(ctx):
+    yield lambda p: ref.set_plan(ctx, p)
+    ref.set_plan(ctx, -1)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("N,K", [(16, 16), (144, 128), (400, 272), (528, 1168), (272, 2576)])
+@pytest.mark.parametrize("M", [1, 63, 64, 65, 128, 200, 257, 513])
+def test_every_kernel(ctx, plan, gated, N, K, M):
+    """Each kernel at and beside every tile height, one block of K to odd and even counts
+    of them, columns and K that end inside a tile; the tiles give the same bits."""
+    W = Weights(ctx, 6000 + N, 1, N, K, gated)
+    x, xs = ref.make_rows(6100 + M, M, K)
+    first = None
+    for p in (0, 1, 2, 3, 4):
+        print(f"case f8 plan {p} gated={gated} N={N} K={K} M={M}", flush=True)
+        plan(p)
+        got = call(ctx, W, x, xs, pad=16 * (p % 2))
+        check(got, W, x, xs)
+        if p == 1:
+            first = got
+        if p > 1:
+            for a, b in zip(first, got):
+                assert np.array_equal(a, b)
+    W.w.close()
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("N,K,counts", [
+    (528, 1088, [1, 64, 65, 0, 127, 128, 129, 63, 2, 200, 130, 100]),
+    (560, 576, [255, 256, 257, 1, 513, 0, 192, 193, 321, 449]),
+    (2064, 64, [300, 700, 15, 0, 1, 900]),
+    (272, 1216, [40, 1000]), (16, 128, [70, 0, 9])])
+def test_every_grouped_kernel(ctx, plan, gated, N, K, counts):
+    E, n = len(counts), sum(counts)
+    W = Weights(ctx, 6200, E, N, K, gated)
+    offsets, order, src = rows_ref.plan_of(counts, n=n + 70, fan=3, seed=N, x_rows=300)
+    x, xs = ref.make_rows(6300, 300, K)
+    # rows in place order: the gathered rows' copies
+    gx, gs = x[src], np.ascontiguousarray(xs[:, src])
+    for p in (0, 2, 4):
+        print(f"case f8 grouped plan {p} gated={gated} N={N} K={K}", flush=True)
+        plan(p)
+        got = call(ctx, W, x, xs, offsets, order, order.size, fan=3, pad=16)
+        check(got, W, x, xs, offsets, src)
+        for a, b in zip(got, call(ctx, W, gx, gs, offsets, None, n)):
+            assert np.array_equal(a, b)
+    W.w.close()
+
+
 @pytest.mark.parametrize("M", [3, 40, 300])
 @pytest.mark.parametrize("gated", [False, True])
 def test_nan_stays_in_its_row(ctx, gated, M):

@@ -1,6 +1,7 @@
 // Host side of the 8-bit floating-point operators: the quantizers, the norm, the
 // resident projections and their products.
 #include <algorithm>
+#include <cmath>
 #include <initializer_list>
 #include <new>
 #include <string>
@@ -20,6 +21,31 @@ struct ming_f8 {
   uint8_t* codes = nullptr;        // [E][KB][NR][128]
   float* scales = nullptr;         // [E][KB][NB]
 };
+
+namespace ming {
+
+int f8_plan(int cus, bool grouped, int E, int NR, int KB, int n) {
+  if (KB > kF8TileBlocks) return 0;
+  if (grouped) {
+    const double live = E * (1.0 - std::exp(-(double)n / E)), rows = n / live;
+    return rows < 32.0 ? 0 : rows < 112.0 ? 2 : 4;
+  }
+  if (n <= 64) return 0;
+  // rounds of the chip, a workgroup a CU, times a tile's time
+  int best = 4;
+  double least = 0.0;
+  for (int rf = 4; rf >= 1; --rf) {
+    const long long tiles = f8_tile_blocks(rf, false, n, 1, NR);
+    const double us = (double)((tiles + cus - 1) / cus) * (24 + 10 * rf);
+    if (rf == 4 || us < least) {
+      best = rf;
+      least = us;
+    }
+  }
+  return best;
+}
+
+}  // namespace ming
 
 namespace {
 
@@ -80,6 +106,17 @@ bool own_memory(const ming_ctx* c, const void* p) {
     return false;
   }
   return at.type == hipMemoryTypeDevice && at.device == ming::rt_device(c);
+}
+
+// The kernel that takes n rows of w on the current device.
+int plan_of(const ming_f8* w, bool grouped, int n) {
+  const int set = ming::rt_f8_plan(w->ctx);
+  if (set >= 0 && w->KB <= ming::kF8TileBlocks) return set;
+  return ming::f8_plan(ming::device_cus(), grouped, w->E, w->NR, w->KB, n);
+}
+// f32 results of the few-row kernel on gated weights, before they are quantized.
+size_t part_bytes(const ming_f8* w, bool grouped, int n) {
+  return w->halves == 2 && plan_of(w, grouped, n) == 0 ? (size_t)n * w->N * 4 : 0;
 }
 
 // What a product's call brings.
@@ -145,15 +182,17 @@ int product(ming_ctx* c, const ming_f8* w, const Product& p) {
       return bad(MING_ERR_ARG, "y must be 16-byte, bias 8-byte aligned");
   }
   DeviceGuard g(ming::rt_device(c));       // (the plan counts its CUs)
-  const size_t need = ming_f8_workspace_bytes(w, p.n);
+  const int plan = plan_of(w, p.grouped, p.n);
+  const size_t need = part_bytes(w, p.grouped, p.n);
   if (need > 0 && (!p.ws || !aligned(p.ws, 16)))
     return bad(MING_ERR_ARG, "ws must be given, 16-byte aligned");
   if (p.ws_bytes < need)
     return rt_fail(MING_ERR_SHAPE, std::string(p.who) + ": the call needs " + std::to_string(need) +
                                        " bytes of workspace, " + std::to_string(p.ws_bytes) +
                                        " given");
-  if (!ming::one_launch(ming::f8_rows_blocks(16, 16, p.grouped, p.n, w->E, w->N), 512) ||
-      !ming::one_launch(ming::f8_finish_blocks(p.n, w->N), 256))
+  if (plan == 0 ? !ming::one_launch(ming::f8_rows_blocks(16, 16, p.grouped, p.n, w->E, w->N), 512) ||
+                      !ming::one_launch(ming::f8_finish_blocks(p.n, w->N), 256)
+                : !ming::one_launch(ming::f8_tile_blocks(plan, p.grouped, p.n, w->E, w->NR), 512))
     return bad(MING_ERR_SHAPE, "more rows times columns than one launch holds");
   const Span out = p.gated ? byte_rows(p.h, p.n, p.ldh, w->N) : bf16_rows(p.y, p.n, p.ldy, w->N);
   const Span outs = bf16_rows(p.hs, p.gated ? blocks_of(w->N) : 0, p.ldhs, p.n);
@@ -178,7 +217,8 @@ int product(ming_ctx* c, const ming_f8* w, const Product& p) {
   const double bytes = wide * w->K * std::min(p.n, w->E) + (double)p.x_rows * w->K +
                        (p.gated ? 1.0 : 2.0) * p.n * w->N;
   const int rc = run(c, p.gated ? ming::kRtF8Swiglu : ming::kRtF8Lin, flops, bytes, p.who, [&] {
-    return ming::launch_f8_rows(p.gated, p.grouped, a, stream_of(c));
+    return plan ? ming::launch_f8_tile(p.gated, p.grouped, a, plan, stream_of(c))
+                : ming::launch_f8_rows(p.gated, p.grouped, a, stream_of(c));
   });
   if (rc != MING_OK) return rc;
   ming::rt_note_rows(c, 8, 2ull * (uint64_t)p.n * (uint64_t)w->N * w->halves * (uint64_t)w->K);
@@ -367,8 +407,9 @@ int ming_f8_shape(const ming_f8* w, int* n_experts, int* N, int* K, int* gated) 
 }
 
 size_t ming_f8_workspace_bytes(const ming_f8* w, int rows) {
-  if (!w || rows <= 0 || w->halves != 2) return 0;
-  return (size_t)rows * w->N * 4;
+  if (!w || rows <= 0) return 0;
+  DeviceGuard g(ming::rt_device(w->ctx));
+  return std::max(part_bytes(w, false, rows), part_bytes(w, true, rows));
 }
 
 int ming_f8_lin(ming_ctx* c, const ming_f8* w, const uint8_t* x, int64_t ldx, const uint16_t* xs,

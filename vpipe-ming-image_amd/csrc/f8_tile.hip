@@ -1,0 +1,433 @@
+// The 8-bit products over many rows, plain or SwiGLU-gated, of one projection or of a
+// mixture's groups: y[m] = sum over blocks b of 128 of xs[b][m] * ws[n / 128][b] *
+// (x . w)_b.
+//
+// MFMA-bound. A workgroup takes 64*RF rows x 256 rows of the resident weights (gated:
+// 128 columns, whose gate and up rows lie side by side in eights of 32), 8 wave64s
+// in 2 x 4, each 32*RF rows x 64 weight rows: 2*RF x 4 tiles of
+// v_mfma_f32_16x16x128_f8f6f4. A stage is a block of 128 of K, so each instruction's
+// result is a whole block's sum: it starts from zero, and four fused multiply-adds take
+// it into the f32 accumulators times both scales, in the shadow of the next ones (16
+// of 32 cycles). A lane's four results are four columns of one row, so a row's scale
+// is one register a row tile, times the weights' one scale.
+//
+// Stages go through an LDS ring filled by direct global->LDS DMA (rows of 128 bytes,
+// chunks swizzled), with the rows' scales; the weights' scales are all taken at the
+// start. One barrier a stage, before its last two row tiles: their operands are in
+// registers by then, so the slot is free for the DMA, and the next stage's first
+// operands are read under their matrix instructions.
+#include <type_traits>
+
+#include "common.h"
+#include "f8.h"
+#include "kernels.h"
+#include "lds_ring.h"
+#include "row_groups.h"
+
+namespace ming {
+namespace {
+
+constexpr int TBN = 256, NW = 8;
+
+// A 16-bit load into LDS, zero-extended to a dword a lane; waits as dma16_sb's.
+__device__ __forceinline__ void dma2_sb(const void* base, uint32_t off, uint32_t lds) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ushort %0, %1"
+               :: "v"(off), "s"(base), "s"(lds) : "m0");
+#pragma clang diagnostic pop
+}
+
+template <int RF>
+struct TileLds {
+  static constexpr int kStages = RF >= 3 ? 2 : 3;
+  static constexpr int kX = 64 * RF * 8, kW = TBN * 8, kS = 16 * RF;   // 16-byte units
+  static constexpr int kStage = kX + kW + kS;
+  static constexpr int kUnits = kStages * kStage + kF8TileBlocks / 2;
+};
+
+// One tile: rows p0 .. p0 + rows - 1, resident weight rows from 256 * tn of expert e.
+template <int RF, bool GATED, bool GROUPED>
+__device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int e, int p0, int rows,
+                                        int tn) {
+  using L = TileLds<RF>;
+  constexpr int NST = L::kStages, MF = 2 * RF, NF = 4;
+  constexpr int XD = RF, WD = 4;           // DMAs a wave and stage, and one of scales
+  float2* const wsc = reinterpret_cast<float2*>(ring + NST * L::kStage);
+
+  const int tid = (int)threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave & 1, wn = wave >> 1;
+  const int KB = a.KB;
+
+  auto source = [&](int r) {               // x's row of tile row r
+    int src = p0 + (r < rows ? r : rows - 1);
+    if constexpr (GROUPED) {
+      if (a.order) src = a.order[src] / a.fan;
+      src = src < 0 ? 0 : src < a.x_rows ? src : a.x_rows - 1;
+      return src;
+    }
+    return src - p0;
+  };
+  const uint8_t* const xbase = GROUPED ? a.x : a.x + (long long)p0 * a.ldx;
+  const uint16_t* const sbase = GROUPED ? a.xs : a.xs + p0;
+  const uint8_t* const wbase =
+      a.w + e * a.w_expert + (long long)tn * (TBN * 128);
+  // LDS chunk p of a tile holds row p >> 3, logical chunk (p & 7) ^ swizzle
+  auto chunk_of = [&](int p) { return (p & 7) ^ ((p >> 4) & 7); };
+  uint32_t xrow[XD], woff[WD];
+#pragma unroll
+  for (int i = 0; i < XD; ++i)
+    xrow[i] = (uint32_t)((long long)source((64 * (XD * wave + i) + lane) >> 3) * a.ldx);
+#pragma unroll
+  for (int i = 0; i < WD; ++i) {
+    const int p = 64 * (WD * wave + i) + lane;
+    int r = p >> 3;
+    // a tile that ends the weights after 128 rows takes those twice
+    if (!GATED && TBN * tn + r >= a.NR) r -= 128;
+    woff[i] = (uint32_t)(r * 128 + 16 * chunk_of(p));
+  }
+  // scales of 64 rows a wave; more waves than that write some twice, the same values (a
+  // branch here would split the stage, and the sums would be sunk past it)
+  const int srow = 64 * (wave % RF);
+  const uint32_t soff = 2u * (uint32_t)source(srow + lane);
+  const int klast = (a.K - 128 * (KB - 1)) / 16;       // the last block's chunks
+
+  // stage t's DMAs; past the last one it is read again into a slot nothing reads, so
+  // that every stage issues and waits alike
+  auto issue_w = [&](int t, const uint4* S) {
+    const uint8_t* base = wbase + (long long)(t < KB ? t : KB - 1) * a.NR * 128;
+#pragma unroll
+    for (int i = 0; i < WD; ++i)
+      dma16_sb(base, woff[i], lds_addr(S + L::kX + 64 * (WD * wave + i)));
+  };
+  auto issue_x = [&](int t, const uint4* S) {
+    const int kb = t < KB ? t : KB - 1;
+    const uint8_t* base = xbase + (long long)kb * 128;
+    // past K the weights are zeros: any chunk of x's own block will do
+    const int cut = kb == KB - 1 ? klast : 8;
+#pragma unroll
+    for (int i = 0; i < XD; ++i) {
+      const int ch = chunk_of(64 * (XD * wave + i) + lane);
+      dma16_sb(base, xrow[i] + (ch < cut ? 16 * ch : 0), lds_addr(S + 64 * (XD * wave + i)));
+    }
+    dma2_sb(sbase + (long long)kb * a.ldxs, soff, lds_addr(S + L::kX + L::kW) + 4 * srow);
+  };
+
+  // the weights' scales of all blocks: the tile's two blocks of rows, or gate and up
+  {
+    const int b0 = 2 * tn, b1 = 2 * tn + 1 < a.NB ? 2 * tn + 1 : 2 * tn;
+    const float* ws = a.ws + e * a.s_expert;
+    for (int k = tid; k < KB; k += 64 * NW)
+      wsc[k] = make_float2(ws[(long long)k * a.NB + b0], ws[(long long)k * a.NB + b1]);
+  }
+
+  floatx4_t acc[NF][MF];
+#pragma unroll
+  for (int j = 0; j < NF; ++j)
+#pragma unroll
+    for (int i = 0; i < MF; ++i) acc[j][i] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
+
+  // fragments: rows 16 apart keep their swizzle
+  const int fx = (32 * RF * wm + c) * 8 + (g ^ (c >> 1)), fw = (64 * wn + c) * 8 + (g ^ (c >> 1));
+  auto read_x = [&](const uint4* S, int i) {
+    return F8Frag{S[fx + 128 * i], S[(fx ^ 4) + 128 * i]};
+  };
+  auto read_w = [&](const uint4* S, int j) {
+    return F8Frag{S[L::kX + fw + 128 * j], S[L::kX + (fw ^ 4) + 128 * j]};
+  };
+  auto read_s = [&](const uint4* S, int i) {
+    return reinterpret_cast<const uint32_t*>(S + L::kX + L::kW)[32 * RF * wm + 16 * i + c];
+  };
+
+  F8Frag w[NF], x[2];
+  uint32_t sx[MF];
+  auto body = [&](auto ph, int t) {
+    constexpr int PH = decltype(ph)::value;
+    const uint4 *const S = ring + PH * L::kStage, *const Sn = ring + (PH + 1) % NST * L::kStage;
+    const float2 sw = wsc[t];
+    const float s0 = GATED ? sw.x : wn < 2 ? sw.x : sw.y;
+    float s[MF], u[MF];
+#pragma unroll
+    for (int i = 0; i < MF; ++i) {
+      const float v = __uint_as_float(sx[i] << 16);
+      s[i] = v * s0;
+      u[i] = GATED ? v * sw.y : 0.0f;
+    }
+    auto add = [&](int j, int i, const floatx4_t& d) {
+      const float f = GATED && j >= 2 ? u[i] : s[i];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[j][i][r] = fmaf(d[r], f, acc[j][i][r]);
+    };
+    F8Frag xa = x[0], xb = x[1];
+    floatx4_t dp[NF];
+#pragma unroll
+    for (int i = 0; i < MF - 2; ++i) {
+      const F8Frag xn = read_x(S, i + 2);
+      floatx4_t d[NF];
+#pragma unroll
+      for (int j = 0; j < NF; ++j) {
+        d[j] = f8_mfma(w[j], xa);
+        if (i > 0) add(j, i - 1, dp[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < NF; ++j) dp[j] = d[j];
+      xa = xb;
+      xb = xn;
+      // a step's matrix instructions, each with a result of the step before
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);     // DS read
+#pragma unroll
+      for (int j = 0; j < NF; ++j) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // MFMA
+        if (i > 0) __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);   // VALU
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    ring_wait<(NST - 2) * (XD + WD + 1)>();
+    __builtin_amdgcn_sched_barrier(0);
+    issue_x(t + NST, S);
+    issue_w(t + NST, S);
+    x[0] = read_x(Sn, 0);
+    floatx4_t e0, e1;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < NF; ++j) {
+      const floatx4_t d0 = f8_mfma(w[j], xa), d1 = f8_mfma(w[j], xb);
+      if (MF > 2) add(j, MF > 2 ? MF - 3 : 0, dp[j]);
+      w[j] = read_w(Sn, j);
+      if (j > 0) {
+        add(j - 1, MF - 2, e0);
+        add(j - 1, MF - 1, e1);
+      }
+      e0 = d0;
+      e1 = d1;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    add(NF - 1, MF - 2, e0);
+    add(NF - 1, MF - 1, e1);
+    x[1] = read_x(Sn, 1);
+#pragma unroll
+    for (int i = 0; i < MF; ++i) sx[i] = read_s(Sn, i);
+  };
+
+#pragma unroll
+  for (int t = 0; t < NST; ++t) {
+    issue_x(t, ring + t * L::kStage);
+    issue_w(t, ring + t * L::kStage);
+  }
+  // stage 0 landed, the weights' scales written (their stores are waited for with the
+  // LDS counter)
+  ring_wait<(NST - 1) * (XD + WD + 1)>();
+#pragma unroll
+  for (int j = 0; j < NF; ++j) w[j] = read_w(ring, j);
+  x[0] = read_x(ring, 0);
+  x[1] = read_x(ring, 1);
+#pragma unroll
+  for (int i = 0; i < MF; ++i) sx[i] = read_s(ring, i);
+  const std::integral_constant<int, 0> p0c{};
+  const std::integral_constant<int, 1> p1c{};
+  int t = 0;
+  if constexpr (NST == 2) {
+    for (; t + 2 <= KB; t += 2) {
+      body(p0c, t);
+      body(p1c, t + 1);
+    }
+    if (t < KB) body(p0c, t);
+  } else {
+    const std::integral_constant<int, 2> p2c{};
+    for (; t + 3 <= KB; t += 3) {
+      body(p0c, t);
+      body(p1c, t + 1);
+      body(p2c, t + 2);
+    }
+    if (KB - t >= 1) body(p0c, t);
+    if (KB - t >= 2) body(p1c, t + 1);
+  }
+  ring_wait<0>();                          // drained; LDS free
+
+  if constexpr (GATED) {
+    // v = silu(gate) * up: fragments 0, 1 are the wave's 32 gate columns, 2, 3 the up
+    // ones. A row's largest over the tile's 128 columns is a block's: over a lane's
+    // columns, the four lane quarters, and the four waves side by side, by LDS.
+    uint32_t* const tops = reinterpret_cast<uint32_t*>(ring);            // [4][64 RF]
+    uint4* const E = ring + RF * 64;                                      // [64 RF][8]
+#pragma unroll
+    for (int i = 0; i < MF; ++i) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float v = silu_f(acc[j][i][r]) * acc[j + 2][i][r];
+          acc[j][i][r] = v;
+          top = f8_top(top, v);
+        }
+#pragma unroll
+      for (int o = 16; o < 64; o <<= 1) {
+        const uint32_t v = (uint32_t)__shfl_xor((int)top, o, 64);
+        top = top > v ? top : v;
+      }
+      if (g == 0) tops[64 * RF * wn + 32 * RF * wm + 16 * i + c] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MF; ++i) {
+      const int row = 32 * RF * wm + 16 * i + c;
+      uint32_t top = tops[row];
+#pragma unroll
+      for (int k = 1; k < 4; ++k) {
+        const uint32_t v = tops[64 * RF * k + row];
+        top = top > v ? top : v;
+      }
+      const float tf = __uint_as_float(top);
+      const bool fine = f8_finite(tf);
+      const uint32_t sb = fine ? f8_scale_bits(tf) : kF8NanScale;
+      const float q = 1.0f / __uint_as_float(sb << 16);
+      if (wn == 0 && g == 0 && row < rows) a.hs[(long long)tn * a.ldhs + p0 + row] = (uint16_t)sb;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const floatx4_t& v = acc[j][i];
+        // chunk of 16 columns 2 wn + j, a lane quarter's dword
+        reinterpret_cast<uint32_t*>(E)[(row * 8 + ((2 * wn + j) ^ ((row >> 1) & 7))) * 4 + g] =
+            fine ? f8_pack4(v[0] * q, v[1] * q, v[2] * q, v[3] * q) : kF8Nan4;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < RF; ++k) {
+      const int p = 512 * k + tid, row = p >> 3, ch = p & 7, n = 128 * tn + 16 * ch;
+      if (row < rows && n < a.N)
+        *reinterpret_cast<uint4*>(a.h + (long long)(p0 + row) * a.ldh + n) =
+            E[row * 8 + (ch ^ ((row >> 1) & 7))];
+    }
+  } else {
+    // each wave turns its 64 columns through its own part of LDS, then stores whole
+    // 128-byte row pieces
+    uint4* const E = ring + 32 * RF * 8 * wave;
+    uint2* const E2 = reinterpret_cast<uint2*>(E);
+    const int nb = TBN * tn + 64 * wn;
+#pragma unroll
+    for (int j = 0; j < NF; ++j) {
+      float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      const int n = nb + 16 * j + 4 * g;
+      if (!GROUPED && a.bias && n < a.N) {
+        const uint2 v = *reinterpret_cast<const uint2*>(a.bias + n);
+        b[0] = bf16_lo(v.x);
+        b[1] = bf16_hi(v.x);
+        b[2] = bf16_lo(v.y);
+        b[3] = bf16_hi(v.y);
+      }
+#pragma unroll
+      for (int i = 0; i < MF; ++i) {
+        const int row = 16 * i + c;
+        const floatx4_t& v = acc[j][i];
+        E2[(row * 8 + ((2 * j + (g >> 1)) ^ ((row >> 1) & 7))) * 2 + (g & 1)] = make_uint2(
+            pack_bf16x2_rne(v[0] + b[0], v[1] + b[1]), pack_bf16x2_rne(v[2] + b[2], v[3] + b[3]));
+      }
+    }
+    const int cl = lane & 7, n = nb + 8 * cl;
+#pragma unroll
+    for (int k = 0; k < 4 * RF; ++k) {
+      const int ml = 8 * k + (lane >> 3), row = 32 * RF * wm + ml;
+      const uint4 v = E[ml * 8 + (cl ^ ((ml >> 1) & 7))];
+      if (row < rows && n < a.N)
+        *reinterpret_cast<uint4*>(a.y + (long long)(p0 + row) * a.ldy + n) = v;
+    }
+  }
+}
+
+template <int RF, bool GATED>
+__global__ __launch_bounds__(64 * NW, 1) void f8_tile_kernel(const F8Args a) {
+  __shared__ uint4 ring[TileLds<RF>::kUnits];
+  constexpr int BM = 64 * RF;
+  const int tiles_m = (a.n + BM - 1) / BM;
+  int tm, tn;
+  tile_of_block((int)blockIdx.x, tiles_m, (a.NR + TBN - 1) / TBN, &tm, &tn);
+  const int p0 = BM * tm, left = a.n - p0;
+  f8_tile<RF, GATED, false>(a, ring, 0, p0, left < BM ? left : BM, tn);
+}
+
+// Groups of more than 64 * MAX places are cut into the fewest tiles that hold them.
+template <int MAX, bool GATED>
+__global__ __launch_bounds__(64 * NW, 1) void f8_group_tile_kernel(const F8Args a) {
+  constexpr int CUT = 64 * MAX;
+  constexpr int kUnits = TileLds<MAX>::kUnits > TileLds<2>::kUnits ? TileLds<MAX>::kUnits
+                                                                     : TileLds<2>::kUnits;
+  __shared__ uint4 ring[kUnits];
+  const int tiles_n = (a.NR + TBN - 1) / TBN;
+  const RowGroup rg = find_group(
+      a.offsets, a.E, a.n, [&](int rows) { return (rows + CUT - 1) / CUT * tiles_n; },
+      [&](int total) {
+        const int b = (int)blockIdx.x, q = total / 8, rem = total % 8, xcd = b % 8;
+        return b < total ? xcd * q + (xcd < rem ? xcd : rem) + b / 8 : -1;
+      });
+  if (rg.e < 0) return;
+  const int tiles_m = (rg.rows + CUT - 1) / CUT;
+  const int tn = rg.index / tiles_m, tm = rg.index - tn * tiles_m;
+  const RowTile rt = row_tile<64>(rg.rows, tiles_m, tm);
+  const int p0 = rg.p0 + rt.first, rows = rt.rows;
+  if constexpr (MAX >= 4) {
+    if (rows > 192) return f8_tile<4, GATED, true>(a, ring, rg.e, p0, rows, tn);
+    if (rows > 128) return f8_tile<3, GATED, true>(a, ring, rg.e, p0, rows, tn);
+  }
+  if (rows > 64)
+    f8_tile<2, GATED, true>(a, ring, rg.e, p0, rows, tn);
+  else
+    f8_tile<1, GATED, true>(a, ring, rg.e, p0, rows, tn);
+}
+
+template <int RF>
+void tile_launch(bool gated, const F8Args& a, hipStream_t s) {
+  const dim3 grid((unsigned)f8_tile_blocks(RF, false, a.n, a.E, a.NR));
+  if (gated)
+    hipLaunchKernelGGL((f8_tile_kernel<RF, true>), grid, dim3(64 * NW), 0, s, a);
+  else
+    hipLaunchKernelGGL((f8_tile_kernel<RF, false>), grid, dim3(64 * NW), 0, s, a);
+}
+template <int MAX>
+void group_launch(bool gated, const F8Args& a, hipStream_t s) {
+  const dim3 grid((unsigned)f8_tile_blocks(MAX, true, a.n, a.E, a.NR));
+  if (gated)
+    hipLaunchKernelGGL((f8_group_tile_kernel<MAX, true>), grid, dim3(64 * NW), 0, s, a);
+  else
+    hipLaunchKernelGGL((f8_group_tile_kernel<MAX, false>), grid, dim3(64 * NW), 0, s, a);
+}
+
+}  // namespace
+
+hipError_t launch_f8_tile(bool gated, bool grouped, const F8Args& a, int rf, hipStream_t s) {
+  if (a.n <= 0) return hipSuccess;
+  if (a.N <= 0 || a.N % (gated ? 16 : 8) || a.K % 16 || a.KB > kF8TileBlocks || a.E < 1 || a.fan < 1)
+    return hipErrorInvalidValue;
+  switch (grouped ? 10 + rf : rf) {
+    case 1: tile_launch<1>(gated, a, s); break;
+    case 2: tile_launch<2>(gated, a, s); break;
+    case 3: tile_launch<3>(gated, a, s); break;
+    case 4: tile_launch<4>(gated, a, s); break;
+    case 12: group_launch<2>(gated, a, s); break;
+    case 14: group_launch<4>(gated, a, s); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+hipError_t validate_f8_tile_kernels() {
+  hipFuncAttributes fa;
+#define MING_F8_TILE(RF)                                          \
+  reinterpret_cast<const void*>(&f8_tile_kernel<RF, false>),      \
+      reinterpret_cast<const void*>(&f8_tile_kernel<RF, true>)
+#define MING_F8_GROUP(MAX)                                        \
+  reinterpret_cast<const void*>(&f8_group_tile_kernel<MAX, false>), \
+      reinterpret_cast<const void*>(&f8_group_tile_kernel<MAX, true>)
+  const void* fns[] = {MING_F8_TILE(1), MING_F8_TILE(2), MING_F8_TILE(3), MING_F8_TILE(4),
+                       MING_F8_GROUP(2), MING_F8_GROUP(4)};
+#undef MING_F8_TILE
+#undef MING_F8_GROUP
+  for (const void* f : fns) {
+    const hipError_t e = hipFuncGetAttributes(&fa, f);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+}  // namespace ming

@@ -646,6 +646,20 @@ inline long long f8_finish_blocks(int n, int N) {
   return ((long long)n * ((N + 127) / 128) + 7) / 8;
 }
 hipError_t validate_f8_rows_kernels();
+// Many rows (f8_tile.hip): 64 * rf rows a tile, rf 1 to 4; over groups cut every 64 * rf
+// places, rf 2 or 4. Up to kF8TileBlocks blocks of K; ungrouped ldx below 2^22, grouped
+// x_rows * ldx below 2^31.
+constexpr int kF8TileBlocks = 1024;
+hipError_t launch_f8_tile(bool gated, bool grouped, const F8Args& a, int rf, hipStream_t s);
+inline long long f8_tile_blocks(int rf, bool grouped, int n, int E, int NR) {
+  const int tm = 64 * rf;
+  const long long tiles_m = grouped ? n / tm + (n < E ? n : E) : ((long long)n + tm - 1) / tm;
+  return tiles_m * ((NR + 255) / 256);
+}
+hipError_t validate_f8_tile_kernels();
+// Which kernel takes n rows (places): 0 the few-row one, else the tiles' rf. On a chip
+// of `cus`.
+int f8_plan(int cus, bool grouped, int E, int NR, int KB, int n);
 
 hipError_t validate_qproj_kernels();
 hipError_t validate_qproj_fast_kernels();

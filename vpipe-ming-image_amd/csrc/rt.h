@@ -61,6 +61,9 @@ int rt_route(const ming_ctx* c);
 // Experts' products on the context take this cut (experts_cut), -1: the plan's (tests).
 void rt_set_experts_cut(ming_ctx* c, int cut);
 int rt_experts_cut(const ming_ctx* c);
+// The same of the 8-bit products (f8_plan).
+void rt_set_f8_plan(ming_ctx* c, int plan);
+int rt_f8_plan(const ming_ctx* c);
 // the device word fp16 copies raise (QprojArgs::range), NULL on routes without
 int* rt_range_word(const ming_ctx* c);
 // Event timing around one launch of a family (ming_ctx_set_profiling): begin

@@ -84,6 +84,7 @@ struct ming_ctx {
   bool part_captured = false;
   size_t part_cap = SIZE_MAX;  // rt_set_part_cap
   int experts_cut = -1;        // rt_set_experts_cut
+  int f8_plan = -1;            // rt_set_f8_plan
   std::vector<void*> part_kept;
   int route = MING_ROUTE_AUTO;
   // device word raised by any fp16 copy that could not hold its value
@@ -456,6 +457,7 @@ hipError_t validate_kernels(int device) {
   if (e == hipSuccess) e = ming::validate_experts_qtile_kernels();
   if (e == hipSuccess) e = ming::validate_f8_quant_kernels();
   if (e == hipSuccess) e = ming::validate_f8_rows_kernels();
+  if (e == hipSuccess) e = ming::validate_f8_tile_kernels();
   if (known) done[device] = e == hipSuccess;
   return e;
 }
@@ -2241,6 +2243,8 @@ namespace ming {
 int rt_route(const ming_ctx* c) { return c->route; }
 void rt_set_experts_cut(ming_ctx* c, int cut) { c->experts_cut = cut; }
 int rt_experts_cut(const ming_ctx* c) { return c->experts_cut; }
+void rt_set_f8_plan(ming_ctx* c, int plan) { c->f8_plan = plan; }
+int rt_f8_plan(const ming_ctx* c) { return c->f8_plan; }
 int* rt_range_word(const ming_ctx* c) { return range_word(c); }
 bool rt_profile_begin(ming_ctx* c, void** ev) {
   *ev = nullptr;
