@@ -172,7 +172,7 @@ def make_weight(seed, E, N, K, gated=False):
 
 
 def set_plan(ctx, plan):
-    """The 8-bit products on ctx run this kernel (0 the few-row one, else tiles of 64 * plan
+    """The 8-bit products on ctx run this kernel (11, 22: the few-row one, else tiles of 64 * plan
     rows, 2 or 4 over groups); -1 the plan's."""
     import ctypes as C
 

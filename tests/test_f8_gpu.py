@@ -344,14 +344,14 @@ def test_every_kernel(ctx, plan, gated, N, K, M):
     W = Weights(ctx, 6000 + N, 1, N, K, gated)
     x, xs = ref.make_rows(6100 + M, M, K)
     first = None
-    for p in (0, 1, 2, 3, 4):
+    for p in (11, 22, 1, 2, 3, 4):
         print(f"case f8 plan {p} gated={gated} N={N} K={K} M={M}", flush=True)
         plan(p)
         got = call(ctx, W, x, xs, pad=16 * (p % 2))
         check(got, W, x, xs)
         if p == 1:
             first = got
-        if p > 1:
+        if 1 < p <= 4:
             for a, b in zip(first, got):
                 assert np.array_equal(a, b)
     W.w.close()
@@ -370,7 +370,7 @@ def test_every_grouped_kernel(ctx, plan, gated, N, K, counts):
     x, xs = ref.make_rows(6300, 300, K)
     # rows in place order: the gathered rows' copies
     gx, gs = x[src], np.ascontiguousarray(xs[:, src])
-    for p in (0, 2, 4):
+    for p in (11, 22, 2, 4):
         print(f"case f8 grouped plan {p} gated={gated} N={N} K={K}", flush=True)
         plan(p)
         got = call(ctx, W, x, xs, offsets, order, order.size, fan=3, pad=16)

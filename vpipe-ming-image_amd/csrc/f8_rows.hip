@@ -222,11 +222,14 @@ __global__ void f8_repack_kernel(const uint8_t* codes, const float* scales, int 
 template <int MF, int NF>
 void rows_launch(bool gated, bool grouped, const F8Args& a, hipStream_t s) {
   const dim3 grid((unsigned)f8_rows_blocks(16 * MF, 16 * NF, grouped, a.n, a.E, a.N));
+  if constexpr (MF * NF < 16) {
   if (gated && grouped)
     hipLaunchKernelGGL((f8_rows_kernel<MF, NF, true, true>), grid, dim3(64 * WK), 0, s, a);
   else if (gated)
     hipLaunchKernelGGL((f8_rows_kernel<MF, NF, true, false>), grid, dim3(64 * WK), 0, s, a);
-  else if (grouped)
+  }
+  if (gated) return;
+  if (grouped)
     hipLaunchKernelGGL((f8_rows_kernel<MF, NF, false, true>), grid, dim3(64 * WK), 0, s, a);
   else
     hipLaunchKernelGGL((f8_rows_kernel<MF, NF, false, false>), grid, dim3(64 * WK), 0, s, a);
@@ -242,14 +245,22 @@ hipError_t launch_f8_repack(const uint8_t* codes, const float* scales, int N, in
   return hipGetLastError();
 }
 
-hipError_t launch_f8_rows(bool gated, bool grouped, const F8Args& a, hipStream_t s) {
+hipError_t launch_f8_rows(bool gated, bool grouped, const F8Args& a, int plan, hipStream_t s) {
   if (a.n <= 0) return hipSuccess;
   if (a.N <= 0 || a.N % (gated ? 16 : 8) || a.K % 16 || (gated && !a.part) || a.E < 1 || a.fan < 1)
     return hipErrorInvalidValue;
-  if (a.n <= 16)
-    rows_launch<1, 1>(gated, grouped, a, s);
-  else
-    rows_launch<2, 2>(gated, grouped, a, s);
+  switch (plan) {
+    case 11: rows_launch<1, 1>(gated, grouped, a, s); break;
+    case 12: rows_launch<1, 2>(gated, grouped, a, s); break;
+    case 14: rows_launch<1, 4>(gated, grouped, a, s); break;
+    case 21: rows_launch<2, 1>(gated, grouped, a, s); break;
+    case 22: rows_launch<2, 2>(gated, grouped, a, s); break;
+    case 24: rows_launch<2, 4>(gated, grouped, a, s); break;
+    case 41: rows_launch<4, 1>(gated, grouped, a, s); break;
+    case 42: rows_launch<4, 2>(gated, grouped, a, s); break;
+    case 44: if (gated) return hipErrorInvalidValue; rows_launch<4, 4>(false, grouped, a, s); break;
+    default: return hipErrorInvalidValue;
+  }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !gated) return e;
   const int blocks = (a.N + 127) / 128;

@@ -25,12 +25,13 @@ struct ming_f8 {
 namespace ming {
 
 int f8_plan(int cus, bool grouped, int E, int NR, int KB, int n) {
-  if (KB > kF8TileBlocks) return 0;
+  if (KB > kF8TileBlocks) return 22;
   if (grouped) {
     const double live = E * (1.0 - std::exp(-(double)n / E)), rows = n / live;
-    return rows < 32.0 ? 0 : rows < 112.0 ? 2 : 4;
+    return rows < 8.0 ? 11 : rows < 32.0 ? 22 : rows < 112.0 ? 2 : 4;
   }
-  if (n <= 64) return 0;
+  if (n <= 16) return 11;
+  if (n <= 64) return 22;
   // rounds of the chip, a workgroup a CU, times a tile's time
   int best = 4;
   double least = 0.0;
@@ -111,12 +112,12 @@ bool own_memory(const ming_ctx* c, const void* p) {
 // The kernel that takes n rows of w on the current device.
 int plan_of(const ming_f8* w, bool grouped, int n) {
   const int set = ming::rt_f8_plan(w->ctx);
-  if (set >= 0 && w->KB <= ming::kF8TileBlocks) return set;
+  if (set > 0 && w->KB <= ming::kF8TileBlocks) return set;
   return ming::f8_plan(ming::device_cus(), grouped, w->E, w->NR, w->KB, n);
 }
 // f32 results of the few-row kernel on gated weights, before they are quantized.
 size_t part_bytes(const ming_f8* w, bool grouped, int n) {
-  return w->halves == 2 && plan_of(w, grouped, n) == 0 ? (size_t)n * w->N * 4 : 0;
+  return w->halves == 2 && plan_of(w, grouped, n) > 4 ? (size_t)n * w->N * 4 : 0;
 }
 
 // What a product's call brings.
@@ -190,7 +191,7 @@ int product(ming_ctx* c, const ming_f8* w, const Product& p) {
     return rt_fail(MING_ERR_SHAPE, std::string(p.who) + ": the call needs " + std::to_string(need) +
                                        " bytes of workspace, " + std::to_string(p.ws_bytes) +
                                        " given");
-  if (plan == 0 ? !ming::one_launch(ming::f8_rows_blocks(16, 16, p.grouped, p.n, w->E, w->N), 512) ||
+  if (plan > 4 ? !ming::one_launch(ming::f8_rows_blocks(16, 16, p.grouped, p.n, w->E, w->N), 512) ||
                       !ming::one_launch(ming::f8_finish_blocks(p.n, w->N), 256)
                 : !ming::one_launch(ming::f8_tile_blocks(plan, p.grouped, p.n, w->E, w->NR), 512))
     return bad(MING_ERR_SHAPE, "more rows times columns than one launch holds");
@@ -217,8 +218,8 @@ int product(ming_ctx* c, const ming_f8* w, const Product& p) {
   const double bytes = wide * w->K * std::min(p.n, w->E) + (double)p.x_rows * w->K +
                        (p.gated ? 1.0 : 2.0) * p.n * w->N;
   const int rc = run(c, p.gated ? ming::kRtF8Swiglu : ming::kRtF8Lin, flops, bytes, p.who, [&] {
-    return plan ? ming::launch_f8_tile(p.gated, p.grouped, a, plan, stream_of(c))
-                : ming::launch_f8_rows(p.gated, p.grouped, a, stream_of(c));
+    return plan <= 4 ? ming::launch_f8_tile(p.gated, p.grouped, a, plan, stream_of(c))
+                : ming::launch_f8_rows(p.gated, p.grouped, a, plan, stream_of(c));
   });
   if (rc != MING_OK) return rc;
   ming::rt_note_rows(c, 8, 2ull * (uint64_t)p.n * (uint64_t)w->N * w->halves * (uint64_t)w->K);

@@ -38,6 +38,16 @@ __device__ __forceinline__ void dma2_sb(const void* base, uint32_t off, uint32_t
 #pragma clang diagnostic pop
 }
 
+// 16 bytes a lane with an offset that moves both addresses.
+template <int OFF>
+__device__ __forceinline__ void dma16_off(const void* base, uint32_t off, uint32_t lds) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3"
+               :: "v"(off), "s"(base), "s"(lds), "n"(OFF) : "m0");
+#pragma clang diagnostic pop
+}
+
 template <int RF>
 struct TileLds {
   static constexpr int kStages = RF >= 3 ? 2 : 3;
@@ -53,7 +63,12 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
   using L = TileLds<RF>;
   constexpr int NST = L::kStages, MF = 2 * RF, NF = 4;
   constexpr int XD = RF, WD = 4;           // DMAs a wave and stage, and one of scales
-  float2* const wsc = reinterpret_cast<float2*>(ring + NST * L::kStage);
+  // Of a stage's DMAs so many follow the barrier that frees its slot, the others lie
+  // between the next stage's first steps: each holds its wave for some 20 cycles (512 x
+  // [3840, 10240] in 256 rows 103.9 us, all at once 113.7).
+  constexpr int kDma = XD + WD + 1, kPost = MF > 2 ? NF : kDma;
+  constexpr int kEach = (kPost + NF - 1) / NF;
+  float* const wsc = reinterpret_cast<float*>(ring + NST * L::kStage);
 
   const int tid = (int)threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -75,51 +90,62 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
       a.w + e * a.w_expert + (long long)tn * (TBN * 128);
   // LDS chunk p of a tile holds row p >> 3, logical chunk (p & 7) ^ swizzle
   auto chunk_of = [&](int p) { return (p & 7) ^ ((p >> 4) & 7); };
-  uint32_t xrow[XD], woff[WD];
+  uint32_t xrow[XD], woff[2];
 #pragma unroll
   for (int i = 0; i < XD; ++i)
     xrow[i] = (uint32_t)((long long)source((64 * (XD * wave + i) + lane) >> 3) * a.ldx);
+  // W's rows 32 wave + 8 i + lane / 8: with i even and odd the swizzles take turns, the
+  // rest of i is an instruction's offset. A tile that ends the weights after 128 rows
+  // takes those twice.
+  const int wrow = !GATED && TBN * tn + 32 * wave >= a.NR ? 32 * wave - 128 : 32 * wave;
 #pragma unroll
-  for (int i = 0; i < WD; ++i) {
-    const int p = 64 * (WD * wave + i) + lane;
-    int r = p >> 3;
-    // a tile that ends the weights after 128 rows takes those twice
-    if (!GATED && TBN * tn + r >= a.NR) r -= 128;
-    woff[i] = (uint32_t)(r * 128 + 16 * chunk_of(p));
-  }
-  // scales of 64 rows a wave; more waves than that write some twice, the same values (a
-  // branch here would split the stage, and the sums would be sunk past it)
-  const int srow = 64 * (wave % RF);
-  const uint32_t soff = 2u * (uint32_t)source(srow + lane);
+  for (int i = 0; i < 2; ++i)
+    woff[i] = (uint32_t)(wrow * 128 + (lane >> 3) * 128 + 16 * chunk_of(64 * i + lane));
+  // Scales of 64 rows a wave; more waves than that write some twice, the same values (a
+  // branch here would split the stage, and the sums would be sunk past it). A lane's MF
+  // rows of a wave's 16 MF lie side by side: dword c * MF + i is row 16 i + c.
+  const int srow = 64 * (wave % RF), sd = srow + lane, si = sd % (16 * MF);
+  const uint32_t soff =
+      2u * (uint32_t)source(sd - si + 16 * (si % MF) + si / MF);
   const int klast = (a.K - 128 * (KB - 1)) / 16;       // the last block's chunks
 
-  // stage t's DMAs; past the last one it is read again into a slot nothing reads, so
-  // that every stage issues and waits alike
-  auto issue_w = [&](int t, const uint4* S) {
-    const uint8_t* base = wbase + (long long)(t < KB ? t : KB - 1) * a.NR * 128;
-#pragma unroll
-    for (int i = 0; i < WD; ++i)
-      dma16_sb(base, woff[i], lds_addr(S + L::kX + 64 * (WD * wave + i)));
-  };
-  auto issue_x = [&](int t, const uint4* S) {
-    const int kb = t < KB ? t : KB - 1;
-    const uint8_t* base = xbase + (long long)kb * 128;
-    // past K the weights are zeros: any chunk of x's own block will do
-    const int cut = kb == KB - 1 ? klast : 8;
-#pragma unroll
-    for (int i = 0; i < XD; ++i) {
-      const int ch = chunk_of(64 * (XD * wave + i) + lane);
-      dma16_sb(base, xrow[i] + (ch < cut ? 16 * ch : 0), lds_addr(S + 64 * (XD * wave + i)));
+  const uint8_t *xnext = xbase, *wnext = wbase;
+  const uint16_t* snext = sbase;
+  int tnext = 0;
+  // The DMAs of the stage that is next to be fetched, one at a time: 0 to XD - 1 x's, then
+  // W's, then the scales'. Its bases move on by a stage at a time; past the last stage it
+  // is read again into a slot nothing reads, so that every stage issues and waits alike.
+  auto issue = [&](int q, const uint4* S) {
+    if (q < XD) {
+      // past K the weights are zeros: any chunk of x's own block will do
+      const int ch = chunk_of(64 * (XD * wave + q) + lane), cut = tnext == KB - 1 ? klast : 8;
+      dma16_sb(xnext, xrow[q] + (ch < cut ? 16 * ch : 0), lds_addr(S + 64 * (XD * wave + q)));
+    } else if (q < XD + WD) {
+      const uint32_t to = lds_addr(S + L::kX + 64 * WD * wave);
+      switch (q - XD) {
+        case 0: dma16_off<0>(wnext, woff[0], to); break;
+        case 1: dma16_off<1024>(wnext, woff[1], to); break;
+        case 2: dma16_off<2048>(wnext, woff[0], to); break;
+        default: dma16_off<3072>(wnext, woff[1], to); break;
+      }
+    } else {
+      dma2_sb(snext, soff, lds_addr(S + L::kX + L::kW) + 4 * srow);
+      const bool more = tnext < KB - 1;
+      tnext += more;
+      xnext += more ? 128 : 0;
+      wnext += more ? a.NR * 128ll : 0;
+      snext += more ? a.ldxs : 0;
     }
-    dma2_sb(sbase + (long long)kb * a.ldxs, soff, lds_addr(S + L::kX + L::kW) + 4 * srow);
   };
 
   // the weights' scales of all blocks: the tile's two blocks of rows, or gate and up
   {
     const int b0 = 2 * tn, b1 = 2 * tn + 1 < a.NB ? 2 * tn + 1 : 2 * tn;
     const float* ws = a.ws + e * a.s_expert;
-    for (int k = tid; k < KB; k += 64 * NW)
-      wsc[k] = make_float2(ws[(long long)k * a.NB + b0], ws[(long long)k * a.NB + b1]);
+    for (int k = tid; k < KB; k += 64 * NW) {
+      wsc[2 * k] = ws[(long long)k * a.NB + b0];
+      wsc[2 * k + 1] = ws[(long long)k * a.NB + b1];
+    }
   }
 
   floatx4_t acc[NF][MF];
@@ -136,35 +162,48 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
   auto read_w = [&](const uint4* S, int j) {
     return F8Frag{S[L::kX + fw + 128 * j], S[L::kX + (fw ^ 4) + 128 * j]};
   };
-  auto read_s = [&](const uint4* S, int i) {
-    return reinterpret_cast<const uint32_t*>(S + L::kX + L::kW)[32 * RF * wm + 16 * i + c];
+  uint32_t sx[MF];
+  float sw[2];
+  auto read_s = [&](const uint4* S, int t) {
+    const uint32_t* p =
+        reinterpret_cast<const uint32_t*>(S + L::kX + L::kW) + 16 * MF * wm + MF * c;
+#pragma unroll
+    for (int i = 0; i < MF; i += 2) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p + i);
+      sx[i] = v.x;
+      sx[i + 1] = v.y;
+    }
+    const float* q = wsc + 2 * t + (GATED ? 0 : wn >> 1);
+    sw[0] = q[0];
+    sw[1] = GATED ? q[1] : 0.0f;
   };
 
   F8Frag w[NF], x[2];
-  uint32_t sx[MF];
   auto body = [&](auto ph, int t) {
     constexpr int PH = decltype(ph)::value;
     const uint4 *const S = ring + PH * L::kStage, *const Sn = ring + (PH + 1) % NST * L::kStage;
-    const float2 sw = wsc[t];
-    const float s0 = GATED ? sw.x : wn < 2 ? sw.x : sw.y;
+    const uint4* const Sl = ring + (PH + NST - 1) % NST * L::kStage;   // freed by stage t - 1
     float s[MF], u[MF];
 #pragma unroll
     for (int i = 0; i < MF; ++i) {
       const float v = __uint_as_float(sx[i] << 16);
-      s[i] = v * s0;
-      u[i] = GATED ? v * sw.y : 0.0f;
+      s[i] = v * sw[0];
+      u[i] = GATED ? v * sw[1] : 0.0f;
     }
     auto add = [&](int j, int i, const floatx4_t& d) {
       const float f = GATED && j >= 2 ? u[i] : s[i];
 #pragma unroll
       for (int r = 0; r < 4; ++r) acc[j][i][r] = fmaf(d[r], f, acc[j][i][r]);
     };
+    constexpr int kSteps = MF > 2 ? MF - 2 : 1, kLate = (kDma - kPost + kSteps - 1) / kSteps;
     F8Frag xa = x[0], xb = x[1];
     floatx4_t dp[NF];
 #pragma unroll
     for (int i = 0; i < MF - 2; ++i) {
       const F8Frag xn = read_x(S, i + 2);
       floatx4_t d[NF];
+#pragma unroll
+      for (int q = kPost + i * kLate; q < kPost + (i + 1) * kLate && q < kDma; ++q) issue(q, Sl);
 #pragma unroll
       for (int j = 0; j < NF; ++j) {
         d[j] = f8_mfma(w[j], xa);
@@ -183,15 +222,16 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    ring_wait<(NST - 2) * (XD + WD + 1)>();
+    ring_wait<(NST - 2) * kDma>();
     __builtin_amdgcn_sched_barrier(0);
-    issue_x(t + NST, S);
-    issue_w(t + NST, S);
     x[0] = read_x(Sn, 0);
+    read_s(Sn, t + 1 < KB ? t + 1 : t);
     floatx4_t e0, e1;
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < NF; ++j) {
+#pragma unroll
+      for (int q = j * kEach; q < (j + 1) * kEach && q < kPost; ++q) issue(q, S);
       const floatx4_t d0 = f8_mfma(w[j], xa), d1 = f8_mfma(w[j], xb);
       if (MF > 2) add(j, MF > 2 ? MF - 3 : 0, dp[j]);
       w[j] = read_w(Sn, j);
@@ -206,24 +246,23 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
     add(NF - 1, MF - 2, e0);
     add(NF - 1, MF - 1, e1);
     x[1] = read_x(Sn, 1);
-#pragma unroll
-    for (int i = 0; i < MF; ++i) sx[i] = read_s(Sn, i);
   };
 
 #pragma unroll
   for (int t = 0; t < NST; ++t) {
-    issue_x(t, ring + t * L::kStage);
-    issue_w(t, ring + t * L::kStage);
+#pragma unroll
+    for (int q = 0; q < kDma; ++q)
+      // (the last one's later ones are stage 0's to issue)
+      if (t < NST - 1 || q < kPost) issue(q, ring + t * L::kStage);
   }
   // stage 0 landed, the weights' scales written (their stores are waited for with the
   // LDS counter)
-  ring_wait<(NST - 1) * (XD + WD + 1)>();
+  ring_wait<(NST - 2) * kDma + kPost>();
 #pragma unroll
   for (int j = 0; j < NF; ++j) w[j] = read_w(ring, j);
   x[0] = read_x(ring, 0);
   x[1] = read_x(ring, 1);
-#pragma unroll
-  for (int i = 0; i < MF; ++i) sx[i] = read_s(ring, i);
+  read_s(ring, 0);
   const std::integral_constant<int, 0> p0c{};
   const std::integral_constant<int, 1> p1c{};
   int t = 0;

@@ -636,7 +636,7 @@ struct F8Args {
 };
 hipError_t launch_f8_repack(const uint8_t* codes, const float* scales, int N, int K, int halves,
                             uint8_t* out, float* souts, hipStream_t s);
-hipError_t launch_f8_rows(bool gated, bool grouped, const F8Args& a, hipStream_t s);
+hipError_t launch_f8_rows(bool gated, bool grouped, const F8Args& a, int plan, hipStream_t s);
 // Blocks of tiles of tm rows x tn columns: every group ends in at most one partial one.
 inline long long f8_rows_blocks(int tm, int tn, bool grouped, int n, int E, int N) {
   const long long tiles_m = grouped ? n / tm + (n < E ? n : E) : ((long long)n + tm - 1) / tm;
