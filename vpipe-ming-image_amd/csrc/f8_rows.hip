@@ -64,7 +64,7 @@ __global__ __launch_bounds__(64 * WK) void f8_rows_kernel(const F8Args a) {
     xp[i] = a.x + (long long)src * a.ldx;
     sp[i] = a.xs + src;
   }
-  const uint8_t* wp = a.w + e * a.w_expert + (long long)c * 128 + 16 * g;
+  const uint8_t* wp = a.w + e * a.w_expert + 16 * lane;
   const float* ws = a.ws + e * a.s_expert;
   int wr[NH];                              // resident rows of the fragments
 #pragma unroll
@@ -84,7 +84,7 @@ __global__ __launch_bounds__(64 * WK) void f8_rows_kernel(const F8Args a) {
 #pragma unroll
     for (int j = 0; j < NH; ++j) {
       b.w[j].lo = *reinterpret_cast<const uint4*>(p + wr[j] * 128);
-      b.w[j].hi = *reinterpret_cast<const uint4*>(p + wr[j] * 128 + 64);
+      b.w[j].hi = *reinterpret_cast<const uint4*>(p + wr[j] * 128 + 1024);
     }
     // past K the weights are zeros, and any chunk of x's own block will do (not one
     // of other memory, whose NaN codes would count)
@@ -190,16 +190,18 @@ __global__ __launch_bounds__(256) void f8_finish_kernel(const F8Args a, int rows
 }
 
 // Codes [halves * N][K] and scales [halves * blocks of N][KB] into the resident order,
-// zeros past N and K: blocks of K outermost, rows of 128 bytes; gated, f8_gate_row's.
+// zeros past N and K: blocks of K outermost, then 16 rows (gated, f8_gate_row's), as the
+// matrix instruction's lanes hold them: chunks g and g + 4 of row c for lane 16 g + c, the
+// first ones of all lanes before the second ones.
 __global__ void f8_repack_kernel(const uint8_t* codes, const float* scales, int N, int K, int halves,
                                  uint8_t* out, float* souts) {
   const int KB = (K + 127) / 128, nb = (N + 127) / 128, NR = halves * nb * 128;
   const long long total = (long long)KB * NR * 8;
   for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total;
        i += (long long)gridDim.x * blockDim.x) {
-    const int ch = (int)(i & 7);
-    const long long q = i >> 3;
-    const int r = (int)(q % NR), kb = (int)(q / NR);
+    const int l = (int)(i & 63), ch = (l >> 4) + 4 * (int)((i >> 6) & 1);
+    const long long q = i >> 7;              // 16 rows of a block
+    const int kb = (int)(q / (NR / 16)), r = 16 * (int)(q % (NR / 16)) + (l & 15);
     int n = r, half = 0;
     if (halves == 2) {
       half = (r >> 5) & 1;

@@ -18,7 +18,7 @@ struct ming_f8 {
   ming_ctx* ctx = nullptr;
   int E = 0, N = 0, K = 0, halves = 0;
   int KB = 0, NR = 0, NB = 0;      // blocks of K, resident rows and scales a block of K
-  uint8_t* codes = nullptr;        // [E][KB][NR][128]
+  uint8_t* codes = nullptr;        // [E][KB][NR][128], in 16 rows at a time
   float* scales = nullptr;         // [E][KB][NB]
 };
 

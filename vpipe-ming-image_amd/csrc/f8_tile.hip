@@ -11,8 +11,8 @@
 // of 32 cycles). A lane's four results are four columns of one row, so a row's scale
 // is one register a row tile, times the weights' one scale.
 //
-// Stages go through an LDS ring filled by direct global->LDS DMA (rows of 128 bytes,
-// chunks swizzled), with the rows' scales; the weights' scales are all taken at the
+// Stages go through an LDS ring filled by direct global->LDS DMA (x in rows of 128 bytes,
+// chunks swizzled; the weights as they lie), with the rows' scales; the weights' scales are all taken at the
 // start. One barrier a stage, before its last two row tiles: their operands are in
 // registers by then, so the slot is free for the DMA, and the next stage's first
 // operands are read under their matrix instructions.
@@ -88,19 +88,16 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
   const uint16_t* const sbase = GROUPED ? a.xs : a.xs + p0;
   const uint8_t* const wbase =
       a.w + e * a.w_expert + (long long)tn * (TBN * 128);
-  // LDS chunk p of a tile holds row p >> 3, logical chunk (p & 7) ^ swizzle
+  // LDS chunk p of x's tile holds row p >> 3, logical chunk (p & 7) ^ swizzle
   auto chunk_of = [&](int p) { return (p & 7) ^ ((p >> 4) & 7); };
-  uint32_t xrow[XD], woff[2];
+  uint32_t xrow[XD];
 #pragma unroll
   for (int i = 0; i < XD; ++i)
     xrow[i] = (uint32_t)((long long)source((64 * (XD * wave + i) + lane) >> 3) * a.ldx);
-  // W's rows 32 wave + 8 i + lane / 8: with i even and odd the swizzles take turns, the
-  // rest of i is an instruction's offset. A tile that ends the weights after 128 rows
-  // takes those twice.
+  // W's 32 rows a wave are 4 KB of memory and of LDS, in the order of the lanes' operands.
+  // A tile that ends the weights after 128 rows takes those twice.
   const int wrow = !GATED && TBN * tn + 32 * wave >= a.NR ? 32 * wave - 128 : 32 * wave;
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    woff[i] = (uint32_t)(wrow * 128 + (lane >> 3) * 128 + 16 * chunk_of(64 * i + lane));
+  const uint32_t woff = (uint32_t)(16 * lane);
   // Scales of 64 rows a wave; more waves than that write some twice, the same values (a
   // branch here would split the stage, and the sums would be sunk past it). A lane's MF
   // rows of a wave's 16 MF lie side by side: dword c * MF + i is row 16 i + c.
@@ -109,7 +106,7 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
       2u * (uint32_t)source(sd - si + 16 * (si % MF) + si / MF);
   const int klast = (a.K - 128 * (KB - 1)) / 16;       // the last block's chunks
 
-  const uint8_t *xnext = xbase, *wnext = wbase;
+  const uint8_t *xnext = xbase, *wnext = wbase + wrow * 128;
   const uint16_t* snext = sbase;
   int tnext = 0;
   // The DMAs of the stage that is next to be fetched, one at a time: 0 to XD - 1 x's, then
@@ -123,10 +120,10 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
     } else if (q < XD + WD) {
       const uint32_t to = lds_addr(S + L::kX + 64 * WD * wave);
       switch (q - XD) {
-        case 0: dma16_off<0>(wnext, woff[0], to); break;
-        case 1: dma16_off<1024>(wnext, woff[1], to); break;
-        case 2: dma16_off<2048>(wnext, woff[0], to); break;
-        default: dma16_off<3072>(wnext, woff[1], to); break;
+        case 0: dma16_off<0>(wnext, woff, to); break;
+        case 1: dma16_off<1024>(wnext, woff, to); break;
+        case 2: dma16_off<2048>(wnext, woff, to); break;
+        default: dma16_off<3072>(wnext, woff, to); break;
       }
     } else {
       dma2_sb(snext, soff, lds_addr(S + L::kX + L::kW) + 4 * srow);
@@ -155,12 +152,12 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
     for (int i = 0; i < MF; ++i) acc[j][i] = floatx4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
   // fragments: rows 16 apart keep their swizzle
-  const int fx = (32 * RF * wm + c) * 8 + (g ^ (c >> 1)), fw = (64 * wn + c) * 8 + (g ^ (c >> 1));
+  const int fx = (32 * RF * wm + c) * 8 + (g ^ (c >> 1)), fw = 64 * 8 * wn + lane;
   auto read_x = [&](const uint4* S, int i) {
     return F8Frag{S[fx + 128 * i], S[(fx ^ 4) + 128 * i]};
   };
   auto read_w = [&](const uint4* S, int j) {
-    return F8Frag{S[L::kX + fw + 128 * j], S[L::kX + (fw ^ 4) + 128 * j]};
+    return F8Frag{S[L::kX + fw + 128 * j], S[L::kX + fw + 128 * j + 64]};
   };
   uint32_t sx[MF];
   float sw[2];

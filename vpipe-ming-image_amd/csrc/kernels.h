@@ -607,8 +607,8 @@ hipError_t validate_f8_quant_kernels();
 // ---- their products (f8_rows.hip) ------------------------------------------------------
 // Row p of the output is x row p, or of a grouped call x row order[p] / fan (p itself
 // without an order; kept inside [0, x_rows)) times the weights of p's group. w is
-// resident as f8_repack leaves it, an expert after another: [KB][NR][128] bytes, NR
-// rows padded to 128 a half, with scales [KB][NB].
+// resident as launch_f8_repack leaves it, an expert after another: [KB][NR / 16] pieces of
+// 2 KB, NR rows padded to 128 a half, with scales [KB][NB].
 struct F8Args {
   const uint8_t* x;
   long long ldx;
