@@ -171,9 +171,15 @@ def make_weight(seed, E, N, K, gated=False):
     return np.stack(codes), np.stack(scales)
 
 
+# The kernels a test can ask for (set_plan): 10 mf + nf of the few-row kernel, the tiles' rf;
+# plain projections' halves of K, 100 * their slices.
+PLANS = (11, 12, 14, 22, 24, 1, 2, 3, 4)
+DUO = (100, 200, 300, 700)
+GROUPED_PLANS = (11, 12, 14, 22, 24, 2, 4)
+
+
 def set_plan(ctx, plan):
-    """The 8-bit products on ctx run this kernel (11, 22: the few-row one, else tiles of 64 * plan
-    rows, 2 or 4 over groups); -1 the plan's."""
+    """The 8-bit products on ctx run this kernel; -1 the plan's."""
     import ctypes as C
 
     import ming_dit_amd as m

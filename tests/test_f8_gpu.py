@@ -224,7 +224,7 @@ def call(ctx, W, x, xs, offsets=None, order=None, n=None, fan=1, bias=None, pad=
     n = rows if n is None else n
     held = n if offsets is None else int(offsets[-1])
     xd, sd = dev8(x, pad), dev_scales(xs, pad)
-    ws = torch.full((max(16, W.w.workspace_bytes(n)),), 255, dtype=torch.uint8, device="cuda")
+    ws = torch.full((W.w.workspace_bytes(n) + 16,), 255, dtype=torch.uint8, device="cuda")
     od = None if order is None else to_dev(order)
     fd = None if offsets is None else to_dev(offsets)
     bd = None if bias is None else to_dev(bias)
@@ -344,14 +344,14 @@ def test_every_kernel(ctx, plan, gated, N, K, M):
     W = Weights(ctx, 6000 + N, 1, N, K, gated)
     x, xs = ref.make_rows(6100 + M, M, K)
     first = None
-    for p in (11, 22, 1, 2, 3, 4):
+    for p in ref.PLANS if gated else ref.PLANS + ref.DUO:
         print(f"case f8 plan {p} gated={gated} N={N} K={K} M={M}", flush=True)
         plan(p)
         got = call(ctx, W, x, xs, pad=16 * (p % 2))
         check(got, W, x, xs)
         if p == 1:
             first = got
-        if 1 < p <= 4:
+        if 1 < p < 10:
             for a, b in zip(first, got):
                 assert np.array_equal(a, b)
     W.w.close()
@@ -370,7 +370,7 @@ def test_every_grouped_kernel(ctx, plan, gated, N, K, counts):
     x, xs = ref.make_rows(6300, 300, K)
     # rows in place order: the gathered rows' copies
     gx, gs = x[src], np.ascontiguousarray(xs[:, src])
-    for p in (11, 22, 2, 4):
+    for p in ref.GROUPED_PLANS:
         print(f"case f8 grouped plan {p} gated={gated} N={N} K={K}", flush=True)
         plan(p)
         got = call(ctx, W, x, xs, offsets, order, order.size, fan=3, pad=16)
@@ -533,13 +533,13 @@ def test_feed_forward_captured(ctx):
     c1, s1 = new((T, H), torch.uint8), new((ref.blocks(H), T), torch.int16)
     ch, sh = new((T, F), torch.uint8), new((ref.blocks(F), T), torch.int16)
     c2, s2 = new((T, H), torch.uint8), new((ref.blocks(H), T), torch.int16)
-    ws = new((max(16, GU.w.workspace_bytes(T)),), torch.uint8)
+    ws = new((16 + max(w.w.workspace_bytes(T) for w in (GU, DN)),), torch.uint8)
     outs = (h1, c1, s1, ch, sh, out, h2, c2, s2)
 
     def step():
         c.f8_rmsnorm(x, nwd, T, H, c1, s1, sub=sub, h=h1)
         c.f8_swiglu(GU.w, c1, s1, ch, sh, T, ws=ws)
-        c.f8_lin(DN.w, ch, sh, out, T)
+        c.f8_lin(DN.w, ch, sh, out, T, ws=ws)
         c.f8_rmsnorm(h1, nwd, T, H, c2, s2, sub=out, h=h2)
 
     sync()
@@ -590,13 +590,14 @@ def test_mixture_of_experts(ctx):
     sh = torch.zeros((ref.blocks(F), n), dtype=torch.int16, device="cuda")
     y = torch.zeros((n, H), dtype=torch.int16, device="cuda")
     out = torch.zeros((T, H), dtype=torch.int16, device="cuda")
-    ws = torch.zeros(max(16, GU.w.workspace_bytes(n)), dtype=torch.uint8, device="cuda")
+    ws = torch.zeros(16 + max(w.w.workspace_bytes(n) for w in (GU, DN)), dtype=torch.uint8,
+                     device="cuda")
     sync()
     ctx.f8_quantize(xd, T, H, c1, s1)
     ctx.topk_route(ld, T, E, k, ids, wt)
     ctx.group_rows(ids, n, E, off, order, place)
     ctx.f8_experts_swiglu(GU.w, c1, s1, T, order, off, n, ch, sh, fan=k, ws=ws)
-    ctx.f8_experts_lin(DN.w, ch, sh, n, None, off, n, y)
+    ctx.f8_experts_lin(DN.w, ch, sh, n, None, off, n, y, ws=ws)
     ctx.experts_combine(y, n, place, wt, T, k, out, H, add=xd)
     ctx.synchronize()
     ho, hi = from_dev(off), from_dev(order)

@@ -157,20 +157,10 @@ __global__ __launch_bounds__(64 * WK) void f8_rows_kernel(const F8Args a) {
   }
 }
 
-// The gated results [n][N] in f32 into codes and scales: 32 lanes a block of 128.
-__global__ __launch_bounds__(256) void f8_finish_kernel(const F8Args a, int rows, int blocks) {
-  const uint32_t unit = blockIdx.x * 8u + (threadIdx.x >> 5);
-  const int l = (int)threadIdx.x & 31;
-  const int b = (int)(unit / (uint32_t)rows), row = (int)(unit - (uint32_t)b * (uint32_t)rows);
-  int held = rows;                         // rows behind the last group stay as they are
-  if (a.offsets) {
-    held = a.offsets[a.E];
-    held = held < rows ? held : rows;
-  }
-  const int n = 128 * b + 4 * l;
-  const bool in = b < blocks && row < held && n < a.N;
-  floatx4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (in) v = *reinterpret_cast<const floatx4_t*>(a.part + (long long)row * a.N + n);
+// Columns n .. n + 3 of a row's block b, lane l of the 32 that hold it (in: they exist;
+// lanes without take part in the shuffles).
+__device__ __forceinline__ void f8_store_block(const F8Args& a, int row, int b, int n, int l, bool in,
+                                               const floatx4_t& v) {
   uint32_t top = 0;
 #pragma unroll
   for (int r = 0; r < 4; ++r) top = f8_top(top, v[r]);
@@ -187,6 +177,23 @@ __global__ __launch_bounds__(256) void f8_finish_kernel(const F8Args a, int rows
   *reinterpret_cast<uint32_t*>(a.h + (long long)row * a.ldh + n) =
       fine ? f8_pack4(v[0] * q, v[1] * q, v[2] * q, v[3] * q) : kF8Nan4;
   if (l == 0) a.hs[(long long)b * a.ldhs + row] = (uint16_t)sb;
+}
+
+// The gated results [n][N] in f32 into codes and scales: 32 lanes a block of 128.
+__global__ __launch_bounds__(256) void f8_finish_kernel(const F8Args a, int rows, int blocks) {
+  const uint32_t unit = blockIdx.x * 8u + (threadIdx.x >> 5);
+  const int l = (int)threadIdx.x & 31;
+  const int b = (int)(unit / (uint32_t)rows), row = (int)(unit - (uint32_t)b * (uint32_t)rows);
+  int held = rows;                         // rows behind the last group stay as they are
+  if (a.offsets) {
+    held = a.offsets[a.E];
+    held = held < rows ? held : rows;
+  }
+  const int n = 128 * b + 4 * l;
+  const bool in = b < blocks && row < held && n < a.N;
+  floatx4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (in) v = *reinterpret_cast<const floatx4_t*>(a.part + (long long)row * a.N + n);
+  f8_store_block(a, row, b, n, l, in, v);
 }
 
 // Codes [halves * N][K] and scales [halves * blocks of N][KB] into the resident order,
@@ -224,14 +231,11 @@ __global__ void f8_repack_kernel(const uint8_t* codes, const float* scales, int 
 template <int MF, int NF>
 void rows_launch(bool gated, bool grouped, const F8Args& a, hipStream_t s) {
   const dim3 grid((unsigned)f8_rows_blocks(16 * MF, 16 * NF, grouped, a.n, a.E, a.N));
-  if constexpr (MF * NF < 16) {
   if (gated && grouped)
     hipLaunchKernelGGL((f8_rows_kernel<MF, NF, true, true>), grid, dim3(64 * WK), 0, s, a);
   else if (gated)
     hipLaunchKernelGGL((f8_rows_kernel<MF, NF, true, false>), grid, dim3(64 * WK), 0, s, a);
-  }
-  if (gated) return;
-  if (grouped)
+  else if (grouped)
     hipLaunchKernelGGL((f8_rows_kernel<MF, NF, false, true>), grid, dim3(64 * WK), 0, s, a);
   else
     hipLaunchKernelGGL((f8_rows_kernel<MF, NF, false, false>), grid, dim3(64 * WK), 0, s, a);
@@ -247,20 +251,17 @@ hipError_t launch_f8_repack(const uint8_t* codes, const float* scales, int N, in
   return hipGetLastError();
 }
 
-hipError_t launch_f8_rows(bool gated, bool grouped, const F8Args& a, int plan, hipStream_t s) {
+hipError_t launch_f8_rows(bool gated, bool grouped, const F8Args& a, int mf, int nf,
+                          hipStream_t s) {
   if (a.n <= 0) return hipSuccess;
   if (a.N <= 0 || a.N % (gated ? 16 : 8) || a.K % 16 || (gated && !a.part) || a.E < 1 || a.fan < 1)
     return hipErrorInvalidValue;
-  switch (plan) {
+  switch (10 * mf + nf) {
     case 11: rows_launch<1, 1>(gated, grouped, a, s); break;
     case 12: rows_launch<1, 2>(gated, grouped, a, s); break;
     case 14: rows_launch<1, 4>(gated, grouped, a, s); break;
-    case 21: rows_launch<2, 1>(gated, grouped, a, s); break;
     case 22: rows_launch<2, 2>(gated, grouped, a, s); break;
     case 24: rows_launch<2, 4>(gated, grouped, a, s); break;
-    case 41: rows_launch<4, 1>(gated, grouped, a, s); break;
-    case 42: rows_launch<4, 2>(gated, grouped, a, s); break;
-    case 44: if (gated) return hipErrorInvalidValue; rows_launch<4, 4>(false, grouped, a, s); break;
     default: return hipErrorInvalidValue;
   }
   hipError_t e = hipGetLastError();
@@ -280,7 +281,8 @@ hipError_t validate_f8_rows_kernels() {
       reinterpret_cast<const void*>(&f8_rows_kernel<MF, NF, true, true>)
   const void* fns[] = {reinterpret_cast<const void*>(&f8_finish_kernel),
                        reinterpret_cast<const void*>(&f8_repack_kernel), MING_F8_ROWS(1, 1),
-                       MING_F8_ROWS(2, 2)};
+                       MING_F8_ROWS(1, 2), MING_F8_ROWS(1, 4), MING_F8_ROWS(2, 2),
+                       MING_F8_ROWS(2, 4)};
 #undef MING_F8_ROWS
   for (const void* f : fns) {
     const hipError_t e = hipFuncGetAttributes(&fa, f);

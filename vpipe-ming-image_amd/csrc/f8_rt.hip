@@ -24,14 +24,16 @@ struct ming_f8 {
 
 namespace ming {
 
-int f8_plan(int cus, bool grouped, int E, int NR, int KB, int n) {
-  if (KB > kF8TileBlocks) return 22;
+F8Plan f8_plan(int cus, bool gated, bool grouped, int E, int NR, int KB, int n) {
+  if (KB > kF8TileBlocks) return {F8Plan::kRows, 2, 2};
   if (grouped) {
     const double live = E * (1.0 - std::exp(-(double)n / E)), rows = n / live;
-    return rows < 8.0 ? 11 : rows < 32.0 ? 22 : rows < 112.0 ? 2 : 4;
+    if (rows < 8.0) return {F8Plan::kRows, 1, 2};
+    if (rows < 24.0) return {F8Plan::kRows, 1, 4};
+    return {F8Plan::kTiles, rows < 112.0 ? 2 : 4, 0};
   }
-  if (n <= 16) return 11;
-  if (n <= 64) return 22;
+  if (n <= 16) return {F8Plan::kRows, 1, 1};
+  if (n <= 64) return {F8Plan::kRows, 1, 4};
   // rounds of the chip, a workgroup a CU, times a tile's time
   int best = 4;
   double least = 0.0;
@@ -43,7 +45,7 @@ int f8_plan(int cus, bool grouped, int E, int NR, int KB, int n) {
       least = us;
     }
   }
-  return best;
+  return {F8Plan::kTiles, best, 0};
 }
 
 }  // namespace ming
@@ -109,15 +111,23 @@ bool own_memory(const ming_ctx* c, const void* p) {
   return at.type == hipMemoryTypeDevice && at.device == ming::rt_device(c);
 }
 
-// The kernel that takes n rows of w on the current device.
-int plan_of(const ming_f8* w, bool grouped, int n) {
+// The kernel that takes n rows of w on the current device. rt_set_f8_plan's choices: rf of
+// the tiles, 10 mf + nf of the few-row kernel, 100 * slices of f8_duo's.
+ming::F8Plan plan_of(const ming_f8* w, bool grouped, int n) {
+  using ming::F8Plan;
   const int set = ming::rt_f8_plan(w->ctx);
-  if (set > 0 && w->KB <= ming::kF8TileBlocks) return set;
-  return ming::f8_plan(ming::device_cus(), grouped, w->E, w->NR, w->KB, n);
+  if (set > 0 && set < 10 && w->KB <= ming::kF8TileBlocks) return {F8Plan::kTiles, set, 0};
+  if (set >= 10 && set < 100) return {F8Plan::kRows, set / 10, set % 10};
+  if (set >= 100 && !grouped && w->halves == 1 && w->KB <= ming::kF8TileBlocks)
+    return {F8Plan::kDuo, std::min(set / 100, w->KB), 0};
+  return ming::f8_plan(ming::device_cus(), w->halves == 2, grouped, w->E, w->NR, w->KB, n);
 }
-// f32 results of the few-row kernel on gated weights, before they are quantized.
-size_t part_bytes(const ming_f8* w, bool grouped, int n) {
-  return w->halves == 2 && plan_of(w, grouped, n) > 4 ? (size_t)n * w->N * 4 : 0;
+// f32 sums on their way (F8Args::part).
+size_t part_bytes(const ming_f8* w, const ming::F8Plan& p, int n) {
+  if (p.kind == ming::F8Plan::kRows) return w->halves == 2 ? (size_t)n * w->N * 4 : 0;
+  return p.kind == ming::F8Plan::kDuo && p.a > 1
+             ? (size_t)p.a * ming::f8_duo_blocks(n, w->NR) * (64 * 128 * 4)
+             : 0;
 }
 
 // What a product's call brings.
@@ -183,17 +193,21 @@ int product(ming_ctx* c, const ming_f8* w, const Product& p) {
       return bad(MING_ERR_ARG, "y must be 16-byte, bias 8-byte aligned");
   }
   DeviceGuard g(ming::rt_device(c));       // (the plan counts its CUs)
-  const int plan = plan_of(w, p.grouped, p.n);
-  const size_t need = part_bytes(w, p.grouped, p.n);
+  const ming::F8Plan plan = plan_of(w, p.grouped, p.n);
+  const size_t need = part_bytes(w, plan, p.n);
   if (need > 0 && (!p.ws || !aligned(p.ws, 16)))
     return bad(MING_ERR_ARG, "ws must be given, 16-byte aligned");
   if (p.ws_bytes < need)
     return rt_fail(MING_ERR_SHAPE, std::string(p.who) + ": the call needs " + std::to_string(need) +
                                        " bytes of workspace, " + std::to_string(p.ws_bytes) +
                                        " given");
-  if (plan > 4 ? !ming::one_launch(ming::f8_rows_blocks(16, 16, p.grouped, p.n, w->E, w->N), 512) ||
-                      !ming::one_launch(ming::f8_finish_blocks(p.n, w->N), 256)
-                : !ming::one_launch(ming::f8_tile_blocks(plan, p.grouped, p.n, w->E, w->NR), 512))
+  using ming::F8Plan;
+  const long long blocks =
+      plan.kind == F8Plan::kTiles  ? ming::f8_tile_blocks(plan.a, p.grouped, p.n, w->E, w->NR)
+      : plan.kind == F8Plan::kDuo ? ming::f8_duo_blocks(p.n, w->NR) * plan.a
+                                   : ming::f8_rows_blocks(16, 16, p.grouped, p.n, w->E, w->N);
+  if (!ming::one_launch(blocks, 512) ||
+      (plan.kind == F8Plan::kRows && !ming::one_launch(ming::f8_finish_blocks(p.n, w->N), 256)))
     return bad(MING_ERR_SHAPE, "more rows times columns than one launch holds");
   const Span out = p.gated ? byte_rows(p.h, p.n, p.ldh, w->N) : bf16_rows(p.y, p.n, p.ldy, w->N);
   const Span outs = bf16_rows(p.hs, p.gated ? blocks_of(w->N) : 0, p.ldhs, p.n);
@@ -218,8 +232,10 @@ int product(ming_ctx* c, const ming_f8* w, const Product& p) {
   const double bytes = wide * w->K * std::min(p.n, w->E) + (double)p.x_rows * w->K +
                        (p.gated ? 1.0 : 2.0) * p.n * w->N;
   const int rc = run(c, p.gated ? ming::kRtF8Swiglu : ming::kRtF8Lin, flops, bytes, p.who, [&] {
-    return plan <= 4 ? ming::launch_f8_tile(p.gated, p.grouped, a, plan, stream_of(c))
-                : ming::launch_f8_rows(p.gated, p.grouped, a, plan, stream_of(c));
+    if (plan.kind == F8Plan::kTiles)
+      return ming::launch_f8_tile(p.gated, p.grouped, a, plan.a, stream_of(c));
+    if (plan.kind == F8Plan::kDuo) return ming::launch_f8_duo(a, plan.a, stream_of(c));
+    return ming::launch_f8_rows(p.gated, p.grouped, a, plan.a, plan.b, stream_of(c));
   });
   if (rc != MING_OK) return rc;
   ming::rt_note_rows(c, 8, 2ull * (uint64_t)p.n * (uint64_t)w->N * w->halves * (uint64_t)w->K);
@@ -410,7 +426,8 @@ int ming_f8_shape(const ming_f8* w, int* n_experts, int* N, int* K, int* gated) 
 size_t ming_f8_workspace_bytes(const ming_f8* w, int rows) {
   if (!w || rows <= 0) return 0;
   DeviceGuard g(ming::rt_device(w->ctx));
-  return std::max(part_bytes(w, false, rows), part_bytes(w, true, rows));
+  const size_t grouped = part_bytes(w, plan_of(w, true, rows), rows);
+  return w->E > 1 ? grouped : std::max(grouped, part_bytes(w, plan_of(w, false, rows), rows));
 }
 
 int ming_f8_lin(ming_ctx* c, const ming_f8* w, const uint8_t* x, int64_t ldx, const uint16_t* xs,

@@ -29,25 +29,6 @@ namespace {
 
 constexpr int TBN = 256, NW = 8;
 
-// A 16-bit load into LDS, zero-extended to a dword a lane; waits as dma16_sb's.
-__device__ __forceinline__ void dma2_sb(const void* base, uint32_t off, uint32_t lds) {
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ushort %0, %1"
-               :: "v"(off), "s"(base), "s"(lds) : "m0");
-#pragma clang diagnostic pop
-}
-
-// 16 bytes a lane with an offset that moves both addresses.
-template <int OFF>
-__device__ __forceinline__ void dma16_off(const void* base, uint32_t off, uint32_t lds) {
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3"
-               :: "v"(off), "s"(base), "s"(lds), "n"(OFF) : "m0");
-#pragma clang diagnostic pop
-}
-
 template <int RF>
 struct TileLds {
   static constexpr int kStages = RF >= 3 ? 2 : 3;
@@ -86,8 +67,7 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
   };
   const uint8_t* const xbase = GROUPED ? a.x : a.x + (long long)p0 * a.ldx;
   const uint16_t* const sbase = GROUPED ? a.xs : a.xs + p0;
-  const uint8_t* const wbase =
-      a.w + e * a.w_expert + (long long)tn * (TBN * 128);
+  const uint8_t* const wbase = a.w + e * a.w_expert + (long long)tn * (TBN * 128);
   // LDS chunk p of x's tile holds row p >> 3, logical chunk (p & 7) ^ swizzle
   auto chunk_of = [&](int p) { return (p & 7) ^ ((p >> 4) & 7); };
   uint32_t xrow[XD];
@@ -137,11 +117,11 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
 
   // the weights' scales of all blocks: the tile's two blocks of rows, or gate and up
   {
-    const int b0 = 2 * tn, b1 = 2 * tn + 1 < a.NB ? 2 * tn + 1 : 2 * tn;
+    const int r0 = 2 * tn, r1 = 2 * tn + 1 < a.NB ? 2 * tn + 1 : 2 * tn;
     const float* ws = a.ws + e * a.s_expert;
     for (int k = tid; k < KB; k += 64 * NW) {
-      wsc[2 * k] = ws[(long long)k * a.NB + b0];
-      wsc[2 * k + 1] = ws[(long long)k * a.NB + b1];
+      wsc[2 * k] = ws[(long long)k * a.NB + r0];
+      wsc[2 * k + 1] = ws[(long long)k * a.NB + r1];
     }
   }
 

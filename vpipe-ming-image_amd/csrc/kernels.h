@@ -627,16 +627,20 @@ struct F8Args {
   const uint16_t* bias;   // optional
   uint16_t* y;
   long long ldy;
-  // gated: codes and scales out, and [n][N] f32 for the few-row kernel
+  // gated: codes and scales out
   uint8_t* h;
   long long ldh;
   uint16_t* hs;           // [blocks of N][ldhs]
   long long ldhs;
+  // f32 sums on their way: of the few-row kernel's gated results [n][N], of the tiles'
+  // slices of K (launch_f8_duo)
   float* part;
 };
 hipError_t launch_f8_repack(const uint8_t* codes, const float* scales, int N, int K, int halves,
                             uint8_t* out, float* souts, hipStream_t s);
-hipError_t launch_f8_rows(bool gated, bool grouped, const F8Args& a, int plan, hipStream_t s);
+// mf * 16 rows x nf * 16 columns a workgroup: 1 x 1, 1 x 2, 1 x 4, 2 x 2, 2 x 4.
+hipError_t launch_f8_rows(bool gated, bool grouped, const F8Args& a, int mf, int nf,
+                          hipStream_t s);
 // Blocks of tiles of tm rows x tn columns: every group ends in at most one partial one.
 inline long long f8_rows_blocks(int tm, int tn, bool grouped, int n, int E, int N) {
   const long long tiles_m = grouped ? n / tm + (n < E ? n : E) : ((long long)n + tm - 1) / tm;
@@ -657,9 +661,19 @@ inline long long f8_tile_blocks(int rf, bool grouped, int n, int E, int NR) {
   return tiles_m * ((NR + 255) / 256);
 }
 hipError_t validate_f8_tile_kernels();
-// Which kernel takes n rows (places): 0 the few-row one, else the tiles' rf. On a chip
-// of `cus`.
-int f8_plan(int cus, bool grouped, int E, int NR, int KB, int n);
+// Some hundred rows of a plain projection (f8_duo.hip), 64 x 128 a tile; with slices > 1
+// K is cut into that many, whose sums meet in part [slices][f8_duo_blocks][64][128]. The
+// limits as the tiles'.
+hipError_t launch_f8_duo(const F8Args& a, int slices, hipStream_t s);
+inline long long f8_duo_blocks(int n, int NR) { return ((long long)n + 63) / 64 * (NR / 128); }
+hipError_t validate_f8_duo_kernels();
+// Which kernel takes n rows (places) on a chip of `cus`: tiles of rf, the few-row one with
+// mf x nf fragments, or f8_duo's with its slices.
+struct F8Plan {
+  enum Kind { kRows, kDuo, kTiles } kind;
+  int a, b;               // kRows mf, nf; kDuo slices; kTiles rf
+};
+F8Plan f8_plan(int cus, bool gated, bool grouped, int E, int NR, int KB, int n);
 
 hipError_t validate_qproj_kernels();
 hipError_t validate_qproj_fast_kernels();

@@ -39,6 +39,17 @@ __device__ __forceinline__ void dma16_v(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
                :: "v"(src), "s"(lds) : "m0");
 }
+// 16 bits a lane, zero-extended to a dword of LDS.
+__device__ __forceinline__ void dma2_sb(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ushort %0, %1"
+               :: "v"(off), "s"(base), "s"(lds) : "m0");
+}
+// 16 bytes a lane with an instruction offset, which moves both addresses.
+template <int OFF>
+__device__ __forceinline__ void dma16_off(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3"
+               :: "v"(off), "s"(base), "s"(lds), "n"(OFF) : "m0");
+}
 #pragma clang diagnostic pop
 
 // LDS byte address of a __shared__ object: the low half of its generic

@@ -458,6 +458,7 @@ hipError_t validate_kernels(int device) {
   if (e == hipSuccess) e = ming::validate_f8_quant_kernels();
   if (e == hipSuccess) e = ming::validate_f8_rows_kernels();
   if (e == hipSuccess) e = ming::validate_f8_tile_kernels();
+  if (e == hipSuccess) e = ming::validate_f8_duo_kernels();
   if (known) done[device] = e == hipSuccess;
   return e;
 }
