@@ -231,12 +231,17 @@ __global__ void f8_repack_kernel(const uint8_t* codes, const float* scales, int 
 template <int MF, int NF>
 void rows_launch(bool gated, bool grouped, const F8Args& a, hipStream_t s) {
   const dim3 grid((unsigned)f8_rows_blocks(16 * MF, 16 * NF, grouped, a.n, a.E, a.N));
-  if (gated && grouped)
-    hipLaunchKernelGGL((f8_rows_kernel<MF, NF, true, true>), grid, dim3(64 * WK), 0, s, a);
-  else if (gated)
+  if constexpr (MF == 1) {
+    if (grouped) {
+      if (gated)
+        hipLaunchKernelGGL((f8_rows_kernel<MF, NF, true, true>), grid, dim3(64 * WK), 0, s, a);
+      else
+        hipLaunchKernelGGL((f8_rows_kernel<MF, NF, false, true>), grid, dim3(64 * WK), 0, s, a);
+      return;
+    }
+  }
+  if (gated)
     hipLaunchKernelGGL((f8_rows_kernel<MF, NF, true, false>), grid, dim3(64 * WK), 0, s, a);
-  else if (grouped)
-    hipLaunchKernelGGL((f8_rows_kernel<MF, NF, false, true>), grid, dim3(64 * WK), 0, s, a);
   else
     hipLaunchKernelGGL((f8_rows_kernel<MF, NF, false, false>), grid, dim3(64 * WK), 0, s, a);
 }
@@ -260,8 +265,10 @@ hipError_t launch_f8_rows(bool gated, bool grouped, const F8Args& a, int mf, int
     case 11: rows_launch<1, 1>(gated, grouped, a, s); break;
     case 12: rows_launch<1, 2>(gated, grouped, a, s); break;
     case 14: rows_launch<1, 4>(gated, grouped, a, s); break;
-    case 22: rows_launch<2, 2>(gated, grouped, a, s); break;
-    case 24: rows_launch<2, 4>(gated, grouped, a, s); break;
+    case 24:
+      if (grouped) return hipErrorInvalidValue;
+      rows_launch<2, 4>(gated, false, a, s);
+      break;
     default: return hipErrorInvalidValue;
   }
   hipError_t e = hipGetLastError();
@@ -276,13 +283,15 @@ hipError_t validate_f8_rows_kernels() {
   hipFuncAttributes fa;
 #define MING_F8_ROWS(MF, NF)                                                    \
   reinterpret_cast<const void*>(&f8_rows_kernel<MF, NF, false, false>),         \
-      reinterpret_cast<const void*>(&f8_rows_kernel<MF, NF, false, true>),      \
-      reinterpret_cast<const void*>(&f8_rows_kernel<MF, NF, true, false>),      \
-      reinterpret_cast<const void*>(&f8_rows_kernel<MF, NF, true, true>)
+      reinterpret_cast<const void*>(&f8_rows_kernel<MF, NF, true, false>)
+#define MING_F8_GROUPS(NF)                                                      \
+  reinterpret_cast<const void*>(&f8_rows_kernel<1, NF, false, true>),           \
+      reinterpret_cast<const void*>(&f8_rows_kernel<1, NF, true, true>)
   const void* fns[] = {reinterpret_cast<const void*>(&f8_finish_kernel),
                        reinterpret_cast<const void*>(&f8_repack_kernel), MING_F8_ROWS(1, 1),
-                       MING_F8_ROWS(1, 2), MING_F8_ROWS(1, 4), MING_F8_ROWS(2, 2),
-                       MING_F8_ROWS(2, 4)};
+                       MING_F8_ROWS(1, 2), MING_F8_ROWS(1, 4), MING_F8_ROWS(2, 4),
+                       MING_F8_GROUPS(1), MING_F8_GROUPS(2), MING_F8_GROUPS(4)};
+#undef MING_F8_GROUPS
 #undef MING_F8_ROWS
   for (const void* f : fns) {
     const hipError_t e = hipFuncGetAttributes(&fa, f);

@@ -24,28 +24,104 @@ struct ming_f8 {
 
 namespace ming {
 
-F8Plan f8_plan(int cus, bool gated, bool grouped, int E, int NR, int KB, int n) {
-  if (KB > kF8TileBlocks) return {F8Plan::kRows, 2, 2};
-  if (grouped) {
-    const double live = E * (1.0 - std::exp(-(double)n / E)), rows = n / live;
-    if (rows < 8.0) return {F8Plan::kRows, 1, 2};
-    if (rows < 24.0) return {F8Plan::kRows, 1, 4};
-    return {F8Plan::kTiles, rows < 112.0 ? 2 : 4, 0};
-  }
-  if (n <= 16) return {F8Plan::kRows, 1, 1};
-  if (n <= 64) return {F8Plan::kRows, 1, 4};
-  // rounds of the chip, a workgroup a CU, times a tile's time
-  int best = 4;
-  double least = 0.0;
-  for (int rf = 4; rf >= 1; --rf) {
-    const long long tiles = f8_tile_blocks(rf, false, n, 1, NR);
-    const double us = (double)((tiles + cus - 1) / cus) * (24 + 10 * rf);
-    if (rf == 4 || us < least) {
-      best = rf;
-      least = us;
+// Times (us) of n rows by each kernel's rounds of the chip, a workgroup a CU, fitted to
+// widths of 512 to 10240 at K = 512 to 10240, 1 to 8704 rows, out of cold caches. The choice
+// is then within 0.5% of the fastest one's time in the geometric mean of 279 shapes (worst
+// 15%), over groups, whose sizes are on the device (what an even router gives), 2.4% of
+// 156. rows: a start, the K blocks and a workgroup's end a round, and the weights' bytes
+// (MB). Two halves: a start a round and its stages, with slices their sum's launch and
+// bytes. Tiles: a start a round and its stages, which take longer where the chip is full.
+namespace {
+double rows_us(int i, bool gated, double wgs, int KB, double mb, int cus) {
+  static const double kPlain[4][4] = {{3.32, 0.062, 0.000, 0.05}, {3.08, 0.074, 0.011, 0.17},
+                                      {3.26, 0.100, 0.033, 0.30}, {1.85, 0.160, 0.035, 1.46}};
+  static const double kGated[4][4] = {{6.33, 0.069, 0.031, 0.14}, {6.08, 0.087, 0.046, 0.41},
+                                      {4.51, 0.149, 0.070, 1.83}, {3.52, 0.209, 0.067, 2.89}};
+  const double* c = gated ? kGated[i] : kPlain[i];
+  const double r = std::ceil(wgs / cus);
+  return c[0] + r * (c[1] * KB + c[3]) + c[2] * mb;
+}
+double tiles_us(int rf, bool gated, long long tiles, int KB, int cus) {
+  static const double kPlain[4][4] = {{1.20, 2.84, 0.439, 0.153}, {0.0, 4.66, 0.543, 0.317},
+                                      {0.0, 4.58, 0.994, 0.322}, {0.20, 5.27, 1.063, 0.607}};
+  static const double kGated[4][4] = {{1.31, 3.41, 0.455, 0.125}, {0.36, 5.63, 0.575, 0.241},
+                                      {0.40, 6.04, 0.992, 0.332}, {0.53, 7.53, 1.123, 0.485}};
+  const double* c = gated ? kGated[rf - 1] : kPlain[rf - 1];
+  const double r = (double)((tiles + cus - 1) / cus), fill = std::min(1.0, (double)tiles / cus);
+  return c[0] + r * (c[1] + KB * (c[2] + c[3] * fill));
+}
+constexpr int kRowShapes[4][2] = {{1, 1}, {1, 2}, {1, 4}, {2, 4}};
+
+F8Plan group_plan(int cus, bool gated, int E, int NR, int KB, int n) {
+  const int N = gated ? NR / 2 : NR, tiles_n = (NR + 255) / 256;
+  const double live = E * (1.0 - std::exp(-(double)n / E)), rows = n / live;
+  const double mb = live * NR * (double)KB * 128e-6;
+  static const double kRows[2][3][4] = {
+      {{3.34, 0.064, 0.000, 0.42}, {2.86, 0.060, 0.071, 0.68}, {2.33, 0.076, 0.097, 1.20}},
+      {{5.80, 0.075, 0.052, 0.83}, {5.15, 0.125, 0.087, 0.91}, {3.97, 0.131, 0.146, 2.06}}};
+  static const double kTile[2][3] = {{3.34, 0.131, 0.343}, {4.97, 0.115, 0.383}};
+  F8Plan best{F8Plan::kTiles, 2, 0};
+  {
+    const double t = live * std::max(1.0, rows / 128 + (rows > 40 ? 0.5 : 0.0)) * tiles_n;
+    const double h = std::min(2.0, std::ceil(rows / 64)), r = std::max(1.0, t / cus);
+    const double* c = kTile[gated];
+    double least = 1.05 * (r * (c[0] + KB * h * c[2]) + c[1] * mb);
+    for (int i = 0; i < 3; ++i) {
+      const int nf = kRowShapes[i][1];
+      const double w = live * (rows > 8 ? std::max(1.0, rows / 16 + 0.5) : 1.0) *
+                       ((N + 16 * nf - 1) / (16 * nf));
+      const double* q = kRows[gated][i];
+      const double us = q[0] + std::max(1.0, w / cus) * (q[1] * KB + q[3]) + q[2] * mb;
+      if (us < least) {
+        best = {F8Plan::kRows, 1, nf};
+        least = us;
+      }
     }
   }
-  return {F8Plan::kTiles, best, 0};
+  // tall tiles read and start less often; low ones fill the chip where there are few
+  if (best.kind == F8Plan::kTiles && rows >= 160.0 &&
+      live * (rows / 256 + 0.5) * tiles_n >= 0.6 * cus)
+    best.a = 4;
+  return best;
+}
+}  // namespace
+
+F8Plan f8_plan(int cus, bool gated, bool grouped, int E, int NR, int KB, int n) {
+  if (KB > kF8TileBlocks) return {F8Plan::kRows, 1, 4};
+  if (grouped) return group_plan(cus, gated, E, NR, KB, n);
+  const int N = gated ? NR / 2 : NR;
+  const double mb = NR * (double)KB * 128e-6;
+  F8Plan best{F8Plan::kTiles, 4, 0};
+  double least = 1e30;
+  auto take = [&](double us, F8Plan p) {
+    if (us < least) {
+      best = p;
+      least = us;
+    }
+  };
+  for (int rf = 4; rf >= 1; --rf)
+    take(tiles_us(rf, gated, f8_tile_blocks(rf, false, n, 1, NR), KB, cus), {F8Plan::kTiles, rf, 0});
+  // whole rounds of 256-row tiles, and what is left of the rows in tiles of 128
+  const int tiles_n = (NR + 255) / 256;
+  const long long whole = (long long)(n / 256) * tiles_n / cus * cus / tiles_n;
+  if (whole > 0 && 256 * whole < n)
+    take(tiles_us(4, gated, whole * tiles_n, KB, cus) +
+             tiles_us(2, gated, (n - 256 * whole + 127) / 128 * tiles_n, KB, cus),
+         {F8Plan::kTiles, 2, (int)whole});
+  for (int i = 0; i < 4; ++i) {
+    const int mf = kRowShapes[i][0], nf = kRowShapes[i][1];
+    const double wgs = (double)((n + 16ll * mf - 1) / (16 * mf)) * ((N + 16 * nf - 1) / (16 * nf));
+    take(rows_us(i, gated, wgs, KB, mb, cus), {F8Plan::kRows, mf, nf});
+  }
+  if (!gated)
+    for (int s = 1; s <= 4 && s <= KB; ++s) {
+      const long long tiles = f8_duo_blocks(n, NR) * s;
+      const double r = (double)((tiles + cus - 1) / cus), stages = (KB + 2 * s - 1) / (2 * s);
+      take(s == 1 ? 0.11 + r * (4.28 + 0.595 * stages)
+                  : 4.60 + r * (2.33 + 0.531 * stages) + 0.418 * 0.0328 * tiles,
+           {F8Plan::kDuo, s, 0});
+    }
+  return best;
 }
 
 }  // namespace ming
@@ -112,11 +188,14 @@ bool own_memory(const ming_ctx* c, const void* p) {
 }
 
 // The kernel that takes n rows of w on the current device. rt_set_f8_plan's choices: rf of
-// the tiles, 10 mf + nf of the few-row kernel, 100 * slices of f8_duo's.
+// the tiles (5: of 256 rows but for the last ones), 10 mf + nf of the few-row kernel, 100 *
+// slices of f8_duo's.
 ming::F8Plan plan_of(const ming_f8* w, bool grouped, int n) {
   using ming::F8Plan;
   const int set = ming::rt_f8_plan(w->ctx);
-  if (set > 0 && set < 10 && w->KB <= ming::kF8TileBlocks) return {F8Plan::kTiles, set, 0};
+  if (set == 5 && !grouped && w->KB <= ming::kF8TileBlocks)
+    return {F8Plan::kTiles, 2, (n - 1) / 256};
+  if (set > 0 && set < 5 && w->KB <= ming::kF8TileBlocks) return {F8Plan::kTiles, set, 0};
   if (set >= 10 && set < 100) return {F8Plan::kRows, set / 10, set % 10};
   if (set >= 100 && !grouped && w->halves == 1 && w->KB <= ming::kF8TileBlocks)
     return {F8Plan::kDuo, std::min(set / 100, w->KB), 0};
@@ -203,9 +282,11 @@ int product(ming_ctx* c, const ming_f8* w, const Product& p) {
                                        " given");
   using ming::F8Plan;
   const long long blocks =
-      plan.kind == F8Plan::kTiles  ? ming::f8_tile_blocks(plan.a, p.grouped, p.n, w->E, w->NR)
-      : plan.kind == F8Plan::kDuo ? ming::f8_duo_blocks(p.n, w->NR) * plan.a
-                                   : ming::f8_rows_blocks(16, 16, p.grouped, p.n, w->E, w->N);
+      plan.kind == F8Plan::kTiles && plan.b > 0 ? ming::f8_mixed_blocks(plan.b, p.n, w->NR)
+      : plan.kind == F8Plan::kTiles ? ming::f8_tile_blocks(plan.a, p.grouped, p.n, w->E, w->NR)
+      : plan.kind == F8Plan::kDuo
+          ? ming::f8_duo_blocks(p.n, w->NR) * plan.a
+          : ming::f8_rows_blocks(16 * plan.a, 16 * plan.b, p.grouped, p.n, w->E, w->N);
   if (!ming::one_launch(blocks, 512) ||
       (plan.kind == F8Plan::kRows && !ming::one_launch(ming::f8_finish_blocks(p.n, w->N), 256)))
     return bad(MING_ERR_SHAPE, "more rows times columns than one launch holds");
@@ -233,7 +314,7 @@ int product(ming_ctx* c, const ming_f8* w, const Product& p) {
                        (p.gated ? 1.0 : 2.0) * p.n * w->N;
   const int rc = run(c, p.gated ? ming::kRtF8Swiglu : ming::kRtF8Lin, flops, bytes, p.who, [&] {
     if (plan.kind == F8Plan::kTiles)
-      return ming::launch_f8_tile(p.gated, p.grouped, a, plan.a, stream_of(c));
+      return ming::launch_f8_tile(p.gated, p.grouped, a, plan.a, plan.b, stream_of(c));
     if (plan.kind == F8Plan::kDuo) return ming::launch_f8_duo(a, plan.a, stream_of(c));
     return ming::launch_f8_rows(p.gated, p.grouped, a, plan.a, plan.b, stream_of(c));
   });

@@ -363,6 +363,25 @@ __global__ __launch_bounds__(64 * NW, 1) void f8_tile_kernel(const F8Args a) {
   f8_tile<RF, GATED, false>(a, ring, 0, p0, left < BM ? left : BM, tn);
 }
 
+// The first `main` tiles of rows are of 256, the others of 128: a last round of the chip that
+// is mostly empty takes half the time.
+template <bool GATED>
+__global__ __launch_bounds__(64 * NW, 1) void f8_mixed_kernel(const F8Args a, int main) {
+  constexpr int kUnits = TileLds<4>::kUnits > TileLds<2>::kUnits ? TileLds<4>::kUnits
+                                                                   : TileLds<2>::kUnits;
+  __shared__ uint4 ring[kUnits];
+  const int tiles_n = (a.NR + TBN - 1) / TBN, first = main * tiles_n, b = (int)blockIdx.x;
+  int tm, tn;
+  if (b < first) {
+    tile_of_block(b, main, tiles_n, &tm, &tn);
+    f8_tile<4, GATED, false>(a, ring, 0, 256 * tm, 256, tn);
+  } else {
+    tile_of_block(b - first, (a.n - 256 * main + 127) / 128, tiles_n, &tm, &tn);
+    const int p0 = 256 * main + 128 * tm, left = a.n - p0;
+    f8_tile<2, GATED, false>(a, ring, 0, p0, left < 128 ? left : 128, tn);
+  }
+}
+
 // Groups of more than 64 * MAX places are cut into the fewest tiles that hold them.
 template <int MAX, bool GATED>
 __global__ __launch_bounds__(64 * NW, 1) void f8_group_tile_kernel(const F8Args a) {
@@ -411,10 +430,21 @@ void group_launch(bool gated, const F8Args& a, hipStream_t s) {
 
 }  // namespace
 
-hipError_t launch_f8_tile(bool gated, bool grouped, const F8Args& a, int rf, hipStream_t s) {
+hipError_t launch_f8_tile(bool gated, bool grouped, const F8Args& a, int rf, int main,
+                          hipStream_t s) {
   if (a.n <= 0) return hipSuccess;
+  if (main < 0 || (main > 0 && (grouped || rf != 2 || 256ll * main >= a.n)))
+    return hipErrorInvalidValue;
   if (a.N <= 0 || a.N % (gated ? 16 : 8) || a.K % 16 || a.KB > kF8TileBlocks || a.E < 1 || a.fan < 1)
     return hipErrorInvalidValue;
+  if (main > 0) {
+    const dim3 grid((unsigned)f8_mixed_blocks(main, a.n, a.NR));
+    if (gated)
+      hipLaunchKernelGGL((f8_mixed_kernel<true>), grid, dim3(64 * NW), 0, s, a, main);
+    else
+      hipLaunchKernelGGL((f8_mixed_kernel<false>), grid, dim3(64 * NW), 0, s, a, main);
+    return hipGetLastError();
+  }
   switch (grouped ? 10 + rf : rf) {
     case 1: tile_launch<1>(gated, a, s); break;
     case 2: tile_launch<2>(gated, a, s); break;
@@ -436,7 +466,9 @@ hipError_t validate_f8_tile_kernels() {
   reinterpret_cast<const void*>(&f8_group_tile_kernel<MAX, false>), \
       reinterpret_cast<const void*>(&f8_group_tile_kernel<MAX, true>)
   const void* fns[] = {MING_F8_TILE(1), MING_F8_TILE(2), MING_F8_TILE(3), MING_F8_TILE(4),
-                       MING_F8_GROUP(2), MING_F8_GROUP(4)};
+                       MING_F8_GROUP(2), MING_F8_GROUP(4),
+                       reinterpret_cast<const void*>(&f8_mixed_kernel<false>),
+                       reinterpret_cast<const void*>(&f8_mixed_kernel<true>)};
 #undef MING_F8_TILE
 #undef MING_F8_GROUP
   for (const void* f : fns) {

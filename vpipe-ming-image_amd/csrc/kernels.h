@@ -638,7 +638,7 @@ struct F8Args {
 };
 hipError_t launch_f8_repack(const uint8_t* codes, const float* scales, int N, int K, int halves,
                             uint8_t* out, float* souts, hipStream_t s);
-// mf * 16 rows x nf * 16 columns a workgroup: 1 x 1, 1 x 2, 1 x 4, 2 x 2, 2 x 4.
+// mf * 16 rows x nf * 16 columns a workgroup: 1 x 1, 1 x 2, 1 x 4 and, ungrouped, 2 x 4.
 hipError_t launch_f8_rows(bool gated, bool grouped, const F8Args& a, int mf, int nf,
                           hipStream_t s);
 // Blocks of tiles of tm rows x tn columns: every group ends in at most one partial one.
@@ -652,9 +652,14 @@ inline long long f8_finish_blocks(int n, int N) {
 hipError_t validate_f8_rows_kernels();
 // Many rows (f8_tile.hip): 64 * rf rows a tile, rf 1 to 4; over groups cut every 64 * rf
 // places, rf 2 or 4. Up to kF8TileBlocks blocks of K; ungrouped ldx below 2^22, grouped
-// x_rows * ldx below 2^31.
 constexpr int kF8TileBlocks = 1024;
-hipError_t launch_f8_tile(bool gated, bool grouped, const F8Args& a, int rf, hipStream_t s);
+// x_rows * ldx below 2^31. main > 0 (ungrouped, rf 2): the first 256 * main rows in tiles
+// of 256.
+hipError_t launch_f8_tile(bool gated, bool grouped, const F8Args& a, int rf, int main,
+                          hipStream_t s);
+inline long long f8_mixed_blocks(int main, int n, int NR) {
+  return (main + ((long long)n - 256ll * main + 127) / 128) * ((NR + 255) / 256);
+}
 inline long long f8_tile_blocks(int rf, bool grouped, int n, int E, int NR) {
   const int tm = 64 * rf;
   const long long tiles_m = grouped ? n / tm + (n < E ? n : E) : ((long long)n + tm - 1) / tm;
@@ -667,11 +672,11 @@ hipError_t validate_f8_tile_kernels();
 hipError_t launch_f8_duo(const F8Args& a, int slices, hipStream_t s);
 inline long long f8_duo_blocks(int n, int NR) { return ((long long)n + 63) / 64 * (NR / 128); }
 hipError_t validate_f8_duo_kernels();
-// Which kernel takes n rows (places) on a chip of `cus`: tiles of rf, the few-row one with
-// mf x nf fragments, or f8_duo's with its slices.
+// Which kernel takes n rows (places) on a chip of `cus`: the few-row one with mf x nf
+// fragments, f8_duo's with its slices, or tiles of rf behind `main` of 256 rows.
 struct F8Plan {
   enum Kind { kRows, kDuo, kTiles } kind;
-  int a, b;               // kRows mf, nf; kDuo slices; kTiles rf
+  int a, b;               // kRows mf, nf; kDuo slices; kTiles rf, main
 };
 F8Plan f8_plan(int cus, bool gated, bool grouped, int E, int NR, int KB, int n);
 
