@@ -67,6 +67,18 @@ __device__ __forceinline__ floatx4_t f8_mfma(const F8Frag& w, const F8Frag& x) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, zero, 0, 0, 0, 0, 0, 0);
 }
 
+// 16 bytes of an output, past the caches if it streams (kernels.h's f8_streams). The empty
+// statements keep the compiler from making one plain store of the two.
+__device__ __forceinline__ void f8_store16(void* p, const uint4& v, int stream) {
+  if (stream) {
+    asm volatile("");
+    store16_nt(p, v);
+    asm volatile("");
+  } else {
+    *reinterpret_cast<uint4*>(p) = v;
+  }
+}
+
 // Where column n of a gated stack has its gate row in the resident order: tiles
 // of 128 columns, 32 gate rows and the same 32 up rows in turn.
 __device__ __host__ __forceinline__ int f8_gate_row(int n) {

@@ -66,8 +66,8 @@ __global__ __launch_bounds__(256) void f8_quantize_kernel(const F8QuantArgs a, i
   const float t = __uint_as_float(top);
   const bool fine = f8_finite(t);
   const uint32_t sb = fine ? f8_scale_bits(t) : kF8NanScale;
-  *reinterpret_cast<uint4*>(a.codes + (long long)row * a.ldc + 16 * c) =
-      fine ? f8_codes16(v, sb) : make_uint4(kF8Nan4, kF8Nan4, kF8Nan4, kF8Nan4);
+  f8_store16(a.codes + (long long)row * a.ldc + 16 * c,
+             fine ? f8_codes16(v, sb) : make_uint4(kF8Nan4, kF8Nan4, kF8Nan4, kF8Nan4), a.stream);
   if ((c & 7) == 0) a.scales[(long long)(c >> 3) * a.lds + row] = (uint16_t)sb;
 }
 

@@ -304,6 +304,7 @@ int product(ming_ctx* c, const ming_f8* w, const Product& p) {
   a.s_expert = (long long)w->KB * w->NB;
   a.N = w->N; a.K = w->K; a.KB = w->KB; a.NR = w->NR; a.NB = w->NB;
   a.n = p.n;
+  a.stream = ming::f8_streams((p.gated ? 1.0 : 2.0) * p.n * w->N);
   a.offsets = p.offsets; a.order = p.order;
   a.E = w->E; a.fan = p.fan; a.x_rows = p.x_rows;
   a.bias = p.bias; a.y = p.y; a.ldy = p.ldy;
@@ -352,7 +353,8 @@ int ming_f8_quantize(ming_ctx* c, const uint16_t* x, int64_t ldx, int rows, int 
              {byte_rows(codes, rows, ldc, D), bf16_rows(scales, blocks_of(D), lds, rows)}))
     return bad(MING_ERR_ARG, "x, codes and scales must not share memory");
   DeviceGuard g(ming::rt_device(c));
-  const ming::F8QuantArgs a = {x, ldx, rows, D, codes, ldc, scales, lds};
+  const ming::F8QuantArgs a = {x,   ldx,    rows, D,  codes,
+                               ldc, scales, lds,  ming::f8_streams(1.0 * rows * D)};
   const int rc = run(c, ming::kRtF8Quant, 0.0, 3.0 * rows * D, "ming_f8_quantize",
                      [&] { return ming::launch_f8_quantize(a, stream_of(c)); });
   if (rc != MING_OK) return rc;

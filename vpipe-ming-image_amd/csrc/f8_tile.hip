@@ -115,13 +115,16 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
     }
   };
 
-  // the weights' scales of all blocks: the tile's two blocks of rows, or gate and up
+  // The weights' scales of all blocks, [KB][2]: of the tile's two blocks of rows, or gate's
+  // and up's. By DMA too, before the others, so that every wait covers them and nothing
+  // waits for them alone.
   {
-    const int r0 = 2 * tn, r1 = 2 * tn + 1 < a.NB ? 2 * tn + 1 : 2 * tn;
-    const float* ws = a.ws + e * a.s_expert;
-    for (int k = tid; k < KB; k += 64 * NW) {
-      wsc[2 * k] = ws[(long long)k * a.NB + r0];
-      wsc[2 * k + 1] = ws[(long long)k * a.NB + r1];
+    const float* const ws = a.ws + e * a.s_expert + 2 * tn;
+    const int odd = 2 * tn + 1 < a.NB ? lane & 1 : 0;
+    for (int i = 64 * wave; i < 2 * KB; i += 64 * NW) {
+      const int k = (i + lane) >> 1;
+      dma4_sb(ws, (uint32_t)(((k < KB ? k : KB - 1) * (long long)a.NB + odd) * 4),
+              lds_addr(wsc + i));
     }
   }
 
@@ -232,8 +235,7 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
       // (the last one's later ones are stage 0's to issue)
       if (t < NST - 1 || q < kPost) issue(q, ring + t * L::kStage);
   }
-  // stage 0 landed, the weights' scales written (their stores are waited for with the
-  // LDS counter)
+  // stage 0 landed, and the weights' scales
   ring_wait<(NST - 2) * kDma + kPost>();
 #pragma unroll
   for (int j = 0; j < NF; ++j) w[j] = read_w(ring, j);
@@ -313,8 +315,8 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
     for (int k = 0; k < RF; ++k) {
       const int p = 512 * k + tid, row = p >> 3, ch = p & 7, n = 128 * tn + 16 * ch;
       if (row < rows && n < a.N)
-        *reinterpret_cast<uint4*>(a.h + (long long)(p0 + row) * a.ldh + n) =
-            E[row * 8 + (ch ^ ((row >> 1) & 7))];
+        f8_store16(a.h + (long long)(p0 + row) * a.ldh + n, E[row * 8 + (ch ^ ((row >> 1) & 7))],
+                   a.stream);
     }
   } else {
     // each wave turns its 64 columns through its own part of LDS, then stores whole
@@ -347,7 +349,7 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
       const int ml = 8 * k + (lane >> 3), row = 32 * RF * wm + ml;
       const uint4 v = E[ml * 8 + (cl ^ ((ml >> 1) & 7))];
       if (row < rows && n < a.N)
-        *reinterpret_cast<uint4*>(a.y + (long long)(p0 + row) * a.ldy + n) = v;
+        f8_store16(a.y + (long long)(p0 + row) * a.ldy + n, v, a.stream);
     }
   }
 }
