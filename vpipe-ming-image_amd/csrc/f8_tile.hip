@@ -266,7 +266,9 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
   if constexpr (GATED) {
     // v = silu(gate) * up: fragments 0, 1 are the wave's 32 gate columns, 2, 3 the up
     // ones. A row's largest over the tile's 128 columns is a block's: over a lane's
-    // columns, the four lane quarters, and the four waves side by side, by LDS.
+    // columns, the four lane quarters, and the four waves side by side, by LDS. Then a
+    // thread makes a row's scale, once for the 16 lanes that multiply by its reciprocal
+    // (NaN for a block that holds a NaN or an inf).
     uint32_t* const tops = reinterpret_cast<uint32_t*>(ring);            // [4][64 RF]
     uint4* const E = ring + RF * 64;                                      // [64 RF][8]
 #pragma unroll
@@ -280,43 +282,44 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
           acc[j][i][r] = v;
           top = f8_top(top, v);
         }
+      top = f8_top_quarters(top);
+      if (g == 0) tops[64 * RF * wn + 32 * RF * wm + 16 * i + c] = top;
+    }
+    __syncthreads();
+    if (tid < 64 * RF) {
+      uint32_t top = tops[tid];
 #pragma unroll
-      for (int o = 16; o < 64; o <<= 1) {
-        const uint32_t v = (uint32_t)__shfl_xor((int)top, o, 64);
+      for (int k = 1; k < 4; ++k) {
+        const uint32_t v = tops[64 * RF * k + tid];
         top = top > v ? top : v;
       }
-      if (g == 0) tops[64 * RF * wn + 32 * RF * wm + 16 * i + c] = top;
+      const float tf = __uint_as_float(top);
+      const uint32_t sb = f8_finite(tf) ? f8_scale_bits(tf) : kF8NanScale;
+      if (tid < rows) a.hs[(long long)tn * a.ldhs + p0 + tid] = (uint16_t)sb;
+      tops[tid] = __float_as_uint(1.0f / __uint_as_float(sb << 16));
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < MF; ++i) {
       const int row = 32 * RF * wm + 16 * i + c;
-      uint32_t top = tops[row];
-#pragma unroll
-      for (int k = 1; k < 4; ++k) {
-        const uint32_t v = tops[64 * RF * k + row];
-        top = top > v ? top : v;
-      }
-      const float tf = __uint_as_float(top);
-      const bool fine = f8_finite(tf);
-      const uint32_t sb = fine ? f8_scale_bits(tf) : kF8NanScale;
-      const float q = 1.0f / __uint_as_float(sb << 16);
-      if (wn == 0 && g == 0 && row < rows) a.hs[(long long)tn * a.ldhs + p0 + row] = (uint16_t)sb;
+      const float q = __uint_as_float(tops[row]);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const floatx4_t& v = acc[j][i];
+        const uint32_t codes = f8_pack4(v[0] * q, v[1] * q, v[2] * q, v[3] * q);
         // chunk of 16 columns 2 wn + j, a lane quarter's dword
         reinterpret_cast<uint32_t*>(E)[(row * 8 + ((2 * wn + j) ^ ((row >> 1) & 7))) * 4 + g] =
-            fine ? f8_pack4(v[0] * q, v[1] * q, v[2] * q, v[3] * q) : kF8Nan4;
+            q == q ? codes : kF8Nan4;
       }
     }
     __syncthreads();
+    const int ch = tid & 7, n = 128 * tn + 16 * ch;
+    uint8_t* to = a.h + (long long)(p0 + (tid >> 3)) * a.ldh + n;
 #pragma unroll
-    for (int k = 0; k < RF; ++k) {
-      const int p = 512 * k + tid, row = p >> 3, ch = p & 7, n = 128 * tn + 16 * ch;
+    for (int k = 0; k < RF; ++k, to += 64 * a.ldh) {
+      const int row = 64 * k + (tid >> 3);
       if (row < rows && n < a.N)
-        f8_store16(a.h + (long long)(p0 + row) * a.ldh + n, E[row * 8 + (ch ^ ((row >> 1) & 7))],
-                   a.stream);
+        f8_store16(to, E[row * 8 + (ch ^ ((row >> 1) & 7))], a.stream);
     }
   } else {
     // each wave turns its 64 columns through its own part of LDS, then stores whole
@@ -326,30 +329,33 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
     const int nb = TBN * tn + 64 * wn;
 #pragma unroll
     for (int j = 0; j < NF; ++j) {
-      float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      const int n = nb + 16 * j + 4 * g;
-      if (!GROUPED && a.bias && n < a.N) {
-        const uint2 v = *reinterpret_cast<const uint2*>(a.bias + n);
-        b[0] = bf16_lo(v.x);
-        b[1] = bf16_hi(v.x);
-        b[2] = bf16_lo(v.y);
-        b[3] = bf16_hi(v.y);
+      if (!GROUPED && a.bias) {
+        const int n = nb + 16 * j + 4 * g;
+        uint2 v = {0, 0};
+        if (n < a.N) v = *reinterpret_cast<const uint2*>(a.bias + n);
+#pragma unroll
+        for (int i = 0; i < MF; ++i) {
+          acc[j][i][0] += bf16_lo(v.x);
+          acc[j][i][1] += bf16_hi(v.x);
+          acc[j][i][2] += bf16_lo(v.y);
+          acc[j][i][3] += bf16_hi(v.y);
+        }
       }
 #pragma unroll
       for (int i = 0; i < MF; ++i) {
         const int row = 16 * i + c;
         const floatx4_t& v = acc[j][i];
-        E2[(row * 8 + ((2 * j + (g >> 1)) ^ ((row >> 1) & 7))) * 2 + (g & 1)] = make_uint2(
-            pack_bf16x2_rne(v[0] + b[0], v[1] + b[1]), pack_bf16x2_rne(v[2] + b[2], v[3] + b[3]));
+        E2[(row * 8 + ((2 * j + (g >> 1)) ^ ((row >> 1) & 7))) * 2 + (g & 1)] =
+            make_uint2(pack_bf16x2_rne(v[0], v[1]), pack_bf16x2_rne(v[2], v[3]));
       }
     }
-    const int cl = lane & 7, n = nb + 8 * cl;
+    const int cl = lane & 7, n = nb + 8 * cl, first = 32 * RF * wm + (lane >> 3);
+    uint16_t* to = a.y + (long long)(p0 + first) * a.ldy + n;
 #pragma unroll
-    for (int k = 0; k < 4 * RF; ++k) {
-      const int ml = 8 * k + (lane >> 3), row = 32 * RF * wm + ml;
+    for (int k = 0; k < 4 * RF; ++k, to += 8 * a.ldy) {
+      const int ml = 8 * k + (lane >> 3);
       const uint4 v = E[ml * 8 + (cl ^ ((ml >> 1) & 7))];
-      if (row < rows && n < a.N)
-        f8_store16(a.y + (long long)(p0 + row) * a.ldy + n, v, a.stream);
+      if (first + 8 * k < rows && n < a.N) f8_store16(to, v, a.stream);
     }
   }
 }

@@ -15,6 +15,18 @@ struct RowGroup {
   int index;   // the block's index inside the group
 };
 
+// The sums over lanes 0 .. lane: inside rows of 16 by shifts, then over the rows by their
+// last lanes.
+__device__ __forceinline__ int scan_sum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);   // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);   // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);   // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);   // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast:15, rows 1, 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);   // row_bcast:31, rows 2, 3
+  return v;
+}
+
 // The group of unit pick(total) where group e has units(rows of e) consecutive
 // ones; none where pick says -1. Offsets are kept inside [0, n] and a group that
 // ends before it begins is empty, so a plan that is not one can name wrong rows
@@ -30,8 +42,9 @@ __device__ __forceinline__ RowGroup find_group(const int32_t* __restrict__ offse
     return v < 0 ? 0 : v < n ? v : n;
   };
   auto count = [&](int lo, int hi) { return hi > lo ? units(hi - lo) : 0; };
-  int sum = 0, lo = at(e0);
-  for (int j = 0; j < per; ++j) {
+  const int lo0 = at(e0), hi0 = at(e0 + 1);
+  int sum = count(lo0, hi0), lo = hi0;
+  for (int j = 1; j < per; ++j) {
     const int hi = at(e0 + j + 1);
     sum += count(lo, hi);
     lo = hi;
@@ -39,18 +52,17 @@ __device__ __forceinline__ RowGroup find_group(const int32_t* __restrict__ offse
   // A launch holds fewer units than 2^24 and no group of a plan more; the lanes of
   // what is no plan are cut so that their total stays an int.
   sum = sum < (1 << 25) - 1 ? sum : (1 << 25) - 1;
-  int run = sum;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int v = __shfl_up(run, o, 64);
-    if (lane >= o) run += v;
-  }
+  const int run = scan_sum(sum);
   RowGroup g = {-1, 0, 0, 0};
   const int b = pick(__builtin_amdgcn_readlane(run, 63));
   const uint64_t past = __ballot(run > b);
   if (b < 0 || !past) return g;
   const int w = __builtin_ctzll(past);     // the lane whose groups hold the block
   int left = b - (__builtin_amdgcn_readlane(run, w) - __builtin_amdgcn_readlane(sum, w));
+  if (per == 1) {                          // the lane has its one group's ends
+    const int p0 = __builtin_amdgcn_readlane(lo0, w);
+    return {w, p0, __builtin_amdgcn_readlane(hi0, w) - p0, left};
+  }
   int e = w * per;
   lo = at(e);                              // wave-uniform from here on
   for (int j = 0; j < per; ++j, ++e) {
