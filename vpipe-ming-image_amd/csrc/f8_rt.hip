@@ -52,7 +52,13 @@ double tiles_us(int rf, bool gated, long long tiles, int KB, int cus) {
 }
 constexpr int kRowShapes[4][2] = {{1, 1}, {1, 2}, {1, 4}, {2, 4}};
 
-F8Plan group_plan(int cus, bool gated, int E, int NR, int KB, int n) {
+// Rows up to which a kernel with sums in the workspace is taken, which keeps the scan of
+// workspace() short: tiles have won by then (groups: by some 40 rows each).
+constexpr int kPartRows = 4096, kPartGroupRows = 64;
+
+F8Plan group_plan(int cus, bool gated, int E, int NR, int KB, int rows_in) {
+  // in steps of an eighth of a row a group, so that the scan has few sizes to look at
+  const int step = std::max(1, E / 8), n = (rows_in + step - 1) / step * step;
   const int N = gated ? NR / 2 : NR, tiles_n = (NR + 255) / 256;
   const double live = E * (1.0 - std::exp(-(double)n / E)), rows = n / live;
   const double mb = live * NR * (double)KB * 128e-6;
@@ -66,7 +72,7 @@ F8Plan group_plan(int cus, bool gated, int E, int NR, int KB, int n) {
     const double h = std::min(2.0, std::ceil(rows / 64)), r = std::max(1.0, t / cus);
     const double* c = kTile[gated];
     double least = 1.05 * (r * (c[0] + KB * h * c[2]) + c[1] * mb);
-    for (int i = 0; i < 3; ++i) {
+    for (int i = 0; i < 3 && n <= kPartGroupRows * E; ++i) {
       const int nf = kRowShapes[i][1];
       const double w = live * (rows > 8 ? std::max(1.0, rows / 16 + 0.5) : 1.0) *
                        ((N + 16 * nf - 1) / (16 * nf));
@@ -108,13 +114,13 @@ F8Plan f8_plan(int cus, bool gated, bool grouped, int E, int NR, int KB, int n) 
     take(tiles_us(4, gated, whole * tiles_n, KB, cus) +
              tiles_us(2, gated, (n - 256 * whole + 127) / 128 * tiles_n, KB, cus),
          {F8Plan::kTiles, 2, (int)whole});
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 4 && n <= kPartRows; ++i) {
     const int mf = kRowShapes[i][0], nf = kRowShapes[i][1];
     const double wgs = (double)((n + 16ll * mf - 1) / (16 * mf)) * ((N + 16 * nf - 1) / (16 * nf));
     take(rows_us(i, gated, wgs, KB, mb, cus), {F8Plan::kRows, mf, nf});
   }
   if (!gated)
-    for (int s = 1; s <= 4 && s <= KB; ++s) {
+    for (int s = 1; s <= (n <= kPartRows ? 4 : 1) && s <= KB; ++s) {
       const long long tiles = f8_duo_blocks(n, NR) * s;
       const double r = (double)((tiles + cus - 1) / cus), stages = (KB + 2 * s - 1) / (2 * s);
       take(s == 1 ? 0.11 + r * (4.28 + 0.595 * stages)
@@ -207,6 +213,21 @@ size_t part_bytes(const ming_f8* w, const ming::F8Plan& p, int n) {
   return p.kind == ming::F8Plan::kDuo && p.a > 1
              ? (size_t)p.a * ming::f8_duo_blocks(n, w->NR) * (64 * 128 * 4)
              : 0;
+}
+
+// The most that a call of up to `rows` rows needs. A plan holds over 16 rows (a group's
+// over a step) and what it needs grows with the rows, so each stretch's last ones do.
+size_t workspace(const ming_f8* w, bool grouped, int rows) {
+  auto need = [&](int n) { return part_bytes(w, plan_of(w, grouped, n), n); };
+  size_t most = need(rows);
+  const int step = grouped ? std::max(1, w->E / 8) : 16;
+  const int last = std::min(rows, grouped ? ming::kPartGroupRows * w->E : ming::kPartRows);
+  for (int n = step; n < last + step; n += step) {
+    const int at = std::min(n, last);
+    most = std::max(most, need(at));
+    if (at > 1) most = std::max(most, need(at - 1));
+  }
+  return most;
 }
 
 // What a product's call brings.
@@ -509,8 +530,8 @@ int ming_f8_shape(const ming_f8* w, int* n_experts, int* N, int* K, int* gated) 
 size_t ming_f8_workspace_bytes(const ming_f8* w, int rows) {
   if (!w || rows <= 0) return 0;
   DeviceGuard g(ming::rt_device(w->ctx));
-  const size_t grouped = part_bytes(w, plan_of(w, true, rows), rows);
-  return w->E > 1 ? grouped : std::max(grouped, part_bytes(w, plan_of(w, false, rows), rows));
+  const size_t grouped = workspace(w, true, rows);
+  return w->E > 1 ? grouped : std::max(grouped, workspace(w, false, rows));
 }
 
 int ming_f8_lin(ming_ctx* c, const ming_f8* w, const uint8_t* x, int64_t ldx, const uint16_t* xs,
