@@ -371,3 +371,36 @@ def test_no_plan_stays_in_bounds(ctx, plan, gated):  # noqa: F811
             assert torch.all(out[:, N:] == 77)
             assert torch.all(hs[0] == 77) and torch.all(hs[-1] == 77) and torch.all(hs[:, n:] == 77)
     W.w.close()
+
+
+def test_profiler_and_counters(ctx):
+    n, N, K = 40, 144, 272
+    L, G = Weights(ctx, 7800, 1, N, K, False), Weights(ctx, 7801, 1, N, K, True)
+    x = torch.randn((n, K), device="cuda").bfloat16()
+    w = torch.ones(K, device="cuda").bfloat16()
+    c = torch.zeros((n, K), dtype=torch.uint8, device="cuda")
+    s = torch.zeros((ref.blocks(K), n), dtype=torch.int16, device="cuda")
+    y = torch.zeros((n, N), dtype=torch.int16, device="cuda")
+    h = torch.zeros((n, N), dtype=torch.uint8, device="cuda")
+    hs = torch.zeros((ref.blocks(N), n), dtype=torch.int16, device="cuda")
+    ws = torch.zeros(16 + G.w.workspace_bytes(n), dtype=torch.uint8, device="cuda")
+    ctx.profile_collect()
+    ctx.set_profiling(True)
+    before = ctx.engagement()
+    sync()
+    ctx.f8_quantize(x, n, K, c, s)
+    ctx.f8_rmsnorm(x, w, n, K, c, s)
+    ctx.f8_lin(L.w, c, s, y, n, ws=ws)
+    ctx.f8_swiglu(G.w, c, s, h, hs, n, ws=ws)
+    prof = ctx.profile_collect()
+    ctx.set_profiling(False)
+    after = ctx.engagement()
+    for b, flops, size in (("f8_quantize", 0, 3 * n * K), ("f8_rmsnorm", 0, 3 * n * K),
+                           ("f8_lin", 2 * n * N * K, N * K + n * K + 2 * n * N),
+                           ("f8_swiglu", 4 * n * N * K, 2 * N * K + n * K + n * N)):
+        assert prof[b]["launches"] == 1 and prof[b]["ms"] > 0, b
+        assert prof[b]["flops"] == flops and prof[b]["bytes"] == size, b
+    for k, v in (("gemm_q8", 2), ("rmsnorm", 1), ("elementwise", 1)):
+        assert after[k] - before[k] == v, k
+    L.w.close()
+    G.w.close()

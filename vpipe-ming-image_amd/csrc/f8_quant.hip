@@ -1,6 +1,11 @@
 // What makes the operands of the 8-bit products: rows of bf16 into e4m3 codes with
 // a scale for each 128 columns, the same from an RMSNorm with the residual's
-// addition before it, and weights in blocks of 128 x 128. HBM-bound.
+// addition before it, and weights in blocks of 128 x 128.
+//
+// HBM-bound, one pass: everything between the loads and the stores is in registers.
+// Measured out of cold caches: quantizing 8704 x 3840 16.1 us (6.2 TB/s), the norm of
+// 8704 x 3840 with the residual 46.0 (5.1), of 203 x 2048 with y 5.1; eight rows or one
+// are a launch, 4.0 and 5.0 (2.5 in the kernel).
 #include "common.h"
 #include "f8.h"
 #include "kernels.h"
@@ -45,7 +50,8 @@ __device__ __forceinline__ uint32_t top8(uint32_t t) {
   return t;
 }
 
-// A thread takes 16 columns, 8 threads a block of 128, `per` threads a row.
+// A thread takes 16 columns, 8 threads a block of 128, `per` threads a row: a block's
+// largest takes three shuffles, and a thread's codes are one store of 16 bytes.
 __global__ __launch_bounds__(256) void f8_quantize_kernel(const F8QuantArgs a, int per) {
   const uint32_t i = blockIdx.x * 256u + threadIdx.x;
   const uint32_t row = i / (uint32_t)per;

@@ -7,7 +7,14 @@
 // in the matrix instruction's own order: no barrier and no LDS before the waves'
 // sums meet, so as many loads as registers hold are in flight. A block of K is one
 // v_mfma_f32_16x16x128 a tile, whose f32 result joins the sum times both scales
-// (f32: the scales are any, not the hardware's powers of two).
+// (f32: the scales are any, not the hardware's powers of two). Gated results go through
+// f32 memory to f8_finish_kernel: a block's 128 columns are several workgroups'.
+//
+// Measured out of cold caches: one row x [3840, 3840] 4.7 us (3.1 TB/s; 2.9 by bytes, the
+// rest a launch's start and end), gated [10240, 3840] 15.1 (5.2 TB/s), eight rows 15.6;
+// 8 x 8 places of [64][1024, 2048] gated 31.2 (5.5 TB/s). With weights in rows of 128
+// bytes, 16 lines a load, the gated ones took 17.6 and 44; more than one block ahead a
+// wave won nothing (occupancy); fp16 products, whose sums would be exact, cost 3 to 20%.
 #include "common.h"
 #include "f8.h"
 #include "kernels.h"
@@ -157,6 +164,12 @@ __global__ __launch_bounds__(64 * WK) void f8_rows_kernel(const F8Args a) {
   }
 }
 
+template <int CTRL>
+__device__ __forceinline__ uint32_t f8_top_row(uint32_t top) {
+  const uint32_t t = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, CTRL, 0xf, 0xf, false);
+  return top > t ? top : t;
+}
+
 // Columns n .. n + 3 of a row's block b, lane l of the 32 that hold it (in: they exist;
 // lanes without take part in the shuffles).
 __device__ __forceinline__ void f8_store_block(const F8Args& a, int row, int b, int n, int l, bool in,
@@ -164,11 +177,12 @@ __device__ __forceinline__ void f8_store_block(const F8Args& a, int row, int b, 
   uint32_t top = 0;
 #pragma unroll
   for (int r = 0; r < 4; ++r) top = f8_top(top, v[r]);
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t t = (uint32_t)__shfl_xor((int)top, o, 64);
-    top = top > t ? top : t;
-  }
+  top = f8_top_row<0x128>(top);            // row_ror by 8, 4, 2, 1, then the other row of 16
+  top = f8_top_row<0x124>(top);
+  top = f8_top_row<0x122>(top);
+  top = f8_top_row<0x121>(top);
+  const auto o = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+  top = o[0] > o[1] ? o[0] : o[1];
   if (!in) return;
   const float t = __uint_as_float(top);
   const bool fine = f8_finite(t);
@@ -179,7 +193,8 @@ __device__ __forceinline__ void f8_store_block(const F8Args& a, int row, int b, 
   if (l == 0) a.hs[(long long)b * a.ldhs + row] = (uint16_t)sb;
 }
 
-// The gated results [n][N] in f32 into codes and scales: 32 lanes a block of 128.
+// The gated results [n][N] in f32 into codes and scales: 32 lanes a block of 128. A
+// dependent launch, 2 to 4.7 us of the above; the results are still in L2.
 __global__ __launch_bounds__(256) void f8_finish_kernel(const F8Args a, int rows, int blocks) {
   const uint32_t unit = blockIdx.x * 8u + (threadIdx.x >> 5);
   const int l = (int)threadIdx.x & 31;
@@ -190,10 +205,10 @@ __global__ __launch_bounds__(256) void f8_finish_kernel(const F8Args a, int rows
     held = held < rows ? held : rows;
   }
   const int n = 128 * b + 4 * l;
-  const bool in = b < blocks && row < held && n < a.N;
-  floatx4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (in) v = *reinterpret_cast<const floatx4_t*>(a.part + (long long)row * a.N + n);
-  f8_store_block(a, row, b, n, l, in, v);
+  floatx4_t v = {0.0f, 0.0f, 0.0f, 0.0f};  // (loaded beside held, not after it)
+  if (b < blocks && n < a.N)
+    v = *reinterpret_cast<const floatx4_t*>(a.part + (long long)row * a.N + n);
+  f8_store_block(a, row, b, n, l, b < blocks && row < held && n < a.N, v);
 }
 
 // Codes [halves * N][K] and scales [halves * blocks of N][KB] into the resident order,

@@ -26,8 +26,8 @@ namespace ming {
 
 // Times (us) of n rows by each kernel's rounds of the chip, a workgroup a CU, fitted to
 // widths of 512 to 10240 at K = 512 to 10240, 1 to 8704 rows, out of cold caches. The choice
-// is then within 0.5% of the fastest one's time in the geometric mean of 279 shapes (worst
-// 15%), over groups, whose sizes are on the device (what an even router gives), 2.4% of
+// is then within 1% of the fastest one's time in the geometric mean of 279 shapes (worst
+// 15%), over groups, whose sizes are on the device (what an even router gives), 2.5% of
 // 156. rows: a start, the K blocks and a workgroup's end a round, and the weights' bytes
 // (MB). Two halves: a start a round and its stages, with slices their sum's launch and
 // bytes. Tiles: a start a round and its stages, which take longer where the chip is full.

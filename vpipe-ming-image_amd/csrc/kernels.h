@@ -661,9 +661,9 @@ inline long long f8_finish_blocks(int n, int N) {
 hipError_t validate_f8_rows_kernels();
 // Many rows (f8_tile.hip): 64 * rf rows a tile, rf 1 to 4; over groups cut every 64 * rf
 // places, rf 2 or 4. Up to kF8TileBlocks blocks of K; ungrouped ldx below 2^22, grouped
-constexpr int kF8TileBlocks = 1024;
 // x_rows * ldx below 2^31. main > 0 (ungrouped, rf 2): the first 256 * main rows in tiles
 // of 256.
+constexpr int kF8TileBlocks = 1024;
 hipError_t launch_f8_tile(bool gated, bool grouped, const F8Args& a, int rf, int main,
                           hipStream_t s);
 inline long long f8_mixed_blocks(int main, int n, int NR) {
