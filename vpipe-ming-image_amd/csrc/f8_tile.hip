@@ -17,9 +17,9 @@
 // operands are in registers by then, so the slot is free for the DMA, and the next
 // stage's first operands are read under their matrix instructions.
 //
-// Measured: 8704 x [3840, 10240] 287 us (2390 TFLOP/s), x [10240, 3840] 294; 4352 rows
-// gated [10240, 3840] 307 (2230); 34816 places of [64][2048, 1024] 112 to 115 (1290, 2.8
-// TB/s). A stage of 256 rows is 1.65 us, 2600 TFLOP/s over the chip: the power limit (the
+// Measured: 8704 x [3840, 10240] 280 to 290 us (2360 to 2440 TFLOP/s), x [10240, 3840]
+// 288 to 295; 4352 rows gated [10240, 3840] 307 (2230); 34816 places of [64][2048, 1024]
+// 110 to 112 (1310, 2.8 TB/s). A stage of 256 rows is 1.65 us, 2600 TFLOP/s over the chip: the power limit (the
 // matrix instruction alone 3400, with the sums, LDS and DMA 2914). Around a tile's stages
 // 0.9 us go to its start, 0.8 to the first stage's arrival, 3 to the results (gated 5) and
 // 1.2 to the change of workgroups, which short K feels. v_mfma_f32_32x32x64 has half the
@@ -332,13 +332,13 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
     }
   } else {
     // each wave turns its 64 columns through its own part of LDS, then stores whole
-    // 128-byte row pieces
+    // 128-byte row pieces; 32 rows at a time, so that the first stores are on their way early
     uint4* const E = ring + 32 * RF * 8 * wave;
     uint2* const E2 = reinterpret_cast<uint2*>(E);
     const int nb = TBN * tn + 64 * wn;
+    if (!GROUPED && a.bias) {
 #pragma unroll
-    for (int j = 0; j < NF; ++j) {
-      if (!GROUPED && a.bias) {
+      for (int j = 0; j < NF; ++j) {
         const int n = nb + 16 * j + 4 * g;
         uint2 v = {0, 0};
         if (n < a.N) v = *reinterpret_cast<const uint2*>(a.bias + n);
@@ -350,21 +350,26 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
           acc[j][i][3] += bf16_hi(v.y);
         }
       }
-#pragma unroll
-      for (int i = 0; i < MF; ++i) {
-        const int row = 16 * i + c;
-        const floatx4_t& v = acc[j][i];
-        E2[(row * 8 + ((2 * j + (g >> 1)) ^ ((row >> 1) & 7))) * 2 + (g & 1)] =
-            make_uint2(pack_bf16x2_rne(v[0], v[1]), pack_bf16x2_rne(v[2], v[3]));
-      }
     }
     const int cl = lane & 7, n = nb + 8 * cl, first = 32 * RF * wm + (lane >> 3);
     uint16_t* to = a.y + (long long)(p0 + first) * a.ldy + n;
 #pragma unroll
-    for (int k = 0; k < 4 * RF; ++k, to += 8 * a.ldy) {
-      const int ml = 8 * k + (lane >> 3);
-      const uint4 v = E[ml * 8 + (cl ^ ((ml >> 1) & 7))];
-      if (first + 8 * k < rows && n < a.N) f8_store16(to, v, a.stream);
+    for (int q = 0; q < RF; ++q) {
+#pragma unroll
+      for (int j = 0; j < NF; ++j)
+#pragma unroll
+        for (int i = 2 * q; i < 2 * q + 2; ++i) {
+          const int row = 16 * i + c;
+          const floatx4_t& v = acc[j][i];
+          E2[(row * 8 + ((2 * j + (g >> 1)) ^ ((row >> 1) & 7))) * 2 + (g & 1)] =
+              make_uint2(pack_bf16x2_rne(v[0], v[1]), pack_bf16x2_rne(v[2], v[3]));
+        }
+#pragma unroll
+      for (int k = 4 * q; k < 4 * q + 4; ++k, to += 8 * a.ldy) {
+        const int ml = 8 * k + (lane >> 3);
+        const uint4 v = E[ml * 8 + (cl ^ ((ml >> 1) & 7))];
+        if (first + 8 * k < rows && n < a.N) f8_store16(to, v, a.stream);
+      }
     }
   }
 }
