@@ -78,7 +78,7 @@ __global__ __launch_bounds__(64 * NW, 1) void f8_duo_kernel(const F8Args a, int 
         case 0: dma16_off<0>(wnext, off, to); break;
         case 1: dma16_off<1024>(wnext, off, to); break;
         case 2: dma16_off<2048>(wnext, off, to); break;
-        default: dma16_off<3072>(wnext, off, to); break;
+        default: dma16_off<3 * 1024>(wnext, off, to); break;
       }
     } else {
       dma2_sb(snext, soff, lds_addr(S + kX + kW));

@@ -15,6 +15,8 @@
 // 8 x 8 places of [64][1024, 2048] gated 31.2 (5.5 TB/s). With weights in rows of 128
 // bytes, 16 lines a load, the gated ones took 17.6 and 44; more than one block ahead a
 // wave won nothing (occupancy); fp16 products, whose sums would be exact, cost 3 to 20%.
+#include <algorithm>
+
 #include "common.h"
 #include "f8.h"
 #include "kernels.h"
@@ -214,11 +216,15 @@ __global__ __launch_bounds__(256) void f8_finish_kernel(const F8Args a, int rows
 // Codes [halves * N][K] and scales [halves * blocks of N][KB] into the resident order,
 // zeros past N and K: blocks of K outermost, then 16 rows (gated, f8_gate_row's), as the
 // matrix instruction's lanes hold them: chunks g and g + 4 of row c for lane 16 g + c, the
-// first ones of all lanes before the second ones.
+// first ones of all lanes before the second ones. blockIdx.y is the expert.
 __global__ void f8_repack_kernel(const uint8_t* codes, const float* scales, int N, int K, int halves,
                                  uint8_t* out, float* souts) {
   const int KB = (K + 127) / 128, nb = (N + 127) / 128, NR = halves * nb * 128;
-  const long long total = (long long)KB * NR * 8;
+  const long long total = (long long)KB * NR * 8, e = blockIdx.y;
+  codes += e * halves * N * K;
+  scales += e * halves * nb * KB;
+  out += e * total * 16;
+  souts += e * halves * nb * KB;
   for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total;
        i += (long long)gridDim.x * blockDim.x) {
     const int l = (int)(i & 63), ch = (l >> 4) + 4 * (int)((i >> 6) & 1);
@@ -263,11 +269,15 @@ void rows_launch(bool gated, bool grouped, const F8Args& a, hipStream_t s) {
 
 }  // namespace
 
-hipError_t launch_f8_repack(const uint8_t* codes, const float* scales, int N, int K, int halves,
-                            uint8_t* out, float* souts, hipStream_t s) {
-  if (N <= 0 || K <= 0 || K % 16) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(f8_repack_kernel, dim3(2048), dim3(256), 0, s, codes, scales, N, K, halves, out,
-                     souts);
+hipError_t launch_f8_repack(const uint8_t* codes, const float* scales, int experts, int N, int K,
+                            int halves, uint8_t* out, float* souts, hipStream_t s) {
+  if (experts < 1 || experts > 65535 || N <= 0 || K <= 0 || K % 16) return hipErrorInvalidValue;
+  const long long units = (K + 127ll) / 128 * ((N + 127ll) / 128) * halves * 128 * 8;
+  const long long each = (2048 + experts - 1) / experts;   // blocks, some 2048 in all
+  hipLaunchKernelGGL(f8_repack_kernel,
+                     dim3((unsigned)std::min(std::max(each, 32ll), (units + 255) / 256),
+                          (unsigned)experts),
+                     dim3(256), 0, s, codes, scales, N, K, halves, out, souts);
   return hipGetLastError();
 }
 

@@ -19,7 +19,7 @@ struct ming_f8 {
   int E = 0, N = 0, K = 0, halves = 0;
   int KB = 0, NR = 0, NB = 0;      // blocks of K, resident rows and scales a block of K
   uint8_t* codes = nullptr;        // [E][KB][NR][128], in 16 rows at a time
-  float* scales = nullptr;         // [E][KB][NB]
+  float* scales = nullptr;         // [E][KB][NB], behind the codes in one allocation
 };
 
 namespace ming {
@@ -451,7 +451,6 @@ int ming_f8_destroy(ming_f8* w) {
   DeviceGuard g(ming::rt_device(w->ctx));
   (void)hipStreamSynchronize(stream_of(w->ctx));
   if (w->codes) (void)hipFree(w->codes);
-  if (w->scales) (void)hipFree(w->scales);
   ming::rt_release(w->ctx);
   delete w;
   return rt_ok();
@@ -487,8 +486,8 @@ int ming_f8_create(ming_ctx* c, int n_experts, int N, int K, int gated, const ui
   const hipMemcpyKind kind = src_on_device ? hipMemcpyDefault : hipMemcpyHostToDevice;
   uint8_t* dc = nullptr;
   float* ds = nullptr;
-  hipError_t e = hipMalloc(&w->codes, E * kept);
-  if (e == hipSuccess) e = hipMalloc(&w->scales, E * ones * 4);
+  hipError_t e = hipMalloc(&w->codes, E * (kept + 4 * ones));
+  if (e == hipSuccess) w->scales = reinterpret_cast<float*>(w->codes + E * kept);
   if (e == hipSuccess && !direct) e = hipMalloc(&dc, some * one);
   if (e == hipSuccess && !direct) e = hipMalloc(&ds, some * ones * 4);
   for (size_t i0 = 0; i0 < E && e == hipSuccess; i0 += some) {
@@ -501,9 +500,9 @@ int ming_f8_create(ming_ctx* c, int n_experts, int N, int K, int gated, const ui
       sc = dc;
       ss = ds;
     }
-    for (size_t i = 0; i < n && e == hipSuccess; ++i)
-      e = ming::launch_f8_repack(sc + i * one, ss + i * ones, N, K, halves,
-                                 w->codes + (i0 + i) * kept, w->scales + (i0 + i) * ones, s);
+    if (e == hipSuccess)
+      e = ming::launch_f8_repack(sc, ss, (int)n, N, K, halves, w->codes + i0 * kept,
+                                 w->scales + i0 * ones, s);
   }
   if (e == hipSuccess) e = hipStreamSynchronize(s);
   if (dc) (void)hipFree(dc);

@@ -112,7 +112,7 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
         case 0: dma16_off<0>(wnext, woff, to); break;
         case 1: dma16_off<1024>(wnext, woff, to); break;
         case 2: dma16_off<2048>(wnext, woff, to); break;
-        default: dma16_off<3072>(wnext, woff, to); break;
+        default: dma16_off<3 * 1024>(wnext, woff, to); break;
       }
     } else {
       dma2_sb(snext, soff, lds_addr(S + L::kX + L::kW) + 4 * srow);

@@ -645,8 +645,8 @@ struct F8Args {
   // slices of K (launch_f8_duo)
   float* part;
 };
-hipError_t launch_f8_repack(const uint8_t* codes, const float* scales, int N, int K, int halves,
-                            uint8_t* out, float* souts, hipStream_t s);
+hipError_t launch_f8_repack(const uint8_t* codes, const float* scales, int experts, int N, int K,
+                            int halves, uint8_t* out, float* souts, hipStream_t s);
 // mf * 16 rows x nf * 16 columns a workgroup: 1 x 1, 1 x 2, 1 x 4 and, ungrouped, 2 x 4.
 hipError_t launch_f8_rows(bool gated, bool grouped, const F8Args& a, int mf, int nf,
                           hipStream_t s);
