@@ -11,7 +11,9 @@
 //
 // Measured out of cold caches: 203 x [2560, 10240] 17.8 us in slices (28.3 in one; the
 // few-row kernel 28, tiles of 64 rows 43.6), 13.5 x [3840, 3840], 1024 rows 22.3 (1350
-// TFLOP/s). A stage of two blocks is 0.53 us a workgroup, near a CU's rate out of L2.
+// TFLOP/s). A stage of two blocks is 0.53 us a workgroup out of L2, 0.7 out of memory, after
+// a start of 3.2 that fills the ring at 107 GB/s a CU; with the weights' scales by DMA that
+// start is 2.7, and the first stage lands as much later.
 #include <type_traits>
 
 #include "common.h"
