@@ -4,8 +4,9 @@
 //
 // HBM-bound, one pass: everything between the loads and the stores is in registers.
 // Measured out of cold caches: quantizing 8704 x 3840 16.1 us (6.2 TB/s), the norm of
-// 8704 x 3840 with the residual 46.0 (5.1), of 203 x 2048 with y 5.1; eight rows or one
-// are a launch, 4.0 and 5.0 (2.5 in the kernel).
+// 8704 x 3840 with the residual 46.0 (5.1). Small ones take what a call costs the host:
+// eight rows quantized 3.8 (2.5 in the kernel), a row's norm 4.6 (2.5), 203 x 2048 with y
+// 4.6 (3.6).
 #include "common.h"
 #include "f8.h"
 #include "kernels.h"

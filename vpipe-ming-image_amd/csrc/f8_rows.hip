@@ -10,8 +10,8 @@
 // (f32: the scales are any, not the hardware's powers of two). Gated results go through
 // f32 memory to f8_finish_kernel: a block's 128 columns are several workgroups'.
 //
-// Measured out of cold caches: one row x [3840, 3840] 4.7 us (3.1 TB/s; 2.9 by bytes, the
-// rest a launch's start and end), gated [10240, 3840] 15.1 (5.2 TB/s), eight rows 15.6;
+// Measured out of cold caches: one row x [3840, 3840] 4.6 us (4.0 in the kernel; 2.9 by
+// bytes, the rest a launch's start and end), gated [10240, 3840] 15.1 (5.2 TB/s), eight rows 15.6;
 // 8 x 8 places of [64][1024, 2048] gated 31.2 (5.5 TB/s). With weights in rows of 128
 // bytes, 16 lines a load, the gated ones took 17.6 and 44; more than one block ahead a
 // wave won nothing (occupancy); fp16 products, whose sums would be exact, cost 3 to 20%.

@@ -135,14 +135,16 @@ F8Plan f8_plan(int cus, bool gated, bool grouped, int E, int NR, int KB, int n) 
 namespace {
 
 struct DeviceGuard {
-  int prev = -1;
+  int prev = -1;                           // the device to go back to, -1: none
   explicit DeviceGuard(int dev) {
     if (hipGetDevice(&prev) != hipSuccess) prev = -1;
-    if (prev != dev) (void)hipSetDevice(dev);
+    if (prev == dev)
+      prev = -1;
+    else
+      (void)hipSetDevice(dev);
   }
   ~DeviceGuard() {
-    int cur = -1;
-    if (prev >= 0 && hipGetDevice(&cur) == hipSuccess && cur != prev) (void)hipSetDevice(prev);
+    if (prev >= 0) (void)hipSetDevice(prev);
   }
 };
 

@@ -321,13 +321,12 @@ def _check(rc: int):
 
 def _ptr(t) -> int:
     """Device (or host numpy) pointer of a tensor / array / int."""
-    if t is None:
-        return None
-    if isinstance(t, int):
+    if t is None or isinstance(t, int):
         return t
-    if hasattr(t, "data_ptr"):
+    try:
         return t.data_ptr()
-    return t.ctypes.data
+    except AttributeError:
+        return t.ctypes.data
 
 
 def _scales(scales):
@@ -597,11 +596,12 @@ class Ctx:
                    eps: float = 1e-6, ldx=None, ldsub=None, ldh=None, ldy=None, ldc=None,
                    lds=None):
         """h = x + sub, then its RMSNorm as e4m3 codes and scales (and bf16 y)."""
-        def at(v):
-            return D if v is None else v
-        _check(lib().ming_f8_rmsnorm(self.h, _ptr(x), at(ldx), _ptr(sub), at(ldsub), _ptr(h),
-                                     at(ldh), _ptr(w), _ptr(y), at(ldy), _ptr(codes), at(ldc),
-                                     _ptr(scales), rows if lds is None else lds, rows, D, eps))
+        _check(lib().ming_f8_rmsnorm(self.h, _ptr(x), D if ldx is None else ldx, _ptr(sub),
+                                     D if ldsub is None else ldsub, _ptr(h),
+                                     D if ldh is None else ldh, _ptr(w), _ptr(y),
+                                     D if ldy is None else ldy, _ptr(codes),
+                                     D if ldc is None else ldc, _ptr(scales),
+                                     rows if lds is None else lds, rows, D, eps))
 
     def f8_quantize_weight(self, w, N: int, K: int, codes, scales):
         """bf16 w [N][K] into codes [N][K] and scales [ceil(N / 128)][ceil(K / 128)]."""
@@ -648,9 +648,7 @@ def _itemsize(t) -> int:
 
 
 def _nbytes(t) -> int:
-    if t is None:
-        return 0
-    return t.numel() * t.element_size() if hasattr(t, "element_size") else t.nbytes
+    return 0 if t is None else t.nbytes
 
 
 def group_rows_workspace_bytes(n: int, n_groups: int) -> int:
