@@ -22,6 +22,7 @@ on a bounded row sample on the host cores.
 from __future__ import annotations
 
 import argparse
+import gc
 import json
 import os
 import sys
@@ -654,6 +655,10 @@ def main():
         # epilogue, lin(w2) -- the same bits as the four separate calls
         ctx.ffn(w1, w3, w2, x, y, M, SCALES, h=g)
 
+    # Python's own collection of garbage goes over every object of the imports (some 20 ms)
+    # whenever its count of allocations says so: now, not between the steps
+    gc.collect()
+    gc.freeze()
     for _ in range(args.warmup):
         step()
     ctx.synchronize()
