@@ -531,7 +531,8 @@ int ming_f8_swiglu(ming_ctx* ctx, const ming_f8* w, const uint8_t* x, int64_t ld
  * offsets, n of ming_group_rows; order NULL: x in place order): place p of expert
  * e's group has x row order[p] / fan and e's weights. x [x_rows][ldx], x_rows * ldx
  * below 2^31; ws by ming_f8_workspace_bytes for n rows. Rows of the outputs (and of
- * hs) from offsets[n_experts] on are left as they were. */
+ * hs) before offsets[0], of a part of a plan, and from offsets[n_experts] on are left
+ * as they were. */
 int ming_f8_experts_lin(ming_ctx* ctx, const ming_f8* w, const uint8_t* x, int64_t ldx,
                         const uint16_t* xs, int64_t ldxs, int x_rows, const int32_t* order,
                         int fan, const int32_t* offsets, int n, uint16_t* y, int64_t ldy,

@@ -1,0 +1,49 @@
+"""Edges of the operators in 8-bit floating point that their documentation allows."""
+import numpy as np
+import pytest
+import torch
+
+import f8_ref as ref
+import ming_dit_amd as m
+import rows_ref
+from helpers import bf16, f32, from_dev, randn, sync, to_dev
+from test_f8_gpu import S8, S16, Weights, call, check, check_norm, norm, plan  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- a part of a plan ------------------------------------------------------------------
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("counts,e0", [([5, 9, 20, 3], 1), ([70, 0, 1, 130], 2), ([3, 0, 300, 40], 1)])
+def test_a_part_of_a_plan(ctx, plan, gated, counts, e0):  # noqa: F811
+    """The experts from e0 on with their part of the plan's offsets: their groups' rows have
+    the whole plan's results, the rows of the groups before stay as they were."""
+    E, N, K = len(counts), 272, 208
+    W = Weights(ctx, 8000, E - e0, N, K, gated)
+    offsets, order, src = rows_ref.plan_of(counts, n=sum(counts) + 11, fan=2, seed=E, x_rows=50)
+    n, first, held = order.size, int(offsets[e0]), int(offsets[-1])
+    x, xs = ref.make_rows(8001, 50, K)
+    xd, sd, od = to_dev(x), to_dev(xs), to_dev(order)
+    fd = to_dev(offsets)
+    for p in (-1,) + ref.GROUPED_PLANS:
+        print(f"case f8 part of a plan {p} gated={gated} {counts}", flush=True)
+        plan(p)
+        ws = torch.full((16 + W.w.workspace_bytes(n),), 0x41, dtype=torch.uint8, device="cuda")
+        out = to_dev(np.full((n, N), S8 if gated else S16, np.uint8 if gated else np.uint16))
+        hs = to_dev(np.full((ref.blocks(N), n), S16, np.uint16))
+        sync()
+        if gated:
+            ctx.f8_experts_swiglu(W.w, xd, sd, 50, od, fd[e0:], n, out, hs, fan=2, ws=ws)
+        else:
+            ctx.f8_experts_lin(W.w, xd, sd, 50, od, fd[e0:], n, out, fan=2, ws=ws)
+        ctx.synchronize()
+        o, s = from_dev(out), from_dev(hs)
+        away = [r for r in range(n) if r < first or r >= held]
+        assert np.all(o[away] == (S8 if gated else S16))
+        if gated:
+            assert np.all(s[:, away] == S16)
+            got = (o[first:held], np.ascontiguousarray(s[:, first:held]))
+        else:
+            got = f32(o[first:held]).astype(np.float64)
+        check(got, W, x, xs, offsets[e0:] - first, src[first:])
+    W.w.close()

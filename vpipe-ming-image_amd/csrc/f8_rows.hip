@@ -201,16 +201,18 @@ __global__ __launch_bounds__(256) void f8_finish_kernel(const F8Args a, int rows
   const uint32_t unit = blockIdx.x * 8u + (threadIdx.x >> 5);
   const int l = (int)threadIdx.x & 31;
   const int b = (int)(unit / (uint32_t)rows), row = (int)(unit - (uint32_t)b * (uint32_t)rows);
-  int held = rows;                         // rows behind the last group stay as they are
+  // rows before the first group and behind the last one stay as they are: part holds
+  // nothing of theirs
+  int first = 0, held = rows;
   if (a.offsets) {
+    first = a.offsets[0];
     held = a.offsets[a.E];
-    held = held < rows ? held : rows;
   }
   const int n = 128 * b + 4 * l;
   floatx4_t v = {0.0f, 0.0f, 0.0f, 0.0f};  // (loaded beside held, not after it)
   if (b < blocks && n < a.N)
     v = *reinterpret_cast<const floatx4_t*>(a.part + (long long)row * a.N + n);
-  f8_store_block(a, row, b, n, l, b < blocks && row < held && n < a.N, v);
+  f8_store_block(a, row, b, n, l, b < blocks && row >= first && row < held && n < a.N, v);
 }
 
 // Codes [halves * N][K] and scales [halves * blocks of N][KB] into the resident order,
