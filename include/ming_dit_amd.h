@@ -480,7 +480,7 @@ int ming_f8_quantize(ming_ctx* ctx, const uint16_t* x, int64_t ldx, int rows, in
  * bf16(x + sub), v = h * rsqrt(mean(h^2) + eps) * w, codes and scales of v, quantized
  * without a rounding before it; with y not NULL also y = bf16(v). Without sub (NULL, and h
  * NULL) h is x and not written; h may be x itself or sub itself, with its stride. A
- * row whose mean square is inf or NaN in f32 has codes and scales of NaN. D % 16
+ * row whose mean square is inf or NaN in f32 has codes, scales and y of NaN. D % 16
  * == 0, D <= 8192, eps 1e-12 to 1; pointers 16-byte aligned, strides multiples of
  * 8, ldc of 16. */
 int ming_f8_rmsnorm(ming_ctx* ctx, const uint16_t* x, int64_t ldx, const uint16_t* sub,

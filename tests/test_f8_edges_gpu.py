@@ -47,3 +47,26 @@ def test_a_part_of_a_plan(ctx, plan, gated, counts, e0):  # noqa: F811
             got = f32(o[first:held]).astype(np.float64)
         check(got, W, x, xs, offsets[e0:] - first, src[first:])
     W.w.close()
+
+
+# ---- norms -----------------------------------------------------------------------------
+@pytest.mark.parametrize("add", [False, True])
+def test_norm_of_a_mean_square_past_f32(ctx, add):
+    """A row whose mean square is inf or NaN in f32 is NaN in y as in its codes, and the
+    rows beside it stay as they are."""
+    D = 400
+    x = randn(8100, (7, D))
+    w = bf16(1.0 + randn(8, (D,), 0.3))
+    w[128:256] = 0                              # (its zeros too)
+    sub = bf16(randn(8101, (7, D))) if add else None
+    keep, odd = [0, 2, 4, 6], [1, 3, 5]
+    a = norm(ctx, bf16(x), w, sub, y=True)
+    x[1] = 1e20
+    x[3, 7] = np.inf
+    x[5, 399] = np.nan
+    h, y, codes, scales = norm(ctx, bf16(x), w, sub, y=True)
+    for p, q in zip((a[0], a[1], a[2], a[3].T), (h, y, codes, scales.T)):
+        if p is not None:
+            assert np.array_equal(p[keep], q[keep])
+    assert np.all((codes[odd] & 0x7f) == ref.NAN) and np.all(scales.T[odd] == 0x7fc0)
+    assert np.all(np.isnan(f32(y[odd])))

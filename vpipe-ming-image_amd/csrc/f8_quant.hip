@@ -151,8 +151,10 @@ __global__ __launch_bounds__(512) void f8_norm_kernel(const F8NormArgs a) {
   if ((c & 7) == 0) a.scales[(long long)(c >> 3) * a.lds + row] = (uint16_t)sb;
   if (a.y) {
     uint32_t y[8];
+    // a row without a mean square has no norm: v would be zeros where inv is 0
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = pack_bf16x2_rne(v[2 * e], v[2 * e + 1]);
+    for (int e = 0; e < 8; ++e)
+      y[e] = inv > 0.0f ? pack_bf16x2_rne(v[2 * e], v[2 * e + 1]) : kF8NanScale * 0x10001u;
     uint4* p = reinterpret_cast<uint4*>(a.y + (long long)row * a.ldy + 16 * c);
     p[0] = make_uint4(y[0], y[1], y[2], y[3]);
     p[1] = make_uint4(y[4], y[5], y[6], y[7]);
