@@ -70,3 +70,18 @@ def test_norm_of_a_mean_square_past_f32(ctx, add):
             assert np.array_equal(p[keep], q[keep])
     assert np.all((codes[odd] & 0x7f) == ref.NAN) and np.all(scales.T[odd] == 0x7fc0)
     assert np.all(np.isnan(f32(y[odd])))
+
+
+def test_norm_of_far_gains(ctx):
+    """Gains so large or small that gain * rsqrt(mean square) leaves f32's range where the
+    result does not."""
+    D = 272
+    x = randn(8110, (5, D))
+    x[0] = 0.0
+    x[1] *= 1e-10
+    x[2] *= 1e18
+    w = 1.0 + randn(8, (D,), 0.3)
+    for size in (1e33, 1e-25):
+        b, g = bf16(x), bf16((w * size).astype(np.float32))
+        _, y, codes, scales = norm(ctx, b, g, y=True, eps=1e-12)
+        check_norm(b, g, None, 1e-12, None, y, codes, scales)

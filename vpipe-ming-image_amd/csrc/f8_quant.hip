@@ -135,7 +135,7 @@ __global__ __launch_bounds__(512) void f8_norm_kernel(const F8NormArgs a) {
     unpack8(w1, w + 8);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      v[e] *= inv * w[e];
+      v[e] = v[e] * inv * w[e];            // (inv * w may leave f32 where this does not)
       top = f8_top(top, v[e]);
     }
   }
