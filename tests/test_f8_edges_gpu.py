@@ -85,3 +85,48 @@ def test_norm_of_far_gains(ctx):
         b, g = bf16(x), bf16((w * size).astype(np.float32))
         _, y, codes, scales = norm(ctx, b, g, y=True, eps=1e-12)
         check_norm(b, g, None, 1e-12, None, y, codes, scales)
+
+
+# ---- gated results on the border of two codes --------------------------------------------
+def border_case():
+    """(codes, scales, x, v): a gated weight of 64 columns whose results v are exact in f32
+    for the row x: 256 times whole numbers of 14 bits, each of four nibbles that x's columns
+    0, 8, 16 and 24 take up. Each block of 128 columns has a scale of another 8-bit
+    significand, and in it the borders of two codes with their neighbours."""
+    N, K = 128 * 128, 64
+    u = np.zeros(N, np.int64)
+    for b in range(128):
+        s = 128 + b
+        near = [sign * (q * s + d) for q in range(17, 32, 2) for sign in (1, -1) for d in (-1, 0, 1)]
+        u[128 * b:128 * b + 128] = np.resize(near, 128)
+        u[128 * b + 127] = 56 * s               # 448 times the scale s / 8
+    x = np.zeros((1, K))
+    codes = np.zeros((1, 2 * N, K))
+    codes[0, :N, 32], x[0, 32] = 16.0, 16.0     # gates of 256, whose sigmoid is 1
+    for k, at, w in ((0, 64.0, 2.0 ** 6), (8, 16.0, 16.0), (16, 1.0, 16.0), (24, 1.0, 1.0)):
+        x[0, k] = at
+        nibble = (np.abs(u) >> int(np.log2(at * w))) & 15
+        codes[0, N:, k] = np.sign(u) * nibble * w
+    scales = np.ones((1, 256, 1), np.float32)
+    v = 256.0 * u[None].astype(np.float64)
+    return ref.encode(codes), scales, ref.encode(x), v
+
+
+@pytest.mark.parametrize("M", [1, 70, 300])
+def test_gated_results_between_two_codes(ctx, plan, M):  # noqa: F811
+    """Codes are the nearest of v over the scale, ties to even, as the row quantizer's are."""
+    codes, scales, x, v = border_case()
+    N, K = codes.shape[1] // 2, codes.shape[2]
+    want, s = ref.quantize(v)
+    W = Weights.__new__(Weights)
+    W.codes, W.scales, W.E, W.N, W.K, W.gated = codes, scales, 1, N, K, True
+    W.w = m.F8(ctx, codes, scales, N, gated=True)
+    x, xs = np.repeat(x, M, 0), np.full((1, M), 0x3f80, np.uint16)
+    offsets = np.array([0, M], np.int32)
+    for p in ref.PLANS + tuple(-q for q in ref.GROUPED_PLANS):
+        print(f"case f8 borders plan {p} M={M}", flush=True)
+        plan(abs(p))
+        got, gs = call(ctx, W, x, xs) if p > 0 else call(ctx, W, x, xs, offsets, None, M)
+        assert np.array_equal(gs, np.repeat(s, M, 1)), p
+        assert np.array_equal(got, np.repeat(want, M, 0)), p
+    W.w.close()

@@ -34,6 +34,15 @@ __device__ __forceinline__ uint32_t f8_scale_bits(float top) {
 }
 constexpr uint32_t kF8NanScale = 0x7fc0u;
 
+// v / s correctly rounded, y = RN(1 / s): the product by y with its residual fed back
+// once (in the signs that leave a zero its own). A quotient of two 8-bit significands
+// lies on the border of two codes often (one in some hundred), where the rounded
+// reciprocal alone would move it.
+__device__ __forceinline__ float f8_quotient(float v, float s, float y) {
+  const float q = v * y;
+  return fmaf(fmaf(q, s, -v), -y, q);
+}
+
 // The largest magnitude's bits: as unsigned integers inf is above every finite
 // value and NaN above inf, so one max finds both.
 __device__ __forceinline__ uint32_t f8_top(uint32_t top, float v) {

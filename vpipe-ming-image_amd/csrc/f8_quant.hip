@@ -14,14 +14,6 @@
 namespace ming {
 namespace {
 
-// v / s correctly rounded, y = RN(1 / s): the product by y with its residual fed back
-// once (in the signs that leave a zero its own). A quotient of two 8-bit significands
-// lies on the border of two codes often (one in some hundred), where the rounded
-// reciprocal alone would move it.
-__device__ __forceinline__ float f8_quotient(float v, float s, float y) {
-  const float q = v * y;
-  return fmaf(fmaf(q, s, -v), -y, q);
-}
 // 16 columns' codes by the scale of bits sb.
 __device__ __forceinline__ uint4 f8_codes16(const float (&v)[16], uint32_t sb) {
   const float s = __uint_as_float(sb << 16), y = 1.0f / s;

@@ -189,9 +189,11 @@ __device__ __forceinline__ void f8_store_block(const F8Args& a, int row, int b, 
   const float t = __uint_as_float(top);
   const bool fine = f8_finite(t);
   const uint32_t sb = fine ? f8_scale_bits(t) : kF8NanScale;
-  const float q = 1.0f / __uint_as_float(sb << 16);
+  const float s = __uint_as_float(sb << 16), y = 1.0f / s;
   *reinterpret_cast<uint32_t*>(a.h + (long long)row * a.ldh + n) =
-      fine ? f8_pack4(v[0] * q, v[1] * q, v[2] * q, v[3] * q) : kF8Nan4;
+      fine ? f8_pack4(f8_quotient(v[0], s, y), f8_quotient(v[1], s, y), f8_quotient(v[2], s, y),
+                      f8_quotient(v[3], s, y))
+           : kF8Nan4;
   if (l == 0) a.hs[(long long)b * a.ldhs + row] = (uint16_t)sb;
 }
 

@@ -276,7 +276,7 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
     // v = silu(gate) * up: fragments 0, 1 are the wave's 32 gate columns, 2, 3 the up
     // ones. A row's largest over the tile's 128 columns is a block's: over a lane's
     // columns, the four lane quarters, and the four waves side by side, by LDS. Then a
-    // thread makes a row's scale, once for the 16 lanes that multiply by its reciprocal
+    // thread makes a row's scale and its reciprocal, once for the 16 lanes that divide by it
     // (NaN for a block that holds a NaN or an inf).
     uint32_t* const tops = reinterpret_cast<uint32_t*>(ring);            // [4][64 RF]
     uint4* const E = ring + RF * 64;                                      // [64 RF][8]
@@ -305,20 +305,23 @@ __device__ __forceinline__ void f8_tile(const F8Args& a, uint4* const ring, int 
       const float tf = __uint_as_float(top);
       const uint32_t sb = f8_finite(tf) ? f8_scale_bits(tf) : kF8NanScale;
       if (tid < rows) a.hs[(long long)tn * a.ldhs + p0 + tid] = (uint16_t)sb;
-      tops[tid] = __float_as_uint(1.0f / __uint_as_float(sb << 16));
+      // (a thread's own entries: no other one reads them before the barrier)
+      tops[tid] = sb << 16;
+      tops[64 * RF + tid] = __float_as_uint(1.0f / __uint_as_float(sb << 16));
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < MF; ++i) {
       const int row = 32 * RF * wm + 16 * i + c;
-      const float q = __uint_as_float(tops[row]);
+      const float s = __uint_as_float(tops[row]), y = __uint_as_float(tops[64 * RF + row]);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const floatx4_t& v = acc[j][i];
-        const uint32_t codes = f8_pack4(v[0] * q, v[1] * q, v[2] * q, v[3] * q);
+        const uint32_t codes = f8_pack4(f8_quotient(v[0], s, y), f8_quotient(v[1], s, y),
+                                        f8_quotient(v[2], s, y), f8_quotient(v[3], s, y));
         // chunk of 16 columns 2 wn + j, a lane quarter's dword
         reinterpret_cast<uint32_t*>(E)[(row * 8 + ((2 * wn + j) ^ ((row >> 1) & 7))) * 4 + g] =
-            q == q ? codes : kF8Nan4;
+            s == s ? codes : kF8Nan4;
       }
     }
     __syncthreads();
