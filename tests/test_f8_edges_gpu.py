@@ -130,3 +130,28 @@ def test_gated_results_between_two_codes(ctx, plan, M):  # noqa: F811
         assert np.array_equal(gs, np.repeat(s, M, 1)), p
         assert np.array_equal(got, np.repeat(want, M, 0)), p
     W.w.close()
+
+
+# ---- scales of inf -----------------------------------------------------------------------
+@pytest.mark.parametrize("K", [128, 272, 640, 1168])
+def test_a_scale_of_inf(ctx, plan, K):  # noqa: F811
+    """A row whose last block has a scale of inf has infinities, of the block's sum's sign,
+    from every kernel; the other rows have their own results."""
+    N, M = 144, 70
+    W = Weights(ctx, 8200, 1, N, K, False)
+    W.w.close()
+    W.codes[..., 128 * ((K - 1) // 128):] = 0x38          # ones
+    W.w = m.F8(ctx, W.codes, W.scales, N)
+    x, xs = ref.make_rows(8201, M, K)
+    x[[3, 69], 128 * ((K - 1) // 128):] = 0x30
+    x[69, 128 * ((K - 1) // 128):] = 0xb0
+    for p in ref.PLANS + ref.DUO:
+        print(f"case f8 inf plan {p} K={K}", flush=True)
+        plan(p)
+        big = xs.copy()
+        big[-1, [3, 69]] = 0x7f80
+        got = call(ctx, W, x, big)
+        assert np.all(got[3] == np.inf) and np.all(got[69] == -np.inf), p
+        keep = [r for r in range(M) if r not in (3, 69)]
+        assert np.array_equal(got[keep], call(ctx, W, x, xs)[keep])
+    W.w.close()

@@ -135,7 +135,9 @@ __global__ __launch_bounds__(64 * NW, 1) void f8_duo_kernel(const F8Args a, int 
     read(Sn, t + 1 < stages ? t + 1 : t, then);
     float s[MF];
 #pragma unroll
-    for (int i = 0; i < MF; ++i) s[i] = __uint_as_float(now.sx[i] << 16) * now.sw;
+    for (int i = 0; i < MF; ++i)
+      // (not a product by the 0 of a block behind the last: x's scale may be inf)
+      s[i] = kb0 + 2 * t + half < KB ? __uint_as_float(now.sx[i] << 16) * now.sw : 0.0f;
     floatx4_t dp[NF];
     constexpr int kEach = (kDma + MF - 1) / MF;
 #pragma unroll
