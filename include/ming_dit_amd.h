@@ -518,8 +518,9 @@ int ming_f8_shape(const ming_f8* w, int* n_experts, int* N, int* K, int* gated);
  * x and h 16-byte aligned with strides multiples of 16, y 16-byte aligned with
  * ldy % 8 == 0, bias 8-byte aligned; ldx below 2^22, M up to 2^28. ws 16-byte
  * aligned, at least the bytes that ming_f8_workspace_bytes names for M rows (which
- * serve calls of fewer rows too; NULL where it is 0); it holds nothing between
- * calls, and calls or graphs that may run at the same time need one each. */
+ * serve calls of fewer rows too; NULL where it is 0; beyond 2^28 rows what those
+ * need); it holds nothing between calls, and calls or graphs that may run at the
+ * same time need one each. */
 size_t ming_f8_workspace_bytes(const ming_f8* w, int rows);
 int ming_f8_lin(ming_ctx* ctx, const ming_f8* w, const uint8_t* x, int64_t ldx, const uint16_t* xs,
                 int64_t ldxs, uint16_t* y, int64_t ldy, int M, const uint16_t* bias, void* ws,

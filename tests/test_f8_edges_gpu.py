@@ -155,3 +155,16 @@ def test_a_scale_of_inf(ctx, plan, K):  # noqa: F811
         keep = [r for r in range(M) if r not in (3, 69)]
         assert np.array_equal(got[keep], call(ctx, W, x, xs)[keep])
     W.w.close()
+
+
+# ---- workspaces --------------------------------------------------------------------------
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("E,N,K", [(1, 272, 400), (64, 48, 144), (1, 16, 131088)])
+def test_workspaces_of_any_count(ctx, gated, E, N, K):
+    """Counts beyond the 2^28 rows that a call takes name what those need."""
+    W = Weights(ctx, 8300, E, N, K, gated)
+    most = W.w.workspace_bytes(1 << 28)
+    assert W.w.workspace_bytes((1 << 28) - 1) <= most
+    for n in ((1 << 28) + 1, 2 ** 31 - 8, 2 ** 31 - 1):
+        assert W.w.workspace_bytes(n) == most
+    W.w.close()

@@ -170,6 +170,9 @@ bool shared(std::initializer_list<Span> ins, std::initializer_list<Span> outs) {
   return false;
 }
 
+// The rows, or places, of a call.
+constexpr int kRowsMax = 1 << 28;
+
 // A stride in elements of b bytes whose rows' last byte 64 bits hold.
 bool stride_fits(int64_t ld) { return ld < (1ll << 30); }
 
@@ -269,7 +272,7 @@ int product(ming_ctx* c, const ming_f8* w, const Product& p) {
   if (p.n == 0) return rt_ok();
   if (!p.x || !p.xs || (p.grouped && !p.offsets) || (p.gated ? !p.h || !p.hs : !p.y))
     return bad(MING_ERR_ARG, "null argument");
-  if (p.n > 1 << 28 || p.x_rows > 1 << 28)
+  if (p.n > kRowsMax || p.x_rows > kRowsMax)
     return bad(MING_ERR_SHAPE, "at most 2^28 rows");
   if (p.x_rows == 0) return bad(MING_ERR_ARG, "places without rows of x");
   if (p.grouped && !p.order && p.x_rows < p.n)
@@ -530,6 +533,7 @@ int ming_f8_shape(const ming_f8* w, int* n_experts, int* N, int* K, int* gated) 
 
 size_t ming_f8_workspace_bytes(const ming_f8* w, int rows) {
   if (!w || rows <= 0) return 0;
+  rows = std::min(rows, kRowsMax);
   DeviceGuard g(ming::rt_device(w->ctx));
   const size_t grouped = workspace(w, true, rows);
   return w->E > 1 ? grouped : std::max(grouped, workspace(w, false, rows));
