@@ -647,6 +647,10 @@ def _itemsize(t) -> int:
     return t.element_size() if hasattr(t, "element_size") else t.itemsize
 
 
+def _dense(t) -> bool:
+    return t.is_contiguous() if hasattr(t, "is_contiguous") else bool(t.flags.c_contiguous)
+
+
 def _nbytes(t) -> int:
     return 0 if t is None else t.nbytes
 
@@ -772,8 +776,12 @@ class F8:
         byte each; scales f32 [E][ceil(N / 128)][ceil(K / 128)] (gated: each half's)."""
         shape = [int(v) for v in codes.shape]
         rows, K = shape[-2:]
-        if _itemsize(codes) != 1 or _itemsize(scales) != 4 or rows != (2 * N if gated else N):
-            raise ValueError("codes of one byte over N (gated 2 N) rows, scales of f32")
+        if len(shape) > 3 or _itemsize(codes) != 1 or rows != (2 * N if gated else N):
+            raise ValueError("codes of one byte over N (gated 2 N) rows")
+        if not str(scales.dtype).endswith("float32"):
+            raise ValueError("scales of f32")
+        if not (_dense(codes) and _dense(scales)):
+            raise ValueError("codes and scales in consecutive memory")
         E = shape[0] if len(shape) == 3 else 1
         blocks = (2 if gated else 1) * -(-N // 128) * -(-K // 128)
         if _nbytes(scales) != 4 * E * blocks:
