@@ -101,7 +101,7 @@ __device__ __forceinline__ void operands(const Raw<BITS>& r, uint4& w0, uint4& w
 // the weights of the experts that have rows, once (w4 and w8, by the loads beside
 // them, x and scales: 6 and 5 weights a ps). Blocks of 16 (gated) or 32 columns leave
 // thousands of them, so loads of many are in flight: [64][2048, 2048] dense, gated,
-// 64 places 59 us, 303 MB at 5.1 TB/s; [60][2048, 1024] w8, 16 places 10.9.
+// 64 places 54 to 56 us, 303 MB at 5.5 TB/s; [60][2048, 1024] w8, 16 places 10.9.
 //
 // WK waves with U groups in flight, by K: 8 with 2 (4 cost registers, so waves: 20 to
 // 55% longer), to K = 1024 with 1 ([60][2048, 1024] w8, 64 places 31.1 -> 26.0 us; K 7168

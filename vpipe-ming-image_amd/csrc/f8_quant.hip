@@ -2,11 +2,14 @@
 // a scale for each 128 columns, the same from an RMSNorm with the residual's
 // addition before it, and weights in blocks of 128 x 128.
 //
-// HBM-bound, one pass: everything between the loads and the stores is in registers.
+// One pass: everything between the loads and the stores is in registers. The quantizer is
+// bound by HBM. The norm stays at a copy's 5.1 TB/s (an addition of two arrays reaches 6.0 to
+// 6.2): a lane's 16 columns are two stores of 16 bytes to h and to y, so a wave's store takes
+// every other 16 bytes, half of each line, and cannot go past the caches (46 -> 72 us).
 // Measured out of cold caches: quantizing 8704 x 3840 16.1 us (6.2 TB/s), the norm of
 // 8704 x 3840 with the residual 46.0 (5.1). Small ones take what a call costs the host:
-// eight rows quantized 3.8 (2.5 in the kernel), a row's norm 4.6 (2.5), 203 x 2048 with y
-// 4.6 (3.6).
+// eight rows quantized 3.8 to 4.1 (2.5 in the kernel), a row's norm 4.6 to 5.0 (2.5), 203 x
+// 2048 with y 4.6 to 5.0 (3.6).
 #include "common.h"
 #include "f8.h"
 #include "kernels.h"

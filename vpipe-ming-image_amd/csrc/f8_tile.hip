@@ -18,8 +18,9 @@
 // stage's first operands are read under their matrix instructions.
 //
 // Measured: 8704 x [3840, 10240] 280 to 290 us (2360 to 2440 TFLOP/s), x [10240, 3840]
-// 288 to 295; 4352 rows gated [10240, 3840] 307 (2230); 34816 places of [64][2048, 1024]
-// 110 to 112 (1310, 2.8 TB/s). A stage of 256 rows is 1.65 us, 2600 TFLOP/s over the chip: the power limit (the
+// 288 to 295; 4352 rows gated [10240, 3840] 298 to 303 (2260 to 2300), 203 rows 26 to 27;
+// 34816 places of [64][2048, 1024] 110 to 113 (1310, 2.8 TB/s), gated of [64][1024, 2048] 191
+// (1530). A stage of 256 rows is 1.65 us, 2600 TFLOP/s over the chip: the power limit (the
 // matrix instruction alone 3400, with the sums, LDS and DMA 2914). Around a tile's stages
 // 0.9 us go to its start, 0.8 to the first stage's arrival, 3 to the results (gated 5) and
 // 1.2 to the change of workgroups, which short K feels. v_mfma_f32_32x32x64 has half the

@@ -570,8 +570,8 @@ int experts_cut_on(int cus, int E, int N, int K, int bits, int n);
 // of the eight L2s of 4 MB before the next call asks for them. Alone, 8704 x [10240, 3840]
 // takes 293 us against 319 and the quantizer of 8704 x 3840 16.1 against 19.7. norm, swiglu
 // and lin in turn, storing every output so: 146 against 136 at 1024 rows (10 MB and 8 MB),
-// 240 against 241 at 2048 (21 MB and 16 MB), 468 against 471 at 4352. Not for the norm, whose lanes store two halves of 32 bytes:
-// 46 -> 72 us at 8704 x 3840.
+// 240 against 241 at 2048 (21 MB and 16 MB), 468 against 471 at 4352. Not for the norm, whose
+// lanes store two halves of 32 bytes: 46 -> 72 us at 8704 x 3840.
 inline int f8_streams(double bytes) { return bytes > 24.0 * 1048576; }
 // Rows of bf16 into e4m3 codes, and scales [blocks of D][lds >= rows] in bf16.
 // D % 16 == 0; x and codes 16-byte aligned, ldx % 8 == 0, ldc % 16 == 0.
